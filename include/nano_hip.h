@@ -228,6 +228,77 @@ int nv_kv_write(nv_context* c, const void* k, const void* v, const void* slots, 
 int nv_sample_parallel_static(nv_context* c, const void* logits, const void* temps, const void* seeds,
                               void* out, int batch, int vocab);
 
+/* Serving with trees of drafted tokens (no counterpart in the reference). A tree
+ * has 1 to max_nodes <= 64 nodes, node 0 the sequence's last committed token, the
+ * others drafted, each after its parent. Sequence s's nodes are the rows
+ * row_starts[s] .. row_starts[s + 1] - 1 (row_starts: [batch + 1] i32) of the step,
+ * and node i's K and V lie at position contexts[s] + i of the sequence
+ * (contexts: [batch] i32, positions committed before node 0), wherever in the
+ * tree it stands. Node i's RoPE position is contexts[s] + its depth. */
+
+/* Bytes of workspace that nv_attention_tree needs for these arguments (0: none,
+ * and NULL will do); a host function, no device work. A workspace's contents do not matter and stay unspecified;
+ * calls that may overlap need one each. */
+int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, int max_nodes, int max_context,
+                                size_t* bytes);
+
+/* Attention of the trees' nodes over the paged cache. q, out: [rows, qh, dim] bf16;
+ * kc, vc: [blocks, bs, kvh, dim] bf16; masks: [rows] u64; tables: [batch, stride]
+ * i32. Row (s, i) attends to the positions before contexts[s] and to node j's for
+ * each bit j of its mask, its own among them if set. Softmax of q . k / sqrt(dim);
+ * fp32 sums and statistics. Rows that see nothing are +0, as are those of
+ * sequences with more than max_nodes nodes or more than min(max_context, stride *
+ * bs) positions, a negative context, or a score that is not finite at the maximum;
+ * positions in blocks outside [0, blocks) are not seen. Rows of no sequence are
+ * left as they were. max_context is any positive bound on a sequence's positions
+ * (contexts[s] + nodes) and, like max_nodes, sizes the launch. Returns -2 for
+ * qh % kvh != 0, an odd head dim or one above 256, max_nodes outside [1, 64]. */
+int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* vc, const void* contexts,
+                      const void* row_starts, const void* masks, const void* tables, void* out, void* workspace,
+                      int rows, int qh, int kvh, int dim, int bs, int blocks, int stride, int batch, int max_nodes,
+                      int max_context);
+
+/* Bytes of workspace that nv_verify_tree needs (16-byte aligned); a host function. */
+int nv_verify_tree_workspace(int rows, int batch, int vocab, size_t* bytes);
+
+/* Rejection sampling of the trees' drafted tokens: the path that the target
+ * accepts, and the token after it. logits: [rows, vocab] bf16, the target's after
+ * each node; draft_logits: the same of the model that drafted, whose distribution
+ * at a node its children were drawn from independently, or NULL for children that
+ * were picked (the most likely, looked up); tokens, parents: [rows] i32 (parents:
+ * node indices below the node's own; node 0's is not read); temps: [batch] f32, <= 0
+ * greedy; uniforms: [rows] f32 in [0, 1), one a drafted token; seeds: [batch] u64,
+ * the Gumbel noise of the last token as nv_sample's. out_tokens: [batch, max_nodes]
+ * i32, the accepted tokens, then the token after them, then -1; out_nodes: [batch,
+ * max_nodes] i32, the path's nodes from 0 on, then -1; out_counts: [batch] i32, how
+ * many of either (0 for a sequence without rows, or with more than max_nodes, or
+ * with rows outside [0, rows)). For temps > 0 the tokens are distributed as the
+ * target's samples; for temps <= 0 they are its argmaxes. With nothing rejected at
+ * the path's last node, the token after it is nv_sample's for that row. */
+int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, const void* tokens,
+                   const void* parents, const void* row_starts, const void* temps, const void* uniforms,
+                   const void* seeds, void* out_tokens, void* out_nodes, void* out_counts, void* workspace, int rows,
+                   int batch, int max_nodes, int vocab);
+
+/* After verification: K and V at position contexts[s] + nodes[s, j] move to contexts[s]
+ * + j for j < counts[s], in every layer. nodes ([batch, max_nodes] i32) and counts
+ * ([batch] i32) are nv_verify_tree's out_nodes and out_counts; a sequence's nodes
+ * must rise from nodes[s, 0] >= 0 (moves stop at the first that does not, or that
+ * is not below max_nodes). kc, vc: [layers, blocks, bs, kvh, dim] bf16 (layers 1 for
+ * a layer by itself). Moves that touch a block outside [0, blocks) or a position
+ * past the table are left out; no sequence may read a slot that another writes. */
+int nv_kv_compact(nv_context* c, void* kc, void* vc, const void* contexts, const void* nodes, const void* counts,
+                  const void* tables, int batch, int max_nodes, int layers, int kvh, int dim, int bs, int blocks,
+                  int stride);
+
+/* The first min(tokens[i], bs) slots of block src[i] are copied to block dst[i], in
+ * every layer (src, dst, tokens: [copies] i32): the block that a forked sequence
+ * and its origin would both write, or any blocks that are to move. Copies of
+ * blocks outside [0, blocks) and onto themselves are left out. No block may be
+ * written twice, or read and written, by one call. */
+int nv_kv_copy_blocks(nv_context* c, void* kc, void* vc, const void* src, const void* dst, const void* tokens,
+                      int copies, int layers, int kvh, int dim, int bs, int blocks);
+
 /* Per-row Gumbel seed of src/runtime.rs:780-790 (host function, no device
  * work): mix(mix(base) ^ mix(request_id) ^ mix(generated)). */
 uint64_t nv_sampling_seed(uint64_t base, uint64_t request_id, uint64_t generated);

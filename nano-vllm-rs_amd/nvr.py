@@ -81,6 +81,12 @@ SIGNATURES = {
     "nv_sample_parallel": (_i, [_vp] * 7 + [_i, _i]),
     "nv_sample_parallel_static": (_i, [_vp] * 5 + [_i, _i]),
     "nv_kv_write": (_i, [_vp] * 6 + [_i] * 5),
+    "nv_attention_tree_workspace": (_i, [_i] * 7 + [ctypes.POINTER(_sz)]),
+    "nv_attention_tree": (_i, [_vp] * 10 + [_i] * 10),
+    "nv_verify_tree_workspace": (_i, [_i] * 3 + [ctypes.POINTER(_sz)]),
+    "nv_verify_tree": (_i, [_vp] * 13 + [_i] * 4),
+    "nv_kv_compact": (_i, [_vp] * 7 + [_i] * 8),
+    "nv_kv_copy_blocks": (_i, [_vp] * 6 + [_i] * 6),
     "nv_sampling_seed": (ctypes.c_uint64, [ctypes.c_uint64] * 3),
 }
 
@@ -143,6 +149,22 @@ def tile_gate_up_rows(gate_up: np.ndarray, intermediate: int) -> np.ndarray:
     rows 8t..8t+7."""
     w = np.asarray(gate_up).reshape(2, intermediate // 8, 8, -1)
     return np.ascontiguousarray(w.transpose(1, 0, 2, 3).reshape(2 * intermediate, -1))
+
+
+MAX_TREE_NODES = 64
+
+
+def tree_masks(parents: Sequence[int]) -> np.ndarray:
+    """The attention masks (u64) of one tree's nodes: each node's own bit and its ancestors'. parents[i] is the
+    node that node i follows, below i; node 0's is not read."""
+    if not 1 <= len(parents) <= MAX_TREE_NODES:
+        raise ArgumentError("value", f"a tree of {len(parents)} nodes; 1 to {MAX_TREE_NODES} are possible")
+    masks = [1]
+    for i, p in enumerate(parents[1:], 1):
+        if not 0 <= p < i:
+            raise ArgumentError("value", f"node {i} follows node {p}, which does not come before it")
+        masks.append(masks[p] | 1 << i)
+    return np.array(masks, np.uint64)
 
 
 def check_status(status: int, lib: ctypes.CDLL | None = None) -> None:
@@ -627,6 +649,115 @@ class Gpu:
         self._admit("sample_parallel_static", self._sampler_args(logits, temperatures, seeds, out, batch, vocab))
         self._call(self.lib.nv_sample_parallel_static(self.handle, logits.ptr, temperatures.ptr, seeds.ptr, out.ptr,
                                                       batch, vocab))
+
+    # ----------------------------------------- trees of drafted tokens ---
+    @staticmethod
+    def _tree_limit(op: str, max_nodes: int) -> None:
+        if not 1 <= max_nodes <= MAX_TREE_NODES:
+            raise ArgumentError("value", f"{op}: max_nodes {max_nodes} outside [1, {MAX_TREE_NODES}]")
+
+    def attention_tree_workspace(self, rows: int, qheads: int, kvheads: int, head_dim: int, batch_size: int,
+                                 max_nodes: int, max_context: int) -> int:
+        """Bytes of workspace that attention_tree needs for these arguments (0: none)."""
+        require_head_layout(qheads, kvheads, head_dim)
+        self._tree_limit("attention_tree_workspace", max_nodes)
+        as_dim(rows), as_dim(batch_size), as_dim(max_context)
+        n, lib = _sz(), self.lib or library()
+        check_status(lib.nv_attention_tree_workspace(rows, qheads, kvheads, head_dim, batch_size, max_nodes,
+                                                     max_context, ctypes.byref(n)), lib)
+        return n.value
+
+    def attention_tree(self, q: Buffer, kcache: Buffer, vcache: Buffer, contexts: Buffer, row_starts: Buffer,
+                       masks: Buffer, block_tables: Buffer, out: Buffer, workspace: Buffer | None, rows: int,
+                       qheads: int, kvheads: int, head_dim: int, block_size: int, num_blocks: int,
+                       table_stride: int, batch_size: int, max_nodes: int, max_context: int) -> None:
+        """Attention of drafted tokens: row row_starts[s] + i reads the positions before contexts[s] and, of its
+        tree, node j (at position contexts[s] + j) for each bit j of its mask. Trees have at most max_nodes (<= 64)
+        nodes, sequences at most max_context positions; workspace holds attention_tree_workspace bytes."""
+        need = self.attention_tree_workspace(rows, qheads, kvheads, head_dim, batch_size, max_nodes, max_context)
+        args = [_r("q", q, 2, rows, qheads, head_dim), _r("kcache", kcache, 2, num_blocks, block_size, kvheads, head_dim),
+                _r("vcache", vcache, 2, num_blocks, block_size, kvheads, head_dim), _r("contexts", contexts, 4, batch_size),
+                _r("row_starts", row_starts, 4, batch_size + 1), _r("masks", masks, 8, rows),
+                _r("block_tables", block_tables, 4, batch_size, table_stride), _w("out", out, 2, rows, qheads, head_dim)]
+        if need:
+            args.append(self._workspace("attention_tree", workspace, need))
+        self._admit("attention_tree", args)
+        self._call(self.lib.nv_attention_tree(
+            self.handle, q.ptr, kcache.ptr, vcache.ptr, contexts.ptr, row_starts.ptr, masks.ptr, block_tables.ptr,
+            out.ptr, workspace.ptr if need else None, rows, qheads, kvheads, head_dim, block_size, num_blocks,
+            table_stride, batch_size, max_nodes, max_context))
+
+    @staticmethod
+    def _workspace(op: str, workspace: Buffer | None, need: int):
+        if workspace is None:
+            raise ArgumentError("extent", f"{op}: needs {need} bytes of workspace")
+        return _w("workspace", workspace, 16, -(-need // 16))
+
+    def verify_tree_workspace(self, rows: int, batch_size: int, vocab: int) -> int:
+        """Bytes of workspace that verify_tree needs for these arguments."""
+        as_dim(rows), as_dim(batch_size), as_dim(vocab)
+        n, lib = _sz(), self.lib or library()
+        check_status(lib.nv_verify_tree_workspace(rows, batch_size, vocab, ctypes.byref(n)), lib)
+        return n.value
+
+    def verify_tree(self, logits: Buffer, draft_logits: Buffer | None, tokens: Buffer, parents: Buffer,
+                    row_starts: Buffer, temperatures: Buffer, uniforms: Buffer, seeds: Buffer, out_tokens: Buffer,
+                    out_nodes: Buffer, out_counts: Buffer, workspace: Buffer, rows: int, batch_size: int,
+                    max_nodes: int, vocab: int) -> None:
+        """Rejection sampling of drafted tokens. logits (and draft_logits, of the model whose distribution the
+        children of each node were drawn from; None where they were picked) [rows, vocab] bf16; parents i32 node
+        indices; f32 temperatures (<= 0 greedy) and u64 seeds a sequence; f32 uniforms a row. Per sequence:
+        out_tokens [max_nodes] i32 the accepted tokens and the one after them, out_nodes [max_nodes] i32 the
+        accepted path from node 0 on, both filled with -1, and out_counts i32 their number."""
+        self._tree_limit("verify_tree", max_nodes)
+        need = self.verify_tree_workspace(rows, batch_size, vocab)
+        args = [_r("logits", logits, 2, rows, vocab), _r("tokens", tokens, 4, rows), _r("parents", parents, 4, rows),
+                _r("row_starts", row_starts, 4, batch_size + 1), _r("temperatures", temperatures, 4, batch_size),
+                _r("uniforms", uniforms, 4, rows), _r("seeds", seeds, 8, batch_size),
+                _w("out_tokens", out_tokens, 4, batch_size, max_nodes),
+                _w("out_nodes", out_nodes, 4, batch_size, max_nodes), _w("out_counts", out_counts, 4, batch_size),
+                self._workspace("verify_tree", workspace, need)]
+        if draft_logits is not None:
+            args.append(_r("draft_logits", draft_logits, 2, rows, vocab))
+        self._admit("verify_tree", args)
+        self._call(self.lib.nv_verify_tree(
+            self.handle, logits.ptr, None if draft_logits is None else draft_logits.ptr, tokens.ptr, parents.ptr,
+            row_starts.ptr, temperatures.ptr, uniforms.ptr, seeds.ptr, out_tokens.ptr, out_nodes.ptr, out_counts.ptr,
+            workspace.ptr, rows, batch_size, max_nodes, vocab))
+
+    def kv_compact(self, kcache: Buffer, vcache: Buffer, contexts: Buffer, nodes: Buffer, counts: Buffer,
+                   block_tables: Buffer, batch_size: int, max_nodes: int, layers: int, kvheads: int, head_dim: int,
+                   block_size: int, num_blocks: int, table_stride: int) -> None:
+        """K and V at position contexts[s] + nodes[s, j] move to contexts[s] + j, for j < counts[s], in every layer
+        of caches [layers, num_blocks, block_size, kvheads, head_dim]."""
+        self._tree_limit("kv_compact", max_nodes)
+        self._cache_width("kv_compact", kvheads, head_dim)
+        self._admit("kv_compact", [
+            _w("kcache", kcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _w("vcache", vcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _r("contexts", contexts, 4, batch_size), _r("nodes", nodes, 4, batch_size, max_nodes),
+            _r("counts", counts, 4, batch_size), _r("block_tables", block_tables, 4, batch_size, table_stride)])
+        self._call(self.lib.nv_kv_compact(self.handle, kcache.ptr, vcache.ptr, contexts.ptr, nodes.ptr, counts.ptr,
+                                          block_tables.ptr, batch_size, max_nodes, layers, kvheads, head_dim,
+                                          block_size, num_blocks, table_stride))
+
+    def kv_copy_blocks(self, kcache: Buffer, vcache: Buffer, sources: Buffer, targets: Buffer, tokens: Buffer,
+                       copies: int, layers: int, kvheads: int, head_dim: int, block_size: int,
+                       num_blocks: int) -> None:
+        """The first tokens[i] slots of block sources[i] are copied to block targets[i], in every layer of caches
+        [layers, num_blocks, block_size, kvheads, head_dim]. No block may be written twice, or read and written."""
+        self._cache_width("kv_copy_blocks", kvheads, head_dim)
+        self._admit("kv_copy_blocks", [
+            _w("kcache", kcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _w("vcache", vcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _r("sources", sources, 4, copies), _r("targets", targets, 4, copies), _r("tokens", tokens, 4, copies)])
+        self._call(self.lib.nv_kv_copy_blocks(self.handle, kcache.ptr, vcache.ptr, sources.ptr, targets.ptr,
+                                              tokens.ptr, copies, layers, kvheads, head_dim, block_size, num_blocks))
+
+    @staticmethod
+    def _cache_width(op: str, kvheads: int, head_dim: int) -> None:
+        if as_dim(kvheads) * as_dim(head_dim) > INT_MAX:
+            raise ArgumentError("dimension", f"{op}: kvheads * head_dim exceeds 2^31 - 1")
 
 
 def bf16_bits(values) -> np.ndarray:
