@@ -22,6 +22,8 @@
 #include "nvr_device.h"
 #include "nvr_internal.h"
 
+#include <algorithm>
+
 namespace {
 
 using nvr::kWave;
@@ -128,6 +130,475 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
     if (int(threadIdx.x) < a.dim) a.out[row * a.dim + threadIdx.x] = nvr::f32_to_bf16(den > 0.0f ? num / den : 0.0f);
 }
 
+// ------------------------------------------------------------- tile form ----
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bf16x8_t operand(const uint4& w) { return __builtin_bit_cast(bf16x8_t, w); }
+
+// Barrier over LDS and everything this wave has copied into it.
+__device__ __forceinline__ void copied_barrier() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Compile-time geometry. DIM: head dim rounded up; QT: tiles of 16 query rows a
+// wave; WQ of the block's four waves hold query rows of their own, the other
+// factor WK splits each tile's positions.
+template <int DIM_, int QT_, int WQ_>
+struct Shape {
+    static constexpr int DIM = DIM_, QT = QT_, WQ = WQ_, WK = 4 / WQ_;
+    static constexpr int T = WK == 4 ? 128 : 64;     // positions a tile
+    static constexpr int KW = T / WK;                // a wave's positions of a tile
+    static constexpr int KT = KW / 16;               // 16-position tiles of those
+    static constexpr int DT = DIM / 16;              // 16-element tiles of a head
+    static constexpr int KS = DIM / 32;              // products of 32 elements a score
+    static constexpr int CH = DIM / 8;               // 16-byte chunks a row
+    static constexpr int R = kWave / CH;             // rows a copy instruction
+    static constexpr int COPIES = T / 4 / R;         // copy instructions a wave, tile and operand
+    static constexpr int ROWS = 16 * QT * WQ;        // query rows a block
+    static constexpr int kTile = T * DIM * 2;        // bytes of K or V
+    static constexpr int kStage = 2 * kTile;
+    static constexpr int kMerge = WK > 1 ? 4 * QT * 16 * (DIM + 2) * 4 : 0;
+    static constexpr int kLds = 2 * kStage > kMerge ? 2 * kStage : kMerge;
+    static constexpr int kBlocks = kLds > 72 * 1024 ? 1 : 2;  // a CU
+    static_assert(KW == 32 || KW == 64, "whole products over positions");
+};
+
+// Where chunk c of a row lies in its LDS row: sixteen rows' same chunk (a K
+// operand) and eight rows' same pair of chunks (a transposed V read) are on all banks.
+template <int CH>
+__device__ __forceinline__ int k_chunk(int row, int c) {
+    return c ^ (CH == 8 ? row >> 1 & 7 : row & 15);
+}
+template <int CH>
+__device__ __forceinline__ int v_chunk(int row, int c) {
+    return c ^ (CH == 8 ? (row >> 1 & 3) << 1 : (row & 7) << 1);
+}
+
+// Two bf16, an Inf or NaN as 0.
+__device__ __forceinline__ uint32_t numbers(uint32_t w) {
+    return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+}
+
+// Partial results of a split: unnormalised outputs, then (maximum, sum) pairs.
+struct Partials {
+    float* out;   // [splits, rows * qh, dim]
+    float2* sum;  // [splits, rows * qh]
+    int splits;
+};
+
+template <typename S>
+__global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs a, Partials part, int chunks) {
+    constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
+    constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES;
+    extern __shared__ __align__(16) unsigned char smem[];  // two stages of K, then V
+    __shared__ int phys[4][T];                             // token rows of four tiles, -1: not there
+    __shared__ uint64_t there[4][T / 64];
+    __shared__ int poison[2];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int n16 = lane & 15, g = lane >> 4;
+    const int wq = wave % WQ, wk = wave / WQ;
+    unsigned idx = blockIdx.x;
+    const int kvhead = int(idx % unsigned(a.kvh));
+    idx /= unsigned(a.kvh);
+    const int chunk = int(idx % unsigned(chunks));
+    idx /= unsigned(chunks);
+    const int split = int(idx % unsigned(part.splits)), s = int(idx / unsigned(part.splits));
+    const TreeSpan span = tree_span(a, s);
+    const int group = a.qh / a.kvh, queries = span.nodes * group, q0 = chunk * S::ROWS;
+    if (span.context < 0) {
+        // Of an invalid sequence each block clears its own rows; the last chunk's those past max_nodes too.
+        if (split == 0) {
+            const int end = chunk + 1 == chunks ? queries : min(queries, q0 + S::ROWS);
+            for (int i = q0 + int(threadIdx.x) / 16; i < end; i += 16) {
+                uint16_t* o = a.out + (int64_t(span.start + i / group) * a.qh + kvhead * group + i % group) * a.dim;
+                for (int d = 8 * n16; d < a.dim; d += 128) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        return;
+    }
+    if (q0 >= queries) return;
+    const int keys = span.context + span.nodes, tiles = (keys + T - 1) / T;
+    const int per = (tiles + part.splits - 1) / part.splits, used = (tiles + per - 1) / per;
+    if (split >= used) return;
+    const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
+
+    // ---- positions' places in the cache ----
+    int entry = -1;
+    auto look_up = [&](int tile) {  // the table's entry of this thread's position, in flight until placed
+        const int pos = tile * T + int(threadIdx.x);
+        entry = int(threadIdx.x) < T && tile < tile1 && pos < keys ? a.tables[int64_t(s) * a.stride + pos / a.bs] : -1;
+    };
+    auto place = [&](int tile) {
+        if (int(threadIdx.x) >= T) return;
+        const int pos = tile * T + int(threadIdx.x);
+        const int at = entry >= 0 && entry < a.blocks ? entry * a.bs + pos % a.bs : -1;
+        phys[tile & 3][threadIdx.x] = at;
+        const uint64_t here = __ballot(at >= 0);
+        if (lane == 0) there[tile & 3][threadIdx.x / 64] = here;
+    };
+    const int64_t pitch = int64_t(a.kvh) * a.dim;
+    const uint16_t* kcol = a.kc + int64_t(kvhead) * a.dim;
+    const uint16_t* vcol = a.vc + int64_t(kvhead) * a.dim;
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem));
+    const int crow = wave * (T / 4) + lane / CH, cslot = lane % CH;  // this lane's row and slot of copy 0
+    auto copy = [&](int tile, int stage) {
+#pragma unroll
+        for (int u = 0; u < COPIES; ++u) {
+            const int row = crow + u * R;
+            const int64_t at = int64_t(max(phys[tile & 3][row], 0)) * pitch;
+            const int ck = k_chunk<CH>(row, cslot), cv = v_chunk<CH>(row, cslot);
+            const uint32_t dst = lds + uint32_t(stage * S::kStage + (wave * (T / 4) + u * R) * DIM * 2);
+            uint32_t saved;
+            if (8 * ck < a.dim)
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                             "s_mov_b32 m0, %0"
+                             : "=&s"(saved)
+                             : "v"(kcol + at + 8 * ck), "s"(dst)
+                             : "memory");
+            if (8 * cv < a.dim)
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
+                             "s_mov_b32 m0, %0"
+                             : "=&s"(saved)
+                             : "v"(vcol + at + 8 * cv), "s"(dst + S::kTile)
+                             : "memory");
+        }
+    };
+    look_up(tile0);
+    if (a.dim < DIM) {  // chunks past the head are never copied
+        for (int i = int(threadIdx.x); i < 2 * S::kStage / 16; i += 256)
+            *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
+    }
+    if (threadIdx.x < 2) poison[threadIdx.x] = -1;
+    place(tile0);
+    look_up(tile0 + 1);
+    place(tile0 + 1);
+    __syncthreads();
+    copy(tile0, 0);
+    look_up(tile0 + 2);
+
+    // ---- this wave's query rows: the B operand of the scores ----
+    const bool working = q0 + wq * QT * 16 < queries;
+    bf16x8_t q[QT][KS];
+    uint64_t mask[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int i = q0 + (wq * QT + t) * 16 + n16;
+        const bool real = i < queries;
+        const int node = real ? i / group : 0;
+        const uint16_t* row = a.q + (int64_t(span.start + node) * a.qh + kvhead * group + (real ? i % group : 0)) * a.dim;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int d = 32 * k + 8 * g;
+            q[t][k] = operand(real && d < a.dim ? *reinterpret_cast<const uint4*>(row + d) : make_uint4(0, 0, 0, 0));
+        }
+        mask[t] = real ? a.masks[span.start + node] : 0;
+    }
+    f32x4_t o[QT][DT];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        m[t] = -kInf;
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
+    }
+
+    for (int tile = tile0; tile < tile1; ++tile) {
+        const int stage = (tile - tile0) & 1, first = tile * T;
+        const unsigned char* kt = smem + stage * S::kStage;
+        unsigned char* vt = smem + stage * S::kStage + S::kTile;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of the tile
+        uint64_t all = there[tile & 3][0];
+        if constexpr (T == 128) all &= there[tile & 3][1];
+        const bool partial = all != ~uint64_t(0), drafted = first + T > span.context;
+        if (partial || drafted) {
+            bool found = false;
+#pragma unroll
+            for (int u = 0; u < COPIES; ++u) {
+                const int row = crow + u * R;
+                uint4* v = reinterpret_cast<uint4*>(vt + (row * CH + cslot) * 16);
+                if (phys[tile & 3][row] < 0) {
+                    *v = make_uint4(0, 0, 0, 0);  // weighs nothing, and must be a number for that
+                } else if (first + row >= span.context) {
+                    // What some rows do not see must be a number for their weight of 0.
+                    uint4 w = *v;
+                    const uint4 whole = make_uint4(numbers(w.x), numbers(w.y), numbers(w.z), numbers(w.w));
+                    if (whole.x != w.x || whole.y != w.y || whole.z != w.z || whole.w != w.w) {
+                        found = true;
+                        *v = whole;
+                    }
+                }
+            }
+            if (__ballot(found) != 0 && lane == 0) poison[tile & 1] = tile;
+        }
+        place(tile + 2);
+        copied_barrier();
+        if (tile + 1 < tile1) copy(tile + 1, stage ^ 1);
+        look_up(tile + 3);
+        if (!working) continue;
+
+        // ---- scores, transposed: positions x query rows ----
+        f32x4_t x[QT][KT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+            for (int j = 0; j < KT; ++j) x[t][j] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+            const int row = wk * S::KW + 16 * j + n16;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const bf16x8_t kv = operand(
+                    *reinterpret_cast<const uint4*>(kt + (row * CH + k_chunk<CH>(row, 4 * k + g)) * 16));
+#pragma unroll
+                for (int t = 0; t < QT; ++t) x[t][j] = mfma(kv, q[t][k], x[t][j]);
+            }
+        }
+        const int w0 = first + (wk * S::KW & ~63);  // the 64 positions that this wave's are among
+        const uint64_t mapped = there[tile & 3][wk * S::KW / 64];
+        bf16x8_t p[QT][KT / 2];
+        auto seen = [&](int t) -> uint64_t {  // of this wave's positions, by row t
+            const int past = span.context - w0;  // positions of the context among the 64
+            const uint64_t sees = past >= 64 ? ~uint64_t(0)
+                                  : past > 0 ? ((uint64_t(1) << past) - 1) | mask[t] << past
+                                  : past > -64 ? mask[t] >> -past : 0;
+            return (sees & mapped) >> (wk * S::KW & 63);
+        };
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const uint64_t sees = partial || drafted ? seen(t) : ~uint64_t(0);
+            float top = m[t];
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = x[t][j][r] * a.scale;
+                    if (partial || drafted) v = (sees >> (16 * j + 4 * g + r) & 1) != 0 ? v : -kInf;
+                    x[t][j][r] = v;
+                    top = fmaxf(top, v);
+                }
+            top = fmaxf(top, nvr::xor_lane(top, 16));
+            top = fmaxf(top, nvr::xor_lane(top, 32));
+            const float base = top == -kInf ? 0.0f : top;
+            if (__ballot(top > m[t]) != 0) {
+                const float old = __builtin_amdgcn_exp2f(m[t] - base);
+                l[t] *= old;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[t][d][r] *= old;
+                m[t] = top;
+            }
+#pragma unroll
+            for (int j = 0; j < KT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[t][j][r] = __builtin_amdgcn_exp2f(x[t][j][r] - base);
+                    l[t] += x[t][j][r];
+                }
+            // Positions 4 g .. 4 g + 3 of two tiles: with V read in the same order, a product's 32 positions.
+#pragma unroll
+            for (int j = 0; j < KT / 2; ++j) {
+                const f32x4_t w = x[t][2 * j], y = x[t][2 * j + 1];
+                p[t][j] = operand(make_uint4(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3]),
+                                             nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3])));
+            }
+        }
+
+        // ---- outputs, transposed: head elements x query rows ----
+        const int vrow = wk * S::KW + 4 * g + (n16 >> 2);
+        auto read = [&](int row, int d) {
+            const int c = 2 * d + (n16 >> 1 & 1);
+            auto* at = (__attribute__((address_space(3))) s16x4_t*)(vt + (row * CH + v_chunk<CH>(row, c)) * 16 + 8 * (n16 & 1));
+            return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
+        };
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < KT / 2; ++j) {
+                const s16x4_t lo = read(vrow + 32 * j, d), hi = read(vrow + 32 * j + 16, d);
+                const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t][j], o[t][d]);
+            }
+        if (drafted && poison[tile & 1] == tile) {
+            // Nodes with an Inf or NaN in V, which went into the products as 0: added for the rows that see them.
+#pragma unroll 1
+            for (int i = 0; i < S::KW; ++i) {
+                const int row = wk * S::KW + i, at = phys[tile & 3][row];
+                if (at < 0 || first + row < span.context) continue;
+                const uint16_t* from = vcol + int64_t(at) * pitch;
+                bool sees[QT];
+#pragma unroll
+                for (int t = 0; t < QT; ++t) sees[t] = (seen(t) >> i & 1) != 0;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int element = 16 * d + 4 * g + e;
+                        const float v = element < a.dim ? nvr::bf16_to_f32(from[element]) : 0.0f;
+                        const float add = __builtin_isfinite(v) ? 0.0f : v;
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) o[t][d][e] += sees[t] ? add : 0.0f;
+                    }
+            }
+        }
+    }
+
+    // ---- the waves' shares, then the output or the split's partial ----
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        l[t] += nvr::xor_lane(l[t], 16);
+        l[t] += nvr::xor_lane(l[t], 32);
+    }
+    if constexpr (WK > 1) {
+        // [wave][query row][DIM + 2]: the output, the maximum and the sum.
+        constexpr int P = DIM + 2;
+        float* merge = reinterpret_cast<float*>(smem);
+        __syncthreads();  // every wave is done with the tiles
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            float* mine = merge + ((wk * WQ + wq) * QT * 16 + t * 16 + n16) * P;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    *reinterpret_cast<float2*>(mine + 16 * d + 4 * g + e) = make_float2(o[t][d][e], o[t][d][e + 1]);
+            if (g == 0) *reinterpret_cast<float2*>(mine + DIM) = make_float2(m[t], l[t]);
+        }
+        __syncthreads();
+        // Sixteen threads a query row.
+        for (int i = int(threadIdx.x) / 16; i < S::ROWS; i += 16) {
+            const int qi = q0 + i;
+            if (qi >= queries) break;
+            float top = -kInf, den = 0.0f, num[DT];
+            float f[WK];
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, merge[(w * WQ * QT * 16 + i) * P + DIM]);
+            const float base = top == -kInf ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+                const float* from = merge + (w * WQ * QT * 16 + i) * P;
+                f[w] = __builtin_amdgcn_exp2f(from[DIM] - base);
+                den = __builtin_fmaf(from[DIM + 1], f[w], den);
+            }
+            const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                num[d] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                    num[d] = __builtin_fmaf(merge[(w * WQ * QT * 16 + i) * P + 16 * d + n16], f[w], num[d]);
+            }
+            if (used == 1) {
+                const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (16 * d + n16 < a.dim)
+                        a.out[out_row * a.dim + 16 * d + n16] = nvr::f32_to_bf16(den > 0.0f ? num[d] * inv : 0.0f);
+            } else {
+                const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+                    if (16 * d + n16 < a.dim) part.out[at * a.dim + 16 * d + n16] = num[d];
+                if (n16 == 0) part.sum[at] = make_float2(top, den);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int qi = q0 + (wq * QT + t) * 16 + n16;
+            if (qi >= queries) continue;
+            const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
+            const float inv = l[t] > 0.0f ? 1.0f / l[t] : 0.0f;
+            const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const int e = 16 * d + 4 * g;
+                if (e >= a.dim) continue;
+                if (used == 1) {
+                    float y[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y[r] = l[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
+                    *reinterpret_cast<uint2*>(a.out + out_row * a.dim + e) =
+                        make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+                } else {
+                    *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = o[t][d];
+                }
+            }
+            if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], l[t]);
+        }
+    }
+}
+
+// The splits of each row, where there was more than one: a block a node.
+__global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int tile) {
+    const int s = int(blockIdx.x) / a.max_nodes, node = int(blockIdx.x) % a.max_nodes;
+    const TreeSpan span = tree_span(a, s);
+    if (node >= span.nodes || span.context < 0) return;
+    const int tiles = (span.context + span.nodes + tile - 1) / tile;
+    const int per = (tiles + part.splits - 1) / part.splits, used = (tiles + per - 1) / per;
+    if (used == 1) return;
+    const int64_t row = int64_t(span.start + node) * a.qh, plane = int64_t(a.rows) * a.qh;
+    const int quads = a.dim / 4;
+    for (int i = int(threadIdx.x); i < a.qh * quads; i += 256) {
+        const int64_t at = row + i / quads;
+        float top = -kInf;
+        for (int w = 0; w < used; ++w) top = fmaxf(top, part.sum[w * plane + at].x);
+        const float base = top == -kInf ? 0.0f : top;
+        float den = 0.0f;
+        f32x4_t num = {0, 0, 0, 0};
+        for (int w = 0; w < used; ++w) {
+            const float2 ml = part.sum[w * plane + at];
+            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(part.out + (w * plane + at) * a.dim + 4 * (i % quads));
+            const float f = __builtin_amdgcn_exp2f(ml.x - base);
+            den = __builtin_fmaf(ml.y, f, den);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) num[r] = __builtin_fmaf(v[r], f, num[r]);
+        }
+        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = den > 0.0f ? num[r] * inv : 0.0f;
+        *reinterpret_cast<uint2*>(a.out + at * a.dim + 4 * (i % quads)) =
+            make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+    }
+}
+
+// The launch's shape: the same for the workspace's size and the launch.
+struct Plan {
+    int dim, rows;  // rounded head dim; query rows a block
+    int tile, chunks, splits;
+};
+Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_context) {
+    Plan p;
+    p.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
+    const int64_t queries = int64_t(max_nodes) * (qh / kvh);
+    if (p.dim == 256) p.rows = queries <= 32 ? 32 : 64;
+    else p.rows = queries <= 16 ? 16 : queries <= 32 ? 32 : queries <= 64 ? 64 : 128;
+    p.tile = p.dim != 256 && p.rows <= 32 ? 128 : 64;
+    p.chunks = int((queries + p.rows - 1) / p.rows);
+    const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + p.tile - 1) / p.tile;
+    const int64_t target = p.tile * p.dim >= 64 * 256 ? 256 : 512;
+    p.splits = int(std::max<int64_t>(1, std::min(most, target / pairs)));
+    return p;
+}
+
+int64_t workspace_bytes(const Plan& p, int rows, int qh, int dim) {
+    return p.splits == 1 ? 0 : int64_t(p.splits) * rows * qh * (4 * int64_t(dim) + int64_t(sizeof(float2)));
+}
+
+template <typename S>
+void launch_tiles(nv_context* c, const TreeArgs& a, const Partials& part, const Plan& p) {
+    const unsigned grid = unsigned(int64_t(a.batch) * a.kvh * p.chunks * p.splits);
+    hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(grid), dim3(256), S::kLds, c->stream, a, part, p.chunks);
+}
+
 }  // namespace
 
 extern "C" {
@@ -136,7 +607,8 @@ int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, i
                                 size_t* bytes) {
     if (rows <= 0 || qh <= 0 || kvh <= 0 || dim <= 0 || batch <= 0 || max_nodes <= 0 || max_context <= 0 || qh % kvh)
         return nvr::fail(-2, "attention_tree_workspace: dimensions must be positive, q heads a multiple of KV heads");
-    *bytes = 0;
+    if (max_nodes > kMaxNodes || dim > 256) return nvr::fail(-2, "attention_tree_workspace: max_nodes %d, head dim %d", max_nodes, dim);
+    *bytes = dim % 8 ? 0 : size_t(workspace_bytes(plan_tiles(qh, kvh, dim, batch, max_nodes, max_context), rows, qh, dim));
     return 0;
 }
 
@@ -152,13 +624,42 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
     if (max_nodes < 1 || max_nodes > kMaxNodes)
         return nvr::fail(-2, "attention_tree: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     if (max_context < 1) return nvr::fail(-2, "attention_tree: max_context %d is not positive", max_context);
-    const int64_t span = int64_t(stride) * bs;
+    const int64_t span = std::min(int64_t(stride) * bs, int64_t(0x7fff0000));  // tiles past the end stay below 2^31
     const TreeArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kc), static_cast<const uint16_t*>(vc),
                      static_cast<const int*>(contexts), static_cast<const int*>(row_starts),
                      static_cast<const uint64_t*>(masks), static_cast<const int*>(tables), static_cast<uint16_t*>(out),
                      rows, qh, kvh, dim, bs, blocks, stride, batch, max_nodes,
                      span < max_context ? span : int64_t(max_context), kLog2e / sqrtf(float(dim))};
     const int64_t grid = int64_t(batch) * max_nodes * qh;
+    const bool fits = dim % 8 == 0 && nvr::aligned(q, 16) && nvr::aligned(kc, 16) && nvr::aligned(vc, 16) &&
+                      nvr::aligned(out, 16) && int64_t(blocks) * bs <= 0x7fffffff;
+    const Plan p = plan_tiles(qh, kvh, dim, batch, max_nodes, max_context);
+    if (fits && int64_t(batch) * kvh * p.chunks * p.splits <= 0x7fffffff) {
+        if (p.splits > 1 && (workspace == nullptr || !nvr::aligned(workspace, 16)))
+            return nvr::fail(-2, "attention_tree: needs a workspace at a multiple of 16 bytes");
+        float* partial = static_cast<float*>(workspace);
+        const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
+        if (p.dim == 256) {
+            if (p.rows == 32) launch_tiles<Shape<256, 1, 2>>(c, a, part, p);
+            else launch_tiles<Shape<256, 1, 4>>(c, a, part, p);
+        } else if (p.dim == 128) {
+            if (p.rows == 16) launch_tiles<Shape<128, 1, 1>>(c, a, part, p);
+            else if (p.rows == 32) launch_tiles<Shape<128, 2, 1>>(c, a, part, p);
+            else if (p.rows == 64) launch_tiles<Shape<128, 2, 2>>(c, a, part, p);
+            else launch_tiles<Shape<128, 2, 4>>(c, a, part, p);
+        } else {
+            if (p.rows == 16) launch_tiles<Shape<64, 1, 1>>(c, a, part, p);
+            else if (p.rows == 32) launch_tiles<Shape<64, 2, 1>>(c, a, part, p);
+            else if (p.rows == 64) launch_tiles<Shape<64, 2, 2>>(c, a, part, p);
+            else launch_tiles<Shape<64, 2, 4>>(c, a, part, p);
+        }
+        if (p.splits > 1) {
+            NVR_HIP(hipGetLastError());
+            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(int64_t(batch) * max_nodes)), dim3(256), 0, c->stream, a,
+                               part, p.tile);
+        }
+        return nvr::launch_status();
+    }
     if (grid > 0x7fffffff) return nvr::fail(-2, "attention_tree: %d sequences of %d nodes exceed one launch", batch, max_nodes);
     hipLaunchKernelGGL(attention_tree_direct, dim3(unsigned(grid)), dim3(256), 0, c->stream, a);
     return nvr::launch_status();
