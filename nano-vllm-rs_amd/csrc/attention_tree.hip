@@ -138,34 +138,41 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4_t mfma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4_t mfma(s16x4_t a, s16x4_t b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, b, c, 0, 0, 0);
+}
 __device__ __forceinline__ bf16x8_t operand(const uint4& w) { return __builtin_bit_cast(bf16x8_t, w); }
 
-// Barrier over LDS and everything this wave has copied into it.
-__device__ __forceinline__ void copied_barrier() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+// At most N of this wave's vector memory operations outstanding.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+constexpr int kPage = 16;  // positions that lie together in the cache: block sizes are multiples
 
 // Compile-time geometry. DIM: head dim rounded up; QT: tiles of 16 query rows a
 // wave; WQ of the block's four waves hold query rows of their own, the other
-// factor WK splits each tile's positions.
-template <int DIM_, int QT_, int WQ_>
+// factor WK splits each tile's T positions; NS: tiles in LDS.
+template <int DIM_, int QT_, int WQ_, int T_, int NS_>
 struct Shape {
-    static constexpr int DIM = DIM_, QT = QT_, WQ = WQ_, WK = 4 / WQ_;
-    static constexpr int T = WK == 4 ? 128 : 64;     // positions a tile
+    static constexpr int DIM = DIM_, QT = QT_, WQ = WQ_, WK = 4 / WQ_, T = T_, NS = NS_;
     static constexpr int KW = T / WK;                // a wave's positions of a tile
     static constexpr int KT = KW / 16;               // 16-position tiles of those
     static constexpr int DT = DIM / 16;              // 16-element tiles of a head
     static constexpr int KS = DIM / 32;              // products of 32 elements a score
     static constexpr int CH = DIM / 8;               // 16-byte chunks a row
     static constexpr int R = kWave / CH;             // rows a copy instruction
-    static constexpr int COPIES = T / 4 / R;         // copy instructions a wave, tile and operand
+    static constexpr int OWN = T / 4;                // rows that a wave copies
+    static constexpr int COPIES = OWN / R;           // copy instructions a wave, tile and operand
     static constexpr int ROWS = 16 * QT * WQ;        // query rows a block
     static constexpr int kTile = T * DIM * 2;        // bytes of K or V
     static constexpr int kStage = 2 * kTile;
     static constexpr int kMerge = WK > 1 ? 4 * QT * 16 * (DIM + 2) * 4 : 0;
-    static constexpr int kLds = 2 * kStage > kMerge ? 2 * kStage : kMerge;
-    static constexpr int kBlocks = kLds > 72 * 1024 ? 1 : 2;  // a CU
-    static_assert(KW == 32 || KW == 64, "whole products over positions");
+    static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
+    static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : 2;  // a CU
+    static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
+    static_assert(T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
 
 // Where chunk c of a row lies in its LDS row: sixteen rows' same chunk (a K
@@ -192,12 +199,11 @@ struct Partials {
 };
 
 template <typename S>
-__global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs a, Partials part, int chunks) {
+__global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
+                                                                        int page_shift) {
     constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
-    constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES;
-    extern __shared__ __align__(16) unsigned char smem[];  // two stages of K, then V
-    __shared__ int phys[4][T];                             // token rows of four tiles, -1: not there
-    __shared__ uint64_t there[4][T / 64];
+    constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS;
+    extern __shared__ __align__(16) unsigned char smem[];  // NS stages of K, then V
     __shared__ int poison[2];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n16 = lane & 15, g = lane >> 4;
@@ -227,60 +233,6 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     if (split >= used) return;
     const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
 
-    // ---- positions' places in the cache ----
-    int entry = -1;
-    auto look_up = [&](int tile) {  // the table's entry of this thread's position, in flight until placed
-        const int pos = tile * T + int(threadIdx.x);
-        entry = int(threadIdx.x) < T && tile < tile1 && pos < keys ? a.tables[int64_t(s) * a.stride + pos / a.bs] : -1;
-    };
-    auto place = [&](int tile) {
-        if (int(threadIdx.x) >= T) return;
-        const int pos = tile * T + int(threadIdx.x);
-        const int at = entry >= 0 && entry < a.blocks ? entry * a.bs + pos % a.bs : -1;
-        phys[tile & 3][threadIdx.x] = at;
-        const uint64_t here = __ballot(at >= 0);
-        if (lane == 0) there[tile & 3][threadIdx.x / 64] = here;
-    };
-    const int64_t pitch = int64_t(a.kvh) * a.dim;
-    const uint16_t* kcol = a.kc + int64_t(kvhead) * a.dim;
-    const uint16_t* vcol = a.vc + int64_t(kvhead) * a.dim;
-    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem));
-    const int crow = wave * (T / 4) + lane / CH, cslot = lane % CH;  // this lane's row and slot of copy 0
-    auto copy = [&](int tile, int stage) {
-#pragma unroll
-        for (int u = 0; u < COPIES; ++u) {
-            const int row = crow + u * R;
-            const int64_t at = int64_t(max(phys[tile & 3][row], 0)) * pitch;
-            const int ck = k_chunk<CH>(row, cslot), cv = v_chunk<CH>(row, cslot);
-            const uint32_t dst = lds + uint32_t(stage * S::kStage + (wave * (T / 4) + u * R) * DIM * 2);
-            uint32_t saved;
-            if (8 * ck < a.dim)
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                             "s_mov_b32 m0, %0"
-                             : "=&s"(saved)
-                             : "v"(kcol + at + 8 * ck), "s"(dst)
-                             : "memory");
-            if (8 * cv < a.dim)
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t"
-                             "s_mov_b32 m0, %0"
-                             : "=&s"(saved)
-                             : "v"(vcol + at + 8 * cv), "s"(dst + S::kTile)
-                             : "memory");
-        }
-    };
-    look_up(tile0);
-    if (a.dim < DIM) {  // chunks past the head are never copied
-        for (int i = int(threadIdx.x); i < 2 * S::kStage / 16; i += 256)
-            *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
-    }
-    if (threadIdx.x < 2) poison[threadIdx.x] = -1;
-    place(tile0);
-    look_up(tile0 + 1);
-    place(tile0 + 1);
-    __syncthreads();
-    copy(tile0, 0);
-    look_up(tile0 + 2);
-
     // ---- this wave's query rows: the B operand of the scores ----
     const bool working = q0 + wq * QT * 16 < queries;
     bf16x8_t q[QT][KS];
@@ -298,6 +250,78 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
         }
         mask[t] = real ? a.masks[span.start + node] : 0;
     }
+
+    // ---- positions' places in the cache, by pages of 16 positions ----
+    using Table = const __attribute__((address_space(4))) int*;  // scalar loads: they do not count with the copies
+    const Table table = (Table)(a.tables + int64_t(s) * a.stride);
+    const int pages = a.bs / kPage, last_page = (keys - 1) / kPage;
+    auto entry_of = [&](int page) { return page_shift >= 0 ? page >> page_shift : page / pages; };
+    // The cache row of a page's first position, or -1.
+    auto place = [&](int page) {
+        const int at = entry_of(page), entry = table[at];
+        return entry >= 0 && entry < a.blocks ? entry * a.bs + (page - at * pages) * kPage : -1;
+    };
+    bool holes = false;
+    for (int i = entry_of(tile0 * T / kPage) + lane; i <= entry_of(min(tile1 * T / kPage - 1, last_page)); i += kWave) {
+        const int entry = a.tables[int64_t(s) * a.stride + i];
+        holes |= entry < 0 || entry >= a.blocks;
+    }
+    const bool any_holes = __ballot(holes) != 0;
+
+    const int64_t pitch = int64_t(a.kvh) * a.dim;
+    const uint16_t* kcol = a.kc + int64_t(kvhead) * a.dim;
+    const uint16_t* vcol = a.vc + int64_t(kvhead) * a.dim;
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem));
+    const int crow = wave * S::OWN + lane / CH, cslot = lane % CH;  // this lane's row and slot of copy 0
+    uint32_t koff[COPIES], voff[COPIES];  // bytes from the page's row
+#pragma unroll
+    for (int u = 0; u < COPIES; ++u) {
+        const int row = crow + u * R;
+        koff[u] = uint32_t((row % kPage) * int(pitch) + 8 * k_chunk<CH>(row, cslot)) * 2;
+        voff[u] = uint32_t((row % kPage) * int(pitch) + 8 * v_chunk<CH>(row, cslot)) * 2;
+    }
+    auto copy = [&](int tile) {
+        const int page = min((tile * T + wave * S::OWN) / kPage, last_page);
+        const int64_t at = int64_t(max(__builtin_amdgcn_readfirstlane(place(page)), 0)) * pitch;
+        const uint16_t* kbase = kcol + at;
+        const uint16_t* vbase = vcol + at;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + uint32_t((tile - tile0) % NS * S::kStage + wave * S::OWN * DIM * 2));
+#pragma unroll
+        for (int u = 0; u < COPIES; ++u) {
+            uint32_t saved;
+            if (k_chunk<CH>(crow + u * R, cslot) * 8 < a.dim)
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+                             "s_mov_b32 m0, %0"
+                             : "=&s"(saved)
+                             : "v"(koff[u]), "s"(kbase), "s"(dst + u * 1024)
+                             : "memory");
+        }
+#pragma unroll
+        for (int u = 0; u < COPIES; ++u) {
+            uint32_t saved;
+            if (v_chunk<CH>(crow + u * R, cslot) * 8 < a.dim)
+                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
+                             "s_mov_b32 m0, %0"
+                             : "=&s"(saved)
+                             : "v"(voff[u]), "s"(vbase), "s"(dst + S::kTile + u * 1024)
+                             : "memory");
+        }
+    };
+    if (a.dim < DIM) {  // chunks past the head are never copied
+        for (int i = int(threadIdx.x); i < NS * S::kStage / 16; i += 256)
+            *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
+    }
+    if (threadIdx.x < 2) poison[threadIdx.x] = -1;
+    __syncthreads();
+    // Every register load is awaited here, so that none is where the copies are counted.
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[t][k]));
+        asm volatile("" : "+v"(mask[t]));
+    }
+    for (int i = 0; i < NS - 1 && tile0 + i < tile1; ++i) copy(tile0 + i);
+
     f32x4_t o[QT][DT];
     float m[QT], l[QT];
 #pragma unroll
@@ -309,24 +333,30 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     }
 
     for (int tile = tile0; tile < tile1; ++tile) {
-        const int stage = (tile - tile0) & 1, first = tile * T;
+        const int stage = (tile - tile0) % NS, first = tile * T;
         const unsigned char* kt = smem + stage * S::kStage;
         unsigned char* vt = smem + stage * S::kStage + S::kTile;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's rows of the tile
-        uint64_t all = there[tile & 3][0];
-        if constexpr (T == 128) all &= there[tile & 3][1];
-        const bool partial = all != ~uint64_t(0), drafted = first + T > span.context;
+        if (tile + NS - 2 < tile1) wait_copies<(NS - 2) * 2 * COPIES>();  // this wave's rows of the tile
+        else wait_copies<0>();
+        const bool drafted = first + T > span.context, partial = any_holes || first + T > keys;
+        uint64_t mapped = T == 64 ? ~uint64_t(0) : (uint64_t(1) << (T & 63)) - 1;
+        if (partial) {
+            if (keys - first < T) mapped = (uint64_t(1) << (keys - first)) - 1;
+#pragma unroll
+            for (int i = 0; i < T / kPage; ++i)
+                if (first + i * kPage < keys && place(first / kPage + i) < 0) mapped &= ~(uint64_t(0xffff) << (i * kPage));
+        }
         if (partial || drafted) {
             bool found = false;
 #pragma unroll
             for (int u = 0; u < COPIES; ++u) {
                 const int row = crow + u * R;
                 uint4* v = reinterpret_cast<uint4*>(vt + (row * CH + cslot) * 16);
-                if (phys[tile & 3][row] < 0) {
+                if ((mapped >> row & 1) == 0) {
                     *v = make_uint4(0, 0, 0, 0);  // weighs nothing, and must be a number for that
                 } else if (first + row >= span.context) {
                     // What some rows do not see must be a number for their weight of 0.
-                    uint4 w = *v;
+                    const uint4 w = *v;
                     const uint4 whole = make_uint4(numbers(w.x), numbers(w.y), numbers(w.z), numbers(w.w));
                     if (whole.x != w.x || whole.y != w.y || whole.z != w.z || whole.w != w.w) {
                         found = true;
@@ -336,10 +366,8 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
             }
             if (__ballot(found) != 0 && lane == 0) poison[tile & 1] = tile;
         }
-        place(tile + 2);
-        copied_barrier();
-        if (tile + 1 < tile1) copy(tile + 1, stage ^ 1);
-        look_up(tile + 3);
+        if (!S::kAlone || drafted) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (tile + NS - 1 < tile1) copy(tile + NS - 1);
         if (!working) continue;
 
         // ---- scores, transposed: positions x query rows ----
@@ -359,20 +387,17 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                 for (int t = 0; t < QT; ++t) x[t][j] = mfma(kv, q[t][k], x[t][j]);
             }
         }
-        const int w0 = first + (wk * S::KW & ~63);  // the 64 positions that this wave's are among
-        const uint64_t mapped = there[tile & 3][wk * S::KW / 64];
-        bf16x8_t p[QT][KT / 2];
         auto seen = [&](int t) -> uint64_t {  // of this wave's positions, by row t
-            const int past = span.context - w0;  // positions of the context among the 64
+            const int past = span.context - first;  // positions of the context in the tile
             const uint64_t sees = past >= 64 ? ~uint64_t(0)
                                   : past > 0 ? ((uint64_t(1) << past) - 1) | mask[t] << past
                                   : past > -64 ? mask[t] >> -past : 0;
-            return (sees & mapped) >> (wk * S::KW & 63);
+            return (sees & mapped) >> (wk * S::KW);
         };
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             const uint64_t sees = partial || drafted ? seen(t) : ~uint64_t(0);
-            float top = m[t];
+            float top = -kInf;
 #pragma unroll
             for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -382,11 +407,12 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                     x[t][j][r] = v;
                     top = fmaxf(top, v);
                 }
-            top = fmaxf(top, nvr::xor_lane(top, 16));
-            top = fmaxf(top, nvr::xor_lane(top, 32));
-            const float base = top == -kInf ? 0.0f : top;
-            if (__ballot(top > m[t]) != 0) {
-                const float old = __builtin_amdgcn_exp2f(m[t] - base);
+            // The weights' common scale follows the maximum only where that outgrows it by 2^8: any scale near it will do.
+            if (__ballot(top > m[t] + 8.0f) != 0) {
+                top = fmaxf(top, m[t]);
+                top = fmaxf(top, nvr::xor_lane(top, 16));
+                top = fmaxf(top, nvr::xor_lane(top, 32));
+                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
                 l[t] *= old;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -394,6 +420,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                     for (int r = 0; r < 4; ++r) o[t][d][r] *= old;
                 m[t] = top;
             }
+            const float base = m[t] == -kInf ? 0.0f : m[t];
 #pragma unroll
             for (int j = 0; j < KT; ++j)
 #pragma unroll
@@ -401,13 +428,6 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                     x[t][j][r] = __builtin_amdgcn_exp2f(x[t][j][r] - base);
                     l[t] += x[t][j][r];
                 }
-            // Positions 4 g .. 4 g + 3 of two tiles: with V read in the same order, a product's 32 positions.
-#pragma unroll
-            for (int j = 0; j < KT / 2; ++j) {
-                const f32x4_t w = x[t][2 * j], y = x[t][2 * j + 1];
-                p[t][j] = operand(make_uint4(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3]),
-                                             nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3])));
-            }
         }
 
         // ---- outputs, transposed: head elements x query rows ----
@@ -417,22 +437,44 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
             auto* at = (__attribute__((address_space(3))) s16x4_t*)(vt + (row * CH + v_chunk<CH>(row, c)) * 16 + 8 * (n16 & 1));
             return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
         };
+        auto pair = [&](const f32x4_t& w) { return make_uint2(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3])); };
+        if constexpr (KT == 1) {
+            s16x4_t p[QT];
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int t = 0; t < QT; ++t) p[t] = __builtin_bit_cast(s16x4_t, pair(x[t][0]));
 #pragma unroll
-            for (int j = 0; j < KT / 2; ++j) {
-                const s16x4_t lo = read(vrow + 32 * j, d), hi = read(vrow + 32 * j + 16, d);
-                const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            for (int d = 0; d < DT; ++d) {
+                const s16x4_t v = read(vrow, d);
 #pragma unroll
-                for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t][j], o[t][d]);
+                for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t], o[t][d]);
             }
+        } else {
+            // Positions 4 g .. 4 g + 3 of two tiles: with V read in the same order, a product's 32 positions.
+            bf16x8_t p[QT][KT / 2];
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+                for (int j = 0; j < KT / 2; ++j) {
+                    const uint2 lo = pair(x[t][2 * j]), hi = pair(x[t][2 * j + 1]);
+                    p[t][j] = operand(make_uint4(lo.x, lo.y, hi.x, hi.y));
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int j = 0; j < KT / 2; ++j) {
+                    const s16x4_t lo = read(vrow + 32 * j, d), hi = read(vrow + 32 * j + 16, d);
+                    const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t][j], o[t][d]);
+                }
+        }
         if (drafted && poison[tile & 1] == tile) {
             // Nodes with an Inf or NaN in V, which went into the products as 0: added for the rows that see them.
 #pragma unroll 1
             for (int i = 0; i < S::KW; ++i) {
-                const int row = wk * S::KW + i, at = phys[tile & 3][row];
-                if (at < 0 || first + row < span.context) continue;
-                const uint16_t* from = vcol + int64_t(at) * pitch;
+                const int row = wk * S::KW + i;
+                if ((mapped >> row & 1) == 0 || first + row < span.context) continue;
+                const uint16_t* from = vcol + int64_t(place((first + row) / kPage) + row % kPage) * pitch;
                 bool sees[QT];
 #pragma unroll
                 for (int t = 0; t < QT; ++t) sees[t] = (seen(t) >> i & 1) != 0;
@@ -575,28 +617,29 @@ struct Plan {
     int dim, rows;  // rounded head dim; query rows a block
     int tile, chunks, splits;
 };
+template <typename F>
+void with_shape(int dim, int rows, F&& f) {
+    if (dim == 256) rows <= 32 ? f(Shape<256, 1, 2, 32, 4>{}) : f(Shape<256, 1, 4, 32, 4>{});
+    else if (dim == 128) rows <= 16 ? f(Shape<128, 1, 1, 64, 4>{}) : rows <= 32 ? f(Shape<128, 2, 1, 64, 4>{}) : rows <= 64 ? f(Shape<128, 2, 2, 32, 4>{}) : f(Shape<128, 2, 4, 32, 4>{});
+    else rows <= 16 ? f(Shape<64, 1, 1, 64, 4>{}) : rows <= 32 ? f(Shape<64, 2, 1, 64, 4>{}) : rows <= 64 ? f(Shape<64, 2, 2, 64, 4>{}) : f(Shape<64, 2, 4, 64, 4>{});
+}
 Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_context) {
     Plan p;
     p.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const int64_t queries = int64_t(max_nodes) * (qh / kvh);
-    if (p.dim == 256) p.rows = queries <= 32 ? 32 : 64;
-    else p.rows = queries <= 16 ? 16 : queries <= 32 ? 32 : queries <= 64 ? 64 : 128;
-    p.tile = p.dim != 256 && p.rows <= 32 ? 128 : 64;
-    p.chunks = int((queries + p.rows - 1) / p.rows);
-    const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + p.tile - 1) / p.tile;
-    const int64_t target = p.tile * p.dim >= 64 * 256 ? 256 : 512;
-    p.splits = int(std::max<int64_t>(1, std::min(most, target / pairs)));
+    with_shape(p.dim, int(std::min<int64_t>(queries, 128)), [&](auto shape) {
+        using S = decltype(shape);
+        p.rows = S::ROWS;
+        p.tile = S::T;
+        p.chunks = int((queries + p.rows - 1) / p.rows);
+        const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + p.tile - 1) / p.tile;
+        p.splits = int(std::max<int64_t>(1, std::min(most, 256 * S::kBlocks / pairs)));
+    });
     return p;
 }
 
 int64_t workspace_bytes(const Plan& p, int rows, int qh, int dim) {
     return p.splits == 1 ? 0 : int64_t(p.splits) * rows * qh * (4 * int64_t(dim) + int64_t(sizeof(float2)));
-}
-
-template <typename S>
-void launch_tiles(nv_context* c, const TreeArgs& a, const Partials& part, const Plan& p) {
-    const unsigned grid = unsigned(int64_t(a.batch) * a.kvh * p.chunks * p.splits);
-    hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(grid), dim3(256), S::kLds, c->stream, a, part, p.chunks);
 }
 
 }  // namespace
@@ -631,7 +674,7 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
                      rows, qh, kvh, dim, bs, blocks, stride, batch, max_nodes,
                      span < max_context ? span : int64_t(max_context), kLog2e / sqrtf(float(dim))};
     const int64_t grid = int64_t(batch) * max_nodes * qh;
-    const bool fits = dim % 8 == 0 && nvr::aligned(q, 16) && nvr::aligned(kc, 16) && nvr::aligned(vc, 16) &&
+    const bool fits = dim % 8 == 0 && bs % kPage == 0 && int64_t(kvh) * dim <= 0x1000000 && nvr::aligned(q, 16) && nvr::aligned(kc, 16) && nvr::aligned(vc, 16) &&
                       nvr::aligned(out, 16) && int64_t(blocks) * bs <= 0x7fffffff;
     const Plan p = plan_tiles(qh, kvh, dim, batch, max_nodes, max_context);
     if (fits && int64_t(batch) * kvh * p.chunks * p.splits <= 0x7fffffff) {
@@ -639,20 +682,13 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
             return nvr::fail(-2, "attention_tree: needs a workspace at a multiple of 16 bytes");
         float* partial = static_cast<float*>(workspace);
         const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
-        if (p.dim == 256) {
-            if (p.rows == 32) launch_tiles<Shape<256, 1, 2>>(c, a, part, p);
-            else launch_tiles<Shape<256, 1, 4>>(c, a, part, p);
-        } else if (p.dim == 128) {
-            if (p.rows == 16) launch_tiles<Shape<128, 1, 1>>(c, a, part, p);
-            else if (p.rows == 32) launch_tiles<Shape<128, 2, 1>>(c, a, part, p);
-            else if (p.rows == 64) launch_tiles<Shape<128, 2, 2>>(c, a, part, p);
-            else launch_tiles<Shape<128, 2, 4>>(c, a, part, p);
-        } else {
-            if (p.rows == 16) launch_tiles<Shape<64, 1, 1>>(c, a, part, p);
-            else if (p.rows == 32) launch_tiles<Shape<64, 2, 1>>(c, a, part, p);
-            else if (p.rows == 64) launch_tiles<Shape<64, 2, 2>>(c, a, part, p);
-            else launch_tiles<Shape<64, 2, 4>>(c, a, part, p);
-        }
+        const int pages = bs / kPage, shift = (pages & (pages - 1)) == 0 ? __builtin_ctz(unsigned(pages)) : -1;
+        const unsigned blocks_all = unsigned(int64_t(batch) * kvh * p.chunks * p.splits);
+        with_shape(p.dim, p.rows, [&](auto shape) {
+            using S = decltype(shape);
+            hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(256), S::kLds, c->stream, a, part,
+                               p.chunks, shift);
+        });
         if (p.splits > 1) {
             NVR_HIP(hipGetLastError());
             hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(int64_t(batch) * max_nodes)), dim3(256), 0, c->stream, a,
