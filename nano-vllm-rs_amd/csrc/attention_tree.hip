@@ -23,6 +23,7 @@
 #include "nvr_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -172,7 +173,7 @@ struct Shape {
     static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
     static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : 2;  // a CU
     static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
-    static_assert(T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
+    static_assert((COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
 
 // Where chunk c of a row lies in its LDS row: sixteen rows' same chunk (a K
@@ -198,9 +199,14 @@ struct Partials {
     int splits;
 };
 
+// Tiles a split, at least `least`.
+__device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
+    return max((tiles + splits - 1) / splits, least);
+}
+
 template <typename S>
 __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
-                                                                        int page_shift) {
+                                                                        int least, int page_shift) {
     constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
     constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS;
     extern __shared__ __align__(16) unsigned char smem[];  // NS stages of K, then V
@@ -229,7 +235,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     }
     if (q0 >= queries) return;
     const int keys = span.context + span.nodes, tiles = (keys + T - 1) / T;
-    const int per = (tiles + part.splits - 1) / part.splits, used = (tiles + per - 1) / per;
+    const int per = split_tiles(tiles, part.splits, least), used = (tiles + per - 1) / per;
     if (split >= used) return;
     const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
 
@@ -273,40 +279,60 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     const uint16_t* vcol = a.vc + int64_t(kvhead) * a.dim;
     const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem));
     const int crow = wave * S::OWN + lane / CH, cslot = lane % CH;  // this lane's row and slot of copy 0
-    uint32_t koff[COPIES], voff[COPIES];  // bytes from the page's row
+    // Bytes from the page's row. A copy's offset field moves both sides by its 1 KB of LDS (whole heads only:
+    // there a row is at least as long in the cache).
+    const bool whole = a.dim == DIM;
+    uint32_t koff[COPIES], voff[COPIES];
 #pragma unroll
     for (int u = 0; u < COPIES; ++u) {
         const int row = crow + u * R;
-        koff[u] = uint32_t((row % kPage) * int(pitch) + 8 * k_chunk<CH>(row, cslot)) * 2;
-        voff[u] = uint32_t((row % kPage) * int(pitch) + 8 * v_chunk<CH>(row, cslot)) * 2;
+        koff[u] = uint32_t((row % kPage) * int(pitch) + 8 * k_chunk<CH>(row, cslot)) * 2 - (whole ? u * 1024 : 0);
+        voff[u] = uint32_t((row % kPage) * int(pitch) + 8 * v_chunk<CH>(row, cslot)) * 2 - (whole ? u * 1024 : 0);
     }
-    auto copy = [&](int tile) {
-        const int page = min((tile * T + wave * S::OWN) / kPage, last_page);
-        const int64_t at = int64_t(max(__builtin_amdgcn_readfirstlane(place(page)), 0)) * pitch;
+    // M0 holds the LDS address and is restored after the copies.
+#define NVR_COPY(n) "global_load_lds_dwordx4 %" #n ", %1 offset:"
+#define NVR_WITH_M0(loads) "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\t" loads "s_mov_b32 m0, %0"
+    auto copy_one = [&](uint32_t offset, const uint16_t* base, uint32_t dst) {
+        uint32_t saved;
+        asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t") : "=&s"(saved) : "s"(base), "s"(dst), "v"(offset) : "memory");
+    };
+    auto copy_all = [&](const uint32_t (&offset)[COPIES], const uint16_t* base, uint32_t dst) {
+        uint32_t saved;
+        if constexpr (COPIES == 4)
+            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "1024\n\t" NVR_COPY(5) "2048\n\t" NVR_COPY(6) "3072\n\t")
+                         : "=&s"(saved)
+                         : "s"(base), "s"(dst), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
+                         : "memory");
+        else
+            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "1024\n\t")
+                         : "=&s"(saved)
+                         : "s"(base), "s"(dst), "v"(offset[0]), "v"(offset[1])
+                         : "memory");
+    };
+#undef NVR_COPY
+#undef NVR_WITH_M0
+    auto copy = [&](int tile, int row0) {  // row0: the cache row of this wave's page
+        const int64_t at = int64_t(max(row0, 0)) * pitch;
         const uint16_t* kbase = kcol + at;
         const uint16_t* vbase = vcol + at;
         const uint32_t dst = __builtin_amdgcn_readfirstlane(lds + uint32_t((tile - tile0) % NS * S::kStage + wave * S::OWN * DIM * 2));
+        if (whole) {
+            copy_all(koff, kbase, dst);
+            copy_all(voff, vbase, dst + S::kTile);
+        } else {
 #pragma unroll
-        for (int u = 0; u < COPIES; ++u) {
-            uint32_t saved;
-            if (k_chunk<CH>(crow + u * R, cslot) * 8 < a.dim)
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-                             "s_mov_b32 m0, %0"
-                             : "=&s"(saved)
-                             : "v"(koff[u]), "s"(kbase), "s"(dst + u * 1024)
-                             : "memory");
-        }
-#pragma unroll
-        for (int u = 0; u < COPIES; ++u) {
-            uint32_t saved;
-            if (v_chunk<CH>(crow + u * R, cslot) * 8 < a.dim)
-                asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\t"
-                             "s_mov_b32 m0, %0"
-                             : "=&s"(saved)
-                             : "v"(voff[u]), "s"(vbase), "s"(dst + S::kTile + u * 1024)
-                             : "memory");
+            for (int u = 0; u < COPIES; ++u) {
+                if (k_chunk<CH>(crow + u * R, cslot) * 8 < a.dim) copy_one(koff[u], kbase, dst + u * 1024);
+                if (v_chunk<CH>(crow + u * R, cslot) * 8 < a.dim) copy_one(voff[u], vbase, dst + S::kTile + u * 1024);
+            }
         }
     };
+    auto own_page = [&](int tile) {
+        return __builtin_amdgcn_readfirstlane(place(min((tile * T + wave * S::OWN) / kPage, last_page)));
+    };
+    int rows0[NS - 1];
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) rows0[i] = own_page(min(tile0 + i, tile1 - 1));
     if (a.dim < DIM) {  // chunks past the head are never copied
         for (int i = int(threadIdx.x); i < NS * S::kStage / 16; i += 256)
             *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
@@ -320,7 +346,10 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
         for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[t][k]));
         asm volatile("" : "+v"(mask[t]));
     }
-    for (int i = 0; i < NS - 1 && tile0 + i < tile1; ++i) copy(tile0 + i);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i)
+        if (tile0 + i < tile1) copy(tile0 + i, rows0[i]);
+    int next_row = own_page(min(tile0 + NS - 1, tile1 - 1));
 
     f32x4_t o[QT][DT];
     float m[QT], l[QT];
@@ -332,21 +361,23 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
     }
 
-    for (int tile = tile0; tile < tile1; ++tile) {
+    // One tile; `masked`: some of its positions are not seen by every row.
+    auto step = [&](int tile, auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
         const int stage = (tile - tile0) % NS, first = tile * T;
         const unsigned char* kt = smem + stage * S::kStage;
         unsigned char* vt = smem + stage * S::kStage + S::kTile;
         if (tile + NS - 2 < tile1) wait_copies<(NS - 2) * 2 * COPIES>();  // this wave's rows of the tile
         else wait_copies<0>();
-        const bool drafted = first + T > span.context, partial = any_holes || first + T > keys;
+        const bool drafted = kMasked && first + T > span.context;
         uint64_t mapped = T == 64 ? ~uint64_t(0) : (uint64_t(1) << (T & 63)) - 1;
-        if (partial) {
+        if constexpr (kMasked) {
             if (keys - first < T) mapped = (uint64_t(1) << (keys - first)) - 1;
 #pragma unroll
             for (int i = 0; i < T / kPage; ++i)
                 if (first + i * kPage < keys && place(first / kPage + i) < 0) mapped &= ~(uint64_t(0xffff) << (i * kPage));
         }
-        if (partial || drafted) {
+        if constexpr (kMasked) {
             bool found = false;
 #pragma unroll
             for (int u = 0; u < COPIES; ++u) {
@@ -367,8 +398,11 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
             if (__ballot(found) != 0 && lane == 0) poison[tile & 1] = tile;
         }
         if (!S::kAlone || drafted) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (tile + NS - 1 < tile1) copy(tile + NS - 1);
-        if (!working) continue;
+        if (tile + NS - 1 < tile1) {
+            copy(tile + NS - 1, next_row);
+            next_row = own_page(min(tile + NS, tile1 - 1));
+        }
+        if (!working) return;
 
         // ---- scores, transposed: positions x query rows ----
         f32x4_t x[QT][KT];
@@ -396,17 +430,20 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
         };
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const uint64_t sees = partial || drafted ? seen(t) : ~uint64_t(0);
+            if constexpr (kMasked) {
+                const uint64_t sees = seen(t);
+#pragma unroll
+                for (int j = 0; j < KT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        x[t][j][r] = (sees >> (16 * j + 4 * g + r) & 1) != 0 ? x[t][j][r] : -kInf;
+            }
             float top = -kInf;
 #pragma unroll
             for (int j = 0; j < KT; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = x[t][j][r] * a.scale;
-                    if (partial || drafted) v = (sees >> (16 * j + 4 * g + r) & 1) != 0 ? v : -kInf;
-                    x[t][j][r] = v;
-                    top = fmaxf(top, v);
-                }
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, x[t][j][r]);
+            top *= a.scale;
             // The weights' common scale follows the maximum only where that outgrows it by 2^8: any scale near it will do.
             if (__ballot(top > m[t] + 8.0f) != 0) {
                 top = fmaxf(top, m[t]);
@@ -425,7 +462,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
             for (int j = 0; j < KT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[t][j][r] = __builtin_amdgcn_exp2f(x[t][j][r] - base);
+                    x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r], a.scale, -base));
                     l[t] += x[t][j][r];
                 }
         }
@@ -490,7 +527,11 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                     }
             }
         }
-    }
+    };
+    const int plain = any_holes ? tile0 : max(tile0, min(tile1, span.context / T));  // tiles that every row sees whole
+    for (int tile = tile0; tile < plain; ++tile) step(tile, std::false_type{});
+#pragma unroll 1
+    for (int tile = plain; tile < tile1; ++tile) step(tile, std::true_type{});
 
     // ---- the waves' shares, then the output or the split's partial ----
 #pragma unroll
@@ -578,44 +619,62 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     }
 }
 
-// The splits of each row, where there was more than one: a block a node.
-__global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int tile) {
-    const int s = int(blockIdx.x) / a.max_nodes, node = int(blockIdx.x) % a.max_nodes;
+// The splits of each row, where there was more than one: a thread four elements
+// of one (node, head), its splits' loads in flight together.
+__global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int tile, int least, int parts) {
+    constexpr int kBatch = 8;
+    const int item = int(blockIdx.x / unsigned(parts));
+    const int s = item / a.max_nodes, node = item % a.max_nodes;
     const TreeSpan span = tree_span(a, s);
     if (node >= span.nodes || span.context < 0) return;
     const int tiles = (span.context + span.nodes + tile - 1) / tile;
-    const int per = (tiles + part.splits - 1) / part.splits, used = (tiles + per - 1) / per;
-    if (used == 1) return;
-    const int64_t row = int64_t(span.start + node) * a.qh, plane = int64_t(a.rows) * a.qh;
-    const int quads = a.dim / 4;
-    for (int i = int(threadIdx.x); i < a.qh * quads; i += 256) {
-        const int64_t at = row + i / quads;
-        float top = -kInf;
-        for (int w = 0; w < used; ++w) top = fmaxf(top, part.sum[w * plane + at].x);
-        const float base = top == -kInf ? 0.0f : top;
-        float den = 0.0f;
-        f32x4_t num = {0, 0, 0, 0};
-        for (int w = 0; w < used; ++w) {
-            const float2 ml = part.sum[w * plane + at];
-            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(part.out + (w * plane + at) * a.dim + 4 * (i % quads));
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            den = __builtin_fmaf(ml.y, f, den);
+    const int per = split_tiles(tiles, part.splits, least), used = (tiles + per - 1) / per;
+    const int quads = a.dim / 4, i = int(blockIdx.x % unsigned(parts)) * 256 + int(threadIdx.x);
+    if (used == 1 || i >= a.qh * quads) return;
+    const int64_t at = int64_t(span.start + node) * a.qh + i / quads, plane = int64_t(a.rows) * a.qh;
+    float top = -kInf, den = 0.0f;
+    f32x4_t num = {0, 0, 0, 0};
+    for (int w0 = 0; w0 < used; w0 += kBatch) {
+        float2 ml[kBatch];
+        f32x4_t v[kBatch];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) num[r] = __builtin_fmaf(v[r], f, num[r]);
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t from = min(w0 + u, used - 1) * plane + at;
+            ml[u] = part.sum[from];
+            v[u] = *reinterpret_cast<const f32x4_t*>(part.out + from * a.dim + 4 * (i % quads));
+            if (w0 + u >= used) ml[u].x = -kInf;
         }
-        const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-        float y[4];
+        float high = top;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = den > 0.0f ? num[r] * inv : 0.0f;
-        *reinterpret_cast<uint2*>(a.out + at * a.dim + 4 * (i % quads)) =
-            make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+        for (int u = 0; u < kBatch; ++u) high = fmaxf(high, ml[u].x);
+        const float base = high == -kInf ? 0.0f : high, old = __builtin_amdgcn_exp2f(top - base);
+        den *= old;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) num[r] *= old;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (w0 + u >= used) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
+            den = __builtin_fmaf(ml[u].y, f, den);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) num[r] = __builtin_fmaf(v[u][r], f, num[r]);
+        }
+        top = high;
     }
+    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
+    float y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = den > 0.0f ? num[r] * inv : 0.0f;
+    *reinterpret_cast<uint2*>(a.out + at * a.dim + 4 * (i % quads)) =
+        make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
 }
+
+constexpr int kSplitPositions = 256;
 
 // The launch's shape: the same for the workspace's size and the launch.
 struct Plan {
     int dim, rows;  // rounded head dim; query rows a block
-    int tile, chunks, splits;
+    int tile, chunks, splits, least;  // positions a tile; blocks a KV head's rows; splits, and the fewest tiles of one
 };
 template <typename F>
 void with_shape(int dim, int rows, F&& f) {
@@ -632,7 +691,8 @@ Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_cont
         p.rows = S::ROWS;
         p.tile = S::T;
         p.chunks = int((queries + p.rows - 1) / p.rows);
-        const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + p.tile - 1) / p.tile;
+        p.least = kSplitPositions / p.tile;
+        const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + kSplitPositions - 1) / kSplitPositions;
         p.splits = int(std::max<int64_t>(1, std::min(most, 256 * S::kBlocks / pairs)));
     });
     return p;
@@ -677,7 +737,7 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
     const bool fits = dim % 8 == 0 && bs % kPage == 0 && int64_t(kvh) * dim <= 0x1000000 && nvr::aligned(q, 16) && nvr::aligned(kc, 16) && nvr::aligned(vc, 16) &&
                       nvr::aligned(out, 16) && int64_t(blocks) * bs <= 0x7fffffff;
     const Plan p = plan_tiles(qh, kvh, dim, batch, max_nodes, max_context);
-    if (fits && int64_t(batch) * kvh * p.chunks * p.splits <= 0x7fffffff) {
+    if (fits && int64_t(batch) * kvh * p.chunks * p.splits <= 0x7fffffff && int64_t(batch) * max_nodes * qh <= 0x3ffffff) {
         if (p.splits > 1 && (workspace == nullptr || !nvr::aligned(workspace, 16)))
             return nvr::fail(-2, "attention_tree: needs a workspace at a multiple of 16 bytes");
         float* partial = static_cast<float*>(workspace);
@@ -687,12 +747,13 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         with_shape(p.dim, p.rows, [&](auto shape) {
             using S = decltype(shape);
             hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(256), S::kLds, c->stream, a, part,
-                               p.chunks, shift);
+                               p.chunks, p.least, shift);
         });
         if (p.splits > 1) {
             NVR_HIP(hipGetLastError());
-            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(int64_t(batch) * max_nodes)), dim3(256), 0, c->stream, a,
-                               part, p.tile);
+            const int parts = (qh * dim / 4 + 255) / 256;
+            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(int64_t(batch) * max_nodes * parts)), dim3(256), 0,
+                               c->stream, a, part, p.tile, p.least, parts);
         }
         return nvr::launch_status();
     }
