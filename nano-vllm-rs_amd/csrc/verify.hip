@@ -34,19 +34,26 @@
 //
 // Launches: 1. verify_stats: maximum, its index and the sum of exponentials over
 // partitions of each row that has children (both models'). 2. verify_walk: a
-// block a sequence folds them and walks the tree. 3. verify_sample: partitions
-// of the last rows. 4. verify_finish: folds those into the last token.
+// block a sequence folds them and walks the tree; with draft logits several
+// blocks a sequence first sum max(p - q, 0), which the second child of a node
+// needs, and the last of them walks. 3. verify_sample: partitions of the last
+// rows; the last block of a sequence stores the token.
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
+
+#include <algorithm>
 
 namespace {
 
 using nvr::kWave;
 constexpr int kMaxNodes = 64;
-constexpr int kPartition = 2048;  // tokens a block of launches 1 and 3
-constexpr int kThreads = kPartition / 8;
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kThreads = 256;
+constexpr int kLoads = 4;             // 16-byte loads in flight a thread of launch 1
+constexpr int kShare = kLoads * kThreads;  // 16-byte chunks a block of launch 1, at least
+constexpr int kSampled = kThreads * 8;               // tokens a block of launch 3
+constexpr int kSlices = 16;                          // blocks a sequence of launch 2, with draft logits
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kInf = __builtin_inff();
 
 // A partition of a row's logits, or the fold of a row's partitions.
@@ -65,6 +72,8 @@ struct Ending {
     float c;             // what rejections took (draft logits)
     float max, inv_sum;  // of the target's row, where c > 0
     float draft_max, draft_inv_sum;
+    int blocks;          // of launch 3 that are done
+    uint64_t best;       // their best (score, token), as keys that compare as they do
     int token[kMaxNodes];
 };
 
@@ -83,15 +92,17 @@ struct VerifyArgs {
     Stats* stats;        // [rows, parts]
     Stats* draft_stats;  // [rows, parts]
     Ending* endings;     // [batch]
-    float* scores;       // [batch, parts]
-    int* ids;            // [batch, parts]
-    int rows, batch, max_nodes, vocab, parts;
+    double* rests;       // [rows, kSlices]: of sum max(p - q, 0)
+    int* arrived;        // [batch]: blocks of launch 2 that are done
+    int rows, batch, max_nodes, vocab;
+    int parts, blocks;  // stats a row has room for; blocks a sequence and model of launch 1
+    int slices;         // blocks a sequence of launch 2
 };
 
-__host__ __device__ inline int partitions(int vocab) {
-    // A row's first token may lie up to 7 tokens behind a 16-byte boundary.
-    return int((int64_t(vocab) + 7 + kPartition - 1) / kPartition);
-}
+// 16-byte chunks that may hold tokens of a row: its first may lie up to 7 tokens behind a boundary.
+__host__ __device__ inline int64_t row_chunks(int vocab) { return (int64_t(vocab) + 7 + 7) / 8; }
+inline int most_parts(int vocab) { return int((row_chunks(vocab) + kShare - 1) / kShare) + 1; }
+inline int sample_blocks(int vocab) { return int((row_chunks(vocab) * 8 + kSampled - 1) / kSampled); }
 
 // Rows of sequence s: the first and how many; none for an invalid sequence.
 __device__ __forceinline__ int tree_rows(const VerifyArgs& a, int s, int* start) {
@@ -101,14 +112,21 @@ __device__ __forceinline__ int tree_rows(const VerifyArgs& a, int s, int* start)
 }
 
 // Eight logits of one row as its 16-byte chunk holds them: tokens t .. t + 7,
-// those outside [0, vocab) NaN, which never wins and weighs nothing.
-__device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t t, int vocab, float (&f)[8]) {
-    if (t >= 0 && t + 8 <= vocab) {
-        nvr::unpack8(nvr::load_stream(row + t), f);
-    } else {
+// those outside [0, vocab) `none`.
+constexpr uint32_t kNaN = 0x7fc0, kMinusInf = 0xff80;
+__device__ __forceinline__ uint4 load_packed(const uint16_t* row, int64_t t, int vocab, uint32_t none) {
+    if (t >= 0 && t + 8 <= vocab) return nvr::load_stream(row + t);
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = t + i >= 0 && t + i < vocab ? nvr::bf16_to_f32(row[t + i]) : __builtin_nanf("");
+    for (int i = 0; i < 4; ++i) {
+        const int64_t lo = t + 2 * i, hi = lo + 1;
+        w[i] = (lo >= 0 && lo < vocab ? uint32_t(row[lo]) : none) | (hi >= 0 && hi < vocab ? uint32_t(row[hi]) : none) << 16;
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The same unpacked, NaN outside: it never wins and weighs nothing.
+__device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t t, int vocab, float (&f)[8]) {
+    nvr::unpack8(load_packed(row, t, vocab, kNaN), f);
 }
 __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinterpret_cast<uintptr_t>(row) >> 1 & 7); }
 
@@ -117,7 +135,6 @@ __device__ __forceinline__ float weight(float x, float top, float scale) {
     if (x == top) return 1.0f;
     return x == x ? __builtin_amdgcn_exp2f((x - top) * scale) : 0.0f;
 }
-
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
 
 struct Best {
@@ -136,88 +153,270 @@ __device__ __forceinline__ Best wave_best(Best b) {
     }
     return b;
 }
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int mask = 1; mask < kWave; mask <<= 1) v = fmaxf(v, nvr::xor_lane(v, mask));
+    return v;
+}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int mask = 1; mask < kWave; mask <<= 1) v += nvr::xor_lane(v, mask);
     return v;
 }
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+    for (int mask = 1; mask < kWave; mask <<= 1) v += __shfl_xor(v, mask);
+    return v;
+}
 
-// A block a (sequence, node, partition); nodes without children have nothing to do.
-__global__ __launch_bounds__(kThreads) void verify_stats(VerifyArgs a) {
-    __shared__ Best tops[kThreads / kWave];
-    __shared__ float sums[kThreads / kWave];
+// Nodes that have children: bit v for node v, the same in every lane. Lane i holds node i's parent, or -1.
+__device__ __forceinline__ uint64_t inner_nodes(int parent) {
+    const uint64_t mine = parent >= 0 ? uint64_t(1) << parent : 0;
+    uint32_t lo = uint32_t(mine), hi = uint32_t(mine >> 32);
+#pragma unroll
+    for (int mask = 1; mask < kWave; mask <<= 1) {
+        lo |= nvr::xor_lane_bits(lo, mask);
+        hi |= nvr::xor_lane_bits(hi, mask);
+    }
+    return uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(hi)))) << 32 | uint32_t(__builtin_amdgcn_readfirstlane(int(lo)));
+}
+
+// How the rows of a sequence's nodes with children are shared by launch 1's
+// blocks: one after the other they are rows * chunks 16-byte chunks, cut evenly,
+// so that every block has as much to do whatever the tree. A row's parts are the
+// blocks that have some of it.
+struct Shares {
+    int64_t chunks, per;  // of a row; of a block
+    __device__ __forceinline__ Shares(int vocab, int rows, int blocks) {
+        chunks = row_chunks(vocab);
+        const int64_t all = chunks * rows;
+        per = max((all + blocks - 1) / blocks, int64_t(kShare));
+    }
+    __device__ __forceinline__ int first_block(int i) const { return int(uint64_t(i) * uint64_t(chunks) / uint64_t(per)); }
+    __device__ __forceinline__ int last_block(int i) const { return int((uint64_t(i + 1) * uint64_t(chunks) - 1) / uint64_t(per)); }
+};
+
+// A block a (sequence, share, model): one pass over its chunks, each thread with a
+// maximum and a sum of its own that it scales again when the maximum grows.
+__global__ __launch_bounds__(kThreads, 8) void verify_stats(VerifyArgs a) {
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ float tops[kWaves], sums[kWaves];
+    __shared__ int first;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int part = int(blockIdx.x % unsigned(a.parts));
-    const int item = int(blockIdx.x / unsigned(a.parts));
-    const int s = item / a.max_nodes, node = item % a.max_nodes;
+    const int block = int(blockIdx.x % unsigned(a.blocks)), item = int(blockIdx.x / unsigned(a.blocks));
+    const int side = item >= a.batch ? 1 : 0, s = item - side * a.batch;
+    if (block == 0 && side == 0 && threadIdx.x == 0) a.arrived[s] = 0;
     int start;
     const int n = tree_rows(a, s, &start);
-    if (node >= n) return;
-    const bool child = lane > node && lane < n && a.parents[start + lane] == node;
-    if (__ballot(child) == 0) return;
+    if (n < 2) return;
     const float temperature = a.temps[s];
     const bool sampled = temperature > 0.0f;
+    if (side == 1 && !sampled) return;
+    int parent = lane > 0 && lane < n ? a.parents[start + lane] : -1;
+    if (parent >= lane) parent = -1;
+    uint64_t inner = inner_nodes(parent);
+    const int count = __popcll(inner);
+    const Shares shares(a.vocab, count, a.blocks);
+    int64_t at = block * shares.per;
+    const int64_t stop = min(at + shares.per, count * shares.chunks);
+    if (at >= stop) return;
     const float scale = kLog2e / temperature;
-    const int row = start + node;
-    for (int side = 0; side < (sampled && a.draft ? 2 : 1); ++side) {
+    int i = int(uint64_t(at) / uint64_t(shares.chunks));
+    for (int skip = 0; skip < i; ++skip) inner &= inner - 1;
+    for (; at < stop; ++i, inner &= inner - 1) {
+        const int row = start + __builtin_ctzll(inner);
         const uint16_t* x = (side ? a.draft : a.logits) + int64_t(row) * a.vocab;
-        const int64_t t = int64_t(part) * kPartition + 8 * int(threadIdx.x) - lead_of(x);
-        float f[8];
-        load_chunk(x, t, a.vocab, f);
-        Best b{-kInf, nvr::kNoIndex};
+        const int lead = lead_of(x);
+        const int64_t base = i * shares.chunks;
+        const int begin = int(at - base), end = int(min(stop - base, shares.chunks));
+        at = base + end;
+        float top = -kInf, sum = 0.0f;
+        int where = -1;  // the chunk from which `top` is
+        for (int k = begin + int(threadIdx.x); k < end; k += kLoads * kThreads) {
+            uint4 packed[kLoads];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
-        b = wave_best(b);
-        if (lane == 0) tops[wave] = b;
-        __syncthreads();
+            for (int u = 0; u < kLoads; ++u) {
+                const int c = k + u * kThreads;
+                packed[u] = load_packed(x, c < end ? 8 * int64_t(c) - lead : int64_t(a.vocab), a.vocab, kMinusInf);
+            }
+            float high = __builtin_nanf("");
 #pragma unroll
-        for (int w = 0; w < kThreads / kWave; ++w) consider(b, tops[w].score, tops[w].index);
-        float sum = 0.0f;
-        if (sampled && b.score > -kInf) {
+            for (int u = 0; u < kLoads; ++u) {
+                float f[8];
+                nvr::unpack8(packed[u], f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += weight(f[i], b.score, scale);
+                for (int j = 0; j < 8; ++j) high = fmaxf(high, f[j]);  // passes over NaN
+            }
+            if (high > top || (high == top && where < 0)) {
+                if (sum > 0.0f) sum *= __builtin_amdgcn_exp2f((top - high) * scale);
+                top = high;
+                where = k;
+            }
+            if (sampled && top > -kInf) {
+#pragma unroll
+                for (int u = 0; u < kLoads; ++u) {
+                    float f[8], eight = 0.0f;
+                    nvr::unpack8(packed[u], f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f((f[j] - top) * scale);
+                    sum += eight;
+                }
+            }
         }
-        sum = wave_sum(sum);
+        if (!(sum < kInf)) {  // a NaN among the logits, or an infinite maximum
+            sum = 0.0f;
+            for (int k = begin + int(threadIdx.x); k < end; k += kThreads) {
+                float f[8];
+                load_chunk(x, 8 * int64_t(k) - lead, a.vocab, f);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += weight(f[j], top, scale);
+            }
+        }
+        const float high = wave_max(top);
+        if (lane == 0) tops[wave] = high;
+        if (threadIdx.x == 0) first = nvr::kNoIndex;
+        __syncthreads();
+        float all = tops[0];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) all = fmaxf(all, tops[w]);
+        if (top == all && where >= 0) {
+            int lowest = nvr::kNoIndex;
+#pragma unroll 1
+            for (int u = kLoads - 1; u >= 0; --u) {
+                const int c = where + u * kThreads;
+                if (c >= end) continue;
+                float f[8];
+                load_chunk(x, 8 * int64_t(c) - lead, a.vocab, f);
+#pragma unroll
+                for (int j = 7; j >= 0; --j)
+                    if (f[j] == all) lowest = int(8 * int64_t(c) - lead) + j;
+            }
+            atomicMin(&first, lowest);
+        }
+        sum = wave_sum(sum > 0.0f ? sum * weight(top, all, scale) : 0.0f);
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         if (threadIdx.x == 0) {
             sum = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kThreads / kWave; ++w) sum += sums[w];
-            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + part] = Stats{b.score, sum, b.index, 0};
+            for (int w = 0; w < kWaves; ++w) sum += sums[w];
+            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + block - shares.first_block(i)] = Stats{all, sum, first, 0};
         }
-        __syncthreads();
     }
 }
 
-// A row's partitions folded, by one wave.
-__device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale, int lane) {
+// A row's partitions folded, by one lane: a wave folds every node of a tree at once.
+__device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale) {
+    constexpr int kBatch = 8;
     Best b{-kInf, nvr::kNoIndex};
-    for (int i = lane; i < parts; i += kWave) consider(b, part[i].max, part[i].best);
-    b = wave_best(b);
-    double sum = 0.0;
-    for (int i = lane; i < parts; i += kWave)
-        if (part[i].max > -kInf) sum += double(part[i].sum) * double(weight(part[i].max, b.score, scale));
+    for (int i0 = 0; i0 < parts; i0 += kBatch) {
+        Stats t[kBatch];
 #pragma unroll
-    for (int mask = 1; mask < kWave; mask <<= 1) sum += __shfl_xor(sum, mask);
+        for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) consider(b, t[u].max, t[u].best);
+    }
+    double sum = 0.0;
+    for (int i0 = 0; i0 < parts; i0 += kBatch) {
+        Stats t[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            if (i0 + u < parts && t[u].max > -kInf) sum += double(t[u].sum * weight(t[u].max, b.score, scale));
+    }
     return Stats{b.score, float(sum), b.index, 0};
 }
 
-constexpr int kWalkThreads = 1024;
+// The target's and the draft model's probabilities of a row's tokens.
+struct Rows {
+    const uint16_t* target;
+    const uint16_t* draft;
+    float max, inv_sum, draft_max, draft_inv_sum;
+};
+
+// p - c q of one token; NaN where p is.
+struct RestTerm {
+    const Rows& r;
+    float scale, cq;
+    bool infinite;
+    __device__ __forceinline__ RestTerm(const Rows& rows, float c, float s)
+        : r(rows), scale(s), cq(c * rows.draft_inv_sum), infinite(!(fabsf(rows.max) < kInf) || !(fabsf(rows.draft_max) < kInf)) {}
+    __device__ __forceinline__ float operator()(float x, float y) const {
+        if (infinite) return weight(x, r.max, scale) * r.inv_sum - weight(y, r.draft_max, scale) * cq;
+        const float wx = __builtin_amdgcn_exp2f((x - r.max) * scale);
+        const float wy = fmaxf(__builtin_amdgcn_exp2f((y - r.draft_max) * scale), 0.0f);  // a NaN is no token of q
+        return __builtin_fmaf(wx, r.inv_sum, -(wy * cq));
+    }
+};
+
+// sum of max(p - c q, 0) over 16-byte chunks [first, end) of a row, this thread's share.
+__device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, float scale, int64_t first, int64_t end,
+                                           int threads) {
+    constexpr int kBatch = 4;
+    const int lead = lead_of(r.target);
+    const bool alike = lead == lead_of(r.draft);
+    const RestTerm term(r, c, scale);
+    double sum = 0.0;
+    for (int64_t k = first + int(threadIdx.x); k < end; k += kBatch * threads) {
+        float x[kBatch][8], y[kBatch][8];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int64_t t = k + u * threads < end ? 8 * (k + u * threads) - lead : int64_t(vocab);
+            load_chunk(r.target, t, vocab, x[u]);
+            if (alike) {
+                load_chunk(r.draft, t, vocab, y[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    y[u][i] = t + i >= 0 && t + i < vocab ? nvr::bf16_to_f32(r.draft[t + i]) : __builtin_nanf("");
+            }
+        }
+        float part = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part += fmaxf(term(x[u][i], y[u][i]), 0.0f);
+        sum += double(part);
+    }
+    return sum;
+}
+
+// Blocks of one launch hand values over by atomics alone, so that no cache has to
+// be written back or dropped for it (a release and an acquire a block do that:
+// 3600 blocks of launch 3 took 102 us with them, 22 without). An atomic that
+// returns a value has been performed when the value is there; the next one is
+// issued after that.
+__device__ __forceinline__ void performed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void publish(double* to, double v) {
+    const uint64_t old = __hip_atomic_exchange(reinterpret_cast<uint64_t*>(to), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("" ::"v"(old));  // the returning form
+    performed();
+}
+__device__ __forceinline__ int arrive(int* count) {
+    performed();
+    return __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+constexpr int kWalkThreads = 512;
 constexpr int kWalkWaves = kWalkThreads / kWave;
 
+// a.slices blocks a sequence.
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ Stats target[kMaxNodes], draft[kMaxNodes];
-    __shared__ double parts[kWalkWaves];
+    __shared__ double parts[kMaxNodes][kWalkWaves], rests[kMaxNodes];
     __shared__ int path[kMaxNodes];
+    __shared__ int last;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int s = int(blockIdx.x);
+    const int s = int(blockIdx.x), slice = int(blockIdx.y);
     Ending* ending = a.endings + s;
     int start;
     const int n = tree_rows(a, s, &start);
     int* tokens = a.out_tokens + int64_t(s) * a.max_nodes;
     int* nodes = a.out_nodes + int64_t(s) * a.max_nodes;
     if (n == 0) {
+        if (slice != 0) return;
         for (int i = int(threadIdx.x); i < a.max_nodes; i += kWalkThreads) tokens[i] = nodes[i] = -1;
         if (threadIdx.x == 0) { a.out_counts[s] = 0; ending->row = -1; }
         return;
@@ -228,36 +427,94 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     // Lane i of every wave holds node i.
     const bool mine = lane > 0 && lane < n;
     int parent = mine ? a.parents[start + lane] : -1;
-    if (parent < 0 || parent >= lane) parent = -1;
     const int token = mine ? a.tokens[start + lane] : -1;
-    const bool known = parent >= 0 && token >= 0 && token < a.vocab;
     const float u = mine ? a.uniforms[start + lane] : 0.0f;
-    for (int v = wave; v < n; v += kWalkWaves) {
-        if (__ballot(parent == v) == 0) continue;
-        const int64_t at = int64_t(start + v) * a.parts;
-        const Stats t = fold(a.stats + at, a.parts, scale, lane);
-        if (lane == 0) target[v] = t;
-        if (drafted) {
-            const Stats d = fold(a.draft_stats + at, a.parts, scale, lane);
-            if (lane == 0) draft[v] = d;
-        }
+    if (parent < 0 || parent >= lane) parent = -1;
+    const bool known = parent >= 0 && token >= 0 && token < a.vocab;
+    const uint64_t inner = inner_nodes(parent);
+    // Only a node with a second child to try needs more than one block.
+    const bool alone = !drafted || __popcll(__ballot(known)) == __popcll(inner_nodes(known ? parent : -1));
+    if (alone && slice != 0) return;
+    // The logits of each node's token, under its parent.
+    float xt = 0.0f, xd = 0.0f;
+    if (sampled && known) {
+        const int64_t at = int64_t(start + parent) * a.vocab + token;
+        xt = nvr::bf16_to_f32(a.logits[at]);
+        if (drafted) xd = nvr::bf16_to_f32(a.draft[at]);
+    }
+    if (wave < (drafted ? 2 : 1) && (inner >> lane & 1) != 0)
+{
+        const Shares shares(a.vocab, __popcll(inner), a.blocks);
+        const int i = __popcll(inner & ((uint64_t(1) << lane) - 1));
+        (wave ? draft : target)[lane] = fold((wave ? a.draft_stats : a.stats) + int64_t(start + lane) * a.parts,
+                                             shares.last_block(i) - shares.first_block(i) + 1, scale);
     }
     __syncthreads();
-    // Each node's probabilities under its parent's rows.
-    auto chance = [&](const uint16_t* logits, const Stats& r) -> double {
-        const float x = nvr::bf16_to_f32(logits[int64_t(start + parent) * a.vocab + token]);
+    auto rows_of = [&](int v) {
+        const int64_t at = int64_t(start + v) * a.vocab;
+        return Rows{a.logits + at, a.draft + at, target[v].max, inverse(target[v].sum), draft[v].max, inverse(draft[v].sum)};
+    };
+    // Each node's probabilities under its parent's rows: 2^y with y = k + f, |f| <= 1/2, in fp64 but for 2^f.
+    auto chance = [&](float x, const Stats& r) -> double {
         if (!(r.max > -kInf) || x != x) return 0.0;
         if (x == r.max) return 1.0 / double(r.sum);
-        const double y = (double(x) - double(r.max)) / double(temperature);
-        return y > -700.0 ? nvr::d_exp(y) / double(r.sum) : 0.0;
+        const double y = (double(x) - double(r.max)) * 1.4426950408889634 / double(temperature), k = rint(y);
+        return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
     };
     double p = 0.0, q = 0.0;
     if (sampled && known) {
-        p = chance(a.logits, target[parent]);
-        if (drafted) q = chance(a.draft, draft[parent]);
+        p = chance(xt, target[parent]);
+        if (drafted) q = chance(xd, draft[parent]);
+    }
+    // Nodes that the walk may come to, have it reject a first child and try a second: those need the first rest's sum.
+    uint64_t several = 0;
+    if (!alone) {
+        uint64_t open = 1;
+        for (int v = 0; v < n - 1; ++v) {
+            uint64_t children = __ballot(known && parent == v);
+            if (children == 0 || (open >> v & 1) == 0) continue;
+            const int i = __builtin_ctzll(children);
+            const double px = __shfl(p, i);
+            if (px > 0.0 && double(__shfl(u, i)) * __shfl(q, i) < px) {
+                open |= uint64_t(1) << i;  // surely the next
+            } else {
+                children &= children - 1;
+                open |= children;
+                several |= uint64_t(children != 0) << v;
+            }
+        }
+        if (several == 0 && slice != 0) return;
+    }
+    const int64_t chunks = row_chunks(a.vocab);
+    if (several != 0) {
+        // This block's share of the rests after one rejection; the last block of the sequence goes on.
+        const int64_t share = (chunks + a.slices - 1) / a.slices, begin = slice * share;
+        for (uint64_t left = several; left != 0; left &= left - 1) {
+            const int v = __builtin_ctzll(left);
+            const double sum = wave_sum(rest_sum(rows_of(v), a.vocab, 1.0f, scale, begin, min(chunks, begin + share), kWalkThreads));
+            if (lane == 0) parts[v][wave] = sum;
+        }
+        __syncthreads();
+        if (threadIdx.x < kMaxNodes && (several >> threadIdx.x & 1) != 0) {
+            double sum = 0.0;
+            for (int w = 0; w < kWalkWaves; ++w) sum += parts[threadIdx.x][w];
+            publish(a.rests + int64_t(start + threadIdx.x) * kSlices + slice, sum);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) last = arrive(a.arrived + s) == a.slices - 1;
+        __syncthreads();
+        if (!last) return;
+        if (threadIdx.x < kMaxNodes && (several >> threadIdx.x & 1) != 0) {
+            double sum = 0.0;
+            for (int w = 0; w < a.slices; ++w)
+                sum += __hip_atomic_load(a.rests + int64_t(start + threadIdx.x) * kSlices + w, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+            rests[threadIdx.x] = sum;
+        }
+        __syncthreads();
     }
     // Every wave walks alike.
-    int v = 0, length = 0, tried = 0;
+    int v = 0, length = 0;
     double c = 0.0, z = 1.0;
     uint64_t rejected = 0;
     while (true) {
@@ -279,26 +536,19 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
             if (drafted) {
                 const double qx = __shfl(q, i), r = fmax(px - c * qx, 0.0);
                 if (r > 0.0 && ux * z * qx < r) { next = i; break; }
+                const bool once = c == 0.0;
                 c += z;
                 if (children == 0) break;
-                // The rest's sum, for the next child.
-                const uint16_t* xt = a.logits + int64_t(start + v) * a.vocab;
-                const uint16_t* xd = a.draft + int64_t(start + v) * a.vocab;
-                const Stats t = target[v], d = draft[v];
-                const float it = inverse(t.sum), id = float(c) * inverse(d.sum);
-                double sum = 0.0;
-                for (int64_t k = threadIdx.x; k < a.vocab; k += kWalkThreads) {
-                    const float wt = weight(nvr::bf16_to_f32(xt[k]), t.max, scale) * it;
-                    const float wd = weight(nvr::bf16_to_f32(xd[k]), d.max, scale) * id;
-                    sum += double(fmaxf(wt - wd, 0.0f));
+                if (once) {
+                    z = rests[v];
+                } else {
+                    const double sum = wave_sum(rest_sum(rows_of(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
+                    if (lane == 0) parts[0][wave] = sum;
+                    __syncthreads();
+                    z = 0.0;
+                    for (int w = 0; w < kWalkWaves; ++w) z += parts[0][w];
+                    __syncthreads();
                 }
-#pragma unroll
-                for (int mask = 1; mask < kWave; mask <<= 1) sum += __shfl_xor(sum, mask);
-                if (lane == 0) parts[wave] = sum;
-                __syncthreads();
-                z = 0.0;
-                for (int w = 0; w < kWalkWaves; ++w) z += parts[w];
-                __syncthreads();
             } else {
                 if (__ballot((rejected >> lane & 1) != 0 && token == x) != 0) continue;
                 if (px > 0.0 && ux * z < px) { next = i; break; }
@@ -318,107 +568,148 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     if (wave == 0) {
         const bool out = (rejected >> lane & 1) != 0;
         const uint64_t all = __ballot(out);
-        tried = __popcll(all);
         if (out) ending->token[__popcll(all & ((uint64_t(1) << lane) - 1))] = token;
+        const bool folded = (inner >> v & 1) != 0;
         if (lane == 0) {
-            const bool inner = c > 0.0;
             a.out_counts[s] = length;
             ending->row = start + v;
             ending->node = length - 1;
-            ending->tried = tried;
+            ending->tried = __popcll(all);
             ending->c = float(c);
-            ending->fallback = 0;
-            ending->max = inner ? target[v].max : 0.0f;
-            ending->inv_sum = inner ? inverse(target[v].sum) : 0.0f;
-            ending->draft_max = inner ? draft[v].max : 0.0f;
-            ending->draft_inv_sum = inner ? inverse(draft[v].sum) : 0.0f;
+            ending->fallback = folded && target[v].best != nvr::kNoIndex ? target[v].best : 0;
+            ending->blocks = 0;
+            ending->best = 0;
+            if (c > 0.0) {
+                const Rows r = rows_of(v);
+                ending->max = r.max;
+                ending->inv_sum = r.inv_sum;
+                ending->draft_max = r.draft_max;
+                ending->draft_inv_sum = r.draft_inv_sum;
+            }
         }
-        if (__ballot(parent == v) != 0 && lane == 0 && target[v].best != nvr::kNoIndex) ending->fallback = target[v].best;
     }
 }
 
-// A block a (sequence, partition of its last row).
+// (score, token) as a number that is larger for what nvr::better prefers; 0: nothing.
+__device__ __forceinline__ uint64_t key_of(const Best& b) {
+    if (b.index == nvr::kNoIndex) return 0;
+    const uint32_t bits = __float_as_uint(b.score + 0.0f);  // -0 as +0: they are equal scores
+    return uint64_t(bits & 0x80000000u ? ~bits : bits | 0x80000000u) << 32 | uint32_t(~b.index);
+}
+
+// A block a (sequence, partition of its last row). A Gumbel score is an integer
+// hash and two logarithms; the noise is at most -ln(1 - u), so one hardware
+// logarithm bounds it, and only a lane's best bound and the bounds that reach
+// the wave's best score are scored in full.
 __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
-    __shared__ Best tops[kThreads / kWave];
+    constexpr int kWaves = kThreads / kWave;
+    __shared__ Best tops[kWaves];
     __shared__ int tried[kMaxNodes];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int part = int(blockIdx.x % unsigned(a.parts));
-    const int s = int(blockIdx.x / unsigned(a.parts));
-    const Ending* e = a.endings + s;
+    const int s = int(blockIdx.x), part = int(blockIdx.y), parts = int(gridDim.y);
+    Ending* e = a.endings + s;
     const int row = e->row;
     if (row < 0) return;
     const int count = e->tried;
-    if (int(threadIdx.x) < count) tried[threadIdx.x] = e->token[threadIdx.x];
-    __syncthreads();
-    const float temperature = a.temps[s];
+    const float temperature = a.temps[s], c = e->c;
     const uint64_t seed = a.seeds[s];
     const uint16_t* x = a.logits + int64_t(row) * a.vocab;
-    const int64_t t = int64_t(part) * kPartition + 8 * int(threadIdx.x) - lead_of(x);
+    const int64_t t = int64_t(part) * kSampled + 8 * int(threadIdx.x) - lead_of(x);
     float f[8];
     load_chunk(x, t, a.vocab, f);
+    if (int(threadIdx.x) < count) tried[threadIdx.x] = e->token[threadIdx.x];
+    __syncthreads();
     Best b{-kInf, nvr::kNoIndex};
     if (!(temperature > 0.0f)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
-    } else if (e->c > 0.0f) {
-        const uint16_t* y = a.draft + int64_t(row) * a.vocab;
-        const float scale = kLog2e / temperature, cq = e->c * e->draft_inv_sum;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (t + i < 0 || t + i >= a.vocab) continue;
-            const float wt = weight(f[i], e->max, scale) * e->inv_sum;
-            const float wd = weight(nvr::bf16_to_f32(y[t + i]), e->draft_max, scale) * cq;
-            const float w = wt - wd;
-            if (!(w >= 0x1p-126f)) continue;
-            const float g = nvr::hash_uniform(nvr::splitmix64(seed ^ (uint64_t(t + i) * nvr::kTokenMix)));
-            consider(b, nvr::nvr_logf(w) - nvr::nvr_logf(-nvr::nvr_logf(g)), int(t) + i);
-        }
     } else {
+        if (c > 0.0f) {  // ln(p - c q) in place of the logits
+            const Rows r{x, a.draft + int64_t(row) * a.vocab, e->max, e->inv_sum, e->draft_max, e->draft_inv_sum};
+            const RestTerm term(r, c, kLog2e / temperature);
+            float y[8];
+            if (lead_of(r.draft) == lead_of(x)) {
+                load_chunk(r.draft, t, a.vocab, y);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    y[i] = t + i >= 0 && t + i < a.vocab ? nvr::bf16_to_f32(r.draft[t + i]) : __builtin_nanf("");
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = term(f[i], y[i]);
+                f[i] = w >= 0x1p-126f ? w : __builtin_nanf("");
+            }
+        }
+        for (int k = 0; k < count; ++k) {
+            const int64_t at = tried[k] - t;
+            if (at >= 0 && at < 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (at == i) f[i] = __builtin_nanf("");
+            }
+        }
+        auto uniform = [&](int i) { return nvr::hash_uniform(nvr::splitmix64(seed ^ (uint64_t(t + i) * nvr::kTokenMix))); };
+        auto score = [&](float v, float u) {
+            return (c > 0.0f ? nvr::nvr_logf(v) : v / temperature) - nvr::nvr_logf(-nvr::nvr_logf(u));
+        };
+        const float inverse_t = 1.0f / temperature;
+        const bool bounded = inverse_t < kInf;
+        float bound[8], high = -kInf;
+        float us[8];
+        int own = -1;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float score = nvr::gumbel_score(f[i], temperature, seed, uint32_t(t + i));
-            if (!nvr::better(score, int(t) + i, b.score, b.index) || (count > 0 && score == -kInf)) continue;
-            bool out = false;
-            for (int k = 0; k < count; ++k) out |= tried[k] == int(t) + i;
-            if (!out) b = Best{score, int(t) + i};
+            us[i] = uniform(i);
+            // Bounds with 2^-20 of the value and 1e-4 to spare: many times what their few roundings can take.
+            const float v = c > 0.0f ? __builtin_amdgcn_logf(f[i]) * kLn2 : f[i] * inverse_t;
+            const float g = __builtin_fmaf(__builtin_amdgcn_logf(1.0f - us[i]), -kLn2, 1e-4f);
+            bound[i] = bounded ? __builtin_fmaf(v, v > 0.0f ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f, g)
+                               : f[i] == f[i] ? kInf : f[i];
+            if (bound[i] > high || (own < 0 && bound[i] == high)) { high = bound[i]; own = i; }
         }
+        if (own >= 0) {
+            float v = f[0], u = us[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i)
+                if (own == i) { v = f[i]; u = us[i]; }
+            consider(b, score(v, u), int(t) + own);
+        }
+        const float reach = wave_max(b.score);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i != own && bound[i] >= reach) consider(b, score(f[i], us[i]), int(t) + i);
+        if (b.score == -kInf && (count > 0 || c > 0.0f)) b.index = nvr::kNoIndex;  // the rest is nothing here
     }
     b = wave_best(b);
     if (lane == 0) tops[wave] = b;
     __syncthreads();
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int w = 0; w < kThreads / kWave; ++w) consider(b, tops[w].score, tops[w].index);
-        a.scores[int64_t(s) * a.parts + part] = b.score;
-        a.ids[int64_t(s) * a.parts + part] = b.index;
+        for (int w = 1; w < kWaves; ++w) consider(b, tops[w].score, tops[w].index);
+        const uint64_t old = __hip_atomic_fetch_max(&e->best, key_of(b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("" ::"v"(old));  // the returning form
+        if (arrive(&e->blocks) == parts - 1) {
+            const uint64_t key = __hip_atomic_load(&e->best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            a.out_tokens[int64_t(s) * a.max_nodes + e->node] = key == 0 ? e->fallback : int(~uint32_t(key));
+        }
     }
-}
-
-__global__ __launch_bounds__(kWave) void verify_finish(VerifyArgs a) {
-    const int s = int(blockIdx.x), lane = int(threadIdx.x);
-    const Ending* e = a.endings + s;
-    if (e->row < 0) return;
-    Best b{-kInf, nvr::kNoIndex};
-    for (int i = lane; i < a.parts; i += kWave)
-        consider(b, a.scores[int64_t(s) * a.parts + i], a.ids[int64_t(s) * a.parts + i]);
-    b = wave_best(b);
-    if (lane == 0) a.out_tokens[int64_t(s) * a.max_nodes + e->node] = b.index == nvr::kNoIndex ? e->fallback : b.index;
 }
 
 // The workspace's parts, each at a multiple of 16 bytes.
 struct Workspace {
-    int64_t stats, draft_stats, endings, scores, ids, bytes;
+    int64_t stats, draft_stats, endings, rests, arrived, bytes;
 };
 Workspace layout(int rows, int batch, int vocab) {
-    const int64_t parts = partitions(vocab);
+    const int64_t parts = most_parts(vocab);
     auto up = [](int64_t b) { return (b + 15) & ~int64_t(15); };
     Workspace w;
     w.stats = 0;
     w.draft_stats = w.stats + up(int64_t(sizeof(Stats)) * rows * parts);
     w.endings = w.draft_stats + up(int64_t(sizeof(Stats)) * rows * parts);
-    w.scores = w.endings + up(int64_t(sizeof(Ending)) * batch);
-    w.ids = w.scores + up(4 * int64_t(batch) * parts);
-    w.bytes = w.ids + up(4 * int64_t(batch) * parts);
+    w.rests = w.endings + up(int64_t(sizeof(Ending)) * batch);
+    w.arrived = w.rests + up(int64_t(sizeof(double)) * kSlices * rows);
+    w.bytes = w.arrived + up(int64_t(sizeof(int)) * batch);
     return w;
 }
 
@@ -441,9 +732,14 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
     if (max_nodes < 1 || max_nodes > kMaxNodes)
         return nvr::fail(-2, "verify_tree: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     if (!nvr::aligned(workspace, 16)) return nvr::fail(-2, "verify_tree: the workspace needs 16-byte alignment");
-    const int parts = partitions(vocab);
-    if (int64_t(batch) * max_nodes > 0x7fffffff / parts)
-        return nvr::fail(-2, "verify_tree: %d sequences of %d nodes over %d tokens exceed one launch", batch, max_nodes, vocab);
+    const int sampled = sample_blocks(vocab);
+    if (sampled > 65535)  // blocks of a grid dimension
+        return nvr::fail(-2, "verify_tree: %d tokens exceed one launch", vocab);
+    // Eight blocks a CU in all, so that none has to wait for another's end.
+    const int sides = draft_logits ? 2 : 1;
+    const int64_t cus = c->cu_count > 0 ? c->cu_count : 256;
+    const int blocks = int(std::min<int64_t>(std::max<int64_t>(8 * cus / (int64_t(batch) * sides), 1),
+                                             int64_t(most_parts(vocab)) * std::max(max_nodes - 1, 1)));
     const Workspace w = layout(rows, batch, vocab);
     char* base = static_cast<char*>(workspace);
     const VerifyArgs a{static_cast<const uint16_t*>(logits), static_cast<const uint16_t*>(draft_logits),
@@ -452,15 +748,14 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
                        static_cast<const float*>(uniforms), static_cast<const uint64_t*>(seeds),
                        static_cast<int*>(out_tokens), static_cast<int*>(out_nodes), static_cast<int*>(out_counts),
                        reinterpret_cast<Stats*>(base + w.stats), reinterpret_cast<Stats*>(base + w.draft_stats),
-                       reinterpret_cast<Ending*>(base + w.endings), reinterpret_cast<float*>(base + w.scores),
-                       reinterpret_cast<int*>(base + w.ids), rows, batch, max_nodes, vocab, parts};
-    hipLaunchKernelGGL(verify_stats, dim3(unsigned(int64_t(batch) * max_nodes * parts)), dim3(kThreads), 0, c->stream, a);
+                       reinterpret_cast<Ending*>(base + w.endings), reinterpret_cast<double*>(base + w.rests),
+                       reinterpret_cast<int*>(base + w.arrived), rows, batch, max_nodes, vocab, most_parts(vocab), blocks,
+                       draft_logits && max_nodes > 2 ? kSlices : 1};
+    hipLaunchKernelGGL(verify_stats, dim3(unsigned(int64_t(batch) * blocks * sides)), dim3(kThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(verify_walk, dim3(unsigned(batch)), dim3(kWalkThreads), 0, c->stream, a);
+    hipLaunchKernelGGL(verify_walk, dim3(unsigned(batch), unsigned(a.slices)), dim3(kWalkThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(verify_sample, dim3(unsigned(int64_t(batch) * parts)), dim3(kThreads), 0, c->stream, a);
-    NVR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(verify_finish, dim3(unsigned(batch)), dim3(kWave), 0, c->stream, a);
+    hipLaunchKernelGGL(verify_sample, dim3(unsigned(batch), unsigned(sampled)), dim3(kThreads), 0, c->stream, a);
     return nvr::launch_status();
 }
 
