@@ -272,7 +272,7 @@ int nv_verify_tree_workspace(int rows, int batch, int vocab, size_t* bytes);
  * i32, the accepted tokens, then the token after them, then -1; out_nodes: [batch,
  * max_nodes] i32, the path's nodes from 0 on, then -1; out_counts: [batch] i32, how
  * many of either (0 for a sequence without rows, or with more than max_nodes, or
- * with rows outside [0, rows)). For temps > 0 the tokens are distributed as the
+ * with rows outside [0, rows)). vocab is at most 2^26 (else -2). For temps > 0 the tokens are distributed as the
  * target's samples; for temps <= 0 they are its argmaxes. With nothing rejected at
  * the path's last node, the token after it is nv_sample's for that row. */
 int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, const void* tokens,

@@ -15,29 +15,31 @@
 //   - T > 0, draft logits (children drawn independently from q_v =
 //     softmax(draft_logits[v] / T)): accepted if p > 0 and u * Z * q_v(x) < p with
 //     p = max(p_v(x) - c q_v(x), 0), where c = 0 and Z = 1 at first, and after each
-//     rejection c += Z and then Z = sum over x of max(p_v - c q_v, 0). (The rest after a
-//     rejection is max(r - Z q, 0) of the rest r before, Z its sum; and
-//     max(max(p - c q, 0) - Z q, 0) = max(p - (c + Z) q, 0), so one number says what every rejection took.) After all are
-//     rejected, the rest is max(p_v - c q_v, 0).
+//     rejection c += Z and then Z = sum over x of max(p_v - c q_v, 0). (A rejection
+//     leaves max(r - Z q, 0) of the rest r before it, Z its sum; and max(max(p - c q,
+//     0) - Z q, 0) = max(p - (c + Z) q, 0), so one number says what all of them took.)
+//     After all are rejected, the rest is max(p_v - c q_v, 0).
 //   - T <= 0 (or NaN): accepted if x is v's argmax.
 // The first accepted child is the next v. Where none is, the path ends and its
 // last token is the argmax of ln(rest) + Gumbel noise, which nv_sample adds from
 // seeds[s] and the token (for T <= 0 of the logits alone): with nothing rejected
 // at v it is nv_sample's token of that row. Where the rest is nothing, it is v's
 // argmax. Drafted tokens outside [0, vocab) are passed over, as are nodes whose
-// parent does not come before them. NaN logits have probability 0; ties go to the lower index; an argmax of nothing is 0.
+// parent does not come before them. NaN logits have probability 0, a logit / T
+// beyond fp32 counts as infinite, and infinite ones share the probability; ties go
+// to the lower index; an argmax of nothing is 0.
 //
 // For T > 0 the emitted tokens are distributed as the target's own samples are.
 // What decides is held in fp32 sums of fp32 exponentials, and in fp64 from there
 // on: a comparison or an argmax goes the other way than exact arithmetic has it
 // only where both sides agree to about 1e-6.
 //
-// Launches: 1. verify_stats: maximum, its index and the sum of exponentials over
-// partitions of each row that has children (both models'). 2. verify_walk: a
-// block a sequence folds them and walks the tree; with draft logits several
-// blocks a sequence first sum max(p - q, 0), which the second child of a node
-// needs, and the last of them walks. 3. verify_sample: partitions of the last
-// rows; the last block of a sequence stores the token.
+// Launches: 1. verify_stats: for each row that has children, the sum of the
+// exponentials (T > 0; both models') or the argmax, by shares of the rows.
+// 2. verify_walk: a block a sequence folds them and walks the tree; with draft
+// logits several blocks a sequence first sum max(p - q, 0), which the second child
+// of a node needs, and the last of them walks. 3. verify_sample: partitions of
+// the last rows; the last block of a sequence stores the token.
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
@@ -48,6 +50,7 @@ namespace {
 
 using nvr::kWave;
 constexpr int kMaxNodes = 64;
+constexpr int kMaxVocab = 1 << 26;
 constexpr int kThreads = 256;
 constexpr int kLoads = 4;             // 16-byte loads in flight a thread of launch 1
 constexpr int kShare = kLoads * kThreads;  // 16-byte chunks a block of launch 1, at least
@@ -56,10 +59,13 @@ constexpr int kSlices = 16;                          // blocks a sequence of lau
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kInf = __builtin_inff();
 
-// A partition of a row's logits, or the fold of a row's partitions.
+// Part of a row's logits, or the fold of its parts. T > 0: sum of 2^(x log2(e) / T -
+// offset), the offset a whole number, so that it is subtracted without an error of
+// its own and sums are brought to another one exactly; +inf where the sum counts
+// infinite logits, -inf where there is nothing. Else: the maximum and its token.
 struct Stats {
-    float max, sum;  // sum of exp((logit - max) / T)
-    int best;        // the maximum's token
+    float offset, sum;
+    int best;
     int pad;
 };
 
@@ -67,11 +73,10 @@ struct Stats {
 struct Ending {
     int row;             // the path's last row, or -1: an invalid sequence
     int node;            // the path's tokens but the last one
-    int fallback;        // the row's argmax where it has children, else 0
     int tried;           // tokens to leave out (no draft logits)
     float c;             // what rejections took (draft logits)
-    float max, inv_sum;  // of the target's row, where c > 0
-    float draft_max, draft_inv_sum;
+    float offset, inv_sum;  // of the target's row, where c > 0
+    float draft_offset, draft_inv_sum;
     int blocks;          // of launch 3 that are done
     uint64_t best;       // their best (score, token), as keys that compare as they do
     int token[kMaxNodes];
@@ -111,31 +116,24 @@ __device__ __forceinline__ int tree_rows(const VerifyArgs& a, int s, int* start)
     return first < 0 || end > a.rows || end <= first || int64_t(end) - first > a.max_nodes ? 0 : end - first;
 }
 
-// Eight logits of one row as its 16-byte chunk holds them: tokens t .. t + 7,
-// those outside [0, vocab) `none`.
-constexpr uint32_t kNaN = 0x7fc0, kMinusInf = 0xff80;
-__device__ __forceinline__ uint4 load_packed(const uint16_t* row, int64_t t, int vocab, uint32_t none) {
-    if (t >= 0 && t + 8 <= vocab) return nvr::load_stream(row + t);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t lo = t + 2 * i, hi = lo + 1;
-        w[i] = (lo >= 0 && lo < vocab ? uint32_t(row[lo]) : none) | (hi >= 0 && hi < vocab ? uint32_t(row[hi]) : none) << 16;
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// The same unpacked, NaN outside: it never wins and weighs nothing.
+// Eight logits of one row as its 16-byte chunk holds them: tokens t .. t + 7, NaN
+// for those outside [0, vocab): it never wins and weighs nothing.
 __device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t t, int vocab, float (&f)[8]) {
-    nvr::unpack8(load_packed(row, t, vocab, kNaN), f);
+    if (t >= 0 && t + 8 <= vocab) {
+        nvr::unpack8(nvr::load_stream(row + t), f);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = t + i >= 0 && t + i < vocab ? nvr::bf16_to_f32(row[t + i]) : __builtin_nanf("");
+    }
 }
 __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinterpret_cast<uintptr_t>(row) >> 1 & 7); }
 
-// exp((x - top) / T) with scale = log2(e) / T; 1 at an infinite maximum, 0 for NaN.
-__device__ __forceinline__ float weight(float x, float top, float scale) {
-    if (x == top) return 1.0f;
-    return x == x ? __builtin_amdgcn_exp2f((x - top) * scale) : 0.0f;
-}
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
+// A sum at one offset, at another that is no smaller.
+__device__ __forceinline__ float at_offset(float sum, float offset, float other) {
+    if (!(sum > 0.0f)) return 0.0f;
+    return offset == other ? sum : __builtin_ldexpf(sum, int(fmaxf(offset - other, -1000.0f)));
+}
 
 struct Best {
     float score;
@@ -186,19 +184,47 @@ __device__ __forceinline__ uint64_t inner_nodes(int parent) {
 // so that every block has as much to do whatever the tree. A row's parts are the
 // blocks that have some of it.
 struct Shares {
-    int64_t chunks, per;  // of a row; of a block
+    uint32_t chunks, per;  // of a row; of a block (64 rows of 2^26 tokens: 2^29)
     __device__ __forceinline__ Shares(int vocab, int rows, int blocks) {
-        chunks = row_chunks(vocab);
-        const int64_t all = chunks * rows;
-        per = max((all + blocks - 1) / blocks, int64_t(kShare));
+        chunks = uint32_t(row_chunks(vocab));
+        per = max((chunks * rows + blocks - 1) / blocks, uint32_t(kShare));
     }
-    __device__ __forceinline__ int first_block(int i) const { return int(uint64_t(i) * uint64_t(chunks) / uint64_t(per)); }
-    __device__ __forceinline__ int last_block(int i) const { return int((uint64_t(i + 1) * uint64_t(chunks) - 1) / uint64_t(per)); }
+    __device__ __forceinline__ int first_block(int i) const { return int(i * chunks / per); }
+    __device__ __forceinline__ int last_block(int i) const { return int(((i + 1) * chunks - 1) / per); }
 };
 
-// A block a (sequence, share, model): one pass over its chunks, each thread with a
-// maximum and a sum of its own that it scales again when the maximum grows.
-__global__ __launch_bounds__(kThreads, 8) void verify_stats(VerifyArgs a) {
+// A thread's chunks begin, begin + kThreads, ... < end of a row and one more value,
+// with their NaN, infinite and huge values looked at one by one.
+__device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int begin, int end, float edge, int vocab,
+                                            float scale, float* offset, float* sum) {
+    float top = fmaxf(edge * scale, -kInf);
+    for (int k = begin; k < end; k += kThreads) {
+        float f[8];
+        load_chunk(x, 8 * int64_t(k) - lead, vocab, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, f[j] * scale);
+    }
+    const float at = __builtin_rintf(top);
+    auto weight = [&](float v) {
+        if (top == kInf) return v * scale == kInf ? 1.0f : 0.0f;
+        return v == v ? __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -at)) : 0.0f;
+    };
+    float total = top > -kInf ? weight(edge) : 0.0f;
+    for (int k = begin; k < end && top > -kInf; k += kThreads) {
+        float f[8];
+        load_chunk(x, 8 * int64_t(k) - lead, vocab, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) total += weight(f[j]);
+    }
+    *offset = at;
+    *sum = total;
+}
+
+// A block a (sequence, share, model). T > 0: one pass with an offset near the
+// maximum of each thread's first loads; a sum that leaves fp32's range, or a NaN,
+// is taken again with care. Bound by the read of the logits and, at four
+// instructions and an exponential a token, nearly as much by its issue.
+__global__ __launch_bounds__(kThreads, 6) void verify_stats(VerifyArgs a) {
     constexpr int kWaves = kThreads / kWave;
     __shared__ float tops[kWaves], sums[kWaves];
     __shared__ int first;
@@ -215,98 +241,120 @@ __global__ __launch_bounds__(kThreads, 8) void verify_stats(VerifyArgs a) {
     int parent = lane > 0 && lane < n ? a.parents[start + lane] : -1;
     if (parent >= lane) parent = -1;
     uint64_t inner = inner_nodes(parent);
-    const int count = __popcll(inner);
+    const uint32_t count = uint32_t(__popcll(inner));
     const Shares shares(a.vocab, count, a.blocks);
-    int64_t at = block * shares.per;
-    const int64_t stop = min(at + shares.per, count * shares.chunks);
+    uint32_t at = block * shares.per;
+    const uint32_t stop = min(at + shares.per, count * shares.chunks);
     if (at >= stop) return;
     const float scale = kLog2e / temperature;
-    int i = int(uint64_t(at) / uint64_t(shares.chunks));
+    int i = int(at / shares.chunks);
     for (int skip = 0; skip < i; ++skip) inner &= inner - 1;
     for (; at < stop; ++i, inner &= inner - 1) {
         const int row = start + __builtin_ctzll(inner);
         const uint16_t* x = (side ? a.draft : a.logits) + int64_t(row) * a.vocab;
         const int lead = lead_of(x);
-        const int64_t base = i * shares.chunks;
+        const uint32_t base = i * shares.chunks;
         const int begin = int(at - base), end = int(min(stop - base, shares.chunks));
         at = base + end;
-        float top = -kInf, sum = 0.0f;
-        int where = -1;  // the chunk from which `top` is
-        for (int k = begin + int(threadIdx.x); k < end; k += kLoads * kThreads) {
-            uint4 packed[kLoads];
+        // Whole chunks, and at either end of a row the tokens of one that is not: one each of the first 16 threads'.
+        const int whole = (a.vocab + lead) / 8, lo = max(begin, lead != 0 ? 1 : 0), hi = min(end, whole);
+        const int lone = threadIdx.x < 8 ? (begin == 0 && lead != 0 ? int(threadIdx.x) - lead : -1)
+                                         : begin <= whole && end > whole && threadIdx.x < 16 ? 8 * whole - lead + int(threadIdx.x) - 8 : -1;
+        float edge = -kInf;
+        if (lone >= 0 && lone < a.vocab) edge = nvr::bf16_to_f32(x[lone]);
+        auto load = [&](int k, uint4 (&packed)[kLoads]) {
 #pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                const int c = k + u * kThreads;
-                packed[u] = load_packed(x, c < end ? 8 * int64_t(c) - lead : int64_t(a.vocab), a.vocab, kMinusInf);
-            }
-            float high = __builtin_nanf("");
+            for (int u = 0; u < kLoads; ++u) packed[u] = nvr::load_stream(x + 8 * int64_t(min(k + u * kThreads, hi - 1)) - lead);
+        };
+        auto loaded = [&](int c, const uint4& packed, float (&f)[8]) {
+            const uint32_t none = 0xff80ff80u;  // -inf: weighs nothing
+            const bool in = c < hi;
+            nvr::unpack8(make_uint4(in ? packed.x : none, in ? packed.y : none, in ? packed.z : none, in ? packed.w : none), f);
+        };
+        auto highest = [&](int k, const uint4 (&packed)[kLoads]) {
+            float high = -kInf;
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) {
                 float f[8];
-                nvr::unpack8(packed[u], f);
+                loaded(k + u * kThreads, packed[u], f);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) high = fmaxf(high, f[j]);  // passes over NaN
             }
-            if (high > top || (high == top && where < 0)) {
-                if (sum > 0.0f) sum *= __builtin_amdgcn_exp2f((top - high) * scale);
-                top = high;
-                where = k;
-            }
-            if (sampled && top > -kInf) {
+            return high;
+        };
+        const int begin_k = lo + int(threadIdx.x);
+        uint4 packed[kLoads];
+        if (begin_k < hi) load(begin_k, packed);
+        Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
+        int where = -2;  // the chunk whose load has the maximum; -1: the edge
+        if (sampled) {
+            float high = edge;
+            if (begin_k < hi) high = fmaxf(high, highest(begin_k, packed));
+            high *= scale;
+            mine.offset = fabsf(high) < kInf ? __builtin_rintf(high) : 0.0f;
+            mine.sum = __builtin_amdgcn_exp2f(__builtin_fmaf(edge, scale, -mine.offset));
+            for (int k = begin_k; k < hi;) {
 #pragma unroll
                 for (int u = 0; u < kLoads; ++u) {
                     float f[8], eight = 0.0f;
-                    nvr::unpack8(packed[u], f);
+                    loaded(k + u * kThreads, packed[u], f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f((f[j] - top) * scale);
-                    sum += eight;
+                    for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], scale, -mine.offset));
+                    mine.sum += eight;
                 }
+                k += kLoads * kThreads;
+                if (k < hi) load(k, packed);
+            }
+            if (!(mine.sum < 0x1p100f)) careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &mine.offset, &mine.sum);
+            if (!(mine.sum > 0.0f)) mine.offset = -kInf;
+        } else {
+            if (edge == edge && lone >= 0 && lone < a.vocab) { mine.offset = edge; where = -1; }
+            for (int k = begin_k; k < hi;) {
+                const float high = highest(k, packed);
+                if (high > mine.offset || (where < 0 && high == mine.offset)) {
+                    mine.offset = high;
+                    where = k;
+                }
+                k += kLoads * kThreads;
+                if (k < hi) load(k, packed);
             }
         }
-        if (!(sum < kInf)) {  // a NaN among the logits, or an infinite maximum
-            sum = 0.0f;
-            for (int k = begin + int(threadIdx.x); k < end; k += kThreads) {
-                float f[8];
-                load_chunk(x, 8 * int64_t(k) - lead, a.vocab, f);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) sum += weight(f[j], top, scale);
-            }
-        }
-        const float high = wave_max(top);
+        const float high = wave_max(mine.offset);
         if (lane == 0) tops[wave] = high;
         if (threadIdx.x == 0) first = nvr::kNoIndex;
         __syncthreads();
         float all = tops[0];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) all = fmaxf(all, tops[w]);
-        if (top == all && where >= 0) {
-            int lowest = nvr::kNoIndex;
+        if (where > -2 && mine.offset == all) {
+            // The lowest of this thread's tokens with that logit.
+            int lowest = lone >= 0 && lone < a.vocab && edge == all ? lone : nvr::kNoIndex;
 #pragma unroll 1
             for (int u = kLoads - 1; u >= 0; --u) {
                 const int c = where + u * kThreads;
-                if (c >= end) continue;
+                if (where < 0 || c >= hi) continue;
                 float f[8];
                 load_chunk(x, 8 * int64_t(c) - lead, a.vocab, f);
 #pragma unroll
                 for (int j = 7; j >= 0; --j)
-                    if (f[j] == all) lowest = int(8 * int64_t(c) - lead) + j;
+                    if (f[j] == all) lowest = min(lowest, int(8 * int64_t(c) - lead) + j);
             }
             atomicMin(&first, lowest);
         }
-        sum = wave_sum(sum > 0.0f ? sum * weight(top, all, scale) : 0.0f);
+        const float sum = wave_sum(at_offset(mine.sum, mine.offset, all));
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         if (threadIdx.x == 0) {
-            sum = 0.0f;
+            float total = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += sums[w];
-            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + block - shares.first_block(i)] = Stats{all, sum, first, 0};
+            for (int w = 0; w < kWaves; ++w) total += sums[w];
+            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + block - shares.first_block(i)] = Stats{all, total, first, 0};
         }
     }
 }
 
-// A row's partitions folded, by one lane: a wave folds every node of a tree at once.
-__device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale) {
+// A row's parts folded, by one lane: a wave folds every node of a tree at once.
+__device__ __forceinline__ Stats fold(const Stats* part, int parts) {
     constexpr int kBatch = 8;
     Best b{-kInf, nvr::kNoIndex};
     for (int i0 = 0; i0 < parts; i0 += kBatch) {
@@ -314,7 +362,7 @@ __device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale)
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u) consider(b, t[u].max, t[u].best);
+        for (int u = 0; u < kBatch; ++u) consider(b, t[u].offset, t[u].best);
     }
     double sum = 0.0;
     for (int i0 = 0; i0 < parts; i0 += kBatch) {
@@ -323,7 +371,7 @@ __device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale)
         for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
-            if (i0 + u < parts && t[u].max > -kInf) sum += double(t[u].sum * weight(t[u].max, b.score, scale));
+            if (i0 + u < parts) sum += double(at_offset(t[u].sum, t[u].offset, b.score));
     }
     return Stats{b.score, float(sum), b.index, 0};
 }
@@ -332,7 +380,7 @@ __device__ __forceinline__ Stats fold(const Stats* part, int parts, float scale)
 struct Rows {
     const uint16_t* target;
     const uint16_t* draft;
-    float max, inv_sum, draft_max, draft_inv_sum;
+    float offset, inv_sum, draft_offset, draft_inv_sum;
 };
 
 // p - c q of one token; NaN where p is.
@@ -341,12 +389,14 @@ struct RestTerm {
     float scale, cq;
     bool infinite;
     __device__ __forceinline__ RestTerm(const Rows& rows, float c, float s)
-        : r(rows), scale(s), cq(c * rows.draft_inv_sum), infinite(!(fabsf(rows.max) < kInf) || !(fabsf(rows.draft_max) < kInf)) {}
+        : r(rows), scale(s), cq(c * rows.draft_inv_sum), infinite(rows.offset == kInf || rows.draft_offset == kInf) {}
+    __device__ __forceinline__ float weight(float x, float offset) const {
+        if (infinite && offset == kInf) return x * scale == kInf ? 1.0f : 0.0f;
+        return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -offset));
+    }
     __device__ __forceinline__ float operator()(float x, float y) const {
-        if (infinite) return weight(x, r.max, scale) * r.inv_sum - weight(y, r.draft_max, scale) * cq;
-        const float wx = __builtin_amdgcn_exp2f((x - r.max) * scale);
-        const float wy = fmaxf(__builtin_amdgcn_exp2f((y - r.draft_max) * scale), 0.0f);  // a NaN is no token of q
-        return __builtin_fmaf(wx, r.inv_sum, -(wy * cq));
+        const float wy = fmaxf(weight(y, r.draft_offset), 0.0f);  // a NaN is no token of q
+        return __builtin_fmaf(weight(x, r.offset), r.inv_sum, -(wy * cq));
     }
 };
 
@@ -447,18 +497,20 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         const Shares shares(a.vocab, __popcll(inner), a.blocks);
         const int i = __popcll(inner & ((uint64_t(1) << lane) - 1));
         (wave ? draft : target)[lane] = fold((wave ? a.draft_stats : a.stats) + int64_t(start + lane) * a.parts,
-                                             shares.last_block(i) - shares.first_block(i) + 1, scale);
+                                             shares.last_block(i) - shares.first_block(i) + 1);
     }
     __syncthreads();
     auto rows_of = [&](int v) {
         const int64_t at = int64_t(start + v) * a.vocab;
-        return Rows{a.logits + at, a.draft + at, target[v].max, inverse(target[v].sum), draft[v].max, inverse(draft[v].sum)};
+        const Stats t = target[v], d = draft[v];
+        return Rows{a.logits + at, a.draft + at, t.sum > 0.0f ? t.offset : 0.0f, inverse(t.sum), d.sum > 0.0f ? d.offset : 0.0f,
+                    inverse(d.sum)};
     };
-    // Each node's probabilities under its parent's rows: 2^y with y = k + f, |f| <= 1/2, in fp64 but for 2^f.
+    // Each node's probabilities under its parent's rows: 2^y, y = k + f, |f| <= 1/2, in fp64 but for 2^f.
     auto chance = [&](float x, const Stats& r) -> double {
-        if (!(r.max > -kInf) || x != x) return 0.0;
-        if (x == r.max) return 1.0 / double(r.sum);
-        const double y = (double(x) - double(r.max)) * 1.4426950408889634 / double(temperature), k = rint(y);
+        if (!(r.sum > 0.0f) || x != x) return 0.0;
+        if (r.offset == kInf) return x * scale == kInf ? 1.0 / double(r.sum) : 0.0;
+        const double y = double(x) * double(scale) - double(r.offset), k = rint(y);
         return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
     };
     double p = 0.0, q = 0.0;
@@ -569,21 +621,19 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         const bool out = (rejected >> lane & 1) != 0;
         const uint64_t all = __ballot(out);
         if (out) ending->token[__popcll(all & ((uint64_t(1) << lane) - 1))] = token;
-        const bool folded = (inner >> v & 1) != 0;
         if (lane == 0) {
             a.out_counts[s] = length;
             ending->row = start + v;
             ending->node = length - 1;
             ending->tried = __popcll(all);
             ending->c = float(c);
-            ending->fallback = folded && target[v].best != nvr::kNoIndex ? target[v].best : 0;
             ending->blocks = 0;
             ending->best = 0;
             if (c > 0.0) {
                 const Rows r = rows_of(v);
-                ending->max = r.max;
+                ending->offset = r.offset;
                 ending->inv_sum = r.inv_sum;
-                ending->draft_max = r.draft_max;
+                ending->draft_offset = r.draft_offset;
                 ending->draft_inv_sum = r.draft_inv_sum;
             }
         }
@@ -625,7 +675,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
     } else {
         if (c > 0.0f) {  // ln(p - c q) in place of the logits
-            const Rows r{x, a.draft + int64_t(row) * a.vocab, e->max, e->inv_sum, e->draft_max, e->draft_inv_sum};
+            const Rows r{x, a.draft + int64_t(row) * a.vocab, e->offset, e->inv_sum, e->draft_offset, e->draft_inv_sum};
             const RestTerm term(r, c, kLog2e / temperature);
             float y[8];
             if (lead_of(r.draft) == lead_of(x)) {
@@ -681,19 +731,37 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
             if (i != own && bound[i] >= reach) consider(b, score(f[i], us[i]), int(t) + i);
         if (b.score == -kInf && (count > 0 || c > 0.0f)) b.index = nvr::kNoIndex;  // the rest is nothing here
     }
-    b = wave_best(b);
-    if (lane == 0) tops[wave] = b;
-    __syncthreads();
-    if (threadIdx.x == 0) {
+    auto block_best = [&] {  // in thread 0
+        b = wave_best(b);
+        if (lane == 0) tops[wave] = b;
+        __syncthreads();
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) consider(b, tops[w].score, tops[w].index);
+    };
+    __shared__ bool nothing;
+    block_best();
+    if (threadIdx.x == 0) {
+        nothing = false;
         const uint64_t old = __hip_atomic_fetch_max(&e->best, key_of(b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("" ::"v"(old));  // the returning form
         if (arrive(&e->blocks) == parts - 1) {
             const uint64_t key = __hip_atomic_load(&e->best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            a.out_tokens[int64_t(s) * a.max_nodes + e->node] = key == 0 ? e->fallback : int(~uint32_t(key));
+            if (key != 0) a.out_tokens[int64_t(s) * a.max_nodes + e->node] = int(~uint32_t(key));
+            else nothing = true;
         }
     }
+    __syncthreads();
+    if (!nothing) return;
+    // Nothing is left: the row's argmax, or 0 where that is nothing either.
+    b = Best{-kInf, nvr::kNoIndex};
+    for (int64_t k = threadIdx.x; k < row_chunks(a.vocab); k += kThreads) {
+        const int64_t t = 8 * k - lead_of(x);
+        load_chunk(x, t, a.vocab, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
+    }
+    block_best();
+    if (threadIdx.x == 0) a.out_tokens[int64_t(s) * a.max_nodes + e->node] = b.index == nvr::kNoIndex ? 0 : b.index;
 }
 
 // The workspace's parts, each at a multiple of 16 bytes.
@@ -733,8 +801,8 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
         return nvr::fail(-2, "verify_tree: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     if (!nvr::aligned(workspace, 16)) return nvr::fail(-2, "verify_tree: the workspace needs 16-byte alignment");
     const int sampled = sample_blocks(vocab);
-    if (sampled > 65535)  // blocks of a grid dimension
-        return nvr::fail(-2, "verify_tree: %d tokens exceed one launch", vocab);
+    if (vocab > kMaxVocab)
+        return nvr::fail(-2, "verify_tree: vocab %d above %d", vocab, kMaxVocab);
     // Eight blocks a CU in all, so that none has to wait for another's end.
     const int sides = draft_logits ? 2 : 1;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256;
