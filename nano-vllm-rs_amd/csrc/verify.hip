@@ -37,9 +37,9 @@
 // Launches: 1. verify_stats: for each row that has children, the sum of the
 // exponentials (T > 0; both models') or the argmax, by shares of the rows.
 // 2. verify_walk: a block a sequence folds them and walks the tree; with draft
-// logits several blocks a sequence first sum max(p - q, 0), which the second child
-// of a node needs, and the last of them walks. 3. verify_sample: partitions of
-// the last rows; the last block of a sequence stores the token.
+// logits several blocks a sequence, in two launches, first sum the rests that the
+// second and third child of a node need. 3. verify_sample: partitions of the last
+// rows; the last block of a sequence stores the token.
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
@@ -55,7 +55,7 @@ constexpr int kThreads = 256;
 constexpr int kLoads = 4;             // 16-byte loads in flight a thread of launch 1
 constexpr int kShare = kLoads * kThreads;  // 16-byte chunks a block of launch 1, at least
 constexpr int kSampled = kThreads * 8;               // tokens a block of launch 3
-constexpr int kSlices = 16;                          // blocks a sequence of launch 2, with draft logits
+constexpr int kSlices = 16;                          // blocks a sequence of the walk, with draft logits
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 constexpr float kInf = __builtin_inff();
 
@@ -97,11 +97,10 @@ struct VerifyArgs {
     Stats* stats;        // [rows, parts]
     Stats* draft_stats;  // [rows, parts]
     Ending* endings;     // [batch]
-    double* rests;       // [rows, kSlices]: of sum max(p - q, 0)
-    int* arrived;        // [batch]: blocks of launch 2 that are done
+    double* rests;       // [2][rows, kSlices]: of the sums of the rests after one and two rejections
+    int* arrived;        // [batch]: blocks of the walk that are done
     int rows, batch, max_nodes, vocab;
     int parts, blocks;  // stats a row has room for; blocks a sequence and model of launch 1
-    int slices;         // blocks a sequence of launch 2
 };
 
 // 16-byte chunks that may hold tokens of a row: its first may lie up to 7 tokens behind a boundary.
@@ -401,9 +400,9 @@ struct RestTerm {
 };
 
 // sum of max(p - c q, 0) over 16-byte chunks [first, end) of a row, this thread's share.
+template <int kBatch>  // chunks in flight a thread
 __device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, float scale, int64_t first, int64_t end,
                                            int threads) {
-    constexpr int kBatch = 4;
     const int lead = lead_of(r.target);
     const bool alike = lead == lead_of(r.draft);
     const RestTerm term(r, c, scale);
@@ -412,7 +411,7 @@ __device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, fl
         float x[kBatch][8], y[kBatch][8];
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int64_t t = k + u * threads < end ? 8 * (k + u * threads) - lead : int64_t(vocab);
+            const int64_t t = 8 * min(k + u * threads, end - 1) - lead;
             load_chunk(r.target, t, vocab, x[u]);
             if (alike) {
                 load_chunk(r.draft, t, vocab, y[u]);
@@ -422,12 +421,13 @@ __device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, fl
                     y[u][i] = t + i >= 0 && t + i < vocab ? nvr::bf16_to_f32(r.draft[t + i]) : __builtin_nanf("");
             }
         }
-        float part = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kBatch; ++u)
+        for (int u = 0; u < kBatch; ++u) {
+            float eight = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) part += fmaxf(term(x[u][i], y[u][i]), 0.0f);
-        sum += double(part);
+            for (int i = 0; i < 8; ++i) eight += fmaxf(term(x[u][i], y[u][i]), 0.0f);
+            sum += k + u * threads < end ? double(eight) : 0.0;
+        }
     }
     return sum;
 }
@@ -452,21 +452,41 @@ __device__ __forceinline__ int arrive(int* count) {
 constexpr int kWalkThreads = 512;
 constexpr int kWalkWaves = kWalkThreads / kWave;
 
-// a.slices blocks a sequence.
+// A lane's value, for every lane.
+__device__ __forceinline__ double lane_value(double v, int i) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits)), i)), hi = uint32_t(__builtin_amdgcn_readlane(int(uint32_t(bits >> 32)), i));
+    return __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+
+// A child's trial against the rest max(p - c q, 0), whose sum is z.
+__device__ __forceinline__ bool accepted(double p, double q, double u, double c, double z) {
+    const double rest = fmax(p - c * q, 0.0);
+    return rest > 0.0 && u * z * q < rest;
+}
+
+// The walk, kSlices blocks a sequence where there are draft logits, else one. A
+// node's second child needs the sum of the rest after one rejection, its third
+// that after two: a pass over the vocabulary, which one block does at the rate
+// of one CU (50257 tokens 7 us). So with draft logits a first launch (kFirst)
+// sums, slice by slice, the first rests that the walk may come to need, and the
+// second launch the second rests; there the last block of a sequence to finish
+// walks. Later rests are summed during the walk.
+template <bool kFirst>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ Stats target[kMaxNodes], draft[kMaxNodes];
-    __shared__ double parts[kMaxNodes][kWalkWaves], rests[kMaxNodes];
+    __shared__ double parts[kMaxNodes][kWalkWaves], rests[2][kMaxNodes];
     __shared__ int path[kMaxNodes];
     __shared__ int last;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int s = int(blockIdx.x), slice = int(blockIdx.y);
+    const int s = int(blockIdx.x), slice = int(blockIdx.y), slices = int(gridDim.y);
     Ending* ending = a.endings + s;
     int start;
     const int n = tree_rows(a, s, &start);
     int* tokens = a.out_tokens + int64_t(s) * a.max_nodes;
     int* nodes = a.out_nodes + int64_t(s) * a.max_nodes;
     if (n == 0) {
-        if (slice != 0) return;
+        if (kFirst || slice != 0) return;
         for (int i = int(threadIdx.x); i < a.max_nodes; i += kWalkThreads) tokens[i] = nodes[i] = -1;
         if (threadIdx.x == 0) { a.out_counts[s] = 0; ending->row = -1; }
         return;
@@ -478,13 +498,13 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     const bool mine = lane > 0 && lane < n;
     int parent = mine ? a.parents[start + lane] : -1;
     const int token = mine ? a.tokens[start + lane] : -1;
-    const float u = mine ? a.uniforms[start + lane] : 0.0f;
+    const double u = mine ? double(a.uniforms[start + lane]) : 0.0;
     if (parent < 0 || parent >= lane) parent = -1;
     const bool known = parent >= 0 && token >= 0 && token < a.vocab;
     const uint64_t inner = inner_nodes(parent);
-    // Only a node with a second child to try needs more than one block.
+    // Rests are summed only where a node has a second child to try.
     const bool alone = !drafted || __popcll(__ballot(known)) == __popcll(inner_nodes(known ? parent : -1));
-    if (alone && slice != 0) return;
+    if (alone && (kFirst || slice != 0)) return;
     // The logits of each node's token, under its parent.
     float xt = 0.0f, xd = 0.0f;
     if (sampled && known) {
@@ -492,8 +512,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         xt = nvr::bf16_to_f32(a.logits[at]);
         if (drafted) xd = nvr::bf16_to_f32(a.draft[at]);
     }
-    if (wave < (drafted ? 2 : 1) && (inner >> lane & 1) != 0)
-{
+    if (wave < (drafted ? 2 : 1) && (inner >> lane & 1) != 0) {
         const Shares shares(a.vocab, __popcll(inner), a.blocks);
         const int i = __popcll(inner & ((uint64_t(1) << lane) - 1));
         (wave ? draft : target)[lane] = fold((wave ? a.draft_stats : a.stats) + int64_t(start + lane) * a.parts,
@@ -518,53 +537,72 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         p = chance(xt, target[parent]);
         if (drafted) q = chance(xd, draft[parent]);
     }
-    // Nodes that the walk may come to, have it reject a first child and try a second: those need the first rest's sum.
-    uint64_t several = 0;
-    if (!alone) {
-        uint64_t open = 1;
-        for (int v = 0; v < n - 1; ++v) {
-            uint64_t children = __ballot(known && parent == v);
-            if (children == 0 || (open >> v & 1) == 0) continue;
-            const int i = __builtin_ctzll(children);
-            const double px = __shfl(p, i);
-            if (px > 0.0 && double(__shfl(u, i)) * __shfl(q, i) < px) {
-                open |= uint64_t(1) << i;  // surely the next
-            } else {
-                children &= children - 1;
-                open |= children;
-                several |= uint64_t(children != 0) << v;
-            }
-        }
-        if (several == 0 && slice != 0) return;
-    }
     const int64_t chunks = row_chunks(a.vocab);
-    if (several != 0) {
-        // This block's share of the rests after one rejection; the last block of the sequence goes on.
-        const int64_t share = (chunks + a.slices - 1) / a.slices, begin = slice * share;
-        for (uint64_t left = several; left != 0; left &= left - 1) {
+    // This block's share of the sums of the nodes' rests, for all slices to see.
+    auto sum_rests = [&](uint64_t which, double* to, auto taken) {
+        const int64_t share = (chunks + slices - 1) / slices, begin = slice * share;
+        for (uint64_t left = which; left != 0; left &= left - 1) {
             const int v = __builtin_ctzll(left);
-            const double sum = wave_sum(rest_sum(rows_of(v), a.vocab, 1.0f, scale, begin, min(chunks, begin + share), kWalkThreads));
+            const double sum = wave_sum(rest_sum<1>(rows_of(v), a.vocab, taken(v), scale, begin, min(chunks, begin + share), kWalkThreads));
             if (lane == 0) parts[v][wave] = sum;
         }
         __syncthreads();
-        if (threadIdx.x < kMaxNodes && (several >> threadIdx.x & 1) != 0) {
+        if (threadIdx.x < kMaxNodes && (which >> threadIdx.x & 1) != 0) {
             double sum = 0.0;
             for (int w = 0; w < kWalkWaves; ++w) sum += parts[threadIdx.x][w];
-            publish(a.rests + int64_t(start + threadIdx.x) * kSlices + slice, sum);
+            publish(to + int64_t(start + threadIdx.x) * kSlices + slice, sum);
         }
-        __syncthreads();
-        if (threadIdx.x == 0) last = arrive(a.arrived + s) == a.slices - 1;
-        __syncthreads();
-        if (!last) return;
-        if (threadIdx.x < kMaxNodes && (several >> threadIdx.x & 1) != 0) {
+    };
+    auto read_rests = [&](uint64_t which, const double* from, double* to) {
+        if (threadIdx.x < kMaxNodes && (which >> threadIdx.x & 1) != 0) {
             double sum = 0.0;
-            for (int w = 0; w < a.slices; ++w)
-                sum += __hip_atomic_load(a.rests + int64_t(start + threadIdx.x) * kSlices + w, __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-            rests[threadIdx.x] = sum;
+            for (int w = 0; w < slices; ++w)
+                sum += __hip_atomic_load(from + int64_t(start + threadIdx.x) * kSlices + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            to[threadIdx.x] = sum;
         }
         __syncthreads();
+    };
+    // Nodes that the walk may come to (open) and have it reject a first child and try a second: those need the first
+    // rest's sum; and those where it rejects a second and tries a third, the second's.
+    uint64_t once = 0, twice = 0;
+    if (!alone) {
+        auto look = [&](bool second) {
+            uint64_t open = 1, found = 0;
+            for (int v = 0; v < n - 1; ++v) {
+                uint64_t children = __ballot(known && parent == v);
+                if (children == 0 || (open >> v & 1) == 0) continue;
+                int i = __builtin_ctzll(children);
+                bool taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 0.0, 1.0);
+                if (!taken && second && (children & (children - 1)) != 0) {
+                    children &= children - 1;
+                    i = __builtin_ctzll(children);
+                    taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 1.0, rests[0][v]);
+                }
+                children &= children - 1;
+                open |= taken ? uint64_t(1) << i : children;
+                // (children: none left where there was no second)
+                if (!taken && children != 0 && (second ? (once >> v & 1) != 0 : true)) found |= uint64_t(1) << v;
+            }
+            return found;
+        };
+        once = look(false);
+        if constexpr (kFirst) {
+            if (once != 0) sum_rests(once, a.rests, [](int) { return 1.0f; });
+            return;
+        }
+        read_rests(once, a.rests, rests[0]);
+        twice = look(true);
+        if (twice == 0 && slice != 0) return;
+        if (twice != 0) {
+            sum_rests(twice, a.rests + int64_t(a.rows) * kSlices, [&](int v) { return float(1.0 + rests[0][v]); });
+            __syncthreads();
+            if (threadIdx.x == 0) last = arrive(a.arrived + s) == slices - 1;
+            __syncthreads();
+            if (!last) return;
+            read_rests(twice, a.rests + int64_t(a.rows) * kSlices, rests[1]);
+        }
     }
+    if constexpr (kFirst) return;
     // Every wave walks alike.
     int v = 0, length = 0;
     double c = 0.0, z = 1.0;
@@ -576,7 +614,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         const int best = children != 0 && target[v].best != nvr::kNoIndex ? target[v].best : 0;
         c = 0.0; z = 1.0; rejected = 0;
         int next = -1;
-        while (children != 0) {
+        for (int tried = 0; children != 0; ++tried) {
             const int i = __builtin_ctzll(children);
             children &= children - 1;
             const int x = __builtin_amdgcn_readlane(token, i);
@@ -584,17 +622,15 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
                 if (x == best) { next = i; break; }
                 continue;
             }
-            const double px = __shfl(p, i), ux = double(__shfl(u, i));
+            const double px = lane_value(p, i), ux = lane_value(u, i);
             if (drafted) {
-                const double qx = __shfl(q, i), r = fmax(px - c * qx, 0.0);
-                if (r > 0.0 && ux * z * qx < r) { next = i; break; }
-                const bool once = c == 0.0;
+                if (accepted(px, lane_value(q, i), ux, c, z)) { next = i; break; }
                 c += z;
                 if (children == 0) break;
-                if (once) {
-                    z = rests[v];
+                if (tried < 2) {
+                    z = rests[tried][v];
                 } else {
-                    const double sum = wave_sum(rest_sum(rows_of(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
+                    const double sum = wave_sum(rest_sum<4>(rows_of(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
                     if (lane == 0) parts[0][wave] = sum;
                     __syncthreads();
                     z = 0.0;
@@ -776,7 +812,7 @@ Workspace layout(int rows, int batch, int vocab) {
     w.draft_stats = w.stats + up(int64_t(sizeof(Stats)) * rows * parts);
     w.endings = w.draft_stats + up(int64_t(sizeof(Stats)) * rows * parts);
     w.rests = w.endings + up(int64_t(sizeof(Ending)) * batch);
-    w.arrived = w.rests + up(int64_t(sizeof(double)) * kSlices * rows);
+    w.arrived = w.rests + up(2 * int64_t(sizeof(double)) * kSlices * rows);
     w.bytes = w.arrived + up(int64_t(sizeof(int)) * batch);
     return w;
 }
@@ -817,11 +853,15 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
                        static_cast<int*>(out_tokens), static_cast<int*>(out_nodes), static_cast<int*>(out_counts),
                        reinterpret_cast<Stats*>(base + w.stats), reinterpret_cast<Stats*>(base + w.draft_stats),
                        reinterpret_cast<Ending*>(base + w.endings), reinterpret_cast<double*>(base + w.rests),
-                       reinterpret_cast<int*>(base + w.arrived), rows, batch, max_nodes, vocab, most_parts(vocab), blocks,
-                       draft_logits && max_nodes > 2 ? kSlices : 1};
+                       reinterpret_cast<int*>(base + w.arrived), rows, batch, max_nodes, vocab, most_parts(vocab), blocks};
     hipLaunchKernelGGL(verify_stats, dim3(unsigned(int64_t(batch) * blocks * sides)), dim3(kThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(verify_walk, dim3(unsigned(batch), unsigned(a.slices)), dim3(kWalkThreads), 0, c->stream, a);
+    const dim3 walk(unsigned(batch), unsigned(draft_logits && max_nodes > 2 ? kSlices : 1));
+    if (walk.y > 1) {
+        hipLaunchKernelGGL(verify_walk<true>, walk, dim3(kWalkThreads), 0, c->stream, a);
+        NVR_HIP(hipGetLastError());
+    }
+    hipLaunchKernelGGL(verify_walk<false>, walk, dim3(kWalkThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
     hipLaunchKernelGGL(verify_sample, dim3(unsigned(batch), unsigned(sampled)), dim3(kThreads), 0, c->stream, a);
     return nvr::launch_status();
