@@ -60,16 +60,14 @@ __global__ __launch_bounds__(256) void copy_blocks(Chunk* __restrict__ kc, Chunk
 // source, and a thread that takes one column of the slots through all moves,
 // reading kBatch of them before it writes, needs no second buffer.
 template <typename Chunk>
-__global__ __launch_bounds__(128) void compact(Chunk* __restrict__ kc, Chunk* __restrict__ vc,
+__global__ __launch_bounds__(256) void compact(Chunk* __restrict__ kc, Chunk* __restrict__ vc,
                                                const int* __restrict__ contexts, const int* __restrict__ nodes,
                                                const int* __restrict__ counts, const int* __restrict__ tables,
-                                               int batch, int max_nodes, int bs, int blocks, int stride,
-                                               int64_t slot_chunks) {
+                                               int max_nodes, int bs, int blocks, int stride, int64_t slot_chunks) {
     constexpr int kBatch = 8;
     __shared__ int64_t from[kMaxNodes], to[kMaxNodes];
     __shared__ int moves;
-    const int s = int(blockIdx.x % unsigned(batch));
-    const int64_t plane = blockIdx.x / unsigned(batch);
+    const int s = int(blockIdx.x);
     if (threadIdx.x < kWave) {
         const int j = int(threadIdx.x), count = counts[s], context = contexts[s];
         const bool named = j < max_nodes && j < count;
@@ -81,8 +79,8 @@ __global__ __launch_bounds__(128) void compact(Chunk* __restrict__ kc, Chunk* __
         const int valid = context < 0 || count > max_nodes ? 0 : bads == 0 ? kWave : __builtin_ctzll(bads);
         auto slot = [&](int64_t pos) -> int64_t {
             if (pos >= int64_t(stride) * bs) return -1;
-            const int entry = tables[int64_t(s) * stride + pos / bs];
-            return entry >= 0 && entry < blocks ? int64_t(entry) * bs + pos % bs : int64_t(-1);
+            const int entry = tables[int64_t(s) * stride + uint32_t(pos) / uint32_t(bs)];
+            return entry >= 0 && entry < blocks ? int64_t(entry) * bs + uint32_t(pos) % uint32_t(bs) : int64_t(-1);
         };
         int64_t a = -1, b = -1;
         if (j < valid && node != j) {
@@ -97,8 +95,10 @@ __global__ __launch_bounds__(128) void compact(Chunk* __restrict__ kc, Chunk* __
     }
     __syncthreads();
     if (moves == 0) return;
-    Chunk* cache = (plane & 1 ? vc : kc) + (plane >> 1) * blocks * bs * slot_chunks;
-    for (int64_t column = threadIdx.x; column < slot_chunks; column += 128) {
+    // Each half of the block takes K or V of one layer.
+    const int64_t layer = blockIdx.y;
+    Chunk* cache = (threadIdx.x & 128 ? vc : kc) + layer * blocks * bs * slot_chunks;
+    for (int64_t column = threadIdx.x & 127; column < slot_chunks; column += 128) {
         for (int j0 = 0; j0 < moves; j0 += kBatch) {
             Chunk v[kBatch];
 #pragma unroll
@@ -153,17 +153,16 @@ int nv_kv_compact(nv_context* c, void* kc, void* vc, const void* contexts, const
         return nvr::fail(-2, "kv_compact: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     const int64_t width = int64_t(kvh) * dim;
     if (width > 0x7fffffff) return nvr::fail(-2, "kv_compact: kvh * dim exceeds int32");
-    if (int64_t(batch) * 2 * layers > 0x7fffffff)
-        return nvr::fail(-2, "kv_compact: %d sequences in %d layers exceed one launch", batch, layers);
+    if (layers > 65535) return nvr::fail(-2, "kv_compact: %d layers exceed one launch", layers);
     auto x = static_cast<const int*>(contexts), n = static_cast<const int*>(nodes);
     auto k = static_cast<const int*>(counts), t = static_cast<const int*>(tables);
-    const dim3 grid(unsigned(int64_t(batch) * 2 * layers));
+    const dim3 grid{unsigned(batch), unsigned(layers)};
     if (chunked(kc, vc, width))
-        hipLaunchKernelGGL(compact<uint4>, grid, dim3(128), 0, c->stream, static_cast<uint4*>(kc),
-                           static_cast<uint4*>(vc), x, n, k, t, batch, max_nodes, bs, blocks, stride, width / 8);
+        hipLaunchKernelGGL(compact<uint4>, grid, dim3(256), 0, c->stream, static_cast<uint4*>(kc),
+                           static_cast<uint4*>(vc), x, n, k, t, max_nodes, bs, blocks, stride, width / 8);
     else
-        hipLaunchKernelGGL(compact<uint16_t>, grid, dim3(128), 0, c->stream, static_cast<uint16_t*>(kc),
-                           static_cast<uint16_t*>(vc), x, n, k, t, batch, max_nodes, bs, blocks, stride, width);
+        hipLaunchKernelGGL(compact<uint16_t>, grid, dim3(256), 0, c->stream, static_cast<uint16_t*>(kc),
+                           static_cast<uint16_t*>(vc), x, n, k, t, max_nodes, bs, blocks, stride, width);
     return nvr::launch_status();
 }
 
