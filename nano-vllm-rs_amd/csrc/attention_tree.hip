@@ -152,28 +152,28 @@ __device__ __forceinline__ void wait_copies() {
 
 constexpr int kPage = 16;  // positions that lie together in the cache: block sizes are multiples
 
-// Compile-time geometry. DIM: head dim rounded up; QT: tiles of 16 query rows a
-// wave; WQ of the block's four waves hold query rows of their own, the other
+// Compile-time geometry. DIM: head dim rounded up; W: waves; QT: tiles of 16
+// query rows a wave; WQ of the waves hold query rows of their own, the other
 // factor WK splits each tile's T positions; NS: tiles in LDS.
-template <int DIM_, int QT_, int WQ_, int T_, int NS_>
+template <int DIM_, int W_, int QT_, int WQ_, int T_, int NS_>
 struct Shape {
-    static constexpr int DIM = DIM_, QT = QT_, WQ = WQ_, WK = 4 / WQ_, T = T_, NS = NS_;
+    static constexpr int DIM = DIM_, W = W_, QT = QT_, WQ = WQ_, WK = W_ / WQ_, T = T_, NS = NS_;
     static constexpr int KW = T / WK;                // a wave's positions of a tile
     static constexpr int KT = KW / 16;               // 16-position tiles of those
     static constexpr int DT = DIM / 16;              // 16-element tiles of a head
     static constexpr int KS = DIM / 32;              // products of 32 elements a score
     static constexpr int CH = DIM / 8;               // 16-byte chunks a row
     static constexpr int R = kWave / CH;             // rows a copy instruction
-    static constexpr int OWN = T / 4;                // rows that a wave copies
+    static constexpr int OWN = T / W;                // rows that a wave copies
     static constexpr int COPIES = OWN / R;           // copy instructions a wave, tile and operand
     static constexpr int ROWS = 16 * QT * WQ;        // query rows a block
     static constexpr int kTile = T * DIM * 2;        // bytes of K or V
     static constexpr int kStage = 2 * kTile;
-    static constexpr int kMerge = WK > 1 ? 4 * QT * 16 * (DIM + 2) * 4 : 0;
+    static constexpr int kMerge = WK > 1 ? W * QT * 16 * (DIM + 2) * 4 : 0;
     static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
     static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : 2;  // a CU
     static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
-    static_assert((COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
+    static_assert((COPIES == 1 || COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
 
 // Where chunk c of a row lies in its LDS row: sixteen rows' same chunk (a K
@@ -205,10 +205,10 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
 }
 
 template <typename S>
-__global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
+__global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
                                                                         int least, int page_shift) {
     constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
-    constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS;
+    constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS, kThreads = kWave * S::W;
     extern __shared__ __align__(16) unsigned char smem[];  // NS stages of K, then V
     __shared__ int poison[2];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -221,19 +221,21 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
     idx /= unsigned(chunks);
     const int split = int(idx % unsigned(part.splits)), s = int(idx / unsigned(part.splits));
     const TreeSpan span = tree_span(a, s);
-    const int group = a.qh / a.kvh, queries = span.nodes * group, q0 = chunk * S::ROWS;
+    const int group = a.qh / a.kvh;
     if (span.context < 0) {
-        // Of an invalid sequence each block clears its own rows; the last chunk's those past max_nodes too.
-        if (split == 0) {
-            const int end = chunk + 1 == chunks ? queries : min(queries, q0 + S::ROWS);
-            for (int i = q0 + int(threadIdx.x) / 16; i < end; i += 16) {
-                uint16_t* o = a.out + (int64_t(span.start + i / group) * a.qh + kvhead * group + i % group) * a.dim;
-                for (int d = 8 * n16; d < a.dim; d += 128) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
-            }
+        if (split != 0) return;
+        for (int64_t i = chunk * (kThreads / 16) + int(threadIdx.x) / 16; i < int64_t(span.nodes) * group;
+             i += int64_t(chunks) * (kThreads / 16)) {
+            uint16_t* o = a.out + ((span.start + i / group) * a.qh + kvhead * group + i % group) * a.dim;
+            for (int d = 8 * n16; d < a.dim; d += 128) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
         }
         return;
     }
-    if (q0 >= queries) return;
+    // A sequence's query rows are dealt evenly to as many blocks as they need.
+    const int all = span.nodes * group, shares = (all + S::ROWS - 1) / S::ROWS;
+    const int share = ((all + shares - 1) / max(shares, 1) + 16 * QT - 1) / (16 * QT) * (16 * QT);
+    const int q0 = chunk * share, queries = min(all, q0 + share);
+    if (chunk >= shares || q0 >= queries) return;
     const int keys = span.context + span.nodes, tiles = (keys + T - 1) / T;
     const int per = split_tiles(tiles, part.splits, least), used = (tiles + per - 1) / per;
     if (split >= used) return;
@@ -303,6 +305,8 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
                          : "=&s"(saved)
                          : "s"(base), "s"(dst), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
                          : "memory");
+        else if constexpr (COPIES == 1)
+            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t") : "=&s"(saved) : "s"(base), "s"(dst), "v"(offset[0]) : "memory");
         else
             asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "1024\n\t")
                          : "=&s"(saved)
@@ -334,7 +338,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
 #pragma unroll
     for (int i = 0; i < NS - 1; ++i) rows0[i] = own_page(min(tile0 + i, tile1 - 1));
     if (a.dim < DIM) {  // chunks past the head are never copied
-        for (int i = int(threadIdx.x); i < NS * S::kStage / 16; i += 256)
+        for (int i = int(threadIdx.x); i < NS * S::kStage / 16; i += kThreads)
             *reinterpret_cast<uint4*>(smem + 16 * i) = make_uint4(0, 0, 0, 0);
     }
     if (threadIdx.x < 2) poison[threadIdx.x] = -1;
@@ -556,7 +560,7 @@ __global__ __launch_bounds__(256, S::kBlocks) void attention_tree_tiles(TreeArgs
         }
         __syncthreads();
         // Sixteen threads a query row.
-        for (int i = int(threadIdx.x) / 16; i < S::ROWS; i += 16) {
+        for (int i = int(threadIdx.x) / 16; i < S::ROWS; i += kThreads / 16) {
             const int qi = q0 + i;
             if (qi >= queries) break;
             float top = -kInf, den = 0.0f, num[DT];
@@ -678,15 +682,22 @@ struct Plan {
 };
 template <typename F>
 void with_shape(int dim, int rows, F&& f) {
-    if (dim == 256) rows <= 32 ? f(Shape<256, 1, 2, 32, 4>{}) : f(Shape<256, 1, 4, 32, 4>{});
-    else if (dim == 128) rows <= 16 ? f(Shape<128, 1, 1, 64, 4>{}) : rows <= 32 ? f(Shape<128, 2, 1, 64, 4>{}) : rows <= 64 ? f(Shape<128, 2, 2, 32, 4>{}) : f(Shape<128, 2, 4, 32, 4>{});
-    else rows <= 16 ? f(Shape<64, 1, 1, 64, 4>{}) : rows <= 32 ? f(Shape<64, 2, 1, 64, 4>{}) : rows <= 64 ? f(Shape<64, 2, 2, 64, 4>{}) : f(Shape<64, 2, 4, 64, 4>{});
+    if (dim == 256) rows <= 32 ? f(Shape<256, 4, 1, 2, 32, 4>{}) : f(Shape<256, 4, 1, 4, 32, 4>{});
+    else if (dim == 128)
+        rows <= 16 ? f(Shape<128, 4, 1, 1, 64, 4>{})
+        : rows <= 32 ? f(Shape<128, 4, 2, 1, 64, 4>{})
+        : rows <= 64 ? f(Shape<128, 8, 2, 2, 64, 4>{}) : f(Shape<128, 8, 2, 4, 64, 4>{});
+    else
+        rows <= 16 ? f(Shape<64, 4, 1, 1, 64, 4>{})
+        : rows <= 32 ? f(Shape<64, 4, 2, 1, 64, 4>{})
+        : rows <= 64 ? f(Shape<64, 8, 2, 2, 64, 6>{})
+        : rows <= 128 ? f(Shape<64, 8, 2, 4, 64, 6>{}) : f(Shape<64, 8, 4, 4, 64, 6>{});
 }
 Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_context) {
     Plan p;
     p.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const int64_t queries = int64_t(max_nodes) * (qh / kvh);
-    with_shape(p.dim, int(std::min<int64_t>(queries, 128)), [&](auto shape) {
+    with_shape(p.dim, int(std::min<int64_t>(queries, 256)), [&](auto shape) {
         using S = decltype(shape);
         p.rows = S::ROWS;
         p.tile = S::T;
@@ -746,7 +757,7 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         const unsigned blocks_all = unsigned(int64_t(batch) * kvh * p.chunks * p.splits);
         with_shape(p.dim, p.rows, [&](auto shape) {
             using S = decltype(shape);
-            hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(256), S::kLds, c->stream, a, part,
+            hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(kWave * S::W), S::kLds, c->stream, a, part,
                                p.chunks, p.least, shift);
         });
         if (p.splits > 1) {
