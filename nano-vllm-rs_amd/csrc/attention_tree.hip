@@ -171,7 +171,7 @@ struct Shape {
     static constexpr int kStage = 2 * kTile;
     static constexpr int kMerge = WK > 1 ? W * QT * 16 * (DIM + 2) * 4 : 0;
     static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
-    static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : 2;  // a CU
+    static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : kLds > 52 * 1024 ? 2 : 3;  // a CU
     static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
     static_assert((COPIES == 1 || COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
@@ -199,9 +199,10 @@ struct Partials {
     int splits;
 };
 
-// Tiles a split, at least `least`.
+// Tiles a split: at least about `least`, the same for every split but the last few.
 __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
-    return max((tiles + splits - 1) / splits, least);
+    const int per = max((tiles + splits - 1) / splits, least), used = (tiles + per - 1) / per;
+    return (tiles + used - 1) / used;
 }
 
 template <typename S>
@@ -690,14 +691,13 @@ void with_shape(int dim, int rows, F&& f) {
     else
         rows <= 16 ? f(Shape<64, 4, 1, 1, 64, 4>{})
         : rows <= 32 ? f(Shape<64, 4, 2, 1, 64, 4>{})
-        : rows <= 64 ? f(Shape<64, 8, 2, 2, 64, 6>{})
-        : rows <= 128 ? f(Shape<64, 8, 2, 4, 64, 6>{}) : f(Shape<64, 8, 4, 4, 64, 6>{});
+        : rows <= 64 ? f(Shape<64, 8, 2, 2, 64, 4>{}) : f(Shape<64, 4, 2, 4, 32, 6>{});
 }
 Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_context) {
     Plan p;
     p.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const int64_t queries = int64_t(max_nodes) * (qh / kvh);
-    with_shape(p.dim, int(std::min<int64_t>(queries, 256)), [&](auto shape) {
+    with_shape(p.dim, int(std::min<int64_t>(queries, 128)), [&](auto shape) {
         using S = decltype(shape);
         p.rows = S::ROWS;
         p.tile = S::T;
