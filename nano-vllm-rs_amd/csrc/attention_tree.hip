@@ -169,9 +169,9 @@ struct Shape {
     static constexpr int ROWS = 16 * QT * WQ;        // query rows a block
     static constexpr int kTile = T * DIM * 2;        // bytes of K or V
     static constexpr int kStage = 2 * kTile;
-    static constexpr int kMerge = WK > 1 ? W * QT * 16 * (DIM + 2) * 4 : 0;
+    static constexpr int kMerge = WK / 2 * WQ * QT * kWave * (16 * DT + 8);  // of half the waves that split positions
     static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
-    static constexpr int kBlocks = kLds > 79 * 1024 ? 1 : kLds > 52 * 1024 ? 2 : 3;  // a CU
+    static constexpr int kFit = 160 * 1024 / (kLds + 64), kBlocks = kFit < 16 / W ? kFit : 16 / W;  // a CU (16 waves)
     static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
     static_assert((COPIES == 1 || COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
@@ -544,83 +544,62 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
         l[t] += nvr::xor_lane(l[t], 16);
         l[t] += nvr::xor_lane(l[t], 32);
     }
-    if constexpr (WK > 1) {
-        // [wave][query row][DIM + 2]: the output, the maximum and the sum.
-        constexpr int P = DIM + 2;
-        float* merge = reinterpret_cast<float*>(smem);
-        __syncthreads();  // every wave is done with the tiles
+    // The upper half of the waves hand theirs to the lower half, until one holds all.
+    f32x4_t* merge = reinterpret_cast<f32x4_t*>(smem);
+    float2* merge_sums = reinterpret_cast<float2*>(smem + (WK / 2 * WQ * QT * DT * kWave) * 16);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            float* mine = merge + ((wk * WQ + wq) * QT * 16 + t * 16 + n16) * P;
+    for (int half = WK / 2; half > 0; half /= 2) {
+        __syncthreads();  // the tiles, or the round before, are read
+        const int from = (wk % max(half, 1) * WQ + wq) * QT;
+        if (wk >= half && wk < 2 * half) {
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int t = 0; t < QT; ++t) {
 #pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    *reinterpret_cast<float2*>(mine + 16 * d + 4 * g + e) = make_float2(o[t][d][e], o[t][d][e + 1]);
-            if (g == 0) *reinterpret_cast<float2*>(mine + DIM) = make_float2(m[t], l[t]);
+                for (int d = 0; d < DT; ++d) merge[((from + t) * DT + d) * kWave + lane] = o[t][d];
+                merge_sums[(from + t) * kWave + lane] = make_float2(m[t], l[t]);
+            }
         }
         __syncthreads();
-        // Sixteen threads a query row.
-        for (int i = int(threadIdx.x) / 16; i < S::ROWS; i += kThreads / 16) {
-            const int qi = q0 + i;
-            if (qi >= queries) break;
-            float top = -kInf, den = 0.0f, num[DT];
-            float f[WK];
+        if (wk < half) {
 #pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, merge[(w * WQ * QT * 16 + i) * P + DIM]);
-            const float base = top == -kInf ? 0.0f : top;
+            for (int t = 0; t < QT; ++t) {
+                const float2 other = merge_sums[(from + t) * kWave + lane];
+                const float top = fmaxf(m[t], other.x), base = top == -kInf ? 0.0f : top;
+                const float f = __builtin_amdgcn_exp2f(m[t] - base), h = __builtin_amdgcn_exp2f(other.x - base);
+                m[t] = top;
+                l[t] = __builtin_fmaf(other.y, h, l[t] * f);
 #pragma unroll
-            for (int w = 0; w < WK; ++w) {
-                const float* from = merge + (w * WQ * QT * 16 + i) * P;
-                f[w] = __builtin_amdgcn_exp2f(from[DIM] - base);
-                den = __builtin_fmaf(from[DIM + 1], f[w], den);
-            }
-            const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
+                for (int d = 0; d < DT; ++d) {
+                    const f32x4_t v = merge[((from + t) * DT + d) * kWave + lane];
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                num[d] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < WK; ++w)
-                    num[d] = __builtin_fmaf(merge[(w * WQ * QT * 16 + i) * P + 16 * d + n16], f[w], num[d]);
-            }
-            if (used == 1) {
-                const float inv = den > 0.0f ? 1.0f / den : 0.0f;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    if (16 * d + n16 < a.dim)
-                        a.out[out_row * a.dim + 16 * d + n16] = nvr::f32_to_bf16(den > 0.0f ? num[d] * inv : 0.0f);
-            } else {
-                const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
-#pragma unroll
-                for (int d = 0; d < DT; ++d)
-                    if (16 * d + n16 < a.dim) part.out[at * a.dim + 16 * d + n16] = num[d];
-                if (n16 == 0) part.sum[at] = make_float2(top, den);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int qi = q0 + (wq * QT + t) * 16 + n16;
-            if (qi >= queries) continue;
-            const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
-            const float inv = l[t] > 0.0f ? 1.0f / l[t] : 0.0f;
-            const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                const int e = 16 * d + 4 * g;
-                if (e >= a.dim) continue;
-                if (used == 1) {
-                    float y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) y[r] = l[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
-                    *reinterpret_cast<uint2*>(a.out + out_row * a.dim + e) =
-                        make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
-                } else {
-                    *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = o[t][d];
+                    for (int e = 0; e < 4; ++e) o[t][d][e] = __builtin_fmaf(v[e], h, o[t][d][e] * f);
                 }
             }
-            if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], l[t]);
         }
+    }
+    if (wk != 0) return;
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        const int qi = q0 + (wq * QT + t) * 16 + n16;
+        if (qi >= queries) continue;
+        const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
+        const float inv = l[t] > 0.0f ? 1.0f / l[t] : 0.0f;
+        const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+            const int e = 16 * d + 4 * g;
+            if (e >= a.dim) continue;
+            if (used == 1) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = l[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
+                *reinterpret_cast<uint2*>(a.out + out_row * a.dim + e) =
+                    make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+            } else {
+                *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = o[t][d];
+            }
+        }
+        if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], l[t]);
     }
 }
 
@@ -678,33 +657,51 @@ constexpr int kSplitPositions = 256;
 
 // The launch's shape: the same for the workspace's size and the launch.
 struct Plan {
-    int dim, rows;  // rounded head dim; query rows a block
+    int dim;              // the head dim, rounded up
+    int64_t queries, pairs;  // query rows a KV head; (sequence, KV head) pairs
     int tile, chunks, splits, least;  // positions a tile; blocks a KV head's rows; splits, and the fewest tiles of one
 };
+// The shape for `queries` query rows a KV head, of sequences and KV heads in
+// `pairs`. Microseconds on MI355X, 16 q heads over 8 KV heads of 128, blocks of 256:
+//  - up to 32 rows four waves split each tile's positions and read only what they
+//    copied themselves, so they need no barrier. Two stages and two blocks a CU beat
+//    four stages and one: 64 sequences of 6 nodes at 200 positions 15.8 against 22.2,
+//    at 1000 44.3, 49.2, at 4090 155, 162.
+//  - up to 64 rows, four waves over stages of 32 positions, two blocks a CU, against
+//    eight waves over stages of 64: 64 of 30 at 300 26.3, 36.6, 8 of 25 at 1030 22.3, 23.3.
+//  - above, the same four waves where there are more pairs than CUs (64 of 60 at 300
+//    30.6 against 43.0, at 1000 62.9, 73.8); else eight waves, which need half the splits
+//    to fill a CU (8 of 64 at 8000 74.3 against 69.9, 4 of 64 at 16000 75.8, 69.5).
+//  - heads of 64, 16 of 33 nodes at 2000 with 8 heads a KV head: three blocks of four
+//    waves a CU 32.8, two of eight 34.3, one of eight with twice the rows 44.6. Heads of
+//    256 with two stages: 16 of 40 at 1000 33.8, with four 37.9.
 template <typename F>
-void with_shape(int dim, int rows, F&& f) {
-    if (dim == 256) rows <= 32 ? f(Shape<256, 4, 1, 2, 32, 4>{}) : f(Shape<256, 4, 1, 4, 32, 4>{});
-    else if (dim == 128)
-        rows <= 16 ? f(Shape<128, 4, 1, 1, 64, 4>{})
-        : rows <= 32 ? f(Shape<128, 4, 2, 1, 64, 4>{})
-        : rows <= 64 ? f(Shape<128, 8, 2, 2, 64, 4>{}) : f(Shape<128, 8, 2, 4, 64, 4>{});
-    else
-        rows <= 16 ? f(Shape<64, 4, 1, 1, 64, 4>{})
-        : rows <= 32 ? f(Shape<64, 4, 2, 1, 64, 4>{})
-        : rows <= 64 ? f(Shape<64, 8, 2, 2, 64, 4>{}) : f(Shape<64, 4, 2, 4, 32, 6>{});
+void with_shape(int dim, int64_t queries, int64_t pairs, F&& f) {
+    if (dim == 256) {
+        queries <= 32 ? f(Shape<256, 4, 1, 2, 32, 2>{}) : f(Shape<256, 4, 1, 4, 32, 2>{});
+    } else if (dim == 128) {
+        queries <= 16   ? f(Shape<128, 4, 1, 1, 64, 2>{})
+        : queries <= 32 ? f(Shape<128, 4, 2, 1, 64, 2>{})
+        : queries <= 64 ? f(Shape<128, 4, 2, 2, 32, 4>{})
+        : pairs > 256   ? f(Shape<128, 4, 2, 4, 32, 4>{}) : f(Shape<128, 8, 2, 4, 64, 4>{});
+    } else {
+        queries <= 16   ? f(Shape<64, 4, 1, 1, 64, 3>{})
+        : queries <= 32 ? f(Shape<64, 4, 2, 1, 64, 3>{})
+        : queries <= 64 ? f(Shape<64, 8, 2, 2, 64, 4>{}) : f(Shape<64, 4, 2, 4, 32, 6>{});
+    }
 }
 Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_context) {
     Plan p;
     p.dim = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-    const int64_t queries = int64_t(max_nodes) * (qh / kvh);
-    with_shape(p.dim, int(std::min<int64_t>(queries, 128)), [&](auto shape) {
+    p.queries = int64_t(max_nodes) * (qh / kvh);
+    p.pairs = int64_t(batch) * kvh;
+    with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
         using S = decltype(shape);
-        p.rows = S::ROWS;
         p.tile = S::T;
-        p.chunks = int((queries + p.rows - 1) / p.rows);
+        p.chunks = int((p.queries + S::ROWS - 1) / S::ROWS);
         p.least = kSplitPositions / p.tile;
-        const int64_t pairs = int64_t(batch) * kvh * p.chunks, most = (int64_t(max_context) + kSplitPositions - 1) / kSplitPositions;
-        p.splits = int(std::max<int64_t>(1, std::min(most, 256 * S::kBlocks / pairs)));
+        const int64_t blocks = p.pairs * p.chunks, most = (int64_t(max_context) + kSplitPositions - 1) / kSplitPositions;
+        p.splits = int(std::max<int64_t>(1, std::min(most, 256 * S::kBlocks / blocks)));
     });
     return p;
 }
@@ -755,7 +752,7 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
         const int pages = bs / kPage, shift = (pages & (pages - 1)) == 0 ? __builtin_ctz(unsigned(pages)) : -1;
         const unsigned blocks_all = unsigned(int64_t(batch) * kvh * p.chunks * p.splits);
-        with_shape(p.dim, p.rows, [&](auto shape) {
+        with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
             using S = decltype(shape);
             hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(kWave * S::W), S::kLds, c->stream, a, part,
                                p.chunks, p.least, shift);
