@@ -561,4 +561,140 @@ void Gpu::kv_write(const Buffer& k, const Buffer& v, const Buffer& slots, const 
                                as_dim(num_blocks)));
 }
 
+// ------------------------------------------------- trees of drafted tokens --
+std::vector<uint64_t> tree_masks(const std::vector<int32_t>& parents) {
+    if (parents.empty() || parents.size() > kMaxTreeNodes)
+        throw Error(Fault::Value, "a tree of " + str(parents.size()) + " nodes; 1 to " + str(kMaxTreeNodes) + " are possible");
+    std::vector<uint64_t> masks{1};
+    for (std::size_t i = 1; i < parents.size(); ++i) {
+        if (parents[i] < 0 || std::size_t(parents[i]) >= i)
+            throw Error(Fault::Value, "node " + str(i) + " follows node " + std::to_string(parents[i]) +
+                                          ", which does not come before it");
+        masks.push_back(masks[std::size_t(parents[i])] | uint64_t(1) << i);
+    }
+    return masks;
+}
+
+namespace {
+
+void require_tree(const char* op, std::size_t max_nodes) {
+    if (max_nodes < 1 || max_nodes > kMaxTreeNodes)
+        throw Error(Fault::Value, std::string(op) + ": max_nodes " + str(max_nodes) + " outside [1, " +
+                                      str(kMaxTreeNodes) + "]");
+}
+
+// Elements of a KV slot, as a dimension.
+std::size_t slot_width(const char* op, std::size_t kvheads, std::size_t head_dim) {
+    as_dim(kvheads);
+    as_dim(head_dim);
+    if (kvheads > std::size_t(INT_MAX) / head_dim)
+        throw Error(Fault::Dimension, std::string(op) + ": kvheads * head_dim exceeds 2^31 - 1");
+    return kvheads * head_dim;
+}
+
+TensorArg workspace_arg(const Buffer& workspace, std::size_t bytes) {
+    return write_arg("workspace", workspace, 16, {(bytes + 15) / 16});
+}
+
+}  // namespace
+
+std::size_t Gpu::attention_tree_workspace(std::size_t rows, std::size_t qheads, std::size_t kvheads,
+                                          std::size_t head_dim, std::size_t batch_size, std::size_t max_nodes,
+                                          std::size_t max_context) const {
+    require_head_layout(qheads, kvheads, head_dim);
+    require_tree("attention_tree_workspace", max_nodes);
+    std::size_t bytes = 0;
+    require_status(nv_attention_tree_workspace(as_dim(rows), as_dim(qheads), as_dim(kvheads), as_dim(head_dim),
+                                               as_dim(batch_size), as_dim(max_nodes), as_dim(max_context), &bytes));
+    return bytes;
+}
+
+void Gpu::attention_tree(const Buffer& q, const Buffer& kcache, const Buffer& vcache, const Buffer& contexts,
+                         const Buffer& row_starts, const Buffer& masks, const Buffer& block_tables, const Buffer& out,
+                         const Buffer& workspace, std::size_t rows, std::size_t qheads, std::size_t kvheads,
+                         std::size_t head_dim, std::size_t block_size, std::size_t num_blocks,
+                         std::size_t table_stride, std::size_t batch_size, std::size_t max_nodes,
+                         std::size_t max_context) const {
+    const std::size_t need =
+        attention_tree_workspace(rows, qheads, kvheads, head_dim, batch_size, max_nodes, max_context);
+    std::vector<TensorArg> args = {read_arg("q", q, 2, {rows, qheads, head_dim}),
+                                   read_arg("kcache", kcache, 2, {num_blocks, block_size, kvheads, head_dim}),
+                                   read_arg("vcache", vcache, 2, {num_blocks, block_size, kvheads, head_dim}),
+                                   read_arg("contexts", contexts, 4, {batch_size}),
+                                   read_arg("row_starts", row_starts, 4, {batch_size + 1}),
+                                   read_arg("masks", masks, 8, {rows}),
+                                   read_arg("block_tables", block_tables, 4, {batch_size, table_stride}),
+                                   write_arg("out", out, 2, {rows, qheads, head_dim})};
+    if (need != 0) args.push_back(workspace_arg(workspace, need));
+    admit("attention_tree", args);
+    require_status(nv_attention_tree(context(), q.address(), kcache.address(), vcache.address(), contexts.address(),
+                                     row_starts.address(), masks.address(), block_tables.address(), out.address(),
+                                     need != 0 ? workspace.address() : nullptr, as_dim(rows), as_dim(qheads),
+                                     as_dim(kvheads), as_dim(head_dim), as_dim(block_size), as_dim(num_blocks),
+                                     as_dim(table_stride), as_dim(batch_size), as_dim(max_nodes), as_dim(max_context)));
+}
+
+std::size_t Gpu::verify_tree_workspace(std::size_t rows, std::size_t batch_size, std::size_t vocab) const {
+    std::size_t bytes = 0;
+    require_status(nv_verify_tree_workspace(as_dim(rows), as_dim(batch_size), as_dim(vocab), &bytes));
+    return bytes;
+}
+
+void Gpu::verify_tree(const Buffer& logits, const Buffer& draft_logits, const Buffer& tokens, const Buffer& parents,
+                      const Buffer& row_starts, const Buffer& temperatures, const Buffer& uniforms,
+                      const Buffer& seeds, const Buffer& out_tokens, const Buffer& out_nodes, const Buffer& out_counts,
+                      const Buffer& workspace, std::size_t rows, std::size_t batch_size, std::size_t max_nodes,
+                      std::size_t vocab) const {
+    require_tree("verify_tree", max_nodes);
+    std::vector<TensorArg> args = {read_arg("logits", logits, 2, {rows, vocab}),
+                                   read_arg("tokens", tokens, 4, {rows}),
+                                   read_arg("parents", parents, 4, {rows}),
+                                   read_arg("row_starts", row_starts, 4, {batch_size + 1}),
+                                   read_arg("temperatures", temperatures, 4, {batch_size}),
+                                   read_arg("uniforms", uniforms, 4, {rows}),
+                                   read_arg("seeds", seeds, 8, {batch_size}),
+                                   write_arg("out_tokens", out_tokens, 4, {batch_size, max_nodes}),
+                                   write_arg("out_nodes", out_nodes, 4, {batch_size, max_nodes}),
+                                   write_arg("out_counts", out_counts, 4, {batch_size}),
+                                   workspace_arg(workspace, verify_tree_workspace(rows, batch_size, vocab))};
+    if (!draft_logits.empty()) args.push_back(read_arg("draft_logits", draft_logits, 2, {rows, vocab}));
+    admit("verify_tree", args);
+    require_status(nv_verify_tree(context(), logits.address(), draft_logits.empty() ? nullptr : draft_logits.address(),
+                                  tokens.address(), parents.address(), row_starts.address(), temperatures.address(),
+                                  uniforms.address(), seeds.address(), out_tokens.address(), out_nodes.address(),
+                                  out_counts.address(), workspace.address(), as_dim(rows), as_dim(batch_size),
+                                  as_dim(max_nodes), as_dim(vocab)));
+}
+
+void Gpu::kv_compact(const Buffer& kcache, const Buffer& vcache, const Buffer& contexts, const Buffer& nodes,
+                     const Buffer& counts, const Buffer& block_tables, std::size_t batch_size, std::size_t max_nodes,
+                     std::size_t layers, std::size_t kvheads, std::size_t head_dim, std::size_t block_size,
+                     std::size_t num_blocks, std::size_t table_stride) const {
+    require_tree("kv_compact", max_nodes);
+    const std::size_t width = slot_width("kv_compact", kvheads, head_dim);
+    admit("kv_compact", {write_arg("kcache", kcache, 2, {layers, num_blocks, block_size, width}),
+                         write_arg("vcache", vcache, 2, {layers, num_blocks, block_size, width}),
+                         read_arg("contexts", contexts, 4, {batch_size}),
+                         read_arg("nodes", nodes, 4, {batch_size, max_nodes}),
+                         read_arg("counts", counts, 4, {batch_size}),
+                         read_arg("block_tables", block_tables, 4, {batch_size, table_stride})});
+    require_status(nv_kv_compact(context(), kcache.address(), vcache.address(), contexts.address(), nodes.address(),
+                                 counts.address(), block_tables.address(), as_dim(batch_size), as_dim(max_nodes),
+                                 as_dim(layers), as_dim(kvheads), as_dim(head_dim), as_dim(block_size),
+                                 as_dim(num_blocks), as_dim(table_stride)));
+}
+
+void Gpu::kv_copy_blocks(const Buffer& kcache, const Buffer& vcache, const Buffer& sources, const Buffer& targets,
+                         const Buffer& tokens, std::size_t copies, std::size_t layers, std::size_t kvheads,
+                         std::size_t head_dim, std::size_t block_size, std::size_t num_blocks) const {
+    const std::size_t width = slot_width("kv_copy_blocks", kvheads, head_dim);
+    admit("kv_copy_blocks", {write_arg("kcache", kcache, 2, {layers, num_blocks, block_size, width}),
+                             write_arg("vcache", vcache, 2, {layers, num_blocks, block_size, width}),
+                             read_arg("sources", sources, 4, {copies}), read_arg("targets", targets, 4, {copies}),
+                             read_arg("tokens", tokens, 4, {copies})});
+    require_status(nv_kv_copy_blocks(context(), kcache.address(), vcache.address(), sources.address(),
+                                     targets.address(), tokens.address(), as_dim(copies), as_dim(layers),
+                                     as_dim(kvheads), as_dim(head_dim), as_dim(block_size), as_dim(num_blocks)));
+}
+
 }  // namespace nvr

@@ -75,6 +75,13 @@ void require_head_layout(std::size_t qheads, std::size_t kvheads, std::size_t he
 std::vector<uint16_t> tile_gate_up_rows(const std::vector<uint16_t>& gate_up, std::size_t intermediate,
                                         std::size_t k);
 
+// Trees of drafted tokens have at most this many nodes.
+constexpr std::size_t kMaxTreeNodes = 64;
+// The attention masks of one tree's nodes: each node's own bit and its
+// ancestors'. parents[i] is the node that node i follows, below i; node 0's is
+// not read.
+std::vector<uint64_t> tree_masks(const std::vector<int32_t>& parents);
+
 namespace detail {
 struct Device;
 struct Allocation;
@@ -248,6 +255,43 @@ public:
     void kv_write(const Buffer& k, const Buffer& v, const Buffer& slots, const Buffer& kcache, const Buffer& vcache,
                   std::size_t rows, std::size_t kvheads, std::size_t head_dim, std::size_t block_size,
                   std::size_t num_blocks) const;
+
+    // ---- trees of drafted tokens (no Rust caller in the reference) ----
+    // Bytes of workspace that attention_tree needs for these arguments (0: none).
+    std::size_t attention_tree_workspace(std::size_t rows, std::size_t qheads, std::size_t kvheads,
+                                         std::size_t head_dim, std::size_t batch_size, std::size_t max_nodes,
+                                         std::size_t max_context) const;
+    // Row row_starts[s] + i reads the positions before contexts[s] and, of its
+    // tree, node j (at position contexts[s] + j) for each bit j of its u64 mask.
+    // Trees have at most max_nodes (<= 64) nodes, sequences max_context positions.
+    void attention_tree(const Buffer& q, const Buffer& kcache, const Buffer& vcache, const Buffer& contexts,
+                        const Buffer& row_starts, const Buffer& masks, const Buffer& block_tables, const Buffer& out,
+                        const Buffer& workspace, std::size_t rows, std::size_t qheads, std::size_t kvheads,
+                        std::size_t head_dim, std::size_t block_size, std::size_t num_blocks,
+                        std::size_t table_stride, std::size_t batch_size, std::size_t max_nodes,
+                        std::size_t max_context) const;
+    std::size_t verify_tree_workspace(std::size_t rows, std::size_t batch_size, std::size_t vocab) const;
+    // Rejection sampling of drafted tokens; draft_logits may be empty (children
+    // that were picked, not drawn). Per sequence: out_tokens [max_nodes] the
+    // accepted tokens and the one after them, out_nodes [max_nodes] the accepted
+    // path from node 0 on, both filled with -1, and out_counts their number.
+    void verify_tree(const Buffer& logits, const Buffer& draft_logits, const Buffer& tokens, const Buffer& parents,
+                     const Buffer& row_starts, const Buffer& temperatures, const Buffer& uniforms,
+                     const Buffer& seeds, const Buffer& out_tokens, const Buffer& out_nodes, const Buffer& out_counts,
+                     const Buffer& workspace, std::size_t rows, std::size_t batch_size, std::size_t max_nodes,
+                     std::size_t vocab) const;
+    // K and V at position contexts[s] + nodes[s, j] move to contexts[s] + j, for
+    // j < counts[s], in every layer of caches [layers, num_blocks, block_size,
+    // kvheads, head_dim].
+    void kv_compact(const Buffer& kcache, const Buffer& vcache, const Buffer& contexts, const Buffer& nodes,
+                    const Buffer& counts, const Buffer& block_tables, std::size_t batch_size, std::size_t max_nodes,
+                    std::size_t layers, std::size_t kvheads, std::size_t head_dim, std::size_t block_size,
+                    std::size_t num_blocks, std::size_t table_stride) const;
+    // The first tokens[i] slots of block sources[i] are copied to block
+    // targets[i], in every layer. No block may be written twice, or read and written.
+    void kv_copy_blocks(const Buffer& kcache, const Buffer& vcache, const Buffer& sources, const Buffer& targets,
+                        const Buffer& tokens, std::size_t copies, std::size_t layers, std::size_t kvheads,
+                        std::size_t head_dim, std::size_t block_size, std::size_t num_blocks) const;
 
 private:
     nv_context* context() const;

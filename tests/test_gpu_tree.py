@@ -92,7 +92,11 @@ class Trees:
     ([11], [50], 3, 1, 6, 5),
     ([4, 40], [33, 260], 64, 2, 32, 8),
     ([2], [60], 5, 5, 128, 7),                        # odd block size
-    ([50, 7], [333, 95], 16, 8, 128, 48),
+    ([50, 7], [333, 95], 16, 8, 128, 48),             # three pages a block
+    ([60] * 34, [17 * i % 90 for i in range(34)], 16, 8, 128, 16),  # more pairs than CUs, wide
+    ([20, 7], [100, 90], 8, 4, 64, 16),
+    ([3], [40], 8, 4, 64, 32),
+    ([14, 5], [1000, 129], 16, 8, 128, 16),
     ([16] * 40, [17 * i for i in range(40)], 2, 1, 64, 16),
 ])
 def test_attention_of_trees(gpu, sizes, contexts, qh, kvh, dim, bs):

@@ -145,6 +145,10 @@ def test_tree_calls_that_keep_the_contract_reach_the_library(call):
     (_attention_call, "alignment", dict(masks=lambda b, a: b(ROWS * 8 + 8).slice(4, ROWS * 8))),
     (_attention_call, "overlap", dict(out=lambda b, a: a["q"])),
     (_attention_call, "overlap", dict(out=lambda b, a: a["kcache"])),
+    (_attention_call, "extent", dict(max_context=lambda b, a: 100000, workspace=lambda b, a: b(1024))),
+    (_attention_call, "extent", dict(max_context=lambda b, a: 100000, workspace=lambda b, a: None)),
+    (_attention_call, "alignment", dict(max_context=lambda b, a: 1000, workspace=lambda b, a: a["workspace"].slice(8, 1 << 20))),
+    (_attention_call, "overlap", dict(max_context=lambda b, a: 1000, kcache=lambda b, a: a["workspace"])),
     (_verify_call, "value", dict(max_nodes=lambda b, a: 65)),
     (_verify_call, "dimension", dict(vocab=lambda b, a: 0)),
     (_verify_call, "extent", dict(draft_logits=lambda b, a: b(ROWS * 100 * 2 - 2))),
