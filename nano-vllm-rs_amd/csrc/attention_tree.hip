@@ -357,11 +357,12 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     int next_row = own_page(min(tile0 + NS - 1, tile1 - 1));
 
     f32x4_t o[QT][DT];
-    float m[QT], l[QT];
+    f32x4_t l[QT];  // the weights' sum, four times
+    float m[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         m[t] = -kInf;
-        l[t] = 0.0f;
+        l[t] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
     }
@@ -468,7 +469,6 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r], a.scale, -base));
-                    l[t] += x[t][j][r];
                 }
         }
 
@@ -483,7 +483,10 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
         if constexpr (KT == 1) {
             s16x4_t p[QT];
 #pragma unroll
-            for (int t = 0; t < QT; ++t) p[t] = __builtin_bit_cast(s16x4_t, pair(x[t][0]));
+            for (int t = 0; t < QT; ++t) {
+                p[t] = __builtin_bit_cast(s16x4_t, pair(x[t][0]));
+                l[t] = mfma(s16x4_t{0x3f80, 0x3f80, 0x3f80, 0x3f80}, p[t], l[t]);
+            }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const s16x4_t v = read(vrow, d);
@@ -499,6 +502,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 for (int j = 0; j < KT / 2; ++j) {
                     const uint2 lo = pair(x[t][2 * j]), hi = pair(x[t][2 * j + 1]);
                     p[t][j] = operand(make_uint4(lo.x, lo.y, hi.x, hi.y));
+                    l[t] = mfma(operand(make_uint4(0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80)), p[t][j], l[t]);
                 }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -539,11 +543,9 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     for (int tile = plain; tile < tile1; ++tile) step(tile, std::true_type{});
 
     // ---- the waves' shares, then the output or the split's partial ----
+    float sum[QT];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-        l[t] += nvr::xor_lane(l[t], 16);
-        l[t] += nvr::xor_lane(l[t], 32);
-    }
+    for (int t = 0; t < QT; ++t) sum[t] = l[t][0];
     // The upper half of the waves hand theirs to the lower half, until one holds all.
     f32x4_t* merge = reinterpret_cast<f32x4_t*>(smem);
     float2* merge_sums = reinterpret_cast<float2*>(smem + (WK / 2 * WQ * QT * DT * kWave) * 16);
@@ -556,7 +558,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int t = 0; t < QT; ++t) {
 #pragma unroll
                 for (int d = 0; d < DT; ++d) merge[((from + t) * DT + d) * kWave + lane] = o[t][d];
-                merge_sums[(from + t) * kWave + lane] = make_float2(m[t], l[t]);
+                merge_sums[(from + t) * kWave + lane] = make_float2(m[t], sum[t]);
             }
         }
         __syncthreads();
@@ -567,7 +569,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 const float top = fmaxf(m[t], other.x), base = top == -kInf ? 0.0f : top;
                 const float f = __builtin_amdgcn_exp2f(m[t] - base), h = __builtin_amdgcn_exp2f(other.x - base);
                 m[t] = top;
-                l[t] = __builtin_fmaf(other.y, h, l[t] * f);
+                sum[t] = __builtin_fmaf(other.y, h, sum[t] * f);
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const f32x4_t v = merge[((from + t) * DT + d) * kWave + lane];
@@ -583,7 +585,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
         const int qi = q0 + (wq * QT + t) * 16 + n16;
         if (qi >= queries) continue;
         const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
-        const float inv = l[t] > 0.0f ? 1.0f / l[t] : 0.0f;
+        const float inv = sum[t] > 0.0f ? 1.0f / sum[t] : 0.0f;
         const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
@@ -592,14 +594,14 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             if (used == 1) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = l[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
+                for (int r = 0; r < 4; ++r) y[r] = sum[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
                 *reinterpret_cast<uint2*>(a.out + out_row * a.dim + e) =
                     make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
             } else {
                 *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = o[t][d];
             }
         }
-        if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], l[t]);
+        if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], sum[t]);
     }
 }
 
