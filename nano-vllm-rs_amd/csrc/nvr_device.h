@@ -203,8 +203,9 @@ __device__ __forceinline__ uint64_t splitmix64(uint64_t v) {
 constexpr uint64_t kTokenMix = 0xd2b74407b1ce6e93ull;
 
 // Uniform in (0,1) from the top 23 hash bits: (k + 0.5) * 2^-23, exact in fp32.
+// Taken from the high word: a shift of all 64 bits compiles to a 64-bit conversion.
 __device__ __forceinline__ float hash_uniform(uint64_t r) {
-    return (float(uint32_t(r >> 41)) + 0.5f) * (1.0f / 8388608.0f);
+    return (float(uint32_t(r >> 32) >> 9) + 0.5f) * (1.0f / 8388608.0f);
 }
 // Gumbel-max score of one vocabulary entry: logit / T - ln(-ln(u)).
 __device__ __forceinline__ float gumbel_score(float logit, float temperature, uint64_t seed, uint32_t token) {

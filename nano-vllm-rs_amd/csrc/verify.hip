@@ -740,20 +740,30 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
             return (c > 0.0f ? nvr::nvr_logf(v) : v / temperature) - nvr::nvr_logf(-nvr::nvr_logf(u));
         };
         const float inverse_t = 1.0f / temperature;
-        const bool bounded = inverse_t < kInf;
-        float bound[8], high = -kInf;
-        float us[8];
-        int own = -1;
+        float bound[8], us[8], high = -kInf;
+        if (c > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bound[i] = __builtin_amdgcn_logf(f[i]) * kLn2;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bound[i] = f[i] * inverse_t;
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             us[i] = uniform(i);
             // Bounds with 2^-20 of the value and 1e-4 to spare: many times what their few roundings can take.
-            const float v = c > 0.0f ? __builtin_amdgcn_logf(f[i]) * kLn2 : f[i] * inverse_t;
             const float g = __builtin_fmaf(__builtin_amdgcn_logf(1.0f - us[i]), -kLn2, 1e-4f);
-            bound[i] = bounded ? __builtin_fmaf(v, v > 0.0f ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f, g)
-                               : f[i] == f[i] ? kInf : f[i];
-            if (bound[i] > high || (own < 0 && bound[i] == high)) { high = bound[i]; own = i; }
+            bound[i] = __builtin_fmaf(bound[i], bound[i] > 0.0f ? 1.0f + 0x1p-20f : 1.0f - 0x1p-20f, g);
         }
+        if (!(inverse_t < kInf)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bound[i] = f[i] == f[i] ? kInf : f[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) high = fmaxf(high, bound[i]);  // passes over NaN
+        int own = -1;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) own = bound[i] == high ? i : own;
         if (own >= 0) {
             float v = f[0], u = us[0];
 #pragma unroll
