@@ -17,7 +17,10 @@
 // min(max_context, stride * bs) positions their rows are +0. Rows of no sequence
 // are left as they were.
 //
-// Scores, maxima, sums and outputs are fp32, rounded to bf16 once at the end.
+// Scores, maxima, sums and outputs are fp32, and the outputs rounded to bf16 once
+// at the end. The tile form rounds each weight p_t to bf16 as an operand of the
+// matrix instructions (a factor within 2^-8, its own for each position), and sums
+// the rounded weights, so that a row's weights still sum to 1.
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
@@ -403,7 +406,9 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             }
             if (__ballot(found) != 0 && lane == 0) poison[tile & 1] = tile;
         }
+        // The tile is whole, and every read of the stage that the next copies fill is done.
         if (!S::kAlone || drafted) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (tile + NS - 1 < tile1) {
             copy(tile + NS - 1, next_row);
             next_row = own_page(min(tile + NS, tile1 - 1));
@@ -712,6 +717,10 @@ int64_t workspace_bytes(const Plan& p, int rows, int qh, int dim) {
     return p.splits == 1 ? 0 : int64_t(p.splits) * rows * qh * (4 * int64_t(dim) + int64_t(sizeof(float2)));
 }
 
+bool too_many(int rows, int qh, int batch, int kvh) {
+    return int64_t(rows) * qh > 0x7fffffff || int64_t(batch) * kvh > 0x7fffffff;
+}
+
 }  // namespace
 
 extern "C" {
@@ -720,6 +729,7 @@ int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, i
                                 size_t* bytes) {
     if (rows <= 0 || qh <= 0 || kvh <= 0 || dim <= 0 || batch <= 0 || max_nodes <= 0 || max_context <= 0 || qh % kvh)
         return nvr::fail(-2, "attention_tree_workspace: dimensions must be positive, q heads a multiple of KV heads");
+    if (too_many(rows, qh, batch, kvh)) return nvr::fail(-2, "attention_tree_workspace: rows * qh or batch * kvh exceed int32");
     if (max_nodes > kMaxNodes || dim > 256) return nvr::fail(-2, "attention_tree_workspace: max_nodes %d, head dim %d", max_nodes, dim);
     *bytes = dim % 8 ? 0 : size_t(workspace_bytes(plan_tiles(qh, kvh, dim, batch, max_nodes, max_context), rows, qh, dim));
     return 0;
@@ -737,37 +747,44 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
     if (max_nodes < 1 || max_nodes > kMaxNodes)
         return nvr::fail(-2, "attention_tree: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     if (max_context < 1) return nvr::fail(-2, "attention_tree: max_context %d is not positive", max_context);
+    if (too_many(rows, qh, batch, kvh)) return nvr::fail(-2, "attention_tree: rows * qh or batch * kvh exceed int32");
     const int64_t span = std::min(int64_t(stride) * bs, int64_t(0x7fff0000));  // tiles past the end stay below 2^31
     const TreeArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(kc), static_cast<const uint16_t*>(vc),
                      static_cast<const int*>(contexts), static_cast<const int*>(row_starts),
                      static_cast<const uint64_t*>(masks), static_cast<const int*>(tables), static_cast<uint16_t*>(out),
                      rows, qh, kvh, dim, bs, blocks, stride, batch, max_nodes,
                      span < max_context ? span : int64_t(max_context), kLog2e / sqrtf(float(dim))};
-    const int64_t grid = int64_t(batch) * max_nodes * qh;
-    const bool fits = dim % 8 == 0 && bs % kPage == 0 && int64_t(kvh) * dim <= 0x1000000 && nvr::aligned(q, 16) && nvr::aligned(kc, 16) && nvr::aligned(vc, 16) &&
-                      nvr::aligned(out, 16) && int64_t(blocks) * bs <= 0x7fffffff;
-    const Plan p = plan_tiles(qh, kvh, dim, batch, max_nodes, max_context);
-    if (fits && int64_t(batch) * kvh * p.chunks * p.splits <= 0x7fffffff && int64_t(batch) * max_nodes * qh <= 0x3ffffff) {
+    const bool fits = dim % 8 == 0 && bs % kPage == 0 && int64_t(kvh) * dim <= 0x1000000 && nvr::aligned(q, 16) &&
+                      nvr::aligned(kc, 16) && nvr::aligned(vc, 16) && nvr::aligned(out, 16) &&
+                      int64_t(blocks) * bs <= 0x7fffffff;
+    // A launch has fewer than 2^32 threads.
+    constexpr int64_t kLaunch = 0xffffffff;
+    const char* const exceeded = "attention_tree: %d sequences of %d nodes and %d heads exceed one launch";
+    if (fits) {
+        const Plan p = plan_tiles(qh, kvh, dim, batch, max_nodes, max_context);
+        const int64_t grid = p.pairs * p.chunks * p.splits, parts = (int64_t(qh) * dim / 4 + 255) / 256;
+        const int64_t joins = int64_t(batch) * max_nodes * parts;
+        if (grid > kLaunch / 512 || (p.splits > 1 && joins > kLaunch / 256))
+            return nvr::fail(-2, exceeded, batch, max_nodes, qh);
         if (p.splits > 1 && (workspace == nullptr || !nvr::aligned(workspace, 16)))
             return nvr::fail(-2, "attention_tree: needs a workspace at a multiple of 16 bytes");
         float* partial = static_cast<float*>(workspace);
         const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
         const int pages = bs / kPage, shift = (pages & (pages - 1)) == 0 ? __builtin_ctz(unsigned(pages)) : -1;
-        const unsigned blocks_all = unsigned(int64_t(batch) * kvh * p.chunks * p.splits);
         with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
             using S = decltype(shape);
-            hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(blocks_all), dim3(kWave * S::W), S::kLds, c->stream, a, part,
-                               p.chunks, p.least, shift);
+            hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(unsigned(grid)), dim3(kWave * S::W), S::kLds, c->stream, a,
+                               part, p.chunks, p.least, shift);
         });
         if (p.splits > 1) {
             NVR_HIP(hipGetLastError());
-            const int parts = (qh * dim / 4 + 255) / 256;
-            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(int64_t(batch) * max_nodes * parts)), dim3(256), 0,
-                               c->stream, a, part, p.tile, p.least, parts);
+            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(joins)), dim3(256), 0, c->stream, a, part, p.tile,
+                               p.least, int(parts));
         }
         return nvr::launch_status();
     }
-    if (grid > 0x7fffffff) return nvr::fail(-2, "attention_tree: %d sequences of %d nodes exceed one launch", batch, max_nodes);
+    const int64_t grid = int64_t(batch) * max_nodes * qh;
+    if (grid > kLaunch / 256) return nvr::fail(-2, exceeded, batch, max_nodes, qh);
     hipLaunchKernelGGL(attention_tree_direct, dim3(unsigned(grid)), dim3(256), 0, c->stream, a);
     return nvr::launch_status();
 }

@@ -131,7 +131,7 @@ int nv_kv_copy_blocks(nv_context* c, void* kc, void* vc, const void* src, const 
     const bool wide = chunked(kc, vc, width);
     const int64_t slot_chunks = wide ? width / 8 : width;
     const int64_t segments = (slot_chunks * bs + kSegment - 1) / kSegment;
-    if (segments > 0x7fffffff / (2 * int64_t(layers)) / copies)
+    if (segments > 0xffffff / (2 * int64_t(layers)) / copies)  // a launch has fewer than 2^32 threads
         return nvr::fail(-2, "kv_copy_blocks: %d copies in %d layers exceed one launch", copies, layers);
     const dim3 grid(unsigned(2 * int64_t(layers) * copies * segments));
     if (wide)
@@ -153,7 +153,8 @@ int nv_kv_compact(nv_context* c, void* kc, void* vc, const void* contexts, const
         return nvr::fail(-2, "kv_compact: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
     const int64_t width = int64_t(kvh) * dim;
     if (width > 0x7fffffff) return nvr::fail(-2, "kv_compact: kvh * dim exceeds int32");
-    if (layers > 65535) return nvr::fail(-2, "kv_compact: %d layers exceed one launch", layers);
+    if (layers > 65535 || batch > 0xffffff)
+        return nvr::fail(-2, "kv_compact: %d sequences in %d layers exceed one launch", batch, layers);
     auto x = static_cast<const int*>(contexts), n = static_cast<const int*>(nodes);
     auto k = static_cast<const int*>(counts), t = static_cast<const int*>(tables);
     const dim3 grid{unsigned(batch), unsigned(layers)};

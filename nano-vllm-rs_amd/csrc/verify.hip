@@ -845,10 +845,13 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
     if (rows <= 0 || batch <= 0 || vocab <= 0) return nvr::fail(-2, "verify_tree: dimensions must be positive");
     if (max_nodes < 1 || max_nodes > kMaxNodes)
         return nvr::fail(-2, "verify_tree: max_nodes %d outside [1, %d]", max_nodes, kMaxNodes);
-    if (!nvr::aligned(workspace, 16)) return nvr::fail(-2, "verify_tree: the workspace needs 16-byte alignment");
+    if (vocab > kMaxVocab) return nvr::fail(-2, "verify_tree: vocab %d above %d", vocab, kMaxVocab);
+    if (workspace == nullptr || !nvr::aligned(workspace, 16))
+        return nvr::fail(-2, "verify_tree: needs a workspace at a multiple of 16 bytes");
+    // A launch has fewer than 2^32 threads.
     const int sampled = sample_blocks(vocab);
-    if (vocab > kMaxVocab)
-        return nvr::fail(-2, "verify_tree: vocab %d above %d", vocab, kMaxVocab);
+    if (batch > 0x3fffff || int64_t(batch) * sampled > 0xffffff)
+        return nvr::fail(-2, "verify_tree: %d sequences over %d tokens exceed one launch", batch, vocab);
     // Eight blocks a CU in all, so that none has to wait for another's end.
     const int sides = draft_logits ? 2 : 1;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256;

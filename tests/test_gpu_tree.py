@@ -315,7 +315,7 @@ class Drafts:
 @pytest.mark.parametrize("sizes,vocab,fan", [
     ([1], 1, 1), ([1, 1, 1], 151936, 1), ([5], 151936, 1), ([2, 3, 2], 2, 2), ([6, 1, 0, 9, 13, 25], 2048, 3),
     ([64, 40, 7], 2049, 4), ([8] * 30, 509, 1), ([13] * 12, 50257, 3), ([9, 17, 4], 32000, 4), ([20] * 9, 7, 3),
-    ([63, 64], 4096, 2), ([33, 5], 20011, 4),
+    ([63, 64], 4096, 2), ([33, 5], 20011, 4), ([3], (1 << 22) + 5, 2),
 ])
 def test_verification_of_trees(gpu, sizes, vocab, fan, draft):
     Drafts(sizes, vocab, 1000 + len(sizes) + vocab % 97, draft, fan).run(gpu)
@@ -545,6 +545,49 @@ def test_tree_operators_replay_in_a_graph(gpu):
         t.buffers[7].upload(t.out)
         t.launch(gpu)
         assert np.array_equal(t.result(), replayed)
+
+
+def test_contexts_run_at_once(gpu):
+    """Two contexts, each with its stream, its buffers and its workspaces: calls of both in flight together give what
+    each gives alone."""
+    other = nvr.Gpu()
+    sides = []
+    for i, g in enumerate((gpu, other)):
+        t = Trees([25, 9, 33], [2000, 700 + i, 90], 16, 8, 128, 16, 3300 + i).upload(g)
+        sides.append((g, t, Drafts([25, 9, 33], 20011, 3310 + i, True).upload(g)))
+        g.sync()
+    for _ in range(20):
+        for g, t, d in sides:
+            t.launch(g)
+            d.launch(g)
+    for g, t, d in sides:
+        g.sync()
+        t.check(t.result())
+        d.check()
+        first = t.result()
+        t.buffers[7].upload(t.out)
+        t.launch(g)
+        assert np.array_equal(t.result(), first)
+
+
+def test_c_entries_refuse_what_does_not_fit(gpu):
+    """Workspaces that are missing or unaligned, vocabularies and launches past the limits: the C entries return -2
+    before they launch anything, whatever the other arguments."""
+    lib, h = gpu.lib, gpu.handle
+    tree = lambda work, rows, qh, kvh, batch, nodes, context, dim=128, bs=16: lib.nv_attention_tree(  # noqa: E731
+        h, *[None] * 8, work, rows, qh, kvh, dim, bs, 4, 4, batch, nodes, context)
+    verify = lambda work, rows, batch, vocab: lib.nv_verify_tree(  # noqa: E731
+        h, *[None] * 11, work, rows, batch, 4, vocab)
+    some = gpu.alloc(64)
+    for status in (tree(None, 25, 16, 8, 1, 25, 4000), tree(some.ptr + 8, 25, 16, 8, 1, 25, 4000),
+                   tree(some.ptr, 2 ** 28, 16, 8, 4, 8, 64), tree(some.ptr, 8, 2 ** 16, 2 ** 16, 2 ** 16, 8, 64),
+                   tree(some.ptr, 8, 8, 8, 2 ** 22, 8, 64), tree(some.ptr, 8, 8, 8, 2 ** 20, 64, 64, bs=5),
+                   verify(None, 8, 2, 100), verify(some.ptr + 8, 8, 2, 100), verify(some.ptr, 8, 2, 2 ** 26 + 1),
+                   verify(some.ptr, 8, 2 ** 22, 100), verify(some.ptr, 8, 2 ** 20, 2 ** 20),
+                   lib.nv_kv_compact(h, *[None] * 6, 2 ** 24, 4, 1, 8, 128, 16, 4, 4),
+                   lib.nv_kv_compact(h, *[None] * 6, 4, 4, 65536, 8, 128, 16, 4, 4),
+                   lib.nv_kv_copy_blocks(h, *[None] * 5, 2 ** 20, 28, 8, 128, 16, 4)):
+        assert status == -2
 
 
 # -------------------------------------------------------- a step as a whole ----

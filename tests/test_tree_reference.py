@@ -187,3 +187,6 @@ def test_workspace_sizes_refuse_bad_dimensions():
         args[i] = 0
         with pytest.raises(nvr.ArgumentError):
             gpu.attention_tree_workspace(*args)
+    for big in ((2 ** 28, 16, 8, 128, 2, 4, 100), (8, 16, 16, 128, 2 ** 28, 4, 100)):
+        with pytest.raises(nvr.BackendError):
+            gpu.attention_tree_workspace(*big)
