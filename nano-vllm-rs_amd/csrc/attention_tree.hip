@@ -62,8 +62,10 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int s) {
     return t;
 }
 
-// Any head dim and alignment: a block per (node, q head), its four waves over
-// every fourth position, lanes over the head's elements.
+// Any head dim, block size and alignment: a block per (node, q head), its four
+// waves over every fourth position, lanes over the head's elements. Bound by the
+// chain of one position's load, dot product and 64-lane sum after the other: with
+// heads of 128, 8 trees of 25 nodes at 1030 positions take 650 us (the tile form 21).
 __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
     constexpr int kWaves = 4, kElems = 4;  // 64 lanes x 4 elements: head dims up to 256
     __shared__ float part_m[kWaves], part_l[kWaves], part_o[kWaves][256];
@@ -208,6 +210,25 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
     return (tiles + used - 1) / used;
 }
 
+// A block a (sequence, KV head, chunk of its query rows, split of its positions).
+// The query rows of a KV head are its tree's nodes times the q heads over it: all
+// of a chunk share one read of K and V, whose tiles of T positions come into a ring
+// of NS stages by copies that bypass the registers, each wave its own rows of every
+// tile. One pass, with each row's running maximum and sum:
+//  - scores transposed, K q^T: a lane then holds four positions of one query row for
+//    each 16, just as the second product wants its weights, which therefore never
+//    leave registers; the row's maximum needs two exchanges, and only where it grew.
+//  - outputs transposed, V^T p: V is read from LDS transposed by the hardware.
+// Chunks lie swizzled in LDS, so that neither read has bank conflicts. Sequences are
+// split, in parts of at least 256 positions, until the blocks fill the CUs; the parts
+// meet in attention_tree_join.
+//
+// What bounds it, on MI355X (times with the join's): with few rows the read of the
+// cache, 64 chains of 6 nodes at 4090 positions 154 us, 5.4 TB/s; with many the copies
+// into LDS, 4 trees of 64 at 16000 65 us, 4.0 TB/s and 0.45 PFLOP/s (as long without
+// the products); with eight q heads a KV head the weights' arithmetic, which the waves
+// of one block do together, 16 trees of 33 at 2000 31 us; small calls the launch (3 us),
+// the tables and the first tiles, one chain of 4 at 180 8.7 us.
 template <typename S>
 __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
                                                                         int least, int page_shift) {
@@ -611,7 +632,9 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 }
 
 // The splits of each row, where there was more than one: a thread four elements
-// of one (node, head), its splits' loads in flight together.
+// of one (node, head), its splits' loads in flight together. Bound by its launch and
+// one memory round trip: 4.2 us for 200 rows of 16 heads in 5 splits, 5.6 for 256 rows
+// in 8 (17 MB of partial outputs).
 __global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int tile, int least, int parts) {
     constexpr int kBatch = 8;
     const int item = int(blockIdx.x / unsigned(parts));

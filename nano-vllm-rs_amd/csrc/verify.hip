@@ -52,8 +52,9 @@ using nvr::kWave;
 constexpr int kMaxNodes = 64;
 constexpr int kMaxVocab = 1 << 26;
 constexpr int kThreads = 256;
-constexpr int kLoads = 4;             // 16-byte loads in flight a thread of launch 1
-constexpr int kShare = kLoads * kThreads;  // 16-byte chunks a block of launch 1, at least
+constexpr int kLoads = 2;             // 16-byte loads a thread and step of launch 1, the next step's in flight
+constexpr int kShare = 4 * kThreads;  // 16-byte chunks a block of launch 1, at least
+constexpr int kResident = 5;          // its blocks a CU
 constexpr int kSampled = kThreads * 8;               // tokens a block of launch 3
 constexpr int kSlices = 16;                          // blocks a sequence of the walk, with draft logits
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
@@ -222,8 +223,12 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
 // A block a (sequence, share, model). T > 0: one pass with an offset near the
 // maximum of each thread's first loads; a sum that leaves fp32's range, or a NaN,
 // is taken again with care. Bound by the read of the logits and, at four
-// instructions and an exponential a token, nearly as much by its issue.
-__global__ __launch_bounds__(kThreads, 6) void verify_stats(VerifyArgs a) {
+// instructions and an exponential a token, nearly as much by its issue; five
+// resident blocks a CU with the next two loads in flight beat eight of four loads
+// that wait for each other, in two rounds (whole calls, vocabulary 151936: 24 trees
+// of 25 31.2 against 36.9 us, 128 chains of 4 58.2, 70.2; six blocks 31.3, 59.6, four
+// 30.8, 59.1, eight 32.1, 61.1).
+__global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a) {
     constexpr int kWaves = kThreads / kWave;
     __shared__ float tops[kWaves], sums[kWaves];
     __shared__ int first;
@@ -265,6 +270,11 @@ __global__ __launch_bounds__(kThreads, 6) void verify_stats(VerifyArgs a) {
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) packed[u] = nvr::load_stream(x + 8 * int64_t(min(k + u * kThreads, hi - 1)) - lead);
         };
+        auto take = [&](int k, uint4 (&packed)[kLoads], uint4 (&now)[kLoads]) {  // step k, the next one's loads under way
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) now[u] = packed[u];
+            if (k + kLoads * kThreads < hi) load(k + kLoads * kThreads, packed);
+        };
         auto loaded = [&](int c, const uint4& packed, float (&f)[8]) {
             const uint32_t none = 0xff80ff80u;  // -inf: weighs nothing
             const bool in = c < hi;
@@ -292,30 +302,30 @@ __global__ __launch_bounds__(kThreads, 6) void verify_stats(VerifyArgs a) {
             high *= scale;
             mine.offset = fabsf(high) < kInf ? __builtin_rintf(high) : 0.0f;
             mine.sum = __builtin_amdgcn_exp2f(__builtin_fmaf(edge, scale, -mine.offset));
-            for (int k = begin_k; k < hi;) {
+            for (int k = begin_k; k < hi; k += kLoads * kThreads) {
+                uint4 now[kLoads];
+                take(k, packed, now);
 #pragma unroll
                 for (int u = 0; u < kLoads; ++u) {
                     float f[8], eight = 0.0f;
-                    loaded(k + u * kThreads, packed[u], f);
+                    loaded(k + u * kThreads, now[u], f);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], scale, -mine.offset));
                     mine.sum += eight;
                 }
-                k += kLoads * kThreads;
-                if (k < hi) load(k, packed);
             }
             if (!(mine.sum < 0x1p100f)) careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &mine.offset, &mine.sum);
             if (!(mine.sum > 0.0f)) mine.offset = -kInf;
         } else {
             if (edge == edge && lone >= 0 && lone < a.vocab) { mine.offset = edge; where = -1; }
-            for (int k = begin_k; k < hi;) {
-                const float high = highest(k, packed);
+            for (int k = begin_k; k < hi; k += kLoads * kThreads) {
+                uint4 now[kLoads];
+                take(k, packed, now);
+                const float high = highest(k, now);
                 if (high > mine.offset || (where < 0 && high == mine.offset)) {
                     mine.offset = high;
                     where = k;
                 }
-                k += kLoads * kThreads;
-                if (k < hi) load(k, packed);
             }
         }
         const float high = wave_max(mine.offset);
@@ -852,10 +862,10 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
     const int sampled = sample_blocks(vocab);
     if (batch > 0x3fffff || int64_t(batch) * sampled > 0xffffff)
         return nvr::fail(-2, "verify_tree: %d sequences over %d tokens exceed one launch", batch, vocab);
-    // Eight blocks a CU in all, so that none has to wait for another's end.
+    // As many blocks as are resident, so that none has to wait for another's end.
     const int sides = draft_logits ? 2 : 1;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256;
-    const int blocks = int(std::min<int64_t>(std::max<int64_t>(8 * cus / (int64_t(batch) * sides), 1),
+    const int blocks = int(std::min<int64_t>(std::max<int64_t>(kResident * cus / (int64_t(batch) * sides), 1),
                                              int64_t(most_parts(vocab)) * std::max(max_nodes - 1, 1)));
     const Workspace w = layout(rows, batch, vocab);
     char* base = static_cast<char*>(workspace);
