@@ -126,6 +126,17 @@ __device__ __forceinline__ void load_chunk(const uint16_t* row, int64_t t, int v
         for (int i = 0; i < 8; ++i) f[i] = t + i >= 0 && t + i < vocab ? nvr::bf16_to_f32(row[t + i]) : __builtin_nanf("");
     }
 }
+// The same as it lies there, for a later unpack8; `whole`: the row's chunks are at multiples of 16 bytes.
+__device__ __forceinline__ uint4 packed_chunk(const uint16_t* row, int64_t t, int vocab, bool whole) {
+    if (whole && t >= 0 && t + 8 <= vocab) return nvr::load_stream(row + t);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t lo = t + 2 * i, hi = lo + 1;
+        w[i] = (lo >= 0 && lo < vocab ? row[lo] : 0x7fc0u) | (hi >= 0 && hi < vocab ? row[hi] : 0x7fc0u) << 16;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinterpret_cast<uintptr_t>(row) >> 1 & 7); }
 
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
@@ -142,19 +153,20 @@ struct Best {
 __device__ __forceinline__ void consider(Best& b, float s, int i) {
     if (nvr::better(s, i, b.score, b.index)) { b.score = s; b.index = i; }
 }
-__device__ __forceinline__ Best wave_best(Best b) {
-#pragma unroll
-    for (int mask = 1; mask < kWave; mask <<= 1) {
-        const float s = nvr::xor_lane(b.score, mask);
-        const int i = nvr::xor_lane(b.index, mask);
-        consider(b, s, i);
-    }
-    return b;
-}
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int mask = 1; mask < kWave; mask <<= 1) v = fmaxf(v, nvr::xor_lane(v, mask));
     return v;
+}
+// The wave's best: its top score, and of the lanes that have it the lowest index.
+__device__ __forceinline__ Best wave_best(Best b) {
+    const float top = wave_max(b.score);
+    int index = b.score == top ? b.index : nvr::kNoIndex;
+    const uint64_t holds = __ballot(index != nvr::kNoIndex);
+    if ((holds & (holds - 1)) == 0) return Best{top, holds != 0 ? __builtin_amdgcn_readlane(index, __builtin_ctzll(holds)) : nvr::kNoIndex};
+#pragma unroll
+    for (int mask = 1; mask < kWave; mask <<= 1) index = min(index, nvr::xor_lane(index, mask));
+    return Best{top, index};
 }
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
@@ -711,6 +723,9 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
     const uint64_t seed = a.seeds[s];
     const uint16_t* x = a.logits + int64_t(row) * a.vocab;
     const int64_t t = int64_t(part) * kSampled + 8 * int(threadIdx.x) - lead_of(x);
+    const Rows rest{x, c > 0.0f ? a.draft + int64_t(row) * a.vocab : x, e->offset, e->inv_sum, e->draft_offset, e->draft_inv_sum};
+    uint4 packed_q = {};
+    if (c > 0.0f) packed_q = packed_chunk(rest.draft, t, a.vocab, lead_of(rest.draft) == lead_of(x));
     float f[8];
     load_chunk(x, t, a.vocab, f);
     if (int(threadIdx.x) < count) tried[threadIdx.x] = e->token[threadIdx.x];
@@ -721,19 +736,12 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
     } else {
         if (c > 0.0f) {  // ln(p - c q) in place of the logits
-            const Rows r{x, a.draft + int64_t(row) * a.vocab, e->offset, e->inv_sum, e->draft_offset, e->draft_inv_sum};
-            const RestTerm term(r, c, kLog2e / temperature);
-            float y[8];
-            if (lead_of(r.draft) == lead_of(x)) {
-                load_chunk(r.draft, t, a.vocab, y);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    y[i] = t + i >= 0 && t + i < a.vocab ? nvr::bf16_to_f32(r.draft[t + i]) : __builtin_nanf("");
-            }
+            const RestTerm term(rest, c, kLog2e / temperature);
+            float q[8];
+            nvr::unpack8(packed_q, q);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float w = term(f[i], y[i]);
+                const float w = term(f[i], q[i]);
                 f[i] = w >= 0x1p-126f ? w : __builtin_nanf("");
             }
         }
