@@ -236,9 +236,10 @@ int nv_sample_parallel_static(nv_context* c, const void* logits, const void* tem
  * (contexts: [batch] i32, positions committed before node 0), wherever in the
  * tree it stands. Node i's RoPE position is contexts[s] + its depth. */
 
-/* Bytes of workspace that nv_attention_tree needs for these arguments (0: none,
- * and NULL will do); a host function, no device work. A workspace's contents do not matter and stay unspecified;
- * calls that may overlap need one each. */
+/* Bytes of workspace that nv_attention_tree needs for these arguments, the call's
+ * own (0: none, and NULL will do); a host function, no device work. A workspace
+ * starts at a multiple of 16 bytes (else -2), its contents do not matter before a
+ * call and are unspecified after; calls that may overlap need one each. */
 int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, int max_nodes, int max_context,
                                 size_t* bytes);
 
@@ -251,14 +252,18 @@ int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, i
  * bs) positions, a negative context, or a score that is not finite at the maximum;
  * positions in blocks outside [0, blocks) are not seen. Rows of no sequence are
  * left as they were. max_context is any positive bound on a sequence's positions
- * (contexts[s] + nodes) and, like max_nodes, sizes the launch. Returns -2 for
- * qh % kvh != 0, an odd head dim or one above 256, max_nodes outside [1, 64]. */
+ * (contexts[s] + nodes) and, like max_nodes, sizes the launch. Head dims that are
+ * multiples of 8 in blocks of multiples of 16 positions, with q, kc, vc and out at
+ * multiples of 16 bytes, take the matrix instructions, which round the weights to
+ * bf16; others a kernel for any layout, many times slower. Returns -2 for
+ * qh % kvh != 0, an odd head dim or one above 256, max_nodes outside [1, 64], and
+ * sizes past one launch (2^32 threads) or past int32 (rows * qh, batch * kvh). */
 int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* vc, const void* contexts,
                       const void* row_starts, const void* masks, const void* tables, void* out, void* workspace,
                       int rows, int qh, int kvh, int dim, int bs, int blocks, int stride, int batch, int max_nodes,
                       int max_context);
 
-/* Bytes of workspace that nv_verify_tree needs (16-byte aligned); a host function. */
+/* Bytes of workspace that nv_verify_tree needs, under the same rules as nv_attention_tree's. */
 int nv_verify_tree_workspace(int rows, int batch, int vocab, size_t* bytes);
 
 /* Rejection sampling of the trees' drafted tokens: the path that the target
@@ -272,9 +277,12 @@ int nv_verify_tree_workspace(int rows, int batch, int vocab, size_t* bytes);
  * i32, the accepted tokens, then the token after them, then -1; out_nodes: [batch,
  * max_nodes] i32, the path's nodes from 0 on, then -1; out_counts: [batch] i32, how
  * many of either (0 for a sequence without rows, or with more than max_nodes, or
- * with rows outside [0, rows)). vocab is at most 2^26 (else -2). For temps > 0 the tokens are distributed as the
+ * with rows outside [0, rows)). For temps > 0 the tokens are distributed as the
  * target's samples; for temps <= 0 they are its argmaxes. With nothing rejected at
- * the path's last node, the token after it is nv_sample's for that row. */
+ * the path's last node, the token after it is nv_sample's for that row. Drafted
+ * tokens outside [0, vocab) and nodes whose parent does not come before them are
+ * passed over. Returns -2 for max_nodes outside [1, 64], vocab above 2^26, and sizes
+ * past one launch (batch above 2^22 - 1, or 2^32 threads over the vocabularies). */
 int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, const void* tokens,
                    const void* parents, const void* row_starts, const void* temps, const void* uniforms,
                    const void* seeds, void* out_tokens, void* out_nodes, void* out_counts, void* workspace, int rows,
@@ -284,9 +292,10 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
  * + j for j < counts[s], in every layer. nodes ([batch, max_nodes] i32) and counts
  * ([batch] i32) are nv_verify_tree's out_nodes and out_counts; a sequence's nodes
  * must rise from nodes[s, 0] >= 0 (moves stop at the first that does not, or that
- * is not below max_nodes). kc, vc: [layers, blocks, bs, kvh, dim] bf16 (layers 1 for
- * a layer by itself). Moves that touch a block outside [0, blocks) or a position
- * past the table are left out; no sequence may read a slot that another writes. */
+ * is not below max_nodes; a count above max_nodes moves nothing). kc, vc: [layers,
+ * blocks, bs, kvh, dim] bf16 (layers 1 for a layer by itself). Moves that touch a
+ * block outside [0, blocks) or a position past the table are left out; no sequence
+ * may read a slot that another writes. */
 int nv_kv_compact(nv_context* c, void* kc, void* vc, const void* contexts, const void* nodes, const void* counts,
                   const void* tables, int batch, int max_nodes, int layers, int kvh, int dim, int bs, int blocks,
                   int stride);
