@@ -374,27 +374,19 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
     }
 }
 
-// A row's parts folded, by one lane: a wave folds every node of a tree at once.
-__device__ __forceinline__ Stats fold(const Stats* part, int parts) {
-    constexpr int kBatch = 8;
-    Best b{-kInf, nvr::kNoIndex};
-    for (int i0 = 0; i0 < parts; i0 += kBatch) {
-        Stats t[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) consider(b, t[u].offset, t[u].best);
-    }
-    double sum = 0.0;
-    for (int i0 = 0; i0 < parts; i0 += kBatch) {
-        Stats t[kBatch];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) t[u] = part[min(i0 + u, parts - 1)];
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-            if (i0 + u < parts) sum += double(at_offset(t[u].sum, t[u].offset, b.score));
-    }
-    return Stats{b.score, float(sum), b.index, 0};
+// Parts folded over a wave, a part a lane (of more than 64 some).
+__device__ __forceinline__ Stats fold(const Stats& mine, double sum) {
+    const Best b = wave_best(Best{mine.offset, mine.best});
+    const double scaled = sum > 0.0 ? ldexp(sum, mine.offset == b.score ? 0 : int(fmaxf(mine.offset - b.score, -1000.0f))) : 0.0;
+    return Stats{b.score, float(wave_sum(scaled)), b.index, 0};
+}
+__device__ __forceinline__ void add_part(Stats& mine, double& sum, const Stats& t) {
+    Best b{mine.offset, mine.best};
+    consider(b, t.offset, t.best);
+    sum = ldexp(sum, sum > 0.0 && mine.offset != b.score ? int(fmaxf(mine.offset - b.score, -1000.0f)) : 0) +
+          double(at_offset(t.sum, t.offset, b.score));
+    mine.offset = b.score;
+    mine.best = b.index;
 }
 
 // The target's and the draft model's probabilities of a row's tokens.
@@ -538,11 +530,38 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         xt = nvr::bf16_to_f32(a.logits[at]);
         if (drafted) xd = nvr::bf16_to_f32(a.draft[at]);
     }
-    if (wave < (drafted ? 2 : 1) && (inner >> lane & 1) != 0) {
-        const Shares shares(a.vocab, __popcll(inner), a.blocks);
-        const int i = __popcll(inner & ((uint64_t(1) << lane) - 1));
-        (wave ? draft : target)[lane] = fold((wave ? a.draft_stats : a.stats) + int64_t(start + lane) * a.parts,
-                                             shares.last_block(i) - shares.first_block(i) + 1);
+    // The stats of the nodes with children, a wave a node and model: kBatch nodes' loads in flight together.
+    {
+        constexpr int kBatch = 4;
+        const int count = __popcll(inner), items = count * (drafted ? 2 : 1);
+        const Shares shares(a.vocab, max(count, 1), a.blocks);
+        uint64_t left = inner;
+        int at = 0;  // nodes taken off left
+        for (int first = wave; first < items; first += kBatch * kWalkWaves) {
+            int node[kBatch], parts[kBatch];
+            const Stats* from[kBatch];
+            Stats t[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int item = min(first + u * kWalkWaves, items - 1), side = item >= count ? 1 : 0, i = item - side * count;
+                if (i < at) { left = inner; at = 0; }
+                for (; at < i; ++at) left &= left - 1;
+                node[u] = __builtin_ctzll(left);
+                parts[u] = shares.last_block(i) - shares.first_block(i) + 1;
+                from[u] = (side ? a.draft_stats : a.stats) + int64_t(start + node[u]) * a.parts;
+                t[u] = from[u][min(lane, parts[u] - 1)];
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (first + u * kWalkWaves >= items) continue;
+                Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
+                double sum = 0.0;
+                if (lane < parts[u]) add_part(mine, sum, t[u]);
+                for (int i = lane + kWave; i < parts[u]; i += kWave) add_part(mine, sum, from[u][i]);
+                const Stats all = fold(mine, sum);
+                if (lane == 0) (first + u * kWalkWaves >= count ? draft : target)[node[u]] = all;
+            }
+        }
     }
     __syncthreads();
     auto rows_of = [&](int v) {
@@ -580,11 +599,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         }
     };
     auto read_rests = [&](uint64_t which, const double* from, double* to) {
-        if (threadIdx.x < kMaxNodes && (which >> threadIdx.x & 1) != 0) {
-            double sum = 0.0;
-            for (int w = 0; w < slices; ++w)
-                sum += __hip_atomic_load(from + int64_t(start + threadIdx.x) * kSlices + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            to[threadIdx.x] = sum;
+        for (int first = 0; first < n; first += kWalkThreads / kSlices) {  // a thread a node and slice
+            const int v = first + int(threadIdx.x) / kSlices, w = int(threadIdx.x) % kSlices;
+            const bool there = v < kMaxNodes && (which >> (v & 63) & 1) != 0;
+            double sum = there && w < slices ? __hip_atomic_load(from + int64_t(start + v) * kSlices + w, __ATOMIC_RELAXED,
+                                                                 __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+#pragma unroll
+            for (int mask = 1; mask < kSlices; mask <<= 1) sum += __shfl_xor(sum, mask);
+            if (there && w == 0) to[v] = sum;
         }
         __syncthreads();
     };
