@@ -39,12 +39,14 @@
 // 2. verify_walk: a block a sequence folds them and walks the tree; with draft
 // logits several blocks a sequence, in two launches, first sum the rests that the
 // second and third child of a node need. 3. verify_sample: partitions of the last
-// rows; the last block of a sequence stores the token.
+// rows; the last block of a sequence stores the token. Small calls without draft
+// logits walk in 3.
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -71,16 +73,19 @@ struct Stats {
 };
 
 // Where a sequence's walk ended.
+struct Path {
+    int row;    // its last row, or -1: an invalid sequence
+    int node;   // its tokens but the last one
+    int tried;  // tokens to leave out (no draft logits)
+    float c;    // what rejections took (draft logits)
+    float offset, inv_sum, draft_offset, draft_inv_sum;  // of the last row, where c > 0
+};
+// The same for launch 3, and its search for the last token.
 struct Ending {
-    int row;             // the path's last row, or -1: an invalid sequence
-    int node;            // the path's tokens but the last one
-    int tried;           // tokens to leave out (no draft logits)
-    float c;             // what rejections took (draft logits)
-    float offset, inv_sum;  // of the target's row, where c > 0
-    float draft_offset, draft_inv_sum;
-    int blocks;          // of launch 3 that are done
-    uint64_t best;       // their best (score, token), as keys that compare as they do
+    Path path;
     int token[kMaxNodes];
+    uint64_t best;  // the best (score, token) of the blocks so far, as keys that compare as they do
+    int blocks;     // that are done
 };
 
 struct VerifyArgs {
@@ -247,7 +252,11 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int block = int(blockIdx.x % unsigned(a.blocks)), item = int(blockIdx.x / unsigned(a.blocks));
     const int side = item >= a.batch ? 1 : 0, s = item - side * a.batch;
-    if (block == 0 && side == 0 && threadIdx.x == 0) a.arrived[s] = 0;
+    if (block == 0 && side == 0 && threadIdx.x == 0) {
+        a.arrived[s] = 0;
+        a.endings[s].best = 0;
+        a.endings[s].blocks = 0;
+    }
     int start;
     const int n = tree_rows(a, s, &start);
     if (n < 2) return;
@@ -479,17 +488,168 @@ __device__ __forceinline__ bool accepted(double p, double q, double u, double c,
     return rest > 0.0 && u * z * q < rest;
 }
 
-// The walk, kSlices blocks a sequence where there are draft logits, else one. A
-// node's second child needs the sum of the rest after one rejection, its third
-// that after two: a pass over the vocabulary, which one block does at the rate
-// of one CU (50257 tokens 7 us). So with draft logits a first launch (kFirst)
-// sums, slice by slice, the first rests that the walk may come to need, and the
-// second launch the second rests; there the last block of a sequence to finish
+// A sequence's tree: lane i of every wave holds node i.
+struct Tree {
+    int start, n;      // n 0: an invalid sequence
+    int parent, token;
+    double u;
+    bool known;        // a drafted node that can be followed
+    uint64_t inner;    // nodes with children
+};
+__device__ __forceinline__ Tree tree_of(const VerifyArgs& a, int s, int lane) {
+    Tree t;
+    t.n = tree_rows(a, s, &t.start);
+    const bool mine = lane > 0 && lane < t.n;
+    t.parent = mine ? a.parents[t.start + lane] : -1;
+    t.token = mine ? a.tokens[t.start + lane] : -1;
+    t.u = mine ? double(a.uniforms[t.start + lane]) : 0.0;
+    if (t.parent < 0 || t.parent >= lane) t.parent = -1;
+    t.known = t.parent >= 0 && t.token >= 0 && t.token < a.vocab;
+    t.inner = inner_nodes(t.parent);
+    return t;
+}
+// Whether no rests have to be summed: picked or greedy, or no node has a second child to try.
+__device__ __forceinline__ bool no_rests(const VerifyArgs& a, const Tree& t, bool sampled) {
+    return a.draft == nullptr || !sampled || __popcll(__ballot(t.known)) == __popcll(inner_nodes(t.known ? t.parent : -1));
+}
+
+// The stats of the nodes with children, a wave a node and model, kBatch of them in flight together.
+template <int kWaves>
+__device__ __forceinline__ void fold_nodes(const VerifyArgs& a, const Tree& t, bool drafted, int wave, int lane, Stats* target,
+                                           Stats* draft) {
+    constexpr int kBatch = 4;
+    const int count = __popcll(t.inner), items = count * (drafted ? 2 : 1);
+    const Shares shares(a.vocab, max(count, 1), a.blocks);
+    uint64_t left = t.inner;
+    int at = 0;  // nodes taken off left
+    for (int first = wave; first < items; first += kBatch * kWaves) {
+        int node[kBatch], parts[kBatch];
+        const Stats* from[kBatch];
+        Stats part[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int item = min(first + u * kWaves, items - 1), side = item >= count ? 1 : 0, i = item - side * count;
+            if (i < at) { left = t.inner; at = 0; }
+            for (; at < i; ++at) left &= left - 1;
+            node[u] = __builtin_ctzll(left);
+            parts[u] = shares.last_block(i) - shares.first_block(i) + 1;
+            from[u] = (side ? a.draft_stats : a.stats) + int64_t(t.start + node[u]) * a.parts;
+            part[u] = from[u][min(lane, parts[u] - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (first + u * kWaves >= items) continue;
+            Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
+            double sum = 0.0;
+            if (lane < parts[u]) add_part(mine, sum, part[u]);
+            for (int i = lane + kWave; i < parts[u]; i += kWave) add_part(mine, sum, from[u][i]);
+            const Stats all = fold(mine, sum);
+            if (lane == 0) (first + u * kWaves >= count ? draft : target)[node[u]] = all;
+        }
+    }
+}
+__device__ __forceinline__ Rows rows_of(const VerifyArgs& a, int row, const Stats& t, const Stats& d) {
+    const int64_t at = int64_t(row) * a.vocab;
+    return Rows{a.logits + at, a.draft + at, t.sum > 0.0f ? t.offset : 0.0f, inverse(t.sum), d.sum > 0.0f ? d.offset : 0.0f,
+                inverse(d.sum)};
+}
+// The probability of a logit of a row: 2^y, y = k + f, |f| <= 1/2, in fp64 but for 2^f.
+__device__ __forceinline__ double chance(float x, float scale, const Stats& r) {
+    if (!(r.sum > 0.0f) || x != x) return 0.0;
+    if (r.offset == kInf) return x * scale == kInf ? 1.0 / double(r.sum) : 0.0;
+    const double y = double(x) * double(scale) - double(r.offset), k = rint(y);
+    return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
+}
+
+// A path's nodes and tokens, and their number; all but its last token, which launch 3 stores.
+__device__ __forceinline__ void write_path(const VerifyArgs& a, int s, int start, const int* path, int length) {
+    const int step = int(threadIdx.x);
+    if (step < a.max_nodes) {
+        a.out_nodes[int64_t(s) * a.max_nodes + step] = step < length ? path[step] : -1;
+        if (step != length - 1) a.out_tokens[int64_t(s) * a.max_nodes + step] = step < length ? a.tokens[start + path[step + 1]] : -1;
+    }
+    if (step == 0) a.out_counts[s] = length;
+}
+__device__ __forceinline__ void write_nothing(const VerifyArgs& a, int s) {
+    if (int(threadIdx.x) < a.max_nodes)
+        a.out_tokens[int64_t(s) * a.max_nodes + threadIdx.x] = a.out_nodes[int64_t(s) * a.max_nodes + threadIdx.x] = -1;
+    if (threadIdx.x == 0) a.out_counts[s] = 0;
+}
+
+// The walk of a block of kWaves where no rests have to be summed.
+template <int kWaves>
+struct SimpleWalk {
+    Stats target[kMaxNodes], draft[kMaxNodes];
+    int path[kMaxNodes], tried[kMaxNodes];
+    __device__ __forceinline__ Path operator()(const VerifyArgs& a, const Tree& t, float temperature, int wave, int lane) {
+        const bool sampled = temperature > 0.0f, drafted = sampled && a.draft != nullptr;
+        const float scale = kLog2e / temperature;
+        const int parent = t.parent;
+        float xt = 0.0f, xd = 0.0f;
+        if (sampled && t.known) {
+            const int64_t at = int64_t(t.start + parent) * a.vocab + t.token;
+            xt = nvr::bf16_to_f32(a.logits[at]);
+            if (drafted) xd = nvr::bf16_to_f32(a.draft[at]);
+        }
+        fold_nodes<kWaves>(a, t, drafted, wave, lane, target, draft);
+        __syncthreads();
+        const double p = sampled && t.known ? chance(xt, scale, target[parent]) : 0.0;
+        const double q = drafted && t.known ? chance(xd, scale, draft[parent]) : 0.0;
+        // Every wave walks alike.
+        Path end{};
+        int v = 0;
+        uint64_t rejected = 0;
+        for (;; ++end.node) {
+            if (threadIdx.x == 0) path[end.node] = v;
+            uint64_t children = __ballot(t.known && parent == v);
+            const int best = children != 0 && target[v].best != nvr::kNoIndex ? target[v].best : 0;
+            int next = -1;
+            rejected = 0;
+            for (double z = 1.0; children != 0; children &= children - 1) {
+                const int i = __builtin_ctzll(children), x = __builtin_amdgcn_readlane(t.token, i);
+                if (!sampled) {
+                    if (x == best) { next = i; break; }
+                    continue;
+                }
+                const double px = lane_value(p, i), ux = lane_value(t.u, i);
+                if (drafted) {  // the only child
+                    if (accepted(px, lane_value(q, i), ux, 0.0, 1.0)) next = i;
+                    else end.c = 1.0f;
+                    break;
+                }
+                if (__ballot((rejected >> lane & 1) != 0 && t.token == x) != 0) continue;
+                if (px > 0.0 && ux * z < px) { next = i; break; }
+                rejected |= uint64_t(1) << i;
+                z -= px;
+            }
+            if (next < 0) break;
+            v = next;
+        }
+        if (wave == 0 && (rejected >> lane & 1) != 0) tried[__popcll(rejected & ((uint64_t(1) << lane) - 1))] = t.token;
+        __syncthreads();  // path, tried
+        end.row = t.start + v;
+        end.tried = __popcll(rejected);
+        if (end.c > 0.0f) {
+            const Rows r = rows_of(a, end.row, target[v], draft[v]);
+            end.offset = r.offset;
+            end.inv_sum = r.inv_sum;
+            end.draft_offset = r.draft_offset;
+            end.draft_inv_sum = r.draft_inv_sum;
+        }
+        return end;
+    }
+};
+
+// The walk. One block a sequence where no rests are summed. Where drafted siblings
+// were sampled, kSlices blocks: a node's second child needs the sum of the rest
+// after one rejection, its third that after two, a pass over the vocabulary, which
+// one block does at the rate of one CU (50257 tokens 7 us). So a first launch
+// (kFirst) sums, slice by slice, the first rests that the walk may come to need, and
+// the second launch the second rests; there the last block of a sequence to finish
 // walks. Later rests are summed during the walk. Bound by the chain of memory round
 // trips (nodes, their logits, the stats' parts, the rests' parts, the hand-over): 6.7
-// us without draft logits, 4.6 + 6.7 with them where every node has one child, 8.5 +
-// 13.5 for 8 trees of 13 with up to three (in one launch of a block a sequence that
-// call took 5.4 us longer as a whole).
+// us without draft logits, 4.5 + 7 with them where every node has one child, 8.2 +
+// 12.2 for 8 trees of 13 with up to three over 50257 tokens.
 template <bool kFirst>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ Stats target[kMaxNodes], draft[kMaxNodes];
@@ -498,97 +658,48 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ int last;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int s = int(blockIdx.x), slice = int(blockIdx.y), slices = int(gridDim.y);
+    const Tree t = tree_of(a, s, lane);
     Ending* ending = a.endings + s;
-    int start;
-    const int n = tree_rows(a, s, &start);
-    int* tokens = a.out_tokens + int64_t(s) * a.max_nodes;
-    int* nodes = a.out_nodes + int64_t(s) * a.max_nodes;
-    if (n == 0) {
-        if (kFirst || slice != 0) return;
-        for (int i = int(threadIdx.x); i < a.max_nodes; i += kWalkThreads) tokens[i] = nodes[i] = -1;
-        if (threadIdx.x == 0) { a.out_counts[s] = 0; ending->row = -1; }
+    const float temperature = a.temps[s];
+    if (t.n == 0 || no_rests(a, t, temperature > 0.0f)) {
+        if constexpr (!kFirst) {
+            if (slice != 0) return;
+            if (t.n == 0) {
+                write_nothing(a, s);
+                if (threadIdx.x == 0) ending->path.row = -1;
+                return;
+            }
+            __shared__ SimpleWalk<kWalkWaves> walk;
+            const Path end = walk(a, t, temperature, wave, lane);
+            write_path(a, s, t.start, walk.path, end.node + 1);
+            if (int(threadIdx.x) < end.tried) ending->token[threadIdx.x] = walk.tried[threadIdx.x];
+            if (threadIdx.x == 0) ending->path = end;
+        }
         return;
     }
-    const float temperature = a.temps[s];
-    const bool sampled = temperature > 0.0f, drafted = sampled && a.draft != nullptr;
     const float scale = kLog2e / temperature;
-    // Lane i of every wave holds node i.
-    const bool mine = lane > 0 && lane < n;
-    int parent = mine ? a.parents[start + lane] : -1;
-    const int token = mine ? a.tokens[start + lane] : -1;
-    const double u = mine ? double(a.uniforms[start + lane]) : 0.0;
-    if (parent < 0 || parent >= lane) parent = -1;
-    const bool known = parent >= 0 && token >= 0 && token < a.vocab;
-    const uint64_t inner = inner_nodes(parent);
-    // Rests are summed only where a node has a second child to try.
-    const bool alone = !drafted || __popcll(__ballot(known)) == __popcll(inner_nodes(known ? parent : -1));
-    if (alone && (kFirst || slice != 0)) return;
+    const int start = t.start, n = t.n, parent = t.parent;
+    const bool known = t.known;
+    const double u = t.u;
     // The logits of each node's token, under its parent.
     float xt = 0.0f, xd = 0.0f;
-    if (sampled && known) {
-        const int64_t at = int64_t(start + parent) * a.vocab + token;
+    if (known) {
+        const int64_t at = int64_t(start + parent) * a.vocab + t.token;
         xt = nvr::bf16_to_f32(a.logits[at]);
-        if (drafted) xd = nvr::bf16_to_f32(a.draft[at]);
+        xd = nvr::bf16_to_f32(a.draft[at]);
     }
-    // The stats of the nodes with children, a wave a node and model: kBatch nodes' loads in flight together.
-    {
-        constexpr int kBatch = 4;
-        const int count = __popcll(inner), items = count * (drafted ? 2 : 1);
-        const Shares shares(a.vocab, max(count, 1), a.blocks);
-        uint64_t left = inner;
-        int at = 0;  // nodes taken off left
-        for (int first = wave; first < items; first += kBatch * kWalkWaves) {
-            int node[kBatch], parts[kBatch];
-            const Stats* from[kBatch];
-            Stats t[kBatch];
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const int item = min(first + u * kWalkWaves, items - 1), side = item >= count ? 1 : 0, i = item - side * count;
-                if (i < at) { left = inner; at = 0; }
-                for (; at < i; ++at) left &= left - 1;
-                node[u] = __builtin_ctzll(left);
-                parts[u] = shares.last_block(i) - shares.first_block(i) + 1;
-                from[u] = (side ? a.draft_stats : a.stats) + int64_t(start + node[u]) * a.parts;
-                t[u] = from[u][min(lane, parts[u] - 1)];
-            }
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                if (first + u * kWalkWaves >= items) continue;
-                Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
-                double sum = 0.0;
-                if (lane < parts[u]) add_part(mine, sum, t[u]);
-                for (int i = lane + kWave; i < parts[u]; i += kWave) add_part(mine, sum, from[u][i]);
-                const Stats all = fold(mine, sum);
-                if (lane == 0) (first + u * kWalkWaves >= count ? draft : target)[node[u]] = all;
-            }
-        }
-    }
+    fold_nodes<kWalkWaves>(a, t, true, wave, lane, target, draft);
     __syncthreads();
-    auto rows_of = [&](int v) {
-        const int64_t at = int64_t(start + v) * a.vocab;
-        const Stats t = target[v], d = draft[v];
-        return Rows{a.logits + at, a.draft + at, t.sum > 0.0f ? t.offset : 0.0f, inverse(t.sum), d.sum > 0.0f ? d.offset : 0.0f,
-                    inverse(d.sum)};
-    };
-    // Each node's probabilities under its parent's rows: 2^y, y = k + f, |f| <= 1/2, in fp64 but for 2^f.
-    auto chance = [&](float x, const Stats& r) -> double {
-        if (!(r.sum > 0.0f) || x != x) return 0.0;
-        if (r.offset == kInf) return x * scale == kInf ? 1.0 / double(r.sum) : 0.0;
-        const double y = double(x) * double(scale) - double(r.offset), k = rint(y);
-        return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
-    };
-    double p = 0.0, q = 0.0;
-    if (sampled && known) {
-        p = chance(xt, target[parent]);
-        if (drafted) q = chance(xd, draft[parent]);
-    }
+    // Each node's probabilities under its parent's rows.
+    const double p = known ? chance(xt, scale, target[parent]) : 0.0, q = known ? chance(xd, scale, draft[parent]) : 0.0;
+    auto rows_at = [&](int v) { return rows_of(a, start + v, target[v], draft[v]); };
     const int64_t chunks = row_chunks(a.vocab);
     // This block's share of the sums of the nodes' rests, for all slices to see.
     auto sum_rests = [&](uint64_t which, double* to, auto taken) {
         const int64_t share = (chunks + slices - 1) / slices, begin = slice * share;
         for (uint64_t left = which; left != 0; left &= left - 1) {
             const int v = __builtin_ctzll(left);
-            const double sum = wave_sum(rest_sum<1>(rows_of(v), a.vocab, taken(v), scale, begin, min(chunks, begin + share), kWalkThreads));
+            const double sum = wave_sum(rest_sum<1>(rows_at(v), a.vocab, taken(v), scale, begin, min(chunks, begin + share), kWalkThreads));
             if (lane == 0) parts[v][wave] = sum;
         }
         __syncthreads();
@@ -612,115 +723,77 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     };
     // Nodes that the walk may come to (open) and have it reject a first child and try a second: those need the first
     // rest's sum; and those where it rejects a second and tries a third, the second's.
-    uint64_t once = 0, twice = 0;
-    if (!alone) {
-        auto look = [&](bool second) {
-            uint64_t open = 1, found = 0;
-            for (int v = 0; v < n - 1; ++v) {
-                uint64_t children = __ballot(known && parent == v);
-                if (children == 0 || (open >> v & 1) == 0) continue;
-                int i = __builtin_ctzll(children);
-                bool taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 0.0, 1.0);
-                if (!taken && second && (children & (children - 1)) != 0) {
-                    children &= children - 1;
-                    i = __builtin_ctzll(children);
-                    taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 1.0, rests[0][v]);
-                }
+    uint64_t once = 0;
+    auto look = [&](bool second) {
+        uint64_t open = 1, found = 0;
+        for (int v = 0; v < n - 1; ++v) {
+            uint64_t children = __ballot(known && parent == v);
+            if (children == 0 || (open >> v & 1) == 0) continue;
+            int i = __builtin_ctzll(children);
+            bool taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 0.0, 1.0);
+            if (!taken && second && (children & (children - 1)) != 0) {
                 children &= children - 1;
-                open |= taken ? uint64_t(1) << i : children;
-                // (children: none left where there was no second)
-                if (!taken && children != 0 && (second ? (once >> v & 1) != 0 : true)) found |= uint64_t(1) << v;
+                i = __builtin_ctzll(children);
+                taken = accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), 1.0, rests[0][v]);
             }
-            return found;
-        };
-        once = look(false);
-        if constexpr (kFirst) {
-            if (once != 0) sum_rests(once, a.rests, [](int) { return 1.0f; });
-            return;
+            children &= children - 1;
+            open |= taken ? uint64_t(1) << i : children;
+            // (children: none left where there was no second)
+            if (!taken && children != 0 && (second ? (once >> v & 1) != 0 : true)) found |= uint64_t(1) << v;
         }
-        read_rests(once, a.rests, rests[0]);
-        twice = look(true);
-        if (twice == 0 && slice != 0) return;
-        if (twice != 0) {
-            sum_rests(twice, a.rests + int64_t(a.rows) * kSlices, [&](int v) { return float(1.0 + rests[0][v]); });
-            __syncthreads();
-            if (threadIdx.x == 0) last = arrive(a.arrived + s) == slices - 1;
-            __syncthreads();
-            if (!last) return;
-            read_rests(twice, a.rests + int64_t(a.rows) * kSlices, rests[1]);
-        }
+        return found;
+    };
+    once = look(false);
+    if constexpr (kFirst) {
+        if (once != 0) sum_rests(once, a.rests, [](int) { return 1.0f; });
+        return;
     }
-    if constexpr (kFirst) return;
+    read_rests(once, a.rests, rests[0]);
+    const uint64_t twice = look(true);
+    if (twice == 0 && slice != 0) return;
+    if (twice != 0) {
+        sum_rests(twice, a.rests + int64_t(a.rows) * kSlices, [&](int v) { return float(1.0 + rests[0][v]); });
+        __syncthreads();
+        if (threadIdx.x == 0) last = arrive(a.arrived + s) == slices - 1;
+        __syncthreads();
+        if (!last) return;
+        read_rests(twice, a.rests + int64_t(a.rows) * kSlices, rests[1]);
+    }
     // Every wave walks alike.
     int v = 0, length = 0;
-    double c = 0.0, z = 1.0;
-    uint64_t rejected = 0;
+    double c = 0.0;
     while (true) {
         if (threadIdx.x == 0) path[length] = v;
         ++length;
         uint64_t children = __ballot(known && parent == v);
-        const int best = children != 0 && target[v].best != nvr::kNoIndex ? target[v].best : 0;
-        c = 0.0; z = 1.0; rejected = 0;
+        double z = 1.0;
+        c = 0.0;
         int next = -1;
         for (int tried = 0; children != 0; ++tried) {
             const int i = __builtin_ctzll(children);
             children &= children - 1;
-            const int x = __builtin_amdgcn_readlane(token, i);
-            if (!sampled) {
-                if (x == best) { next = i; break; }
-                continue;
-            }
-            const double px = lane_value(p, i), ux = lane_value(u, i);
-            if (drafted) {
-                if (accepted(px, lane_value(q, i), ux, c, z)) { next = i; break; }
-                c += z;
-                if (children == 0) break;
-                if (tried < 2) {
-                    z = rests[tried][v];
-                } else {
-                    const double sum = wave_sum(rest_sum<4>(rows_of(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
-                    if (lane == 0) parts[0][wave] = sum;
-                    __syncthreads();
-                    z = 0.0;
-                    for (int w = 0; w < kWalkWaves; ++w) z += parts[0][w];
-                    __syncthreads();
-                }
+            if (accepted(lane_value(p, i), lane_value(q, i), lane_value(u, i), c, z)) { next = i; break; }
+            c += z;
+            if (children == 0) break;
+            if (tried < 2) {
+                z = rests[tried][v];
             } else {
-                if (__ballot((rejected >> lane & 1) != 0 && token == x) != 0) continue;
-                if (px > 0.0 && ux * z < px) { next = i; break; }
-                rejected |= uint64_t(1) << i;
-                z -= px;
+                const double sum = wave_sum(rest_sum<4>(rows_at(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
+                if (lane == 0) parts[0][wave] = sum;
+                __syncthreads();
+                z = 0.0;
+                for (int w = 0; w < kWalkWaves; ++w) z += parts[0][w];
+                __syncthreads();
             }
         }
         if (next < 0) break;
         v = next;
     }
     __syncthreads();  // path
-    const int step = int(threadIdx.x);
-    if (step < a.max_nodes) {
-        nodes[step] = step < length ? path[step] : -1;
-        tokens[step] = step + 1 < length ? a.tokens[start + path[step + 1]] : -1;
-    }
-    if (wave == 0) {
-        const bool out = (rejected >> lane & 1) != 0;
-        const uint64_t all = __ballot(out);
-        if (out) ending->token[__popcll(all & ((uint64_t(1) << lane) - 1))] = token;
-        if (lane == 0) {
-            a.out_counts[s] = length;
-            ending->row = start + v;
-            ending->node = length - 1;
-            ending->tried = __popcll(all);
-            ending->c = float(c);
-            ending->blocks = 0;
-            ending->best = 0;
-            if (c > 0.0) {
-                const Rows r = rows_of(v);
-                ending->offset = r.offset;
-                ending->inv_sum = r.inv_sum;
-                ending->draft_offset = r.draft_offset;
-                ending->draft_inv_sum = r.draft_inv_sum;
-            }
-        }
+    write_path(a, s, start, path, length);
+    if (threadIdx.x == 0) {
+        const Rows r = rows_at(v);
+        ending->path = Path{start + v, length - 1, 0, float(c), r.offset, r.inv_sum, r.draft_offset, r.draft_inv_sum};
     }
 }
 
@@ -738,34 +811,53 @@ __device__ __forceinline__ uint64_t key_of(const Best& b) {
 // a token, six of them multiplications at a quarter of the rate; 48 rows of 151936
 // tokens take 21 us, 24 rows 10.5. Blocks of two or four times the tokens gained 1 us
 // in 49 there and lost as much at 24 rows.
+// kWalks: every block walks its tree by itself, which saves launch 2.
+template <bool kWalks>
 __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
     constexpr int kWaves = kThreads / kWave;
     __shared__ Best tops[kWaves];
+    __shared__ std::conditional_t<kWalks, SimpleWalk<kWaves>, int> walk;
     __shared__ int tried[kMaxNodes];
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int s = int(blockIdx.x), part = int(blockIdx.y), parts = int(gridDim.y);
     Ending* e = a.endings + s;
-    const int row = e->row;
-    if (row < 0) return;
-    const int count = e->tried;
-    const float temperature = a.temps[s], c = e->c;
+    const float temperature = a.temps[s], scale = kLog2e / temperature;
     const uint64_t seed = a.seeds[s];
+    Path path;
+    if constexpr (kWalks) {
+        const Tree tree = tree_of(a, s, lane);
+        if (tree.n == 0) {
+            if (part == 0) write_nothing(a, s);
+            return;
+        }
+        path = walk(a, tree, temperature, wave, lane);
+        if (part == 0) write_path(a, s, tree.start, walk.path, path.node + 1);
+    } else {
+        path = e->path;
+    }
+    const int row = path.row, node = path.node, count = path.tried;
+    if (row < 0) return;
+    const float c = path.c;
     const uint16_t* x = a.logits + int64_t(row) * a.vocab;
     const int64_t t = int64_t(part) * kSampled + 8 * int(threadIdx.x) - lead_of(x);
-    const Rows rest{x, c > 0.0f ? a.draft + int64_t(row) * a.vocab : x, e->offset, e->inv_sum, e->draft_offset, e->draft_inv_sum};
+    const Rows rest{x, c > 0.0f ? a.draft + int64_t(row) * a.vocab : x, path.offset, path.inv_sum, path.draft_offset, path.draft_inv_sum};
     uint4 packed_q = {};
     if (c > 0.0f) packed_q = packed_chunk(rest.draft, t, a.vocab, lead_of(rest.draft) == lead_of(x));
     float f[8];
     load_chunk(x, t, a.vocab, f);
-    if (int(threadIdx.x) < count) tried[threadIdx.x] = e->token[threadIdx.x];
-    __syncthreads();
+    if constexpr (!kWalks) {
+        if (int(threadIdx.x) < count) tried[threadIdx.x] = e->token[threadIdx.x];
+        __syncthreads();
+    }
+    const int* out = tried;
+    if constexpr (kWalks) out = walk.tried;
     Best b{-kInf, nvr::kNoIndex};
     if (!(temperature > 0.0f)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
     } else {
         if (c > 0.0f) {  // ln(p - c q) in place of the logits
-            const RestTerm term(rest, c, kLog2e / temperature);
+            const RestTerm term(rest, c, scale);
             float q[8];
             nvr::unpack8(packed_q, q);
 #pragma unroll
@@ -775,7 +867,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
             }
         }
         for (int k = 0; k < count; ++k) {
-            const int64_t at = tried[k] - t;
+            const int64_t at = out[k] - t;
             if (at >= 0 && at < 8) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -839,7 +931,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
         asm volatile("" ::"v"(old));  // the returning form
         if (arrive(&e->blocks) == parts - 1) {
             const uint64_t key = __hip_atomic_load(&e->best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (key != 0) a.out_tokens[int64_t(s) * a.max_nodes + e->node] = int(~uint32_t(key));
+            if (key != 0) a.out_tokens[int64_t(s) * a.max_nodes + node] = int(~uint32_t(key));
             else nothing = true;
         }
     }
@@ -854,7 +946,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
     }
     block_best();
-    if (threadIdx.x == 0) a.out_tokens[int64_t(s) * a.max_nodes + e->node] = b.index == nvr::kNoIndex ? 0 : b.index;
+    if (threadIdx.x == 0) a.out_tokens[int64_t(s) * a.max_nodes + node] = b.index == nvr::kNoIndex ? 0 : b.index;
 }
 
 // The workspace's parts, each at a multiple of 16 bytes.
@@ -916,14 +1008,21 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
                        reinterpret_cast<int*>(base + w.arrived), rows, batch, max_nodes, vocab, most_parts(vocab), blocks};
     hipLaunchKernelGGL(verify_stats, dim3(unsigned(int64_t(batch) * blocks * sides)), dim3(kThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    const dim3 walk(unsigned(batch), unsigned(draft_logits && max_nodes > 2 ? kSlices : 1));
+    // Up to a block a CU, launch 3 walks by itself (one chain of 5 14.2 us against 16.5, 4 trees of 60 with more
+    // blocks 25.8 against 24.7, 24 of 25 35.0, 30.8).
+    const dim3 sample{unsigned(batch), unsigned(sampled)};
+    if (!draft_logits && int64_t(batch) * sampled <= cus) {
+        hipLaunchKernelGGL(verify_sample<true>, sample, dim3(kThreads), 0, c->stream, a);
+        return nvr::launch_status();
+    }
+    const dim3 walk{unsigned(batch), unsigned(draft_logits && max_nodes > 2 ? kSlices : 1)};
     if (walk.y > 1) {
         hipLaunchKernelGGL(verify_walk<true>, walk, dim3(kWalkThreads), 0, c->stream, a);
         NVR_HIP(hipGetLastError());
     }
     hipLaunchKernelGGL(verify_walk<false>, walk, dim3(kWalkThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    hipLaunchKernelGGL(verify_sample, dim3(unsigned(batch), unsigned(sampled)), dim3(kThreads), 0, c->stream, a);
+    hipLaunchKernelGGL(verify_sample<false>, sample, dim3(kThreads), 0, c->stream, a);
     return nvr::launch_status();
 }
 

@@ -417,6 +417,19 @@ def test_verification_of_invalid_nodes_and_sequences(gpu):
         d.run(gpu)
 
 
+def test_verification_of_invalid_sequences_in_large_calls(gpu):
+    """The same where the call has more blocks than a GPU has CUs, so that the walk is a launch of its own."""
+    d = Drafts([6, 6, 0, 6, 9, 6], 120011, 1650, False, fan=4, temps=(0.9, 0.0, 1.1))
+    d.max_nodes = 6
+    d.tokens[1], d.tokens[8], d.parents[9], d.parents[15] = -1, 120011, -7, 64
+    d.tokens[20] = d.tokens[19]
+    d.uniforms[18:24] = 0.999
+    d.run(gpu)
+    assert d.result()[2][2] == 0 and d.result()[2][4] == 0
+    d.row_starts = np.array([0, 6, 3, 12, -1, 20, 34], np.int32)
+    d.run(gpu)
+
+
 def test_verification_of_unaligned_rows(gpu):
     """Logits whose rows start at every alignment, in a view that starts at any."""
     for draft in (False, True):
