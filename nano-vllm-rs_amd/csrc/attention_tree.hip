@@ -231,7 +231,7 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
 // the tables and the first tiles, one chain of 4 at 180 8.7 us.
 template <typename S>
 __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
-                                                                        int least, int page_shift) {
+                                                                        int least, int page_shift, int spread) {
     constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
     constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS, kThreads = kWave * S::W;
     extern __shared__ __align__(16) unsigned char smem[];  // NS stages of K, then V
@@ -239,12 +239,13 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int n16 = lane & 15, g = lane >> 4;
     const int wq = wave % WQ, wk = wave / WQ;
-    unsigned idx = blockIdx.x;
-    const int kvhead = int(idx % unsigned(a.kvh));
-    idx /= unsigned(a.kvh);
-    const int chunk = int(idx % unsigned(chunks));
-    idx /= unsigned(chunks);
-    const int split = int(idx % unsigned(part.splits)), s = int(idx / unsigned(part.splits));
+    // spread 3: blocks go round the eight XCDs, so the chunks of one part of the cache follow each other on one, whose L2 they share.
+    const unsigned turn = blockIdx.x >> spread;
+    const int chunk = int(turn % unsigned(chunks));
+    unsigned item = turn / unsigned(chunks) << spread | (blockIdx.x & ((1u << spread) - 1));
+    const int kvhead = int(item % unsigned(a.kvh));
+    item /= unsigned(a.kvh);
+    const int split = int(item % unsigned(part.splits)), s = int(item / unsigned(part.splits));
     const TreeSpan span = tree_span(a, s);
     const int group = a.qh / a.kvh;
     if (span.context < 0) {
@@ -794,10 +795,12 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         float* partial = static_cast<float*>(workspace);
         const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
         const int pages = bs / kPage, shift = (pages & (pages - 1)) == 0 ? __builtin_ctz(unsigned(pages)) : -1;
+        // Chunks on one XCD: 32 trees of 24 at 2000 with 8 heads a KV head of 64 37.4 us against 40.6, 16 of 33 31.9, 32.9.
+        const int spread = p.chunks > 1 && p.pairs * p.splits % 8 == 0 ? 3 : 0;
         with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
             using S = decltype(shape);
             hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(unsigned(grid)), dim3(kWave * S::W), S::kLds, c->stream, a,
-                               part, p.chunks, p.least, shift);
+                               part, p.chunks, p.least, shift, spread);
         });
         if (p.splits > 1) {
             NVR_HIP(hipGetLastError());
