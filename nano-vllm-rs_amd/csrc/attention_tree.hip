@@ -226,9 +226,9 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
 // What bounds it, on MI355X (times with the join's): with few rows the read of the
 // cache, 64 chains of 6 nodes at 4090 positions 154 us, 5.4 TB/s; with many the copies
 // into LDS, 4 trees of 64 at 16000 65 us, 4.0 TB/s and 0.45 PFLOP/s (as long without
-// the products); with eight q heads a KV head the weights' arithmetic, which the waves
-// of one block do together, 16 trees of 33 at 2000 31 us; small calls the launch (3 us),
-// the tables and the first tiles, one chain of 4 at 180 8.7 us.
+// the products); with eight q heads a KV head each tile's chain of LDS reads, products
+// and exponentials, 16 trees of 33 at 2000 30 us; small calls the launch (3 us),
+// the tables and the first tiles, one chain of 4 at 180 9 us.
 template <typename S>
 __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
                                                                         int least, int page_shift, int spread) {
@@ -704,8 +704,9 @@ struct Plan {
 //    30.6 against 43.0, at 1000 62.9, 73.8); else eight waves, which need half the splits
 //    to fill a CU (8 of 64 at 8000 74.3 against 69.9, 4 of 64 at 16000 75.8, 69.5).
 //  - heads of 64, 16 of 33 nodes at 2000 with 8 heads a KV head: three blocks of four
-//    waves a CU 32.8, two of eight 34.3, one of eight with twice the rows 44.6. Heads of
-//    256 with two stages: 16 of 40 at 1000 33.8, with four 37.9.
+//    waves a CU 32.8, two of eight 34.3, one of eight with twice the rows 44.6 (each
+//    before its chunks shared an XCD). Heads of 256 with two stages: 16 of 40 at 1000
+//    33.8, with four 37.9.
 template <typename F>
 void with_shape(int dim, int64_t queries, int64_t pairs, F&& f) {
     if (dim == 256) {

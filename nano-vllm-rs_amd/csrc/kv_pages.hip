@@ -18,7 +18,7 @@ constexpr int kMaxNodes = 64;
 // contiguous, so a copy is cut into segments of kSegment chunks whatever the
 // slot size, one a block, all loads of a thread in flight before its stores.
 // Reads and writes bypass the caches' retention: 12 copies of partly filled blocks
-// of 256 positions in 28 layers (559 MB moved) take 84 us, 6.7 TB/s.
+// of 256 positions in 28 layers (559 MB moved) take 84 to 86 us, 6.6 TB/s.
 constexpr int kCopyLoads = 8;
 constexpr int kSegment = 256 * kCopyLoads;
 

@@ -647,9 +647,9 @@ struct SimpleWalk {
 // (kFirst) sums, slice by slice, the first rests that the walk may come to need, and
 // the second launch the second rests; there the last block of a sequence to finish
 // walks. Later rests are summed during the walk. Bound by the chain of memory round
-// trips (nodes, their logits, the stats' parts, the rests' parts, the hand-over): 6.7
-// us without draft logits, 4.5 + 7 with them where every node has one child, 8.2 +
-// 12.2 for 8 trees of 13 with up to three over 50257 tokens.
+// trips (nodes, their logits, the stats' parts, the rests' parts, the hand-over): 6.5
+// us without draft logits, 4.5 + 6.9 with them where every node has one child, 8.8 +
+// 11 for 8 trees of 13 with up to three over 50257 tokens.
 template <bool kFirst>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ Stats target[kMaxNodes], draft[kMaxNodes];
@@ -809,7 +809,7 @@ __device__ __forceinline__ uint64_t key_of(const Best& b) {
 // logarithm bounds it, and only a lane's best bound and the bounds that reach
 // the wave's best score are scored in full. Bound by the hash: about 60 instructions
 // a token, six of them multiplications at a quarter of the rate; 48 rows of 151936
-// tokens take 21 us, 24 rows 10.5. Blocks of two or four times the tokens gained 1 us
+// tokens take 21 us, 24 rows 11. Blocks of two or four times the tokens gained 1 us
 // in 49 there and lost as much at 24 rows.
 // kWalks: every block walks its tree by itself, which saves launch 2.
 template <bool kWalks>
