@@ -144,6 +144,8 @@ __device__ __forceinline__ uint4 packed_chunk(const uint16_t* row, int64_t t, in
 }
 __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinterpret_cast<uintptr_t>(row) >> 1 & 7); }
 
+// log2(e) / T, finite, so that a logit of 0 stays 0.
+__device__ __forceinline__ float scale_of(float temperature) { return fminf(kLog2e / temperature, 0x1.fffffep127f); }
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
 // A sum at one offset, at another that is no smaller.
 __device__ __forceinline__ float at_offset(float sum, float offset, float other) {
@@ -224,7 +226,8 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
     const float at = __builtin_rintf(top);
     auto weight = [&](float v) {
         if (top == kInf) return v * scale == kInf ? 1.0f : 0.0f;
-        return v == v ? __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -at)) : 0.0f;
+        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -at));
+        return w == w ? w : 0.0f;  // nor has an infinite logit a weight where T is infinite
     };
     float total = top > -kInf ? weight(edge) : 0.0f;
     for (int k = begin; k < end && top > -kInf; k += kThreads) {
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
     uint32_t at = block * shares.per;
     const uint32_t stop = min(at + shares.per, count * shares.chunks);
     if (at >= stop) return;
-    const float scale = kLog2e / temperature;
+    const float scale = scale_of(temperature);
     int i = int(at / shares.chunks);
     for (int skip = 0; skip < i; ++skip) inner &= inner - 1;
     for (; at < stop; ++i, inner &= inner - 1) {
@@ -583,7 +586,7 @@ struct SimpleWalk {
     int path[kMaxNodes], tried[kMaxNodes];
     __device__ __forceinline__ Path operator()(const VerifyArgs& a, const Tree& t, float temperature, int wave, int lane) {
         const bool sampled = temperature > 0.0f, drafted = sampled && a.draft != nullptr;
-        const float scale = kLog2e / temperature;
+        const float scale = scale_of(temperature);
         const int parent = t.parent;
         float xt = 0.0f, xd = 0.0f;
         if (sampled && t.known) {
@@ -677,7 +680,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
         }
         return;
     }
-    const float scale = kLog2e / temperature;
+    const float scale = scale_of(temperature);
     const int start = t.start, n = t.n, parent = t.parent;
     const bool known = t.known;
     const double u = t.u;
@@ -821,7 +824,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int s = int(blockIdx.x), part = int(blockIdx.y), parts = int(gridDim.y);
     Ending* e = a.endings + s;
-    const float temperature = a.temps[s], scale = kLog2e / temperature;
+    const float temperature = a.temps[s], scale = scale_of(temperature);
     const uint64_t seed = a.seeds[s];
     Path path;
     if constexpr (kWalks) {

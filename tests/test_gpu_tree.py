@@ -403,6 +403,31 @@ def test_verification_leaves_out_what_was_rejected(gpu):
     d.run(gpu)
 
 
+@pytest.mark.parametrize("vocab", [1000, 120011])  # walks in the last launch, and in one of its own
+def test_verification_at_extreme_temperatures(gpu, vocab):
+    """T infinite: the tokens that are not masked are equally likely. T below the smallest normal number: the largest
+    logits share, zeros among them. Two such tokens have 1/2 each, so u decides, and a rejected one leaves the other."""
+    cases = [(np.inf, -np.inf, 1.0, 0.4, [3, 5]), (np.inf, -np.inf, 1.0, 0.6, [5]), (np.inf, -np.inf, -2.0, 0.6, [5]),
+             (1e-40, -1.0, 0.0, 0.4, [3, 5]), (1e-40, -1.0, 0.0, 0.6, [5]),
+             (1e-40, -1.0, 2.0, 0.4, [3, 5]), (1e-40, -1.0, 2.0, 0.6, [5])]
+    for draft in (False, True):
+        d = Drafts([2] * len(cases), vocab, 1450, draft, fan=1)
+        for s, (t, low, high, u, want) in enumerate(cases):
+            x = np.full((2, vocab), low)
+            x[0, [3, 5]] = high
+            x[1, 5] = high
+            d.logits[2 * s:2 * s + 2] = nvr.bf16_bits(x)
+            if draft:  # every sample is of token 3, which the target accepts with 1/2
+                x[:] = low
+                x[:, 3] = high
+                d.draft[2 * s:2 * s + 2] = nvr.bf16_bits(x)
+            d.temps[s], d.uniforms[2 * s + 1], d.tokens[2 * s + 1] = t, u, 3
+        d.upload(gpu).launch(gpu)
+        tokens, _, counts = d.result()
+        for s, case in enumerate(cases):
+            assert tokens[s, :counts[s]].tolist() == case[4], (draft, s)
+
+
 def test_verification_of_invalid_nodes_and_sequences(gpu):
     """Tokens outside the vocabulary, parents that do not come before their node, sequences without rows, with too
     many, or outside the rows: none is followed, and what is not a sequence gives no tokens."""
