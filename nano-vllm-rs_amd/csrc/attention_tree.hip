@@ -204,8 +204,14 @@ struct Partials {
     int splits;
 };
 
-// Tiles a split: at least about `least`, the same for every split but the last few.
-__device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
+// The fewest positions of a split. One chain of 4 at 180 whole 9.1 us, in two 10.7;
+// parts of 128 against 256: 4 trees of 13 at 500 14.9, 16.1, one chain of 8 at 1000 11.9,
+// 12.9, 8 of 9 at 700 with heads of 64 13.2, 15.3; but one tree of 25 at 4000 19.7, 18.6.
+constexpr int kWhole = 256, kShort = 1024;  // positions that are not split, that are split finely
+
+// Tiles (of 2^shift positions) a split: the same for every split but the last.
+__device__ __forceinline__ int split_tiles(int tiles, int splits, int shift) {
+    const int least = tiles <= kWhole >> shift ? tiles : (tiles <= kShort >> shift ? 128 : 256) >> shift;
     const int per = max((tiles + splits - 1) / splits, least), used = (tiles + per - 1) / per;
     return (tiles + used - 1) / used;
 }
@@ -220,7 +226,7 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
 //    leave registers; the row's maximum needs two exchanges, and only where it grew.
 //  - outputs transposed, V^T p: V is read from LDS transposed by the hardware.
 // Chunks lie swizzled in LDS, so that neither read has bank conflicts. Sequences are
-// split, in parts of at least 256 positions, until the blocks fill the CUs; the parts
+// split, in parts of at least 128 or 256 positions, until the blocks fill the CUs; the parts
 // meet in attention_tree_join.
 //
 // What bounds it, on MI355X (times with the join's): with few rows the read of the
@@ -231,7 +237,7 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int least) {
 // the tables and the first tiles, one chain of 4 at 180 9 us.
 template <typename S>
 __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
-                                                                        int least, int page_shift, int spread) {
+                                                                        int page_shift, int spread) {
     constexpr int DIM = S::DIM, QT = S::QT, WQ = S::WQ, WK = S::WK, T = S::T, KT = S::KT, DT = S::DT, KS = S::KS;
     constexpr int CH = S::CH, R = S::R, COPIES = S::COPIES, NS = S::NS, kThreads = kWave * S::W;
     extern __shared__ __align__(16) unsigned char smem[];  // NS stages of K, then V
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     const int q0 = chunk * share, queries = min(all, q0 + share);
     if (chunk >= shares || q0 >= queries) return;
     const int keys = span.context + span.nodes, tiles = (keys + T - 1) / T;
-    const int per = split_tiles(tiles, part.splits, least), used = (tiles + per - 1) / per;
+    const int per = split_tiles(tiles, part.splits, __builtin_ctz(T)), used = (tiles + per - 1) / per;
     if (split >= used) return;
     const int tile0 = split * per, tile1 = min(tiles, tile0 + per);
 
@@ -327,14 +333,14 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     auto copy_all = [&](const uint32_t (&offset)[COPIES], const uint16_t* base, uint32_t dst) {
         uint32_t saved;
         if constexpr (COPIES == 4)
-            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "1024\n\t" NVR_COPY(5) "2048\n\t" NVR_COPY(6) "3072\n\t")
+            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "0x400\n\t" NVR_COPY(5) "0x800\n\t" NVR_COPY(6) "0xc00\n\t")
                          : "=&s"(saved)
                          : "s"(base), "s"(dst), "v"(offset[0]), "v"(offset[1]), "v"(offset[2]), "v"(offset[3])
                          : "memory");
         else if constexpr (COPIES == 1)
             asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t") : "=&s"(saved) : "s"(base), "s"(dst), "v"(offset[0]) : "memory");
         else
-            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "1024\n\t")
+            asm volatile(NVR_WITH_M0(NVR_COPY(3) "0\n\t" NVR_COPY(4) "0x400\n\t")
                          : "=&s"(saved)
                          : "s"(base), "s"(dst), "v"(offset[0]), "v"(offset[1])
                          : "memory");
@@ -636,14 +642,14 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 // of one (node, head), its splits' loads in flight together. Bound by its launch and
 // one memory round trip: 4.2 us for 200 rows of 16 heads in 5 splits, 5.6 for 256 rows
 // in 8 (17 MB of partial outputs).
-__global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int tile, int least, int parts) {
+__global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int shift, int parts) {
     constexpr int kBatch = 8;
     const int item = int(blockIdx.x / unsigned(parts));
     const int s = item / a.max_nodes, node = item % a.max_nodes;
     const TreeSpan span = tree_span(a, s);
     if (node >= span.nodes || span.context < 0) return;
-    const int tiles = (span.context + span.nodes + tile - 1) / tile;
-    const int per = split_tiles(tiles, part.splits, least), used = (tiles + per - 1) / per;
+    const int tiles = (span.context + span.nodes + (1 << shift) - 1) >> shift;
+    const int per = split_tiles(tiles, part.splits, shift), used = (tiles + per - 1) / per;
     const int quads = a.dim / 4, i = int(blockIdx.x % unsigned(parts)) * 256 + int(threadIdx.x);
     if (used == 1 || i >= a.qh * quads) return;
     const int64_t at = int64_t(span.start + node) * a.qh + i / quads, plane = int64_t(a.rows) * a.qh;
@@ -684,13 +690,11 @@ __global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials 
         make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
 }
 
-constexpr int kSplitPositions = 256;
-
 // The launch's shape: the same for the workspace's size and the launch.
 struct Plan {
     int dim;              // the head dim, rounded up
     int64_t queries, pairs;  // query rows a KV head; (sequence, KV head) pairs
-    int tile, chunks, splits, least;  // positions a tile; blocks a KV head's rows; splits, and the fewest tiles of one
+    int tile, chunks, splits;  // positions a tile; blocks a KV head's rows; splits of the longest sequence
 };
 // The shape for `queries` query rows a KV head, of sequences and KV heads in
 // `pairs`. Microseconds on MI355X, 16 q heads over 8 KV heads of 128, blocks of 256:
@@ -731,8 +735,9 @@ Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_cont
         using S = decltype(shape);
         p.tile = S::T;
         p.chunks = int((p.queries + S::ROWS - 1) / S::ROWS);
-        p.least = kSplitPositions / p.tile;
-        const int64_t blocks = p.pairs * p.chunks, most = (int64_t(max_context) + kSplitPositions - 1) / kSplitPositions;
+        const int64_t blocks = p.pairs * p.chunks, context = max_context;
+        const int64_t fine = (std::min<int64_t>(context, kShort) + 127) / 128;
+        const int64_t most = context <= kWhole ? 1 : std::max(fine, (context + 255) / 256);
         p.splits = int(std::max<int64_t>(1, std::min(most, 256 * S::kBlocks / blocks)));
     });
     return p;
@@ -801,12 +806,12 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
             using S = decltype(shape);
             hipLaunchKernelGGL(attention_tree_tiles<S>, dim3(unsigned(grid)), dim3(kWave * S::W), S::kLds, c->stream, a,
-                               part, p.chunks, p.least, shift, spread);
+                               part, p.chunks, shift, spread);
         });
         if (p.splits > 1) {
             NVR_HIP(hipGetLastError());
-            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(joins)), dim3(256), 0, c->stream, a, part, p.tile,
-                               p.least, int(parts));
+            hipLaunchKernelGGL(attention_tree_join, dim3(unsigned(joins)), dim3(256), 0, c->stream, a, part,
+                               __builtin_ctz(unsigned(p.tile)), int(parts));
         }
         return nvr::launch_status();
     }
