@@ -284,10 +284,12 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
         const uint32_t base = i * shares.chunks;
         const int begin = int(at - base), end = int(min(stop - base, shares.chunks));
         at = base + end;
-        // Whole chunks, and at either end of a row the tokens of one that is not: one each of the first 16 threads'.
+        // Whole chunks, and at either end of a row the tokens of one that is not: one each of the first 16 threads'. A
+        // row in one chunk has one such end.
         const int whole = (a.vocab + lead) / 8, lo = max(begin, lead != 0 ? 1 : 0), hi = min(end, whole);
-        const int lone = threadIdx.x < 8 ? (begin == 0 && lead != 0 ? int(threadIdx.x) - lead : -1)
-                                         : begin <= whole && end > whole && threadIdx.x < 16 ? 8 * whole - lead + int(threadIdx.x) - 8 : -1;
+        const bool head = begin == 0 && lead != 0, tail = begin <= whole && end > whole && (whole > 0 || lead == 0);
+        const int lone = threadIdx.x < 8 ? (head ? int(threadIdx.x) - lead : -1)
+                                         : tail && threadIdx.x < 16 ? 8 * whole - lead + int(threadIdx.x) - 8 : -1;
         float edge = -kInf;
         if (lone >= 0 && lone < a.vocab) edge = nvr::bf16_to_f32(x[lone]);
         auto load = [&](int k, uint4 (&packed)[kLoads]) {

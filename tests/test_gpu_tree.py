@@ -322,6 +322,13 @@ def test_verification_of_trees(gpu, sizes, vocab, fan, draft):
 
 
 @pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("vocab", [1, 2, 3, 4, 5, 6, 7, 8, 9, 15, 16, 17])
+def test_verification_over_few_tokens(gpu, vocab, draft):
+    """Rows that begin and end inside 16 bytes, at every offset."""
+    Drafts([5, 9, 2, 13] * 8, vocab, 1150 + vocab, draft, fan=3, temps=(0.7, 1.0, 0.0, 1.4), likely=2).run(gpu)
+
+
+@pytest.mark.parametrize("draft", [False, True])
 def test_verification_accepts_and_rejects(gpu, draft):
     """Over many sequences every length of path occurs."""
     d = Drafts([6] * 400, 61, 1100, draft, fan=2, temps=(0.7, 1.0, 1.4), likely=3)
