@@ -743,8 +743,10 @@ Plan plan_tiles(int qh, int kvh, int dim, int batch, int max_nodes, int max_cont
     return p;
 }
 
+// A multiple of 16 bytes.
 int64_t workspace_bytes(const Plan& p, int rows, int qh, int dim) {
-    return p.splits == 1 ? 0 : int64_t(p.splits) * rows * qh * (4 * int64_t(dim) + int64_t(sizeof(float2)));
+    const int64_t bytes = int64_t(p.splits) * rows * qh * (4 * int64_t(dim) + int64_t(sizeof(float2)));
+    return p.splits == 1 ? 0 : (bytes + 15) / 16 * 16;
 }
 
 bool too_many(int rows, int qh, int batch, int kvh) {

@@ -190,3 +190,12 @@ def test_workspace_sizes_refuse_bad_dimensions():
     for big in ((2 ** 28, 16, 8, 128, 2, 4, 100), (8, 16, 16, 128, 2 ** 28, 4, 100)):
         with pytest.raises(nvr.BackendError):
             gpu.attention_tree_workspace(*big)
+
+
+@pytest.mark.parametrize("rows,qheads,head_dim", [(7, 5, 128), (1, 1, 8), (3, 3, 40), (64, 16, 128)])
+def test_workspaces_are_as_large_as_a_call_asks(rows, qheads, head_dim):
+    """A buffer of the size that is told is admitted: sizes are whole numbers of the 16 bytes that it is aligned to."""
+    gpu, _ = _fake()
+    for max_context in (1, 300, 700, 1280, 1800, 5000):
+        assert gpu.attention_tree_workspace(rows, qheads, 1, head_dim, 1, min(rows, 64), max_context) % 16 == 0
+    assert gpu.verify_tree_workspace(rows, 3, 77) % 16 == 0
