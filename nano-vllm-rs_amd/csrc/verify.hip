@@ -64,8 +64,10 @@ constexpr float kInf = __builtin_inff();
 
 // Part of a row's logits, or the fold of its parts. T > 0: sum of 2^(x log2(e) / T -
 // offset), the offset a whole number, so that it is subtracted without an error of
-// its own and sums are brought to another one exactly; +inf where the sum counts
-// infinite logits, -inf where there is nothing. Else: the maximum and its token.
+// its own and sums are brought to another one exactly; -inf where there is nothing.
+// An offset that is not below 2^24 (infinite, or the type's lowest value as a mask)
+// is the scaled maximum itself and the sum counts the logits that have it: others
+// are at least 2^15 below. Else: the maximum and its token.
 struct Stats {
     float offset, sum;
     int best;
@@ -146,6 +148,7 @@ __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinter
 
 // log2(e) / T, finite, so that a logit of 0 stays 0.
 __device__ __forceinline__ float scale_of(float temperature) { return fminf(kLog2e / temperature, 0x1.fffffep127f); }
+__device__ __forceinline__ bool vast(float offset) { return !(fabsf(offset) < 0x1p24f); }
 __device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
 // A sum at one offset, at another that is no smaller.
 __device__ __forceinline__ float at_offset(float sum, float offset, float other) {
@@ -225,7 +228,7 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
     }
     const float at = __builtin_rintf(top);
     auto weight = [&](float v) {
-        if (top == kInf) return v * scale == kInf ? 1.0f : 0.0f;
+        if (vast(top)) return v * scale == top ? 1.0f : 0.0f;
         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -at));
         return w == w ? w : 0.0f;  // nor has an infinite logit a weight where T is infinite
     };
@@ -241,8 +244,8 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
 }
 
 // A block a (sequence, share, model). T > 0: one pass with an offset near the
-// maximum of each thread's first loads; a sum that leaves fp32's range, or a NaN,
-// is taken again with care. Bound by the read of the logits and, at four
+// maximum of each thread's first loads; a sum that comes near the ends of fp32's
+// range, or a NaN, is taken again with care. Bound by the read of the logits and, at four
 // instructions and an exponential a token, nearly as much by its issue; five
 // resident blocks a CU with the next two loads in flight beat eight of four loads
 // that wait for each other, in two rounds (whole calls, vocabulary 151936: 24 trees
@@ -326,7 +329,7 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
             float high = edge;
             if (begin_k < hi) high = fmaxf(high, highest(begin_k, packed));
             high *= scale;
-            mine.offset = fabsf(high) < kInf ? __builtin_rintf(high) : 0.0f;
+            mine.offset = vast(high) ? 0.0f : __builtin_rintf(high);
             mine.sum = __builtin_amdgcn_exp2f(__builtin_fmaf(edge, scale, -mine.offset));
             for (int k = begin_k; k < hi; k += kLoads * kThreads) {
                 uint4 now[kLoads];
@@ -340,7 +343,8 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
                     mine.sum += eight;
                 }
             }
-            if (!(mine.sum < 0x1p100f)) careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &mine.offset, &mine.sum);
+            if (!(mine.sum >= 0x1p-20f && mine.sum < 0x1p100f))
+                careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &mine.offset, &mine.sum);
             if (!(mine.sum > 0.0f)) mine.offset = -kInf;
         } else {
             if (edge == edge && lone >= 0 && lone < a.vocab) { mine.offset = edge; where = -1; }
@@ -414,11 +418,11 @@ struct Rows {
 struct RestTerm {
     const Rows& r;
     float scale, cq;
-    bool infinite;
+    bool any_vast;
     __device__ __forceinline__ RestTerm(const Rows& rows, float c, float s)
-        : r(rows), scale(s), cq(c * rows.draft_inv_sum), infinite(rows.offset == kInf || rows.draft_offset == kInf) {}
+        : r(rows), scale(s), cq(c * rows.draft_inv_sum), any_vast(vast(rows.offset) || vast(rows.draft_offset)) {}
     __device__ __forceinline__ float weight(float x, float offset) const {
-        if (infinite && offset == kInf) return x * scale == kInf ? 1.0f : 0.0f;
+        if (any_vast && vast(offset)) return x * scale == offset ? 1.0f : 0.0f;
         return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -offset));
     }
     __device__ __forceinline__ float operator()(float x, float y) const {
@@ -561,7 +565,7 @@ __device__ __forceinline__ Rows rows_of(const VerifyArgs& a, int row, const Stat
 // The probability of a logit of a row: 2^y, y = k + f, |f| <= 1/2, in fp64 but for 2^f.
 __device__ __forceinline__ double chance(float x, float scale, const Stats& r) {
     if (!(r.sum > 0.0f) || x != x) return 0.0;
-    if (r.offset == kInf) return x * scale == kInf ? 1.0 / double(r.sum) : 0.0;
+    if (vast(r.offset)) return x * scale == r.offset ? 1.0 / double(r.sum) : 0.0;
     const double y = double(x) * double(scale) - double(r.offset), k = rint(y);
     return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
 }

@@ -410,6 +410,29 @@ def test_verification_leaves_out_what_was_rejected(gpu):
     d.run(gpu)
 
 
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("mask", [0xFF80, 0xFF7F, 0x7FC0])
+def test_verification_of_masks_at_any_level(gpu, draft, mask):
+    """Most tokens masked by -inf, the lowest value or NaN, whole stretches among them, the others far below or above
+    0, at temperatures at which the lowest value's scaled products round up and down; rows of -inf or NaN alone."""
+    rng = np.random.default_rng(1470 + mask)
+    d = Drafts([6] * 40, 9001, 1471, draft, fan=3, temps=(0.3, 0.7, 1.0, 1.5, 0.9))
+    for s in range(40):
+        rows = slice(6 * s, 6 * s + 6)
+        keep = rng.random(9001) < (0.3, 0.003)[s % 2]
+        keep[:4096 * (s % 3)] = False
+        keep[rng.integers(0, 9001, 2)] = True
+        level = (0.0, -300.0, 250.0, -500.0)[s % 4]
+        for x in ([d.logits] if d.draft is None else [d.logits, d.draft]):
+            x[rows] = nvr.bf16_bits(nvr.bf16_values(x[rows]).astype(np.float64) + level)
+            x[rows][:, ~keep] = mask
+        if s % 8 == 5 and mask != 0xFF7F:
+            d.logits[rows] = mask
+        allowed = np.flatnonzero(keep)
+        d.tokens[rows] = rng.choice(allowed, 6)
+    d.run(gpu)
+
+
 @pytest.mark.parametrize("vocab", [1000, 120011])  # walks in the last launch, and in one of its own
 def test_verification_at_extreme_temperatures(gpu, vocab):
     """T infinite: the tokens that are not masked are equally likely. T below the smallest normal number: the largest
