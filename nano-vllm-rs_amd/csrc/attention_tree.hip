@@ -390,6 +390,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     f32x4_t o[QT][DT];
     f32x4_t l[QT];  // the weights' sum, four times
     float m[QT];
+    bool vast = false;
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         m[t] = -kInf;
@@ -488,6 +489,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 top = fmaxf(top, m[t]);
                 top = fmaxf(top, nvr::xor_lane(top, 16));
                 top = fmaxf(top, nvr::xor_lane(top, 32));
+                vast |= __ballot(fabsf(top) >= 0x1p28f && top != -kInf) != 0;
                 const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
                 l[t] *= old;
 #pragma unroll
@@ -574,6 +576,65 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     for (int tile = tile0; tile < plain; ++tile) step(tile, std::false_type{});
 #pragma unroll 1
     for (int tile = plain; tile < tile1; ++tile) step(tile, std::true_type{});
+
+    if (__builtin_expect(vast, 0)) {
+        // A scaled maximum of 2^28 or more: its rounding, which the fma of a score and its maximum leaves out, is more
+        // than a weight's exponent can hold. This wave's positions again, one by one.
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            m[t] = -kInf;
+            l[t] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll 1
+        for (int pos = tile0 * T; pos < min(tile1 * T, keys); ++pos) {
+            const int row = pos % T / S::KW == wk ? place(pos / kPage) : -1;
+            if (row < 0) continue;
+            const int64_t at = int64_t(row + pos % kPage) * pitch;
+            float x[QT] = {};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const int d = 32 * k + 8 * g;
+                if (d >= a.dim) continue;
+                float kv[8];
+                nvr::unpack8(*reinterpret_cast<const uint4*>(kcol + at + d), kv);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    float qv[8];
+                    nvr::unpack8(__builtin_bit_cast(uint4, q[t][k]), qv);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[t] = __builtin_fmaf(qv[i], kv[i], x[t]);
+                }
+            }
+            float old[QT], w[QT];
+            bool sees[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                x[t] += nvr::xor_lane(x[t], 16);
+                x[t] += nvr::xor_lane(x[t], 32);
+                x[t] *= a.scale;
+                sees[t] = (pos < span.context || (mask[t] >> (pos - span.context) & 1) != 0) && x[t] != -kInf;
+                const float top = sees[t] ? fmaxf(m[t], x[t]) : m[t];
+                old[t] = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
+                w[t] = __builtin_amdgcn_exp2f(x[t] - top);
+                if (sees[t]) {
+                    l[t][0] = __builtin_fmaf(l[t][0], old[t], w[t]);
+                    m[t] = top;
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int element = 16 * d + 4 * g + e;
+                    const float v = element < a.dim ? nvr::bf16_to_f32(vcol[at + element]) : 0.0f;
+#pragma unroll
+                    for (int t = 0; t < QT; ++t)
+                        if (sees[t]) o[t][d][e] = __builtin_fmaf(w[t], v, o[t][d][e] * old[t]);
+                }
+        }
+    }
 
     // ---- the waves' shares, then the output or the split's partial ----
     float sum[QT];

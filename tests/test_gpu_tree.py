@@ -194,6 +194,31 @@ def test_attention_of_infinite_and_nan_operands(gpu, what):
             assert np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("dim", [128, 64, 256, 10])
+@pytest.mark.parametrize("size", [1e4, 3e8, 5e12, -3e8, -5e12])
+def test_attention_of_vast_scores(gpu, dim, size):
+    """Scores of up to 2^80, and as far below 0: the positions with the largest one share the weight. The mean of their
+    V to the sums' roundings (2^-16 of their magnitudes) and the output's (2^-8 of it)."""
+    t = Trees([9, 3], [700, 35], 8, 4, dim, 16, 650)
+    q = np.zeros(t.q.shape, np.float32)
+    q[..., 0] = abs(size)
+    k = nvr.bf16_values(t.kc).copy()
+    k[..., 0] = np.where(np.arange(len(k)) % 7 == 3, 1.0, 0.5 if size > 0 else 2.0)[:, None] * size
+    t.q, t.kc = nvr.bf16_bits(q), nvr.bf16_bits(k)
+    t.upload(gpu).launch(gpu)
+    got, v = nvr.bf16_values(t.result()), nvr.bf16_values(t.vc).astype(np.float64)
+    for s, (n, c) in enumerate(zip(t.sizes, t.contexts)):
+        for i in range(n):
+            row = int(t.row_starts[s]) + i
+            seen = [p for p in range(c + n) if p < c or int(t.masks[row]) >> (p - c) & 1]
+            at = np.array([t.tables[s, p // 16] * 16 + p % 16 for p in seen])
+            if (at % 7 == 3).any():
+                at = at[at % 7 == 3]
+            want = np.repeat(v[at].mean(0), 2, 0)
+            bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -16 * np.repeat(np.abs(v[at]).mean(0), 2, 0)
+            assert (np.abs(got[row] - want) <= bound).all(), (s, i)
+
+
 def test_attention_of_one_node_trees_is_the_decode_attention(gpu):
     """A tree of one node is a decode row: nv_attention's result to both kernels' roundings."""
     t = Trees([1] * 12, [0, 1, 15, 16, 31, 100, 255, 256, 700, 1023, 64, 3], 16, 8, 128, 16, 700)
