@@ -523,6 +523,34 @@ def test_verification_of_unaligned_rows(gpu):
         d.check()
 
 
+@pytest.mark.parametrize("draft", [False, True])
+def test_verification_with_offsets_past_32_bits(gpu, draft):
+    """Logits of more than 2^32 elements, with a tree at either end (between them a sequence with too many rows)."""
+    vocab = (1 << 20) + 3
+    d = Drafts([5, 5], vocab, 1800, draft, fan=2, temps=(0.8, 1.1))
+    d.run(gpu)
+    want = d.result()
+    rows = 2 ** 32 // vocab + 20
+    place = np.concatenate([np.arange(5), np.arange(rows - 5, rows)])
+    for i in range(2 if draft else 1):
+        big = gpu.alloc(rows * vocab * 2)
+        for row, values in zip(place, (d.logits, d.draft)[i]):
+            big.slice(int(row) * vocab * 2, vocab * 2).upload(values)
+        d.inputs[i] = big
+    for i, a in ((2, d.tokens), (3, d.parents), (6, d.uniforms)):
+        wide = np.zeros(rows, a.dtype)
+        wide[place] = a
+        d.inputs[i] = put(gpu, wide)
+    d.inputs[4] = put(gpu, np.array([0, 5, rows - 5, rows], np.int32))
+    d.inputs[5], d.inputs[7] = put(gpu, d.temps[[0, 0, 1]]), put(gpu, d.seeds[[0, 0, 1]])
+    outputs = [gpu.alloc(3 * 5 * 4), gpu.alloc(3 * 5 * 4), gpu.alloc(12)]
+    gpu.verify_tree(*d.inputs, *outputs, gpu.alloc(gpu.verify_tree_workspace(rows, 3, vocab)), rows, 3, 5, vocab)
+    got = [b.download(np.int32, n).reshape(3, -1) for b, n in zip(outputs, (15, 15, 3))]
+    for a, b in zip(got, want):
+        assert np.array_equal(a[[0, 2]].reshape(b.shape), b)
+    assert got[2][1] == 0
+
+
 # -------------------------------------------------------------------- pages ----
 @pytest.mark.parametrize("layers,kvh,dim,bs", [(1, 8, 128, 256), (28, 8, 128, 16), (3, 4, 80, 16), (2, 3, 10, 5),
                                                (2, 1, 7, 1), (1, 16, 256, 32)])
@@ -586,6 +614,47 @@ def test_compaction_of_unaligned_caches(gpu):
     nodes = np.array([[0, 2, 5, 7], [1, 2, 3, 11]], np.int32)
     nodes = np.concatenate([nodes, np.full((2, 8), -1, np.int32)], 1)
     _compact_both(gpu, 2, 2, 64, 4, 12, np.array([5, 9], np.int32), nodes, np.array([4, 4], np.int32), tables, offset=2)
+
+
+def test_moves_with_offsets_past_32_bits(gpu):
+    """Caches of more than 2^32 elements in three layers: moves in the first block and in the last ones."""
+    layers, kvh, dim, bs = 3, 8, 128, 16
+    width, slots = kvh * dim, 2 ** 32 // (3 * kvh * dim) + 64 * bs
+    blocks = slots // bs
+    rng = np.random.default_rng(2050)
+    used = [0, blocks - 3, blocks - 2, blocks - 1]
+    buffers, hosts = [], []
+    for _ in range(2):
+        cache = gpu.alloc(layers * blocks * bs * width * 2)
+        host = rng.integers(0, 2 ** 16, (layers, len(used) * bs, width), dtype=np.uint16)
+        for layer in range(layers):
+            for i, b in enumerate(used):
+                cache.slice((layer * blocks + b) * bs * width * 2, bs * width * 2).upload(host[layer, i * bs:(i + 1) * bs])
+        buffers.append(cache)
+        hosts.append(host)
+
+    def check():
+        for cache, host in zip(buffers, hosts):
+            for layer in range(layers):
+                for i, b in enumerate(used):
+                    got = cache.slice((layer * blocks + b) * bs * width * 2, bs * width * 2).download(np.uint16, bs * width)
+                    assert np.array_equal(got, host[layer, i * bs:(i + 1) * bs].reshape(-1)), (layer, b)
+
+    contexts, counts = np.array([2, 9], np.int32), np.array([4, 5], np.int32)
+    nodes = np.array([[0, 3, 4, 9, -1], [1, 2, 7, 12, 19]], np.int32)
+    nodes = np.concatenate([nodes, np.full((2, 20), -1, np.int32)], 1)
+    small = np.array([[0, 2], [1, 3]], np.int32)
+    gpu.kv_compact(*buffers, put(gpu, contexts), put(gpu, nodes), put(gpu, counts),
+                   put(gpu, np.array(used, np.int32)[small]), 2, 25, layers, kvh, dim, bs, blocks, 2)
+    for host in hosts:
+        ref.compact(host, contexts, nodes, counts, small, bs, len(used), 25)
+    check()
+    gpu.kv_copy_blocks(*buffers, *(put(gpu, np.array(a, np.int32)) for a in ([0, blocks - 1], [blocks - 2, blocks - 3], [16, 7])),
+                       2, layers, kvh, dim, bs, blocks)
+    for host in hosts:
+        host[:, 2 * bs:3 * bs] = host[:, :bs]
+        host[:, bs:bs + 7] = host[:, 3 * bs:3 * bs + 7]
+    check()
 
 
 @pytest.mark.parametrize("layers,kvh,dim,bs,offset", [(1, 8, 128, 256, 0), (28, 8, 128, 16, 0), (3, 4, 80, 16, 0),
