@@ -34,6 +34,9 @@ using nvr::kWave;
 constexpr int kMaxNodes = 64;  // a row's mask is one 64-bit word
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
+// Weights are at most 2^-24 (2^-16 in the tile form), so that sums over 65536 positions hold any V; m, the exponent that
+// they are scaled by, is that much above the maximum.
+constexpr float kBias = 24.0f;
 
 struct TreeArgs {
     const uint16_t* q;
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
         for (int w = 1; w < kWave; w <<= 1) dot += nvr::xor_lane(dot, w);
         const float x = dot * a.scale;
         if (x == -kInf) continue;
-        const float top = fmaxf(m, x);  // a NaN leaves m, and makes l NaN
+        const float top = fmaxf(m, x + kBias);  // a NaN leaves m, and makes l NaN
         const float old = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
         const float p = __builtin_amdgcn_exp2f(x - top);
         m = top;
@@ -485,11 +488,12 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, x[t][j][r]);
             top *= a.scale;
             // The weights' common scale follows the maximum only where that outgrows it by 2^8: any scale near it will do.
-            if (__ballot(top > m[t] + 8.0f) != 0) {
-                top = fmaxf(top, m[t]);
+            if (__ballot(top > m[t] + (8.0f - kBias)) != 0) {
+                top = fmaxf(top, m[t] - kBias);
                 top = fmaxf(top, nvr::xor_lane(top, 16));
                 top = fmaxf(top, nvr::xor_lane(top, 32));
                 vast |= __ballot(fabsf(top) >= 0x1p28f && top != -kInf) != 0;
+                top += kBias;
                 const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
                 l[t] *= old;
 #pragma unroll
@@ -615,7 +619,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 x[t] += nvr::xor_lane(x[t], 32);
                 x[t] *= a.scale;
                 sees[t] = (pos < span.context || (mask[t] >> (pos - span.context) & 1) != 0) && x[t] != -kInf;
-                const float top = sees[t] ? fmaxf(m[t], x[t]) : m[t];
+                const float top = sees[t] ? fmaxf(m[t], x[t] + kBias) : m[t];
                 old[t] = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
                 w[t] = __builtin_amdgcn_exp2f(x[t] - top);
                 if (sees[t]) {

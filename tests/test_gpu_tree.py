@@ -219,6 +219,18 @@ def test_attention_of_vast_scores(gpu, dim, size):
             assert (np.abs(got[row] - want) <= bound).all(), (s, i)
 
 
+@pytest.mark.parametrize("dim,size", [(128, 3.2e38), (64, 3.2e38), (256, 3.2e38), (10, 3.2e38), (128, 1e-30), (10, 1e-30)])
+def test_attention_of_the_largest_and_smallest_values(gpu, dim, size):
+    """V of one magnitude, with a sign a head element: the outputs are that, to the weights' sums' roundings (2^-16)
+    and the output's (2^-8), however many positions share the weight."""
+    t = Trees([9, 3], [2100, 35], 8, 4, dim, 16, 660, spread=0.01)
+    signs = np.where(np.arange(dim) % 3 == 0, -size, size)
+    t.vc = nvr.bf16_bits(np.broadcast_to(signs, t.vc.shape))
+    t.upload(gpu).launch(gpu)
+    got, want = nvr.bf16_values(t.result()).astype(np.float64), nvr.bf16_values(t.vc)[0, 0].astype(np.float64)
+    assert (np.abs(got - want) <= (2.0 ** -8 + 2.0 ** -16) * np.abs(want)).all()
+
+
 def test_attention_of_one_node_trees_is_the_decode_attention(gpu):
     """A tree of one node is a decode row: nv_attention's result to both kernels' roundings."""
     t = Trees([1] * 12, [0, 1, 15, 16, 31, 100, 255, 256, 700, 1023, 64, 3], 16, 8, 128, 16, 700)
