@@ -110,7 +110,11 @@ __global__ __launch_bounds__(256) void compact(Chunk* __restrict__ kc, Chunk* __
                 if (j0 + u < moves) v[u] = cache[from[j0 + u] * slot_chunks + column];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u)
-                if (j0 + u < moves) cache[to[j0 + u] * slot_chunks + column] = v[u];
+                if (j0 + u < moves) {
+                    Chunk* at = cache + to[j0 + u] * slot_chunks + column;
+                    if constexpr (sizeof(Chunk) == 16) nvr::store_stream(at, v[u]);
+                    else *at = v[u];
+                }
         }
     }
 }
