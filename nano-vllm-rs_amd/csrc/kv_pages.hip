@@ -17,9 +17,11 @@ constexpr int kMaxNodes = 64;
 // The first min(tokens[i], bs) slots of block src[i] to block dst[i]: they are
 // contiguous, so a copy is cut into segments of kSegment chunks whatever the
 // slot size, one a block, all loads of a thread in flight before its stores.
-// Reads and writes bypass the caches' retention: 12 copies of partly filled blocks
-// of 256 positions in 28 layers (559 MB moved) take 84 to 86 us, 6.6 TB/s.
-constexpr int kCopyLoads = 8;
+// Bound by HBM: 12 copies of partly filled blocks of 256 positions from 4 sources in
+// 28 layers (559 MB moved) take 62 us, 9 TB/s. Writes bypass the caches, which would
+// hold them in the way of sources read again (98 us); reads do not (80), nor do more
+// loads a thread hide more (eight 78, two 66).
+constexpr int kCopyLoads = 4;
 constexpr int kSegment = 256 * kCopyLoads;
 
 template <typename Chunk>  // uint4, or uint16_t where sizes or addresses are no multiples of 16 bytes
@@ -42,10 +44,7 @@ __global__ __launch_bounds__(256) void copy_blocks(Chunk* __restrict__ kc, Chunk
 #pragma unroll
     for (int u = 0; u < kCopyLoads; ++u) {
         const int64_t at = first + u * 256;
-        if (at < end) {
-            if constexpr (sizeof(Chunk) == 16) v[u] = nvr::load_stream(s + at);
-            else v[u] = s[at];
-        }
+        if (at < end) v[u] = s[at];
     }
 #pragma unroll
     for (int u = 0; u < kCopyLoads; ++u) {
