@@ -18,7 +18,7 @@ constexpr int kMaxNodes = 64;
 // contiguous, so a copy is cut into segments of kSegment chunks whatever the
 // slot size, one a block, all loads of a thread in flight before its stores.
 // Bound by HBM: 12 copies of partly filled blocks of 256 positions from 4 sources in
-// 28 layers (559 MB moved) take 62 us, 9 TB/s. Writes bypass the caches, which would
+// 28 layers (559 MB moved) take 63 to 67 us, 8.6 TB/s. Writes bypass the caches, which would
 // hold them in the way of sources read again (98 us); reads do not (80), nor do more
 // loads a thread hide more (eight 78, two 66).
 constexpr int kCopyLoads = 4;
@@ -60,8 +60,9 @@ __global__ __launch_bounds__(256) void copy_blocks(Chunk* __restrict__ kc, Chunk
 // order. The nodes rise, so nodes[j] >= j: a move's target is no later move's
 // source, and a thread that takes one column of the slots through all moves,
 // reading kBatch of them before it writes, needs no second buffer. A block a
-// (sequence, layer): its time is the chain nodes, table, slots, store: 4.2 us for 8
-// sequences in 28 layers (2.5 MB), 9.2 for 64 (16 MB).
+// (sequence, layer): its time is the chain nodes, table, slots, store: 3.6 us for 8
+// sequences in 28 layers (2.5 MB), 5.3 for 64 (16 MB). Stores bypass the caches: 10
+// us for the 64 with plain ones.
 template <typename Chunk>
 __global__ __launch_bounds__(256) void compact(Chunk* __restrict__ kc, Chunk* __restrict__ vc,
                                                const int* __restrict__ contexts, const int* __restrict__ nodes,
