@@ -731,10 +731,10 @@ class Gpu:
         """K and V at position contexts[s] + nodes[s, j] move to contexts[s] + j, for j < counts[s], in every layer
         of caches [layers, num_blocks, block_size, kvheads, head_dim]."""
         self._tree_limit("kv_compact", max_nodes)
-        self._cache_width("kv_compact", kvheads, head_dim)
+        width = self._cache_width("kv_compact", kvheads, head_dim)
         self._admit("kv_compact", [
-            _w("kcache", kcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
-            _w("vcache", vcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _w("kcache", kcache, 2, layers, num_blocks, block_size, width),
+            _w("vcache", vcache, 2, layers, num_blocks, block_size, width),
             _r("contexts", contexts, 4, batch_size), _r("nodes", nodes, 4, batch_size, max_nodes),
             _r("counts", counts, 4, batch_size), _r("block_tables", block_tables, 4, batch_size, table_stride)])
         self._call(self.lib.nv_kv_compact(self.handle, kcache.ptr, vcache.ptr, contexts.ptr, nodes.ptr, counts.ptr,
@@ -746,18 +746,20 @@ class Gpu:
                        num_blocks: int) -> None:
         """The first tokens[i] slots of block sources[i] are copied to block targets[i], in every layer of caches
         [layers, num_blocks, block_size, kvheads, head_dim]. No block may be written twice, or read and written."""
-        self._cache_width("kv_copy_blocks", kvheads, head_dim)
+        width = self._cache_width("kv_copy_blocks", kvheads, head_dim)
         self._admit("kv_copy_blocks", [
-            _w("kcache", kcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
-            _w("vcache", vcache, 2, layers, num_blocks, block_size, kvheads, head_dim),
+            _w("kcache", kcache, 2, layers, num_blocks, block_size, width),
+            _w("vcache", vcache, 2, layers, num_blocks, block_size, width),
             _r("sources", sources, 4, copies), _r("targets", targets, 4, copies), _r("tokens", tokens, 4, copies)])
         self._call(self.lib.nv_kv_copy_blocks(self.handle, kcache.ptr, vcache.ptr, sources.ptr, targets.ptr,
                                               tokens.ptr, copies, layers, kvheads, head_dim, block_size, num_blocks))
 
     @staticmethod
-    def _cache_width(op: str, kvheads: int, head_dim: int) -> None:
-        if as_dim(kvheads) * as_dim(head_dim) > INT_MAX:
-            raise ArgumentError("dimension", f"{op}: kvheads * head_dim exceeds 2^31 - 1")
+    def _cache_width(op: str, kvheads: int, head_dim: int) -> int:
+        """Elements of a cache slot, as a dimension."""
+        if kvheads < 1 or head_dim < 1 or int(kvheads) * int(head_dim) > INT_MAX:
+            raise ArgumentError("dimension", f"{op}: {kvheads} KV heads of {head_dim} are no slot of 1 to 2^31 - 1 elements")
+        return int(kvheads) * int(head_dim)
 
 
 def bf16_bits(values) -> np.ndarray:
