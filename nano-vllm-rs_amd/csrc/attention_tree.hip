@@ -18,9 +18,8 @@
 // are left as they were.
 //
 // Scores, maxima, sums and outputs are fp32, and the outputs rounded to bf16 once
-// at the end. The tile form rounds each weight p_t to bf16 as an operand of the
-// matrix instructions (a factor within 2^-8, its own for each position), and sums
-// the rounded weights, so that a row's weights still sum to 1.
+// at the end. The tile form hands each weight p_t to the matrix instructions as the
+// sum of two bf16 (within 2^-18 of it).
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
@@ -391,7 +390,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     int next_row = own_page(min(tile0 + NS - 1, tile1 - 1));
 
     f32x4_t o[QT][DT];
-    f32x4_t l[QT];  // the weights' sum, four times
+    f32x4_t l[QT];  // the weights' sum: of this lane's positions, by the last two bits of their index
     float m[QT];
     bool vast = false;
 #pragma unroll
@@ -508,6 +507,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r], a.scale, -base));
+                    l[t][r] += x[t][j][r];
                 }
         }
 
@@ -518,30 +518,41 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             auto* at = (__attribute__((address_space(3))) s16x4_t*)(vt + (row * CH + v_chunk<CH>(row, c)) * 16 + 8 * (n16 & 1));
             return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
         };
-        auto pair = [&](const f32x4_t& w) { return make_uint2(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3])); };
+        // Four weights as two bf16 each, the nearest one and what it leaves: 2^-18 of a weight is lost, not 2^-9.
+        auto halves = [&](const f32x4_t& w, uint2& hi, uint2& lo) {
+            hi = make_uint2(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3]));
+            lo = make_uint2(nvr::pack_bf16x2(w[0] - nvr::bf16_lo(hi.x), w[1] - nvr::bf16_hi(hi.x)),
+                            nvr::pack_bf16x2(w[2] - nvr::bf16_lo(hi.y), w[3] - nvr::bf16_hi(hi.y)));
+        };
         if constexpr (KT == 1) {
-            s16x4_t p[QT];
+            s16x4_t p[QT], rest[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-                p[t] = __builtin_bit_cast(s16x4_t, pair(x[t][0]));
-                l[t] = mfma(s16x4_t{0x3f80, 0x3f80, 0x3f80, 0x3f80}, p[t], l[t]);
+                uint2 hi, lo;
+                halves(x[t][0], hi, lo);
+                p[t] = __builtin_bit_cast(s16x4_t, hi);
+                rest[t] = __builtin_bit_cast(s16x4_t, lo);
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 const s16x4_t v = read(vrow, d);
 #pragma unroll
                 for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t], o[t][d]);
+#pragma unroll
+                for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, rest[t], o[t][d]);
             }
         } else {
             // Positions 4 g .. 4 g + 3 of two tiles: with V read in the same order, a product's 32 positions.
-            bf16x8_t p[QT][KT / 2];
+            bf16x8_t p[QT][KT / 2], rest[QT][KT / 2];
 #pragma unroll
             for (int t = 0; t < QT; ++t)
 #pragma unroll
                 for (int j = 0; j < KT / 2; ++j) {
-                    const uint2 lo = pair(x[t][2 * j]), hi = pair(x[t][2 * j + 1]);
-                    p[t][j] = operand(make_uint4(lo.x, lo.y, hi.x, hi.y));
-                    l[t] = mfma(operand(make_uint4(0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80)), p[t][j], l[t]);
+                    uint2 hi[2], lo[2];
+                    halves(x[t][2 * j], hi[0], lo[0]);
+                    halves(x[t][2 * j + 1], hi[1], lo[1]);
+                    p[t][j] = operand(make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y));
+                    rest[t][j] = operand(make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y));
                 }
 #pragma unroll
             for (int d = 0; d < DT; ++d)
@@ -551,6 +562,8 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                     const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
                     for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, p[t][j], o[t][d]);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) o[t][d] = mfma(v, rest[t][j], o[t][d]);
                 }
         }
         if (drafted && poison[tile & 1] == tile) {
@@ -581,13 +594,21 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 #pragma unroll 1
     for (int tile = plain; tile < tile1; ++tile) step(tile, std::true_type{});
 
+    float sum[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+        sum[t] = (l[t][0] + l[t][1]) + (l[t][2] + l[t][3]);
+        sum[t] += nvr::xor_lane(sum[t], 16);
+        sum[t] += nvr::xor_lane(sum[t], 32);
+    }
+
     if (__builtin_expect(vast, 0)) {
         // A scaled maximum of 2^28 or more: its rounding, which the fma of a score and its maximum leaves out, is more
         // than a weight's exponent can hold. This wave's positions again, one by one.
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
             m[t] = -kInf;
-            l[t] = f32x4_t{0, 0, 0, 0};
+            sum[t] = 0.0f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
         }
@@ -623,7 +644,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                 old[t] = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
                 w[t] = __builtin_amdgcn_exp2f(x[t] - top);
                 if (sees[t]) {
-                    l[t][0] = __builtin_fmaf(l[t][0], old[t], w[t]);
+                    sum[t] = __builtin_fmaf(sum[t], old[t], w[t]);
                     m[t] = top;
                 }
             }
@@ -641,9 +662,6 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     }
 
     // ---- the waves' shares, then the output or the split's partial ----
-    float sum[QT];
-#pragma unroll
-    for (int t = 0; t < QT; ++t) sum[t] = l[t][0];
     // The upper half of the waves hand theirs to the lower half, until one holds all.
     f32x4_t* merge = reinterpret_cast<f32x4_t*>(smem);
     float2* merge_sums = reinterpret_cast<float2*>(smem + (WK / 2 * WQ * QT * DT * kWave) * 16);
