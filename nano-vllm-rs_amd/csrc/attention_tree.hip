@@ -33,8 +33,8 @@ using nvr::kWave;
 constexpr int kMaxNodes = 64;  // a row's mask is one 64-bit word
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
-// Weights are at most 2^-24 (2^-16 in the tile form), so that sums over 65536 positions hold any V; m, the exponent that
-// they are scaled by, is that much above the maximum.
+// Weights are at most 2^-24 (2^-16 in the tile form), so that sums over 65536 positions hold any V. They are of a score's
+// distance from the maximum, which is exact to its own 2^-24 however large both are.
 constexpr float kBias = 24.0f;
 
 struct TreeArgs {
@@ -108,11 +108,10 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
         }
 #pragma unroll
         for (int w = 1; w < kWave; w <<= 1) dot += nvr::xor_lane(dot, w);
-        const float x = dot * a.scale;
-        if (x == -kInf) continue;
-        const float top = fmaxf(m, x + kBias);  // a NaN leaves m, and makes l NaN
-        const float old = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        const float p = __builtin_amdgcn_exp2f(x - top);
+        if (dot == -kInf) continue;
+        const float top = fmaxf(m, dot);  // a NaN leaves m, and makes l NaN
+        const float old = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.scale);
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot - top, a.scale, -kBias));
         m = top;
         l = __builtin_fmaf(l, old, p);
 #pragma unroll
@@ -131,7 +130,7 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
         if (part_m[w] == -kInf && part_l[w] == 0.0f) continue;  // saw nothing
-        const float f = __builtin_amdgcn_exp2f(part_m[w] - top);
+        const float f = __builtin_amdgcn_exp2f((part_m[w] - top) * a.scale);
         den = __builtin_fmaf(part_l[w], f, den);
         num = __builtin_fmaf(part_o[w][threadIdx.x], f, num);
     }
@@ -390,13 +389,11 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     int next_row = own_page(min(tile0 + NS - 1, tile1 - 1));
 
     f32x4_t o[QT][DT];
-    f32x4_t l[QT];  // the weights' sum: of this lane's positions, by the last two bits of their index
-    float m[QT];
-    bool vast = false;
+    float m[QT], l[QT];  // the weights' scale; their sum, of this lane's positions
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         m[t] = -kInf;
-        l[t] = f32x4_t{0, 0, 0, 0};
+        l[t] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
     }
@@ -485,15 +482,12 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int j = 0; j < KT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, x[t][j][r]);
-            top *= a.scale;
             // The weights' common scale follows the maximum only where that outgrows it by 2^8: any scale near it will do.
-            if (__ballot(top > m[t] + (8.0f - kBias)) != 0) {
-                top = fmaxf(top, m[t] - kBias);
+            if (__ballot((top - m[t]) * a.scale > 8.0f) != 0) {
+                top = fmaxf(top, m[t]);
                 top = fmaxf(top, nvr::xor_lane(top, 16));
                 top = fmaxf(top, nvr::xor_lane(top, 32));
-                vast |= __ballot(fabsf(top) >= 0x1p28f && top != -kInf) != 0;
-                top += kBias;
-                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
+                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m[t] - top) * a.scale);
                 l[t] *= old;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -503,12 +497,12 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             }
             const float base = m[t] == -kInf ? 0.0f : m[t];
 #pragma unroll
-            for (int j = 0; j < KT; ++j)
+            for (int j = 0; j < KT; ++j) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r], a.scale, -base));
-                    l[t][r] += x[t][j][r];
-                }
+                for (int r = 0; r < 4; ++r)
+                    x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r] - base, a.scale, -kBias));
+                l[t] += (x[t][j][0] + x[t][j][1]) + (x[t][j][2] + x[t][j][3]);
+            }
         }
 
         // ---- outputs, transposed: head elements x query rows ----
@@ -597,68 +591,8 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     float sum[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        sum[t] = (l[t][0] + l[t][1]) + (l[t][2] + l[t][3]);
-        sum[t] += nvr::xor_lane(sum[t], 16);
+        sum[t] = l[t] + nvr::xor_lane(l[t], 16);
         sum[t] += nvr::xor_lane(sum[t], 32);
-    }
-
-    if (__builtin_expect(vast, 0)) {
-        // A scaled maximum of 2^28 or more: its rounding, which the fma of a score and its maximum leaves out, is more
-        // than a weight's exponent can hold. This wave's positions again, one by one.
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            m[t] = -kInf;
-            sum[t] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
-        }
-#pragma unroll 1
-        for (int pos = tile0 * T; pos < min(tile1 * T, keys); ++pos) {
-            const int row = pos % T / S::KW == wk ? place(pos / kPage) : -1;
-            if (row < 0) continue;
-            const int64_t at = int64_t(row + pos % kPage) * pitch;
-            float x[QT] = {};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const int d = 32 * k + 8 * g;
-                if (d >= a.dim) continue;
-                float kv[8];
-                nvr::unpack8(*reinterpret_cast<const uint4*>(kcol + at + d), kv);
-#pragma unroll
-                for (int t = 0; t < QT; ++t) {
-                    float qv[8];
-                    nvr::unpack8(__builtin_bit_cast(uint4, q[t][k]), qv);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[t] = __builtin_fmaf(qv[i], kv[i], x[t]);
-                }
-            }
-            float old[QT], w[QT];
-            bool sees[QT];
-#pragma unroll
-            for (int t = 0; t < QT; ++t) {
-                x[t] += nvr::xor_lane(x[t], 16);
-                x[t] += nvr::xor_lane(x[t], 32);
-                x[t] *= a.scale;
-                sees[t] = (pos < span.context || (mask[t] >> (pos - span.context) & 1) != 0) && x[t] != -kInf;
-                const float top = sees[t] ? fmaxf(m[t], x[t] + kBias) : m[t];
-                old[t] = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(m[t] - top);
-                w[t] = __builtin_amdgcn_exp2f(x[t] - top);
-                if (sees[t]) {
-                    sum[t] = __builtin_fmaf(sum[t], old[t], w[t]);
-                    m[t] = top;
-                }
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int element = 16 * d + 4 * g + e;
-                    const float v = element < a.dim ? nvr::bf16_to_f32(vcol[at + element]) : 0.0f;
-#pragma unroll
-                    for (int t = 0; t < QT; ++t)
-                        if (sees[t]) o[t][d][e] = __builtin_fmaf(w[t], v, o[t][d][e] * old[t]);
-                }
-        }
     }
 
     // ---- the waves' shares, then the output or the split's partial ----
@@ -683,7 +617,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int t = 0; t < QT; ++t) {
                 const float2 other = merge_sums[(from + t) * kWave + lane];
                 const float top = fmaxf(m[t], other.x), base = top == -kInf ? 0.0f : top;
-                const float f = __builtin_amdgcn_exp2f(m[t] - base), h = __builtin_amdgcn_exp2f(other.x - base);
+                const float f = __builtin_amdgcn_exp2f((m[t] - base) * a.scale), h = __builtin_amdgcn_exp2f((other.x - base) * a.scale);
                 m[t] = top;
                 sum[t] = __builtin_fmaf(other.y, h, sum[t] * f);
 #pragma unroll
@@ -751,14 +685,14 @@ __global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials 
         float high = top;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) high = fmaxf(high, ml[u].x);
-        const float base = high == -kInf ? 0.0f : high, old = __builtin_amdgcn_exp2f(top - base);
+        const float base = high == -kInf ? 0.0f : high, old = __builtin_amdgcn_exp2f((top - base) * a.scale);
         den *= old;
 #pragma unroll
         for (int r = 0; r < 4; ++r) num[r] *= old;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if (w0 + u >= used) continue;
-            const float f = __builtin_amdgcn_exp2f(ml[u].x - base);
+            const float f = __builtin_amdgcn_exp2f((ml[u].x - base) * a.scale);
             den = __builtin_fmaf(ml[u].y, f, den);
 #pragma unroll
             for (int r = 0; r < 4; ++r) num[r] = __builtin_fmaf(v[u][r], f, num[r]);

@@ -65,3 +65,27 @@ def test_attention_holds_its_weights(gpu, shape):
     t = trees(shape, 150, 600, 5000)
     t.upload(gpu).launch(gpu)
     check_tightly(t, t.result())
+
+
+def constant_values(t, gpu, size):
+    """The outputs for V of one size, with a sign a head element, and what they are: that, however many positions share
+    the weight, to the roundings of two sums of up to 2^12 weights (2^-12 each) and the output's."""
+    signs = np.where(np.arange(t.dim) % 3 == 0, -size, size)
+    t.vc = nvr.bf16_bits(np.broadcast_to(signs, t.vc.shape))
+    t.upload(gpu).launch(gpu)
+    want = values(t.vc)[0, 0]
+    return values(t.result()), want, (2.0 ** -8 + 2 * 2.0 ** -12) * np.abs(want)
+
+
+@pytest.mark.parametrize("dim", [128, 64, 256, 10])
+@pytest.mark.parametrize("level", [22.7, 24.4, 25.3, 25.9, 26.6, 27.2, 27.8, 28.5, 29.9])
+def test_attention_of_the_largest_values_under_vast_scores(gpu, dim, level):
+    """All scores alike, 2^level as powers of two, where a maximum's own rounding is whole powers of two: the weights
+    are of a score's distance from it, and the largest V's sums stay finite."""
+    t = Trees([9, 3], [2100, 35], 8, 4, dim, 16, 5100, spread=0.01)
+    size = np.sqrt(2.0 ** level * np.sqrt(dim) / np.log2(np.e))
+    for x in (t.q, t.kc):
+        x[:] = 0
+        x[..., 0] = nvr.bf16_bits(np.array([size]))[0]
+    got, want, bound = constant_values(t, gpu, 3.2e38)
+    assert (np.abs(got - want) <= bound).all()
