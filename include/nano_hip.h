@@ -247,7 +247,7 @@ int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, i
  * kc, vc: [blocks, bs, kvh, dim] bf16; masks: [rows] u64; tables: [batch, stride]
  * i32. Row (s, i) attends to the positions before contexts[s] and to node j's for
  * each bit j of its mask, its own among them if set. Softmax of q . k / sqrt(dim);
- * fp32 sums and statistics. Rows that see nothing are +0, as are those of
+ * sums and statistics of 32 bits or more, finite for any finite V. Rows that see nothing are +0, as are those of
  * sequences with more than max_nodes nodes or more than min(max_context, stride *
  * bs) positions, a negative context, or a score that is not finite at the maximum;
  * positions in blocks outside [0, blocks) are not seen. Rows of no sequence are

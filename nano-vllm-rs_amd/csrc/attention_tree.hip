@@ -33,10 +33,6 @@ using nvr::kWave;
 constexpr int kMaxNodes = 64;  // a row's mask is one 64-bit word
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kInf = __builtin_inff();
-// Weights are at most 2^-24 (2^-16 in the tile form), so that sums over 65536 positions hold any V. They are of a score's
-// distance from the maximum, which is exact to its own 2^-24 however large both are.
-constexpr float kBias = 24.0f;
-
 struct TreeArgs {
     const uint16_t* q;
     const uint16_t* kc;
@@ -70,7 +66,8 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int s) {
 // heads of 128, 8 trees of 25 nodes at 1030 positions take 650 us (the tile form 21).
 __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
     constexpr int kWaves = 4, kElems = 4;  // 64 lanes x 4 elements: head dims up to 256
-    __shared__ float part_m[kWaves], part_l[kWaves], part_o[kWaves][256];
+    __shared__ float part_m[kWaves];
+    __shared__ double part_l[kWaves], part_o[kWaves][256];  // as the sums: of V of any size
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int head = int(blockIdx.x % unsigned(a.qh));
     const int item = int(blockIdx.x / unsigned(a.qh));
@@ -87,13 +84,14 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
     const int64_t row = int64_t(t.start + node) * a.qh + head;
     const uint64_t mask = a.masks[t.start + node];
     const int64_t pitch = int64_t(a.kvh) * a.dim, column = int64_t(head / (a.qh / a.kvh)) * a.dim;
-    float q[kElems], o[kElems] = {};
+    float q[kElems];
+    double o[kElems] = {}, l = 0.0;
 #pragma unroll
     for (int e = 0; e < kElems; ++e) {
         const int d = lane + e * kWave;
         q[e] = d < a.dim ? nvr::bf16_to_f32(a.q[row * a.dim + d]) : 0.0f;
     }
-    float m = -kInf, l = 0.0f;
+    float m = -kInf;
     const int keys = t.context + t.nodes;
     for (int pos = wave; pos < keys; pos += kWaves) {
         if (pos >= t.context && (mask >> (pos - t.context) & 1) == 0) continue;
@@ -110,31 +108,34 @@ __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
         for (int w = 1; w < kWave; w <<= 1) dot += nvr::xor_lane(dot, w);
         if (dot == -kInf) continue;
         const float top = fmaxf(m, dot);  // a NaN leaves m, and makes l NaN
+        // Of the scores' distances, which are exact to their own 2^-24 however large both are.
         const float old = m == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m - top) * a.scale);
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(dot - top, a.scale, -kBias));
+        const float p = __builtin_amdgcn_exp2f((dot - top) * a.scale);
         m = top;
-        l = __builtin_fmaf(l, old, p);
+        l = __builtin_fma(l, double(old), double(p));
 #pragma unroll
         for (int e = 0; e < kElems; ++e) {
             const int d = lane + e * kWave;
-            if (d < a.dim) o[e] = __builtin_fmaf(p, nvr::bf16_to_f32(a.vc[at + d]), o[e] * old);
+            if (d < a.dim) o[e] = __builtin_fma(double(p), double(nvr::bf16_to_f32(a.vc[at + d])), o[e] * double(old));
         }
     }
     if (lane == 0) { part_m[wave] = m; part_l[wave] = l; }
 #pragma unroll
     for (int e = 0; e < kElems; ++e) part_o[wave][lane + e * kWave] = o[e];
     __syncthreads();
-    float top = -kInf, den = 0.0f, num = 0.0f;
+    float top = -kInf;
+    double den = 0.0, num = 0.0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) top = fmaxf(top, part_m[w]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-        if (part_m[w] == -kInf && part_l[w] == 0.0f) continue;  // saw nothing
-        const float f = __builtin_amdgcn_exp2f((part_m[w] - top) * a.scale);
-        den = __builtin_fmaf(part_l[w], f, den);
-        num = __builtin_fmaf(part_o[w][threadIdx.x], f, num);
+        if (part_m[w] == -kInf && part_l[w] == 0.0) continue;  // saw nothing
+        const double f = double(__builtin_amdgcn_exp2f((part_m[w] - top) * a.scale));
+        den = __builtin_fma(part_l[w], f, den);
+        num = __builtin_fma(part_o[w][threadIdx.x], f, num);
     }
-    if (int(threadIdx.x) < a.dim) a.out[row * a.dim + threadIdx.x] = nvr::f32_to_bf16(den > 0.0f ? num / den : 0.0f);
+    if (int(threadIdx.x) < a.dim)
+        a.out[row * a.dim + threadIdx.x] = nvr::f32_to_bf16(den > 0.0 ? float(num / den) : 0.0f);
 }
 
 // ------------------------------------------------------------- tile form ----
@@ -158,6 +159,16 @@ __device__ __forceinline__ void wait_copies() {
 
 constexpr int kPage = 16;  // positions that lie together in the cache: block sizes are multiples
 
+// A weight is 2^(d - bias) of its score's distance d, in powers of two, from a scale m, which is exact to its own 2^-24
+// however large both are. m follows the maximum, and the bias the weights' sum, so that a wave's sum stays below 1: fp32
+// sums of the largest V are finite, over any number of positions. The maximum may outgrow m by 2^kLag before o and l are
+// scaled again; where a lane's sum has passed kFull, they shrink by 2^kShrink. The largest weight is 2^-kBias at
+// least (11 to 13), so that the sum of 32 positions' products, which fp32 rounds by 2^-150 at most, is off by 2^-137 of the
+// smallest V's outputs, whose last bit is 2^-133. A lag of 2 with 2^-10 would keep three bits more (8 trees of 25 at 1030
+// 24.2 us against 23.1, 16 of 33 at 2000 39.5, 37.0), one of 8 with 2^-15 two less (22.9, 37.0). At the end the waves' and
+// the splits' outputs meet by their shares of 1.
+constexpr float kLag = 6.0f, kFull = 0x1p-5f, kShrink = 4.0f;
+
 // Compile-time geometry. DIM: head dim rounded up; W: waves; QT: tiles of 16
 // query rows a wave; WQ of the waves hold query rows of their own, the other
 // factor WK splits each tile's T positions; NS: tiles in LDS.
@@ -166,6 +177,7 @@ struct Shape {
     static constexpr int DIM = DIM_, W = W_, QT = QT_, WQ = WQ_, WK = W_ / WQ_, T = T_, NS = NS_;
     static constexpr int KW = T / WK;                // a wave's positions of a tile
     static constexpr int KT = KW / 16;               // 16-position tiles of those
+    static constexpr float kBias = 11 + KT / 2;      // a lane's 4 KT weights of a tile, up to 2^(kLag - kBias), are 2^-3 at most
     static constexpr int DT = DIM / 16;              // 16-element tiles of a head
     static constexpr int KS = DIM / 32;              // products of 32 elements a score
     static constexpr int CH = DIM / 8;               // 16-byte chunks a row
@@ -179,6 +191,7 @@ struct Shape {
     static constexpr int kLds = NS * kStage > kMerge ? NS * kStage : kMerge;
     static constexpr int kFit = 160 * 1024 / (kLds + 64), kBlocks = kFit < 16 / W ? kFit : 16 / W;  // a CU (16 waves)
     static constexpr bool kAlone = WQ == 1;          // a wave reads only the rows that it copied
+    static_assert(KT == 1 || KT == 2 || KT == 4, "kBias");
     static_assert((COPIES == 1 || COPIES == 2 || COPIES == 4) && T <= 64 && kPage % OWN == 0 && KW % 16 == 0 && (!kAlone || KW == OWN), "tiles");
 };
 
@@ -198,7 +211,7 @@ __device__ __forceinline__ uint32_t numbers(uint32_t w) {
     return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
 }
 
-// Partial results of a split: unnormalised outputs, then (maximum, sum) pairs.
+// Partial results of a split: its outputs by themselves, then (m, sum of 2^d) pairs.
 struct Partials {
     float* out;   // [splits, rows * qh, dim]
     float2* sum;  // [splits, rows * qh]
@@ -389,11 +402,12 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     int next_row = own_page(min(tile0 + NS - 1, tile1 - 1));
 
     f32x4_t o[QT][DT];
-    float m[QT], l[QT];  // the weights' scale; their sum, of this lane's positions
+    float m[QT], l[QT], bias[QT];  // l: the weights' sum, of this lane's positions
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
         m[t] = -kInf;
         l[t] = 0.0f;
+        bias[t] = S::kBias;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[t][d] = f32x4_t{0, 0, 0, 0};
     }
@@ -482,12 +496,18 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int j = 0; j < KT; ++j)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, x[t][j][r]);
-            // The weights' common scale follows the maximum only where that outgrows it by 2^8: any scale near it will do.
-            if (__ballot((top - m[t]) * a.scale > 8.0f) != 0) {
+            if (__ballot((top - m[t]) * a.scale > kLag || l[t] > kFull) != 0) {
                 top = fmaxf(top, m[t]);
                 top = fmaxf(top, nvr::xor_lane(top, 16));
                 top = fmaxf(top, nvr::xor_lane(top, 32));
-                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f((m[t] - top) * a.scale);
+                float shrink = 0.0f;
+                if (__ballot(l[t] > kFull) != 0) {
+                    shrink = l[t] > kFull ? kShrink : 0.0f;
+                    shrink = fmaxf(shrink, nvr::xor_lane(shrink, 16));
+                    shrink = fmaxf(shrink, nvr::xor_lane(shrink, 32));
+                }
+                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(m[t] - top, a.scale, -shrink));
+                bias[t] += shrink;
                 l[t] *= old;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)
@@ -500,7 +520,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int j = 0; j < KT; ++j) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r] - base, a.scale, -kBias));
+                    x[t][j][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][j][r] - base, a.scale, -bias[t]));
                 l[t] += (x[t][j][0] + x[t][j][1]) + (x[t][j][2] + x[t][j][3]);
             }
         }
@@ -588,14 +608,20 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 #pragma unroll 1
     for (int tile = plain; tile < tile1; ++tile) step(tile, std::true_type{});
 
+    // ---- the waves' shares, then the output or the split's partial ----
+    // From here on outputs are by themselves, of whatever share of 1, and sums of 2^d.
     float sum[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-        sum[t] = l[t] + nvr::xor_lane(l[t], 16);
-        sum[t] += nvr::xor_lane(sum[t], 32);
+        float all = l[t] + nvr::xor_lane(l[t], 16);
+        all += nvr::xor_lane(all, 32);
+        const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+        sum[t] = all * __builtin_amdgcn_exp2f(bias[t]);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][d][r] *= inv;
     }
-
-    // ---- the waves' shares, then the output or the split's partial ----
     // The upper half of the waves hand theirs to the lower half, until one holds all.
     f32x4_t* merge = reinterpret_cast<f32x4_t*>(smem);
     float2* merge_sums = reinterpret_cast<float2*>(smem + (WK / 2 * WQ * QT * DT * kWave) * 16);
@@ -617,9 +643,11 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             for (int t = 0; t < QT; ++t) {
                 const float2 other = merge_sums[(from + t) * kWave + lane];
                 const float top = fmaxf(m[t], other.x), base = top == -kInf ? 0.0f : top;
-                const float f = __builtin_amdgcn_exp2f((m[t] - base) * a.scale), h = __builtin_amdgcn_exp2f((other.x - base) * a.scale);
+                const float mine = sum[t] * __builtin_amdgcn_exp2f((m[t] - base) * a.scale);
+                const float its = other.y * __builtin_amdgcn_exp2f((other.x - base) * a.scale);
                 m[t] = top;
-                sum[t] = __builtin_fmaf(other.y, h, sum[t] * f);
+                sum[t] = mine + its;
+                const float inv = sum[t] > 0.0f ? 1.0f / sum[t] : 0.0f, f = mine * inv, h = its * inv;
 #pragma unroll
                 for (int d = 0; d < DT; ++d) {
                     const f32x4_t v = merge[((from + t) * DT + d) * kWave + lane];
@@ -635,20 +663,19 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
         const int qi = q0 + (wq * QT + t) * 16 + n16;
         if (qi >= queries) continue;
         const int64_t out_row = int64_t(span.start + qi / group) * a.qh + kvhead * group + qi % group;
-        const float inv = sum[t] > 0.0f ? 1.0f / sum[t] : 0.0f;
         const int64_t at = int64_t(split) * a.rows * a.qh + out_row;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
             const int e = 16 * d + 4 * g;
             if (e >= a.dim) continue;
-            if (used == 1) {
-                float y[4];
+            f32x4_t y;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = sum[t] > 0.0f ? o[t][d][r] * inv : 0.0f;
+            for (int r = 0; r < 4; ++r) y[r] = sum[t] > 0.0f ? o[t][d][r] : 0.0f;
+            if (used == 1) {
                 *reinterpret_cast<uint2*>(a.out + out_row * a.dim + e) =
                     make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
             } else {
-                *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = o[t][d];
+                *reinterpret_cast<f32x4_t*>(part.out + at * a.dim + e) = y;
             }
         }
         if (used != 1 && g == 0) part.sum[at] = make_float2(m[t], sum[t]);
@@ -670,39 +697,54 @@ __global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials 
     const int quads = a.dim / 4, i = int(blockIdx.x % unsigned(parts)) * 256 + int(threadIdx.x);
     if (used == 1 || i >= a.qh * quads) return;
     const int64_t at = int64_t(span.start + node) * a.qh + i / quads, plane = int64_t(a.rows) * a.qh;
-    float top = -kInf, den = 0.0f;
-    f32x4_t num = {0, 0, 0, 0};
-    for (int w0 = 0; w0 < used; w0 += kBatch) {
-        float2 ml[kBatch];
-        f32x4_t v[kBatch];
+    float2 ml[kBatch];
+    f32x4_t v[kBatch];
+    auto sums = [&](int w0) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int64_t from = min(w0 + u, used - 1) * plane + at;
-            ml[u] = part.sum[from];
-            v[u] = *reinterpret_cast<const f32x4_t*>(part.out + from * a.dim + 4 * (i % quads));
-            if (w0 + u >= used) ml[u].x = -kInf;
+            ml[u] = part.sum[min(w0 + u, used - 1) * plane + at];
+            if (w0 + u >= used) ml[u] = make_float2(-kInf, 0.0f);
         }
+    };
+    auto outs = [&](int w0) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            v[u] = *reinterpret_cast<const f32x4_t*>(part.out + (min(w0 + u, used - 1) * plane + at) * a.dim + 4 * (i % quads));
+    };
+    // The splits' shares of 1 first, so that no sum of theirs passes the outputs' own range.
+    sums(0);
+    outs(0);
+    float top = -kInf, den = 0.0f;
+    for (int w0 = 0;;) {
         float high = top;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) high = fmaxf(high, ml[u].x);
-        const float base = high == -kInf ? 0.0f : high, old = __builtin_amdgcn_exp2f((top - base) * a.scale);
-        den *= old;
+        const float base = high == -kInf ? 0.0f : high;
+        den *= __builtin_amdgcn_exp2f((top - base) * a.scale);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) num[r] *= old;
+        for (int u = 0; u < kBatch; ++u) den = __builtin_fmaf(ml[u].y, __builtin_amdgcn_exp2f((ml[u].x - base) * a.scale), den);
+        top = high;
+        if ((w0 += kBatch) >= used) break;
+        sums(w0);
+    }
+    if (used > kBatch) sums(0);
+    const float base = top == -kInf ? 0.0f : top, inv = den > 0.0f ? 1.0f / den : 0.0f;
+    f32x4_t num = {0, 0, 0, 0};
+    for (int w0 = 0;;) {
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if (w0 + u >= used) continue;
-            const float f = __builtin_amdgcn_exp2f((ml[u].x - base) * a.scale);
-            den = __builtin_fmaf(ml[u].y, f, den);
+            const float f = ml[u].y * __builtin_amdgcn_exp2f((ml[u].x - base) * a.scale) * inv;
 #pragma unroll
             for (int r = 0; r < 4; ++r) num[r] = __builtin_fmaf(v[u][r], f, num[r]);
         }
-        top = high;
+        if ((w0 += kBatch) >= used) break;
+        sums(w0);
+        outs(w0);
     }
-    const float inv = den > 0.0f ? 1.0f / den : 0.0f;
     float y[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) y[r] = den > 0.0f ? num[r] * inv : 0.0f;
+    for (int r = 0; r < 4; ++r) y[r] = den > 0.0f ? num[r] : 0.0f;
     *reinterpret_cast<uint2*>(a.out + at * a.dim + 4 * (i % quads)) =
         make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
 }

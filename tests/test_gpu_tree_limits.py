@@ -36,7 +36,9 @@ def check_tightly(t, got):
     """As Trees.check, with weights held in more than 16 bits. Off against the formula: a weight by 2^-17 at most
     where it is two bf16 (2^-18 each, and as much in the normaliser), by the exponential's few roundings (2^-18, twice
     likewise) and by its score (dim roundings of the sum of its products' sizes; twice); a sum of N weights or
-    products by N roundings, twice; the output by its own."""
+    products by N roundings, twice; the output by its own, which is 2^-134 where it is subnormal: bf16's last bit is
+    2^-133 there. Sums of subnormal products round by 2^-150, once in 32 positions, at weights of 2^-13 for the largest:
+    2^-137 of the output."""
     with np.errstate(all="ignore"):
         want, _ = ref.attention(values(t.q), values(t.kc), values(t.vc), t.contexts, t.row_starts, t.masks, t.tables,
                                 t.kvh, t.bs, t.blocks, t.max_nodes, t.max_context, values(t.out))
@@ -54,7 +56,7 @@ def check_tightly(t, got):
                 p = np.exp(score - score.max())
                 score_off = t.dim * 2.0 ** -24 * (np.abs(k) @ np.abs(q[a + i, h])).max() / np.sqrt(t.dim)
                 part = 2 * 2.0 ** -17 + 2 * score_off + 2 * len(at) * 2.0 ** -24
-                bound = p @ vc[at, h // group] / p.sum() * part + 2.0 ** -8 * np.abs(want[a + i, h])
+                bound = p @ vc[at, h // group] / p.sum() * part + 2.0 ** -8 * np.abs(want[a + i, h]) + 2.0 ** -134 + -(-len(at) // 32) * 2.0 ** -137
                 assert (off[a + i, h] <= bound).all(), (s, i, h, float((off[a + i, h] / bound).max()))
 
 
@@ -89,3 +91,63 @@ def test_attention_of_the_largest_values_under_vast_scores(gpu, dim, level):
         x[..., 0] = nvr.bf16_bits(np.array([size]))[0]
     got, want, bound = constant_values(t, gpu, 3.2e38)
     assert (np.abs(got - want) <= bound).all()
+
+
+@each_shape
+@pytest.mark.parametrize("size", [1e-38, 3e-38, 1e-36, 1e-20, 1e20, 1e30, 3.3e38])
+def test_attention_of_values_of_any_size(gpu, shape, size):
+    """V of one size, from the smallest normal numbers to the largest, its weight spread over 700 positions."""
+    t = trees(shape, 700, 150, 5200, spread=0.01)
+    got, want, bound = constant_values(t, gpu, size)
+    assert (np.abs(got - want) <= bound).all()
+
+
+@each_shape
+@pytest.mark.parametrize("size", [1e-37, 1e37])
+def test_attention_holds_values_of_any_size(gpu, shape, size):
+    """Values of both signs near either end of the type: as exact as those near 1."""
+    t = trees(shape, 600, 150, 5300)
+    t.vc = nvr.bf16_bits(values(t.vc) * size)
+    t.upload(gpu).launch(gpu)
+    check_tightly(t, t.result())
+
+
+@pytest.mark.parametrize("dim", [128, 64, 256, 80, 10])
+def test_attention_of_small_values_beside_large_ones(gpu, dim):
+    """Head elements of the largest V, of the smallest and of subnormals in one head: each is as exact as by itself. A
+    subnormal output is off by half its last bit, 2^-134."""
+    t = Trees([9, 3], [2100, 35], 8, 4, dim, 16, 5400, spread=0.01)
+    sizes = np.resize(np.array([3.2e38, 1e-38, 1.0, -4e-39, -3.2e38, 2e-40]), dim)
+    t.vc = nvr.bf16_bits(np.broadcast_to(sizes, t.vc.shape))
+    t.upload(gpu).launch(gpu)
+    got, want = values(t.result()), values(t.vc)[0, 0]
+    assert (np.abs(got - want) <= (2.0 ** -8 + 2 * 2.0 ** -12) * np.abs(want) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("dim,bs", [(64, 256), (128, 256), (256, 64), (64, 7)])
+def test_attention_of_the_largest_values_at_many_positions(gpu, dim, bs):
+    """More than 2^17 positions that share the weight: two sums of n weights are off by n roundings each at most, which
+    is 2^-5.9 for the 137000 of them."""
+    positions = 137000
+    t = Trees([4], [positions], 1, 1, dim, bs, 5500, spread=0.01)
+    t.vc = nvr.bf16_bits(np.broadcast_to(np.where(np.arange(dim) % 3 == 0, -3.2e38, 3.2e38), t.vc.shape))
+    t.upload(gpu).launch(gpu)
+    got, want = values(t.result()), values(t.vc)[0, 0]
+    bound = (2.0 ** -8 + 2 * positions * 2.0 ** -24) * np.abs(want)
+    assert (np.abs(got - want) <= bound).all()
+
+
+@each_shape
+@pytest.mark.parametrize("value", [0x7F80, 0xFF80, 0x7FC0])
+def test_attention_of_infinite_values_in_the_context(gpu, shape, value):
+    """An Inf or NaN in V at a committed position stays in its head element of every row of its KV head, and changes no
+    other."""
+    t = trees(shape, 300, 700, 5600)
+    clean = t.run(gpu)
+    group = t.qh // t.kvh
+    t.vc[t.tables[0][100 // 16] * 16 + 100 % 16, 1 % t.kvh, 5] = value
+    t.upload(gpu).launch(gpu)
+    got, heads = t.result(), slice(1 % t.kvh * group, (1 % t.kvh + 1) * group)
+    assert not np.isfinite(values(got[:t.sizes[0], heads, 5])).any()
+    got[:t.sizes[0], heads, 5] = clean[:t.sizes[0], heads, 5]
+    assert np.array_equal(got, clean)
