@@ -30,9 +30,12 @@
 // to the lower index; an argmax of nothing is 0.
 //
 // For T > 0 the emitted tokens are distributed as the target's own samples are.
-// What decides is held in fp32 sums of fp32 exponentials, and in fp64 from there
-// on: a comparison or an argmax goes the other way than exact arithmetic has it
-// only where both sides agree to about 1e-6.
+// What decides is held in fp64 sums of fp32 exponentials (added by eights first),
+// and in fp64 from there on: a comparison or an argmax goes the other way than exact
+// arithmetic has it only where both sides agree to about 1e-6 of the p and c q that
+// they are made of, over any vocabulary. The largest exponential of a row is the same
+// number wherever it is taken, so that where one token has nearly all of p, what is
+// left of 1 is that exact as well.
 //
 // Launches: 1. verify_stats: for each row that has children, the sum of the
 // exponentials (T > 0; both models') or the argmax, by shares of the rows.
@@ -69,9 +72,9 @@ constexpr float kInf = __builtin_inff();
 // is the scaled maximum itself and the sum counts the logits that have it: others
 // are at least 2^15 below. Else: the maximum and its token.
 struct Stats {
-    float offset, sum;
+    float offset;
     int best;
-    int pad;
+    double sum;
 };
 
 // Where a sequence's walk ended.
@@ -79,8 +82,9 @@ struct Path {
     int row;    // its last row, or -1: an invalid sequence
     int node;   // its tokens but the last one
     int tried;  // tokens to leave out (no draft logits)
-    float c;    // what rejections took (draft logits)
-    float offset, inv_sum, draft_offset, draft_inv_sum;  // of the last row, where c > 0
+    double c;   // what rejections took (draft logits)
+    double inv_sum, draft_inv_sum;  // of the last row, where c > 0
+    float offset, draft_offset;
 };
 // The same for launch 3, and its search for the last token.
 struct Ending {
@@ -151,11 +155,11 @@ __device__ __forceinline__ int lead_of(const uint16_t* row) { return int(reinter
 // log2(e) / T, finite, so that a logit of 0 stays 0.
 __device__ __forceinline__ float scale_of(float temperature) { return fminf(kLog2e / temperature, 0x1.fffffep127f); }
 __device__ __forceinline__ bool vast(float offset) { return !(fabsf(offset) < 0x1p24f); }
-__device__ __forceinline__ float inverse(float sum) { return sum > 0.0f ? 1.0f / sum : 0.0f; }
+__device__ __forceinline__ double inverse(double sum) { return sum > 0.0 ? 1.0 / sum : 0.0; }
 // A sum at one offset, at another that is no smaller.
-__device__ __forceinline__ float at_offset(float sum, float offset, float other) {
-    if (!(sum > 0.0f)) return 0.0f;
-    return offset == other ? sum : __builtin_ldexpf(sum, int(fmaxf(offset - other, -1000.0f)));
+__device__ __forceinline__ double at_offset(double sum, float offset, float other) {
+    if (!(sum > 0.0)) return 0.0;
+    return offset == other ? sum : ldexp(sum, int(fmaxf(offset - other, -1000.0f)));
 }
 
 struct Best {
@@ -179,11 +183,6 @@ __device__ __forceinline__ Best wave_best(Best b) {
 #pragma unroll
     for (int mask = 1; mask < kWave; mask <<= 1) index = min(index, nvr::xor_lane(index, mask));
     return Best{top, index};
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int mask = 1; mask < kWave; mask <<= 1) v += nvr::xor_lane(v, mask);
-    return v;
 }
 __device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
@@ -220,7 +219,7 @@ struct Shares {
 // A thread's chunks begin, begin + kThreads, ... < end of a row and one more value,
 // with their NaN, infinite and huge values looked at one by one.
 __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int begin, int end, float edge, int vocab,
-                                            float scale, float* offset, float* sum) {
+                                            float scale, float* offset, double* sum) {
     float top = fmaxf(edge * scale, -kInf);
     for (int k = begin; k < end; k += kThreads) {
         float f[8];
@@ -234,12 +233,13 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
         const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(v, scale, -at));
         return w == w ? w : 0.0f;  // nor has an infinite logit a weight where T is infinite
     };
-    float total = top > -kInf ? weight(edge) : 0.0f;
+    double total = top > -kInf ? double(weight(edge)) : 0.0;
     for (int k = begin; k < end && top > -kInf; k += kThreads) {
-        float f[8];
+        float f[8], eight = 0.0f;
         load_chunk(x, 8 * int64_t(k) - lead, vocab, f);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) total += weight(f[j]);
+        for (int j = 0; j < 8; ++j) eight += weight(f[j]);
+        total += double(eight);
     }
     *offset = at;
     *sum = total;
@@ -255,7 +255,8 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
 // 30.8, 59.1, eight 32.1, 61.1).
 __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a) {
     constexpr int kWaves = kThreads / kWave;
-    __shared__ float tops[kWaves], sums[kWaves];
+    __shared__ float tops[kWaves];
+    __shared__ double sums[kWaves];
     __shared__ int first;
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const int block = int(blockIdx.x % unsigned(a.blocks)), item = int(blockIdx.x / unsigned(a.blocks));
@@ -325,49 +326,56 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
         const int begin_k = lo + int(threadIdx.x);
         uint4 packed[kLoads];
         if (begin_k < hi) load(begin_k, packed);
-        Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
+        float offset = -kInf;
+        double total = 0.0;
         int where = -2;  // the chunk whose load has the maximum; -1: the edge
         if (sampled) {
             float high = edge;
             if (begin_k < hi) high = fmaxf(high, highest(begin_k, packed));
             high *= scale;
-            mine.offset = vast(high) ? 0.0f : __builtin_rintf(high);
-            mine.sum = __builtin_amdgcn_exp2f(__builtin_fmaf(edge, scale, -mine.offset));
+            offset = vast(high) ? 0.0f : __builtin_rintf(high);
+            total = double(__builtin_amdgcn_exp2f(__builtin_fmaf(edge, scale, -offset)));
             for (int k = begin_k; k < hi; k += kLoads * kThreads) {
                 uint4 now[kLoads];
                 take(k, packed, now);
+                const float grown = highest(k, now) * scale;
+                if (grown > offset + 0.5f && !vast(grown)) {
+                    const float to = __builtin_rintf(grown);
+                    total = at_offset(total, offset, to);
+                    offset = to;
+                }
 #pragma unroll
                 for (int u = 0; u < kLoads; ++u) {
                     float f[8], eight = 0.0f;
                     loaded(k + u * kThreads, now[u], f);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], scale, -mine.offset));
-                    mine.sum += eight;
+                    for (int j = 0; j < 8; ++j) eight += __builtin_amdgcn_exp2f(__builtin_fmaf(f[j], scale, -offset));
+                    total += double(eight);
                 }
             }
-            if (!(mine.sum >= 0x1p-20f && mine.sum < 0x1p100f))
-                careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &mine.offset, &mine.sum);
-            if (!(mine.sum > 0.0f)) mine.offset = -kInf;
+            if (!(total >= 0x1p-20 && total < 0x1p100))
+                careful_sum(x, lead, begin_k, hi, edge, a.vocab, scale, &offset, &total);
+            if (!(total > 0.0)) offset = -kInf;
         } else {
-            if (edge == edge && lone >= 0 && lone < a.vocab) { mine.offset = edge; where = -1; }
+            if (edge == edge && lone >= 0 && lone < a.vocab) { offset = edge; where = -1; }
             for (int k = begin_k; k < hi; k += kLoads * kThreads) {
                 uint4 now[kLoads];
                 take(k, packed, now);
                 const float high = highest(k, now);
-                if (high > mine.offset || (where < 0 && high == mine.offset)) {
-                    mine.offset = high;
+                if (high > offset || (where < 0 && high == offset)) {
+                    offset = high;
                     where = k;
                 }
             }
         }
-        const float high = wave_max(mine.offset);
+        const float high = wave_max(offset);
         if (lane == 0) tops[wave] = high;
         if (threadIdx.x == 0) first = nvr::kNoIndex;
         __syncthreads();
         float all = tops[0];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) all = fmaxf(all, tops[w]);
-        if (where > -2 && mine.offset == all) {
+        if (where > -2 && offset == all) {
             // The lowest of this thread's tokens with that logit.
             int lowest = lone >= 0 && lone < a.vocab && edge == all ? lone : nvr::kNoIndex;
 #pragma unroll 1
@@ -382,14 +390,14 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
             }
             atomicMin(&first, lowest);
         }
-        const float sum = wave_sum(at_offset(mine.sum, mine.offset, all));
+        const double sum = wave_sum(at_offset(total, offset, all));
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         if (threadIdx.x == 0) {
-            float total = 0.0f;
+            double parts = 0.0;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) total += sums[w];
-            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + block - shares.first_block(i)] = Stats{all, total, first, 0};
+            for (int w = 0; w < kWaves; ++w) parts += sums[w];
+            (side ? a.draft_stats : a.stats)[int64_t(row) * a.parts + block - shares.first_block(i)] = Stats{all, first, parts};
         }
     }
 }
@@ -398,13 +406,13 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
 __device__ __forceinline__ Stats fold(const Stats& mine, double sum) {
     const Best b = wave_best(Best{mine.offset, mine.best});
     const double scaled = sum > 0.0 ? ldexp(sum, mine.offset == b.score ? 0 : int(fmaxf(mine.offset - b.score, -1000.0f))) : 0.0;
-    return Stats{b.score, float(wave_sum(scaled)), b.index, 0};
+    return Stats{b.score, b.index, wave_sum(scaled)};
 }
 __device__ __forceinline__ void add_part(Stats& mine, double& sum, const Stats& t) {
     Best b{mine.offset, mine.best};
     consider(b, t.offset, t.best);
     sum = ldexp(sum, sum > 0.0 && mine.offset != b.score ? int(fmaxf(mine.offset - b.score, -1000.0f)) : 0) +
-          double(at_offset(t.sum, t.offset, b.score));
+          at_offset(t.sum, t.offset, b.score);
     mine.offset = b.score;
     mine.best = b.index;
 }
@@ -413,29 +421,31 @@ __device__ __forceinline__ void add_part(Stats& mine, double& sum, const Stats& 
 struct Rows {
     const uint16_t* target;
     const uint16_t* draft;
-    float offset, inv_sum, draft_offset, draft_inv_sum;
+    float offset, draft_offset;
+    double inv_sum, draft_inv_sum;
 };
 
-// p - c q of one token; NaN where p is.
+// p - c q of one token, in fp64, since both may be near 1 and agree; NaN where p is.
 struct RestTerm {
     const Rows& r;
-    float scale, cq;
+    float scale;
+    double cq;
     bool any_vast;
-    __device__ __forceinline__ RestTerm(const Rows& rows, float c, float s)
+    __device__ __forceinline__ RestTerm(const Rows& rows, double c, float s)
         : r(rows), scale(s), cq(c * rows.draft_inv_sum), any_vast(vast(rows.offset) || vast(rows.draft_offset)) {}
     __device__ __forceinline__ float weight(float x, float offset) const {
         if (any_vast && vast(offset)) return x * scale == offset ? 1.0f : 0.0f;
         return __builtin_amdgcn_exp2f(__builtin_fmaf(x, scale, -offset));
     }
-    __device__ __forceinline__ float operator()(float x, float y) const {
+    __device__ __forceinline__ double operator()(float x, float y) const {
         const float wy = fmaxf(weight(y, r.draft_offset), 0.0f);  // a NaN is no token of q
-        return __builtin_fmaf(weight(x, r.offset), r.inv_sum, -(wy * cq));
+        return __builtin_fma(double(weight(x, r.offset)), r.inv_sum, -(double(wy) * cq));
     }
 };
 
 // sum of max(p - c q, 0) over 16-byte chunks [first, end) of a row, this thread's share.
 template <int kBatch>  // chunks in flight a thread
-__device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, float scale, int64_t first, int64_t end,
+__device__ __forceinline__ double rest_sum(const Rows& r, int vocab, double c, float scale, int64_t first, int64_t end,
                                            int threads) {
     const int lead = lead_of(r.target);
     const bool alike = lead == lead_of(r.draft);
@@ -457,10 +467,10 @@ __device__ __forceinline__ double rest_sum(const Rows& r, int vocab, float c, fl
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            float eight = 0.0f;
+            double eight = 0.0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) eight += fmaxf(term(x[u][i], y[u][i]), 0.0f);
-            sum += k + u * threads < end ? double(eight) : 0.0;
+            for (int i = 0; i < 8; ++i) eight += fmax(term(x[u][i], y[u][i]), 0.0);
+            sum += k + u * threads < end ? eight : 0.0;
         }
     }
     return sum;
@@ -550,7 +560,7 @@ __device__ __forceinline__ void fold_nodes(const VerifyArgs& a, const Tree& t, b
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if (first + u * kWaves >= items) continue;
-            Stats mine{-kInf, 0.0f, nvr::kNoIndex, 0};
+            Stats mine{-kInf, nvr::kNoIndex, 0.0};
             double sum = 0.0;
             if (lane < parts[u]) add_part(mine, sum, part[u]);
             for (int i = lane + kWave; i < parts[u]; i += kWave) add_part(mine, sum, from[u][i]);
@@ -561,15 +571,15 @@ __device__ __forceinline__ void fold_nodes(const VerifyArgs& a, const Tree& t, b
 }
 __device__ __forceinline__ Rows rows_of(const VerifyArgs& a, int row, const Stats& t, const Stats& d) {
     const int64_t at = int64_t(row) * a.vocab;
-    return Rows{a.logits + at, a.draft + at, t.sum > 0.0f ? t.offset : 0.0f, inverse(t.sum), d.sum > 0.0f ? d.offset : 0.0f,
+    return Rows{a.logits + at, a.draft + at, t.sum > 0.0 ? t.offset : 0.0f, d.sum > 0.0 ? d.offset : 0.0f, inverse(t.sum),
                 inverse(d.sum)};
 }
 // The probability of a logit of a row: 2^y, y = k + f, |f| <= 1/2, in fp64 but for 2^f.
 __device__ __forceinline__ double chance(float x, float scale, const Stats& r) {
-    if (!(r.sum > 0.0f) || x != x) return 0.0;
-    if (vast(r.offset)) return x * scale == r.offset ? 1.0 / double(r.sum) : 0.0;
+    if (!(r.sum > 0.0) || x != x) return 0.0;
+    if (vast(r.offset)) return x * scale == r.offset ? 1.0 / r.sum : 0.0;
     const double y = double(x) * double(scale) - double(r.offset), k = rint(y);
-    return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / double(r.sum) : 0.0;
+    return y > -1000.0 ? ldexp(double(__builtin_amdgcn_exp2f(float(y - k))), int(k)) / r.sum : 0.0;
 }
 
 // A path's nodes and tokens, and their number; all but its last token, which launch 3 stores.
@@ -625,7 +635,7 @@ struct SimpleWalk {
                 const double px = lane_value(p, i), ux = lane_value(t.u, i);
                 if (drafted) {  // the only child
                     if (accepted(px, lane_value(q, i), ux, 0.0, 1.0)) next = i;
-                    else end.c = 1.0f;
+                    else end.c = 1.0;
                     break;
                 }
                 if (__ballot((rejected >> lane & 1) != 0 && t.token == x) != 0) continue;
@@ -640,7 +650,7 @@ struct SimpleWalk {
         __syncthreads();  // path, tried
         end.row = t.start + v;
         end.tried = __popcll(rejected);
-        if (end.c > 0.0f) {
+        if (end.c > 0.0) {
             const Rows r = rows_of(a, end.row, target[v], draft[v]);
             end.offset = r.offset;
             end.inv_sum = r.inv_sum;
@@ -757,14 +767,14 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     };
     once = look(false);
     if constexpr (kFirst) {
-        if (once != 0) sum_rests(once, a.rests, [](int) { return 1.0f; });
+        if (once != 0) sum_rests(once, a.rests, [](int) { return 1.0; });
         return;
     }
     read_rests(once, a.rests, rests[0]);
     const uint64_t twice = look(true);
     if (twice == 0 && slice != 0) return;
     if (twice != 0) {
-        sum_rests(twice, a.rests + int64_t(a.rows) * kSlices, [&](int v) { return float(1.0 + rests[0][v]); });
+        sum_rests(twice, a.rests + int64_t(a.rows) * kSlices, [&](int v) { return 1.0 + rests[0][v]; });
         __syncthreads();
         if (threadIdx.x == 0) last = arrive(a.arrived + s) == slices - 1;
         __syncthreads();
@@ -790,7 +800,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
             if (tried < 2) {
                 z = rests[tried][v];
             } else {
-                const double sum = wave_sum(rest_sum<4>(rows_at(v), a.vocab, float(c), scale, 0, chunks, kWalkThreads));
+                const double sum = wave_sum(rest_sum<4>(rows_at(v), a.vocab, c, scale, 0, chunks, kWalkThreads));
                 if (lane == 0) parts[0][wave] = sum;
                 __syncthreads();
                 z = 0.0;
@@ -805,7 +815,7 @@ __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     write_path(a, s, start, path, length);
     if (threadIdx.x == 0) {
         const Rows r = rows_at(v);
-        ending->path = Path{start + v, length - 1, 0, float(c), r.offset, r.inv_sum, r.draft_offset, r.draft_inv_sum};
+        ending->path = Path{start + v, length - 1, 0, c, r.inv_sum, r.draft_inv_sum, r.offset, r.draft_offset};
     }
 }
 
@@ -849,12 +859,12 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
     }
     const int row = path.row, node = path.node, count = path.tried;
     if (row < 0) return;
-    const float c = path.c;
+    const double c = path.c;
     const uint16_t* x = a.logits + int64_t(row) * a.vocab;
     const int64_t t = int64_t(part) * kSampled + 8 * int(threadIdx.x) - lead_of(x);
-    const Rows rest{x, c > 0.0f ? a.draft + int64_t(row) * a.vocab : x, path.offset, path.inv_sum, path.draft_offset, path.draft_inv_sum};
+    const Rows rest{x, c > 0.0 ? a.draft + int64_t(row) * a.vocab : x, path.offset, path.draft_offset, path.inv_sum, path.draft_inv_sum};
     uint4 packed_q = {};
-    if (c > 0.0f) packed_q = packed_chunk(rest.draft, t, a.vocab, lead_of(rest.draft) == lead_of(x));
+    if (c > 0.0) packed_q = packed_chunk(rest.draft, t, a.vocab, lead_of(rest.draft) == lead_of(x));
     float f[8];
     load_chunk(x, t, a.vocab, f);
     if constexpr (!kWalks) {
@@ -868,13 +878,13 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) consider(b, f[i], int(t) + i);
     } else {
-        if (c > 0.0f) {  // ln(p - c q) in place of the logits
+        if (c > 0.0) {  // ln(p - c q) in place of the logits
             const RestTerm term(rest, c, scale);
             float q[8];
             nvr::unpack8(packed_q, q);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float w = term(f[i], q[i]);
+                const float w = float(term(f[i], q[i]));
                 f[i] = w >= 0x1p-126f ? w : __builtin_nanf("");
             }
         }
@@ -888,11 +898,11 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
         }
         auto uniform = [&](int i) { return nvr::hash_uniform(nvr::splitmix64(seed ^ (uint64_t(t + i) * nvr::kTokenMix))); };
         auto score = [&](float v, float u) {
-            return (c > 0.0f ? nvr::nvr_logf(v) : v / temperature) - nvr::nvr_logf(-nvr::nvr_logf(u));
+            return (c > 0.0 ? nvr::nvr_logf(v) : v / temperature) - nvr::nvr_logf(-nvr::nvr_logf(u));
         };
         const float inverse_t = 1.0f / temperature;
         float bound[8], us[8], high = -kInf;
-        if (c > 0.0f) {
+        if (c > 0.0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) bound[i] = __builtin_amdgcn_logf(f[i]) * kLn2;
         } else {
@@ -926,7 +936,7 @@ __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i != own && bound[i] >= reach) consider(b, score(f[i], us[i]), int(t) + i);
-        if (b.score == -kInf && (count > 0 || c > 0.0f)) b.index = nvr::kNoIndex;  // the rest is nothing here
+        if (b.score == -kInf && (count > 0 || c > 0.0)) b.index = nvr::kNoIndex;  // the rest is nothing here
     }
     auto block_best = [&] {  // in thread 0
         b = wave_best(b);

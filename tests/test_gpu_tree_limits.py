@@ -5,7 +5,7 @@ import pytest
 
 import nvr
 import tree_reference as ref
-from test_gpu_tree import Trees
+from test_gpu_tree import Drafts, Trees
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,58 @@ def test_attention_of_infinite_values_in_the_context(gpu, shape, value):
     assert not np.isfinite(values(got[:t.sizes[0], heads, 5])).any()
     got[:t.sizes[0], heads, 5] = clean[:t.sizes[0], heads, 5]
     assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_verification_sums_large_vocabularies(gpu, masked):
+    """Rows of about a million equal logits (with `masked`, every other one a NaN), each summed by one block: drafted
+    tokens of probability 1 / n are accepted by a uniform 3e-6 below that and rejected by one 3e-6 above it. The sum is
+    within 1e-6: additions of eight exponentials and their own roundings (2^-21), the parts' to fp32 (2^-23)."""
+    batch, nodes, vocab = 20, 64, 1_000_003
+    rng = np.random.default_rng(6000)
+    levels = nvr.bf16_bits(rng.normal(size=batch * nodes) * 3.0)
+    logits = gpu.alloc(batch * nodes * vocab * 2)
+    row = np.empty(vocab, np.uint16)
+    for i, level in enumerate(levels):
+        row[:] = level
+        if masked:
+            row[1::2] = 0x7FC0
+        logits.slice(i * vocab * 2, vocab * 2).upload(row)
+    p = 1.0 / (vocab - vocab // 2 if masked else vocab)
+    uniforms = np.full((batch, nodes), p * (1 - 3e-6), np.float32)
+    ends = rng.integers(1, nodes, batch)  # the node that is rejected
+    uniforms[np.arange(batch), ends] = p * (1 + 3e-6)
+    tokens = (2 * rng.integers(0, vocab // 2, batch * nodes)).astype(np.int32)
+    inputs = [gpu.upload_array(a) for a in (
+        tokens, np.tile(np.arange(-1, nodes - 1, dtype=np.int32), batch), np.arange(batch + 1, dtype=np.int32) * nodes,
+        rng.uniform(0.5, 1.5, batch).astype(np.float32), uniforms, rng.integers(0, 2 ** 64, batch, dtype=np.uint64))]
+    outputs = [gpu.alloc(batch * nodes * 4), gpu.alloc(batch * nodes * 4), gpu.alloc(batch * 4)]
+    gpu.verify_tree(logits, None, *inputs, *outputs, gpu.alloc(gpu.verify_tree_workspace(batch * nodes, batch, vocab)),
+                    batch * nodes, batch, nodes, vocab)
+    assert outputs[2].download(np.int32, batch).tolist() == ends.tolist()
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("vocab", [9001, 50257])
+def test_verification_of_what_one_token_leaves(gpu, vocab, draft):
+    """One token has all but 1e-5 (picked) or 1e-9 (drawn) of both models' probabilities, somewhere in the row, and the
+    drafted ones are others, but the first of the picked ones it: what is left of 1 and the rest's sum are differences
+    of numbers near 1, and the path and its last token those of the 64-bit walk all the same."""
+    d = Drafts([4] * 150, vocab, 6100 + vocab % 7, draft, fan=3, temps=(0.3, 0.7, 1.0))
+    rng = np.random.default_rng(6101)
+    d.parents = np.tile(np.array([-1, 0, 0, 0], np.int32), 150)
+    scale = np.repeat(np.resize(np.array([0.3, 0.7, 1.0]), 150), 4)[:, None]
+    x = rng.normal(size=(600, vocab)) * scale  # a mass of about vocab * exp(1/2) without the one token
+    at = rng.integers(0, vocab, 600)
+    high = np.log(vocab) + 0.5 + (9 if draft else 5) * np.log(10)
+    for logits in [d.logits] + ([d.draft] if draft else []):
+        y = x if logits is d.logits else x + 0.5 * rng.normal(size=x.shape) * scale
+        y[np.arange(600), at] = (high + 0.3 * rng.normal(size=600)) * scale[:, 0]
+        logits[:] = nvr.bf16_bits(y)
+    d.tokens = rng.integers(0, vocab, 600).astype(np.int32)
+    d.uniforms = rng.random(600, dtype=np.float32)
+    if not draft:
+        d.tokens[1::4] = at[0::4]
+        d.uniforms[1::4] = np.nextafter(np.float32(1), np.float32(0))
+    counts = d.run(gpu)
+    assert (d.result()[0][counts == 1, 0] != at[0::4][counts == 1]).any()
