@@ -378,10 +378,10 @@ __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a
         if (where > -2 && offset == all) {
             // The lowest of this thread's tokens with that logit.
             int lowest = lone >= 0 && lone < a.vocab && edge == all ? lone : nvr::kNoIndex;
+            // Where that is -inf, loads of NaN alone had it too: all of the thread's are looked at.
+            const int from = all == -kInf ? begin_k : where, until = all == -kInf ? hi : min(hi, from + kLoads * kThreads);
 #pragma unroll 1
-            for (int u = kLoads - 1; u >= 0; --u) {
-                const int c = where + u * kThreads;
-                if (where < 0 || c >= hi) continue;
+            for (int c = from; c < until && where >= 0; c += kThreads) {
                 float f[8];
                 load_chunk(x, 8 * int64_t(c) - lead, a.vocab, f);
 #pragma unroll

@@ -206,3 +206,18 @@ def test_verification_of_what_one_token_leaves(gpu, vocab, draft):
         d.uniforms[1::4] = np.nextafter(np.float32(1), np.float32(0))
     counts = d.run(gpu)
     assert (d.result()[0][counts == 1, 0] != at[0::4][counts == 1]).any()
+
+
+@pytest.mark.parametrize("vocab", [30011, 120011])  # walks in the last launch, and in one of its own
+def test_greedy_verification_of_rows_without_numbers(gpu, vocab):
+    """Rows of NaN and some -inf: their argmax is the first -inf, wherever it lies; of NaN alone, token 0."""
+    d = Drafts([3] * 6, vocab, 6200, False, fan=1, temps=(0.0,))
+    d.logits[:] = 0x7FC0
+    firsts = [6000, vocab - 1, 4100, 0, 20007, None]
+    for s, first in enumerate(firsts):
+        if first is not None:
+            d.logits[3 * s:3 * s + 3, [first, min(first + 4000, vocab - 1)]] = 0xFF80
+        d.tokens[3 * s + 1:3 * s + 3] = first or 0
+    d.run(gpu)
+    tokens, _, counts = d.result()
+    assert (counts == 3).all() and tokens.tolist() == [[first or 0] * 3 for first in firsts]
