@@ -255,7 +255,7 @@ int nv_attention_tree_workspace(int rows, int qh, int kvh, int dim, int batch, i
  * (contexts[s] + nodes) and, like max_nodes, sizes the launch. Head dims that are
  * multiples of 8 in blocks of multiples of 16 positions, with q, kc, vc and out at
  * multiples of 16 bytes, take the matrix instructions, with each weight as two bf16
- * (within 2^-18 of it); others a kernel for any layout, many times slower. Returns -2 for
+ * (within 2^-15 of it); others a kernel for any layout, many times slower. Returns -2 for
  * qh % kvh != 0, an odd head dim or one above 256, max_nodes outside [1, 64], and
  * sizes past one launch (2^32 threads) or past int32 (rows * qh, batch * kvh). */
 int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* vc, const void* contexts,

@@ -19,7 +19,7 @@
 //
 // Scores, maxima, sums and outputs are fp32, and the outputs rounded to bf16 once
 // at the end. The tile form hands each weight p_t to the matrix instructions as the
-// sum of two bf16 (within 2^-18 of it).
+// sum of two bf16 (within 2^-15 of it).
 #include "../../include/nano_hip.h"
 #include "nvr_device.h"
 #include "nvr_internal.h"
@@ -168,6 +168,7 @@ constexpr int kPage = 16;  // positions that lie together in the cache: block si
 // 24.2 us against 23.1, 16 of 33 at 2000 39.5, 37.0), one of 8 with 2^-15 two less (22.9, 37.0). At the end the waves' and
 // the splits' outputs meet by their shares of 1.
 constexpr float kLag = 6.0f, kFull = 0x1p-5f, kShrink = 4.0f;
+constexpr float kAbove = 1.0f + 0x1p-18f;
 
 // Compile-time geometry. DIM: head dim rounded up; W: waves; QT: tiles of 16
 // query rows a wave; WQ of the waves hold query rows of their own, the other
@@ -532,11 +533,13 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
             auto* at = (__attribute__((address_space(3))) s16x4_t*)(vt + (row * CH + v_chunk<CH>(row, c)) * 16 + 8 * (n16 & 1));
             return __builtin_amdgcn_ds_read_tr16_b64_v4i16(at);
         };
-        // Four weights as two bf16 each, the nearest one and what it leaves: 2^-18 of a weight is lost, not 2^-9.
+        // Four weights, times kAbove, as two bf16 each: their upper halves and what those leave, rounded (up to 2^-15 of
+        // the weight). Both are positive where the weight is, so that an Inf in V stays one.
         auto halves = [&](const f32x4_t& w, uint2& hi, uint2& lo) {
-            hi = make_uint2(nvr::pack_bf16x2(w[0], w[1]), nvr::pack_bf16x2(w[2], w[3]));
-            lo = make_uint2(nvr::pack_bf16x2(w[0] - nvr::bf16_lo(hi.x), w[1] - nvr::bf16_hi(hi.x)),
-                            nvr::pack_bf16x2(w[2] - nvr::bf16_lo(hi.y), w[3] - nvr::bf16_hi(hi.y)));
+            auto upper = [](float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u); };
+            auto left = [](float f) { return __builtin_fmaf(f, kAbove, -__uint_as_float(__float_as_uint(f) & 0xffff0000u)); };
+            hi = make_uint2(upper(w[0], w[1]), upper(w[2], w[3]));
+            lo = make_uint2(nvr::pack_bf16x2(left(w[0]), left(w[1])), nvr::pack_bf16x2(left(w[2]), left(w[3])));
         };
         if constexpr (KT == 1) {
             s16x4_t p[QT], rest[QT];
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
     for (int t = 0; t < QT; ++t) {
         float all = l[t] + nvr::xor_lane(l[t], 16);
         all += nvr::xor_lane(all, 32);
-        const float inv = all > 0.0f ? 1.0f / all : 0.0f;
+        const float inv = all > 0.0f ? 1.0f / (all * kAbove) : 0.0f;
         sum[t] = all * __builtin_amdgcn_exp2f(bias[t]);
 #pragma unroll
         for (int d = 0; d < DT; ++d)

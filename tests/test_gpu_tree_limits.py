@@ -33,10 +33,10 @@ def values(bits):
 
 
 def check_tightly(t, got):
-    """As Trees.check, with weights held in more than 16 bits. Off against the formula: a weight by 2^-17 at most
-    where it is two bf16 (2^-18 each, and as much in the normaliser), by the exponential's few roundings (2^-18, twice
-    likewise) and by its score (dim roundings of the sum of its products' sizes; twice); a sum of N weights or
-    products by N roundings, twice; the output by its own, which is 2^-134 where it is subnormal: bf16's last bit is
+    """As Trees.check, with weights held in more than 16 bits. Off against the formula: a weight by 2^-15 where
+    it is two bf16 (the upper half leaves up to 2^-7 of it, which rounds by 2^-8 of that), by the exponential's few
+    roundings (2^-18, and as much in the normaliser) and by its score (dim roundings of the sum of its products' sizes;
+    twice); a sum of N weights or products by N roundings, twice; the output by its own, which is 2^-134 where it is subnormal: bf16's last bit is
     2^-133 there. Sums of subnormal products round by 2^-150, once in 32 positions, at weights of 2^-13 for the largest:
     2^-137 of the output."""
     with np.errstate(all="ignore"):
@@ -55,7 +55,7 @@ def check_tightly(t, got):
                 score = k @ q[a + i, h] / np.sqrt(t.dim)
                 p = np.exp(score - score.max())
                 score_off = t.dim * 2.0 ** -24 * (np.abs(k) @ np.abs(q[a + i, h])).max() / np.sqrt(t.dim)
-                part = 2 * 2.0 ** -17 + 2 * score_off + 2 * len(at) * 2.0 ** -24
+                part = 2.0 ** -15 + 2 * 2.0 ** -18 + 2 * score_off + 2 * len(at) * 2.0 ** -24
                 bound = p @ vc[at, h // group] / p.sum() * part + 2.0 ** -8 * np.abs(want[a + i, h]) + 2.0 ** -134 + -(-len(at) // 32) * 2.0 ** -137
                 assert (off[a + i, h] <= bound).all(), (s, i, h, float((off[a + i, h] / bound).max()))
 
@@ -221,3 +221,34 @@ def test_greedy_verification_of_rows_without_numbers(gpu, vocab):
     d.run(gpu)
     tokens, _, counts = d.result()
     assert (counts == 3).all() and tokens.tolist() == [[first or 0] * 3 for first in firsts]
+
+
+@each_shape
+@pytest.mark.parametrize("poison", [0x7FC0, 0x7F80, 0xFF80])
+def test_attention_never_sees_masked_values_in_any_shape(gpu, shape, poison):
+    """NaN and Inf in K and V of slots past the trees, of no sequence and of unmapped blocks change nothing; in K or V
+    of a node, a context's position of one sequence and a block's last slot, only rows that see them."""
+    t = trees(shape, 70, 333, 5700, spare=3)
+    clean = t.run(gpu)
+    used = np.zeros(t.blocks * t.bs, bool)
+    for s, (n, c) in enumerate(zip(t.sizes, t.contexts.tolist())):
+        pos = np.arange(c + n)
+        used[t.tables[s][pos // t.bs] * t.bs + pos % t.bs] = True
+    t.kc[~used] = poison
+    t.vc[~used] = poison
+    t.upload(gpu).launch(gpu)
+    assert np.array_equal(t.result(), clean)
+    first = t.sizes[0]
+    for position in {70 + first // 2, 70 + first - 1, 69, 15}:  # a node in the middle, the last, the context's last, one more
+        node = position - 70
+        sees = np.ones(first, bool) if node < 0 else (t.masks[:first] >> np.uint64(node) & np.uint64(1)) != 0
+        at = t.tables[0][position // 16] * 16 + position % 16
+        for cache in (t.vc, t.kc):
+            kept = cache[at].copy()
+            cache[at] = poison
+            t.upload(gpu).launch(gpu)
+            got = t.result()
+            assert np.array_equal(got[:first][~sees], clean[:first][~sees])
+            assert np.array_equal(got[first:], clean[first:])
+            t.check(got)
+            cache[at] = kept
