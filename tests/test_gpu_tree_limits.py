@@ -252,3 +252,50 @@ def test_attention_never_sees_masked_values_in_any_shape(gpu, shape, poison):
             assert np.array_equal(got[first:], clean[first:])
             t.check(got)
             cache[at] = kept
+
+
+@each_shape
+def test_attention_passes_over_unmapped_blocks_in_any_shape(gpu, shape):
+    """Holes in tiles of the context that every row would see whole, in the tile where the nodes begin and among the
+    nodes; a sequence with no block at all."""
+    t = trees(shape, 300, 700, 5800)
+    holes = [(0, 3, -1), (0, 7, t.blocks), (1, 0, 2 ** 31 - 1), (1, 21, -1), (1, 22, -2 ** 31), (0, 300 // 16, -1)]
+    for s, entry, value in holes:
+        t.tables[s, entry] = value
+    t.run(gpu)
+    at = np.where((t.tables[1] >= 0) & (t.tables[1] < t.blocks))[0]
+    unseen = np.ones(t.blocks, bool)
+    for s in range(t.batch):
+        unseen[t.tables[s][(t.tables[s] >= 0) & (t.tables[s] < t.blocks)]] = False
+    assert len(at) and unseen.any()
+    clean = t.result()
+    for cache in (t.kc, t.vc):  # block 0 is read in a hole's place
+        cache.reshape(t.blocks, -1)[unseen] = 0x7FC0
+    t.upload(gpu).launch(gpu)
+    assert np.array_equal(t.result(), clean)
+    t.tables[1, :] = -1
+    n = t.sizes[0]
+    assert not t.run(gpu)[n:n + t.sizes[1]].any()
+
+
+@each_shape
+@pytest.mark.parametrize("size", [1e4, 3e8, -3e8, 5e12, -5e12])
+def test_attention_of_vast_scores_in_any_shape(gpu, shape, size):
+    """Scores of up to 2^80, and as far below 0, in chains: the positions with the largest one share the weight. The
+    mean of their V to the sums' roundings (2^-13 of their magnitudes for up to 400) and the output's."""
+    t = trees(shape, 700, 35, 5900, fan=1)
+    q, k = np.zeros(t.q.shape, np.float32), nvr.bf16_values(t.kc).copy()
+    q[..., 0] = abs(size)
+    best = np.arange(len(k)) % 7 == 3
+    k[..., 0] = np.where(best, 1.0, 0.5 if size > 0 else 2.0)[:, None] * size
+    t.q, t.kc = nvr.bf16_bits(q), nvr.bf16_bits(k)
+    t.upload(gpu).launch(gpu)
+    got, v = values(t.result()), values(t.vc)
+    for s, (n, c) in enumerate(zip(t.sizes, t.contexts.tolist())):
+        for i in range(n):
+            pos = np.arange(c + i + 1)
+            at = t.tables[s, pos // 16] * 16 + pos % 16
+            at = at[best[at]] if best[at].any() else at
+            want = np.repeat(v[at].mean(0), t.qh // t.kvh, 0)
+            bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -13 * np.repeat(np.abs(v[at]).mean(0), t.qh // t.kvh, 0)
+            assert (np.abs(got[t.row_starts[s] + i] - want) <= bound).all(), (s, i)
