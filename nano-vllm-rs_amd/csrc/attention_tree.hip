@@ -63,7 +63,8 @@ __device__ __forceinline__ TreeSpan tree_span(const TreeArgs& a, int s) {
 // Any head dim, block size and alignment: a block per (node, q head), its four
 // waves over every fourth position, lanes over the head's elements. Bound by the
 // chain of one position's load, dot product and 64-lane sum after the other: with
-// heads of 128, 8 trees of 25 nodes at 1030 positions take 650 us (the tile form 21).
+// heads of 128, 8 trees of 25 nodes at 1030 positions in blocks of 8 take 785 us (the
+// tile form in blocks of 256 22), as many as with fp32 sums.
 __global__ __launch_bounds__(256) void attention_tree_direct(TreeArgs a) {
     constexpr int kWaves = 4, kElems = 4;  // 64 lanes x 4 elements: head dims up to 256
     __shared__ float part_m[kWaves];
@@ -219,9 +220,11 @@ struct Partials {
     int splits;
 };
 
-// The fewest positions of a split. One chain of 4 at 180 whole 9.1 us, in two 10.7;
-// parts of 128 against 256: 4 trees of 13 at 500 14.9, 16.1, one chain of 8 at 1000 11.9,
-// 12.9, 8 of 9 at 700 with heads of 64 13.2, 15.3; but one tree of 25 at 4000 19.7, 18.6.
+// The fewest positions of a split. One chain of 4 at 180 whole 9.4 us, in two 11.1;
+// parts of 128 against 256: 4 trees of 13 at 500 15.7, 17.0, one chain of 8 at 1000 12.1,
+// 13.1, 8 of 9 at 700 with heads of 64 14.2, 17.3, one tree of 25 at 4000 21.3, 21.7. (One
+// number of splits for all sequences of a call: where one is far longer than the others,
+// the call lasts as long as that one's parts.)
 constexpr int kWhole = 256, kShort = 1024;  // positions that are not split, that are split finely
 
 // Tiles (of 2^shift positions) a split: the same for every split but the last.
@@ -245,11 +248,11 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int shift) {
 // meet in attention_tree_join.
 //
 // What bounds it, on MI355X (times with the join's): with few rows the read of the
-// cache, 64 chains of 6 nodes at 4090 positions 154 us, 5.4 TB/s; with many the copies
-// into LDS, 4 trees of 64 at 16000 65 us, 4.0 TB/s and 0.45 PFLOP/s (as long without
-// the products); with eight q heads a KV head each tile's chain of LDS reads, products
-// and exponentials, 16 trees of 33 at 2000 30 us; small calls the launch (3 us),
-// the tables and the first tiles, one chain of 4 at 180 9 us.
+// cache, 64 chains of 6 nodes at 4090 positions 155 us, 5.4 TB/s; with many each tile's
+// chain of copies, LDS reads, products and exponentials, which the waves of a block go
+// through in step: 4 trees of 64 at 16000 78 us, 3.6 TB/s, the matrix instructions busy
+// for 27% of it, and with eight q heads a KV head 16 trees of 33 at 2000 35 us; small
+// calls the launch (3 us), the tables and the first tiles, one chain of 4 at 180 9 us.
 template <typename S>
 __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_tree_tiles(TreeArgs a, Partials part, int chunks,
                                                                         int page_shift, int spread) {
@@ -687,8 +690,8 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
 
 // The splits of each row, where there was more than one: a thread four elements
 // of one (node, head), its splits' loads in flight together. Bound by its launch and
-// one memory round trip: 4.2 us for 200 rows of 16 heads in 5 splits, 5.6 for 256 rows
-// in 8 (17 MB of partial outputs).
+// one memory round trip: 4.3 us for 168 rows of 16 heads in up to 8 splits (10 MB of
+// partial outputs), 5.1 for 226 rows in 8 (15 MB).
 __global__ __launch_bounds__(256) void attention_tree_join(TreeArgs a, Partials part, int shift, int parts) {
     constexpr int kBatch = 8;
     const int item = int(blockIdx.x / unsigned(parts));
@@ -762,17 +765,17 @@ struct Plan {
 // `pairs`. Microseconds on MI355X, 16 q heads over 8 KV heads of 128, blocks of 256:
 //  - up to 32 rows four waves split each tile's positions and read only what they
 //    copied themselves, so they need no barrier. Two stages and two blocks a CU beat
-//    four stages and one: 64 sequences of 6 nodes at 200 positions 15.8 against 22.2,
-//    at 1000 44.3, 49.2, at 4090 155, 162.
+//    four stages and one: 64 sequences of 6 nodes at 200 positions 16.4 against 24.4,
+//    at 1000 44.1, 52.6, at 4090 155, 165.
 //  - up to 64 rows, four waves over stages of 32 positions, two blocks a CU, against
-//    eight waves over stages of 64: 64 of 30 at 300 26.3, 36.6, 8 of 25 at 1030 22.3, 23.3.
+//    eight waves over stages of 64: 64 of 30 at 300 29.2, 40.1, 8 of 25 at 1030 23.6, 24.5.
 //  - above, the same four waves where there are more pairs than CUs (64 of 60 at 300
-//    30.6 against 43.0, at 1000 62.9, 73.8); else eight waves, which need half the splits
-//    to fill a CU (8 of 64 at 8000 74.3 against 69.9, 4 of 64 at 16000 75.8, 69.5).
+//    35.1 against 46.7, at 1000 77, 84); else eight waves, which need half the splits
+//    to fill a CU (8 of 64 at 8000 86.5 against 82.9, 4 of 64 at 16000 86.1, 84.6).
 //  - heads of 64, 16 of 33 nodes at 2000 with 8 heads a KV head: three blocks of four
-//    waves a CU 32.8, two of eight 34.3, one of eight with twice the rows 44.6 (each
-//    before its chunks shared an XCD). Heads of 256 with two stages: 16 of 40 at 1000
-//    33.8, with four 37.9.
+//    waves a CU 37.5, one of eight over stages of 64 46.9, the same with twice the rows,
+//    which spills, 155. Heads of 256 with two stages: 16 of 40 at 1000 33.0, with four 40.3.
+//    (256 in these rules is the CUs of an MI355X; on another number they cost time only.)
 template <typename F>
 void with_shape(int dim, int64_t queries, int64_t pairs, F&& f) {
     if (dim == 256) {
@@ -865,7 +868,7 @@ int nv_attention_tree(nv_context* c, const void* q, const void* kc, const void* 
         float* partial = static_cast<float*>(workspace);
         const Partials part{partial, reinterpret_cast<float2*>(partial + int64_t(p.splits) * rows * qh * dim), p.splits};
         const int pages = bs / kPage, shift = (pages & (pages - 1)) == 0 ? __builtin_ctz(unsigned(pages)) : -1;
-        // Chunks on one XCD: 32 trees of 24 at 2000 with 8 heads a KV head of 64 37.4 us against 40.6, 16 of 33 31.9, 32.9.
+        // Chunks on one XCD: 32 trees of 24 at 2000 with 8 heads a KV head of 64 46.5 us against 47.3, 16 of 33 37.5, 38.5.
         const int spread = p.chunks > 1 && p.pairs * p.splits % 8 == 0 ? 3 : 0;
         with_shape(p.dim, p.queries, p.pairs, [&](auto shape) {
             using S = decltype(shape);

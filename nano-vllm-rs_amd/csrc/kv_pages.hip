@@ -18,8 +18,9 @@ constexpr int kMaxNodes = 64;
 // contiguous, so a copy is cut into segments of kSegment chunks whatever the
 // slot size, one a block, all loads of a thread in flight before its stores.
 // Bound by HBM: 12 copies of partly filled blocks of 256 positions from 4 sources in
-// 28 layers (559 MB moved) take 63 to 67 us, 8.6 TB/s. Writes bypass the caches, which would
-// hold them in the way of sources read again (98 us); reads do not (80), nor do more
+// 28 layers (280 MB written, 385 MB with each source read once) take 63 us, the call 67:
+// 5.7 to 6.2 TB/s; a source's second and third read hit the caches. Writes bypass them, or
+// they would be in the way of sources read again (98 us); reads do not (80), nor do more
 // loads a thread hide more (eight 78, two 66).
 constexpr int kCopyLoads = 4;
 constexpr int kSegment = 256 * kCopyLoads;

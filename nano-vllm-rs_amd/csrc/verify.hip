@@ -245,14 +245,14 @@ __device__ __forceinline__ void careful_sum(const uint16_t* x, int lead, int beg
     *sum = total;
 }
 
-// A block a (sequence, share, model). T > 0: one pass with an offset near the
-// maximum of each thread's first loads; a sum that comes near the ends of fp32's
-// range, or a NaN, is taken again with care. Bound by the read of the logits and, at four
-// instructions and an exponential a token, nearly as much by its issue; five
-// resident blocks a CU with the next two loads in flight beat eight of four loads
-// that wait for each other, in two rounds (whole calls, vocabulary 151936: 24 trees
-// of 25 31.2 against 36.9 us, 128 chains of 4 58.2, 70.2; six blocks 31.3, 59.6, four
-// 30.8, 59.1, eight 32.1, 61.1).
+// A block a (sequence, share, model). T > 0: one pass with an offset that follows
+// each thread's maximum; a sum that comes near the ends of fp32's range, or a NaN, is
+// taken again with care. Bound by the read of the logits (48 chains of 6 with draft
+// logits, 117 MB, in 22 us, 5.2 TB/s) and, at five instructions and an exponential a
+// token, nearly as much by its issue (24 trees of 25, 55 MB, in 15 us, 3.6 TB/s). Five
+// resident blocks a CU, with the next two loads in flight: whole calls, vocabulary
+// 151936, 24 trees of 25 31.8 us, 128 chains of 4 61.0; six blocks 31.9, 62.6, four 31.6,
+// 61.7, eight 32.7, 64.3.
 __global__ __launch_bounds__(kThreads, kResident) void verify_stats(VerifyArgs a) {
     constexpr int kWaves = kThreads / kWave;
     __shared__ float tops[kWaves];
@@ -668,10 +668,11 @@ struct SimpleWalk {
 // (kFirst) sums, slice by slice, the first rests that the walk may come to need, and
 // the second launch the second rests; there the last block of a sequence to finish
 // walks. Later rests are summed during the walk. Bound by the chain of memory round
-// trips (nodes, their logits, the stats' parts, the rests' parts, the hand-over): 6.5
-// us without draft logits, 4.5 + 6.9 with them where every node has one child, 8.8 +
-// 10 for 8 trees of 13 with up to three over 50257 tokens. (8 trees of 40 with up to
-// four over 151936: 89 us the whole call, 117 with loads that bypass the caches.)
+// trips (nodes, their logits, the stats' parts, the rests' parts, the hand-over): 6.4
+// us without draft logits, 4.4 + 7.0 with them where every node has one child (the first
+// launch finds nothing to sum there), 9 + 12 for 8 trees of 13 with up to three over
+// 50257 tokens. Fourth children cost a pass by one block each, which 16 slices whatever the
+// batch leave far from a bound: 8 trees of 40 with up to four over 151936 tokens take 93 us.
 template <bool kFirst>
 __global__ __launch_bounds__(kWalkThreads) void verify_walk(VerifyArgs a) {
     __shared__ Stats target[kMaxNodes], draft[kMaxNodes];
@@ -830,9 +831,9 @@ __device__ __forceinline__ uint64_t key_of(const Best& b) {
 // hash and two logarithms; the noise is at most -ln(1 - u), so one hardware
 // logarithm bounds it, and only a lane's best bound and the bounds that reach
 // the wave's best score are scored in full. Bound by the hash: about 60 instructions
-// a token, six of them multiplications at a quarter of the rate; 48 rows of 151936
-// tokens take 21 us, 24 rows 11. Blocks of two or four times the tokens gained 1 us
-// in 49 there and lost as much at 24 rows.
+// a token, six of them multiplications at a quarter of the rate, also for tokens whose
+// rest is nothing; 48 rows of 151936 tokens take 22 us, 24 rows 11. Blocks of two or four
+// times the tokens gained 1 us in 49 there and lost as much at 24 rows (with fp32 rests).
 // kWalks: every block walks its tree by itself, which saves launch 2.
 template <bool kWalks>
 __global__ __launch_bounds__(kThreads) void verify_sample(VerifyArgs a) {
@@ -1030,8 +1031,8 @@ int nv_verify_tree(nv_context* c, const void* logits, const void* draft_logits, 
                        reinterpret_cast<int*>(base + w.arrived), rows, batch, max_nodes, vocab, most_parts(vocab), blocks};
     hipLaunchKernelGGL(verify_stats, dim3(unsigned(int64_t(batch) * blocks * sides)), dim3(kThreads), 0, c->stream, a);
     NVR_HIP(hipGetLastError());
-    // Up to a block a CU, launch 3 walks by itself (one chain of 5 14.2 us against 16.5, 4 trees of 60 with more
-    // blocks 25.8 against 24.7, 24 of 25 35.0, 30.8).
+    // Up to a block a CU, launch 3 walks by itself (one chain of 5 14.5 us against 16.8, 4 trees of 60 with more
+    // blocks 25.2 against 25.5, 24 of 25 36.2, 31.8).
     const dim3 sample{unsigned(batch), unsigned(sampled)};
     if (!draft_logits && int64_t(batch) * sampled <= cus) {
         hipLaunchKernelGGL(verify_sample<true>, sample, dim3(kThreads), 0, c->stream, a);
