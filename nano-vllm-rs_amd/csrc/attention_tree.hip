@@ -163,8 +163,8 @@ constexpr int kPage = 16;  // positions that lie together in the cache: block si
 // A weight is 2^(d - bias) of its score's distance d, in powers of two, from a scale m, which is exact to its own 2^-24
 // however large both are. m follows the maximum, and the bias the weights' sum, so that a wave's sum stays below 1: fp32
 // sums of the largest V are finite, over any number of positions. The maximum may outgrow m by 2^kLag before o and l are
-// scaled again; where a lane's sum has passed kFull, they shrink by 2^kShrink. The largest weight is 2^-kBias at
-// least (11 to 13), so that the sum of 32 positions' products, which fp32 rounds by 2^-150 at most, is off by 2^-137 of the
+// scaled again; where a lane's sum has passed kFull, they shrink by 2^kShrink, which the bias gives back as the maximum
+// grows. So the sum is 2^-kBias at least (11 to 13), and that of 32 positions' products, which fp32 rounds by 2^-150 at most, is off by 2^-137 of the
 // smallest V's outputs, whose last bit is 2^-133. A lag of 2 with 2^-10 would keep three bits more (8 trees of 25 at 1030
 // 24.2 us against 23.1, 16 of 33 at 2000 39.5, 37.0), one of 8 with 2^-15 two less (22.9, 37.0). At the end the waves' and
 // the splits' outputs meet by their shares of 1.
@@ -510,8 +510,10 @@ __global__ __launch_bounds__(kWave* S::W, S::kBlocks* S::W / 4) void attention_t
                     shrink = fmaxf(shrink, nvr::xor_lane(shrink, 16));
                     shrink = fmaxf(shrink, nvr::xor_lane(shrink, 32));
                 }
-                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(m[t] - top, a.scale, -shrink));
-                bias[t] += shrink;
+                // Where the maximum grew, the bias comes back by as much, to a multiple of 2^-8: it stays exact.
+                const float grown = (top - m[t]) * a.scale, back = fminf(bias[t] - S::kBias, __builtin_floorf(grown * 256.0f) * (1.0f / 256.0f));
+                const float old = m[t] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(back - shrink - grown);
+                bias[t] += shrink - back;
                 l[t] *= old;
 #pragma unroll
                 for (int d = 0; d < DT; ++d)

@@ -299,3 +299,23 @@ def test_attention_of_vast_scores_in_any_shape(gpu, shape, size):
             want = np.repeat(v[at].mean(0), t.qh // t.kvh, 0)
             bound = 2.0 ** -8 * np.abs(want) + 2.0 ** -13 * np.repeat(np.abs(v[at]).mean(0), t.qh // t.kvh, 0)
             assert (np.abs(got[t.row_starts[s] + i] - want) <= bound).all(), (s, i)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_a_late_key_after_many_positions(gpu, dim):
+    """137000 positions that share the weight, V 0, in long parts (64 sequences over the same blocks), then a key whose
+    score is 2^60 of theirs, with the smallest V: the outputs are that V, to the roundings of its products (2^-137) and
+    the output's."""
+    t = Trees([2], [137000], 8, 4, dim, 256, 6300)
+    last = t.tables[0][137000 // 256] * 256 + 137000 % 256
+    q, k = np.zeros(t.q.shape), np.zeros(t.kc.shape)
+    q[..., 0], k[last, :, 0] = 1.0, 60 / np.log2(np.e) * np.sqrt(dim)
+    t.q, t.kc = nvr.bf16_bits(q), nvr.bf16_bits(k)
+    t.vc[:] = 0
+    t.vc[last] = nvr.bf16_bits(np.resize(np.array([1.2e-38, -2e-38, 5e-38]), dim))
+    t.batch, t.rows, t.row_starts = 64, 128, 2 * np.arange(65, dtype=np.int32)
+    t.tables, t.contexts, t.masks = np.tile(t.tables, (64, 1)), np.tile(t.contexts, 64), np.tile(t.masks, 64)
+    t.q, t.out = np.tile(t.q, (64, 1, 1)), np.tile(t.out, (64, 1, 1))
+    t.upload(gpu).launch(gpu)
+    got, want = values(t.result()), values(t.vc[last])[0]
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -136).all()
