@@ -164,10 +164,10 @@ constexpr int kPage = 16;  // positions that lie together in the cache: block si
 // however large both are. m follows the maximum, and the bias the weights' sum, so that a wave's sum stays below 1: fp32
 // sums of the largest V are finite, over any number of positions. The maximum may outgrow m by 2^kLag before o and l are
 // scaled again; where a lane's sum has passed kFull, they shrink by 2^kShrink, which the bias gives back as the maximum
-// grows. So the sum is 2^-kBias at least (11 to 13), and that of 32 positions' products, which fp32 rounds by 2^-150 at most, is off by 2^-137 of the
-// smallest V's outputs, whose last bit is 2^-133. A lag of 2 with 2^-10 would keep three bits more (8 trees of 25 at 1030
-// 24.2 us against 23.1, 16 of 33 at 2000 39.5, 37.0), one of 8 with 2^-15 two less (22.9, 37.0). At the end the waves' and
-// the splits' outputs meet by their shares of 1.
+// grows. So the sum is 2^-kBias at least (11 to 13), and what fp32 rounds of a sum over 32 positions, 2^-150 at most, is
+// 2^-137 of the smallest V's outputs, whose last bit is 2^-133. A lag of 2 with 2^-10 would keep three bits more (8 trees
+// of 25 at 1030 24.2 us against 23.1, 16 of 33 at 2000 39.5, 37.0), one of 8 with 2^-15 two less (22.9, 37.0). At the end
+// the waves' and the splits' outputs meet by their shares of 1.
 constexpr float kLag = 6.0f, kFull = 0x1p-5f, kShrink = 4.0f;
 constexpr float kAbove = 1.0f + 0x1p-18f;
 
@@ -250,7 +250,7 @@ __device__ __forceinline__ int split_tiles(int tiles, int splits, int shift) {
 // What bounds it, on MI355X (times with the join's): with few rows the read of the
 // cache, 64 chains of 6 nodes at 4090 positions 155 us, 5.4 TB/s; with many each tile's
 // chain of copies, LDS reads, products and exponentials, which the waves of a block go
-// through in step: 4 trees of 64 at 16000 78 us, 3.6 TB/s, the matrix instructions busy
+// through in step: 4 trees of 64 at 16000 76 us, 3.6 TB/s, the matrix instructions busy
 // for 27% of it, and with eight q heads a KV head 16 trees of 33 at 2000 35 us; small
 // calls the launch (3 us), the tables and the first tiles, one chain of 4 at 180 9 us.
 template <typename S>
