@@ -145,9 +145,9 @@ def prepare(case, seed):
         torch.cuda.synchronize()
         return state
     # The library takes its own buffers; a program keeps its workspace, and its weights in 8 bits.
+    g, b = gpu(), {}
     import nvr
 
-    g, b = gpu(), {}
     m, n, k = case["m"], case["n"], case["k"]
     for name, t in list(v.items()):
         b[name], mine = _buffer(*t.shape)
