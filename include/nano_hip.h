@@ -308,6 +308,49 @@ int nv_kv_compact(nv_context* c, void* kc, void* vc, const void* contexts, const
 int nv_kv_copy_blocks(nv_context* c, void* kc, void* vc, const void* src, const void* dst, const void* tokens,
                       int copies, int layers, int kvh, int dim, int bs, int blocks);
 
+/* Serving with weights in 8-bit integers (no counterpart in the reference, whose
+ * projections are bf16). A weight [n, k] is kept as rows of k int8 at multiples of
+ * 16 bytes (k rounded up to a multiple of 16 is a row's pitch, and w starts at a
+ * multiple of 16 bytes) and a scale (f32) a row, its channel. k is at most 131071,
+ * so that sums of products are exact in 32 bits; a longer one is refused (-2).
+ *
+ * Rows of bf16 as 8-bit integers: x [rows, k] bf16; q [rows, pitch] i8, zeros
+ * behind k; scales [rows] f32. With a = max |x_j| of a row, its scale is a / 127 and
+ * q_j = 127 x_j / a to the nearest whole number, half to even; 0 where a is 0. A
+ * row that holds a NaN or an infinity has a scale of NaN and integers 0. */
+int nv_quantize_rows(nv_context* c, const void* x, void* q, void* scales, int rows, int k);
+
+/* Bytes of workspace that nv_gemm_i8 needs; a host function, no device work. A
+ * workspace starts at a multiple of 16 bytes (else -2), its contents do not matter
+ * before a call and are unspecified after; calls that may overlap need one each. */
+int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
+
+/* y[m, n] = bf16(sum_l xq[i, l] w[j, l] * xs[i] * w_scales[j]), where xq and xs are
+ * the tokens as nv_quantize_rows makes them of
+ *   x                            norm_weight NULL (residual and residual_out too),
+ *   RMSNorm(x)                   residual NULL (residual_out too),
+ *   RMSNorm(x + residual)        with residual_out <- bf16(x + residual), unless NULL;
+ * the norm in fp32 (as nv_rms up to the order of its sum) and not rounded to bf16
+ * before. x, residual, residual_out: [m, k] bf16, residual_out another buffer than
+ * the others; norm_weight: [k] bf16; w, w_scales as nv_quantize_rows' q and scales
+ * (integers of any source; -128 too); y: [m, n] bf16. Sums of products are exact,
+ * so a token's outputs are the same bits in any batch. A token with a NaN or an
+ * infinity (after the norm) has NaN in its row of y, and in no other. eps is read
+ * with a norm_weight only. */
+int nv_gemm_i8(nv_context* c, const void* x, const void* residual, void* residual_out, const void* norm_weight,
+               const void* w, const void* w_scales, void* y, void* workspace, int m, int n, int k, float eps);
+
+int nv_gemm_i8_silu_workspace(int m, int intermediate, int k, size_t* bytes);
+
+/* The gated feed-forward block's first half, both projections and SiLU·up in one
+ * product: w is [2 * intermediate, k], the gate's rows, then the up projection's
+ * (as a bf16 gate_up weight has them), and act[m, intermediate] =
+ * bf16(g / (1 + e^-g) * u) with g and u the products of nv_gemm_i8 before its
+ * rounding. Everything else as nv_gemm_i8. */
+int nv_gemm_i8_silu(nv_context* c, const void* x, const void* residual, void* residual_out, const void* norm_weight,
+                    const void* w, const void* w_scales, void* act, void* workspace, int m, int intermediate, int k,
+                    float eps);
+
 /* Per-row Gumbel seed of src/runtime.rs:780-790 (host function, no device
  * work): mix(mix(base) ^ mix(request_id) ^ mix(generated)). */
 uint64_t nv_sampling_seed(uint64_t base, uint64_t request_id, uint64_t generated);

@@ -598,6 +598,72 @@ TensorArg workspace_arg(const Buffer& workspace, std::size_t bytes) {
 
 }  // namespace
 
+namespace {
+
+void require_i8(const char* op, std::size_t k) {
+    if (k < 1 || k > kI8MaxK)
+        throw Error(Fault::Value, std::string(op) + ": k " + std::to_string(k) + " outside [1, " +
+                                      std::to_string(kI8MaxK) + "]");
+}
+
+}  // namespace
+
+void Gpu::quantize_rows(const Buffer& x, const Buffer& q, const Buffer& scales, std::size_t rows, std::size_t k) const {
+    require_i8("quantize_rows", k);
+    admit("quantize_rows", {read_arg("x", x, 2, {rows, k}), write_arg("q", q, 16, {rows, i8_pitch(k) / 16}),
+                            write_arg("scales", scales, 4, {rows})});
+    require_status(nv_quantize_rows(context(), x.address(), q.address(), scales.address(), as_dim(rows), as_dim(k)));
+}
+
+std::size_t Gpu::gemm_i8_workspace(std::size_t m, std::size_t n, std::size_t k) const {
+    require_i8("gemm_i8_workspace", k);
+    std::size_t bytes = 0;
+    require_status(nv_gemm_i8_workspace(as_dim(m), as_dim(n), as_dim(k), &bytes));
+    return bytes;
+}
+
+std::size_t Gpu::gemm_i8_silu_workspace(std::size_t m, std::size_t intermediate, std::size_t k) const {
+    require_i8("gemm_i8_silu_workspace", k);
+    std::size_t bytes = 0;
+    require_status(nv_gemm_i8_silu_workspace(as_dim(m), as_dim(intermediate), as_dim(k), &bytes));
+    return bytes;
+}
+
+void Gpu::product_i8(bool gated, const Buffer& x, const Buffer& residual, const Buffer& residual_out,
+                     const Buffer& norm_weight, const Buffer& w, const Buffer& w_scales, const Buffer& y,
+                     const Buffer& workspace, std::size_t m, std::size_t n, std::size_t k, float eps) const {
+    const char* op = gated ? "gemm_i8_silu" : "gemm_i8";
+    if (!norm_weight.empty()) require_positive(eps, "gemm_i8 eps");
+    else if (!residual.empty()) throw Error(Fault::Value, std::string(op) + ": a residual needs a norm_weight");
+    if (residual.empty() && !residual_out.empty())
+        throw Error(Fault::Value, std::string(op) + ": residual_out needs a residual to add");
+    const std::size_t need = gated ? gemm_i8_silu_workspace(m, n, k) : gemm_i8_workspace(m, n, k);
+    const std::size_t channels = gated ? 2 * n : n;
+    std::vector<TensorArg> args = {read_arg("x", x, 2, {m, k}), read_arg("w", w, 16, {channels, i8_pitch(k) / 16}),
+                                   read_arg("w_scales", w_scales, 4, {channels}), write_arg("y", y, 2, {m, n})};
+    if (need != 0) args.push_back(workspace_arg(workspace, need));
+    if (!residual.empty()) args.push_back(read_arg("residual", residual, 2, {m, k}));
+    if (!residual_out.empty()) args.push_back(write_arg("residual_out", residual_out, 2, {m, k}));
+    if (!norm_weight.empty()) args.push_back(read_arg("norm_weight", norm_weight, 2, {k}));
+    admit(op, args);
+    auto ptr = [](const Buffer& b) { return b.empty() ? nullptr : b.address(); };
+    const auto call = gated ? nv_gemm_i8_silu : nv_gemm_i8;
+    require_status(call(context(), x.address(), ptr(residual), ptr(residual_out), ptr(norm_weight), w.address(),
+                        w_scales.address(), y.address(), ptr(workspace), as_dim(m), as_dim(n), as_dim(k), eps));
+}
+
+void Gpu::gemm_i8(const Buffer& x, const Buffer& residual, const Buffer& residual_out, const Buffer& norm_weight,
+                  const Buffer& w, const Buffer& w_scales, const Buffer& y, const Buffer& workspace, std::size_t m,
+                  std::size_t n, std::size_t k, float eps) const {
+    product_i8(false, x, residual, residual_out, norm_weight, w, w_scales, y, workspace, m, n, k, eps);
+}
+
+void Gpu::gemm_i8_silu(const Buffer& x, const Buffer& residual, const Buffer& residual_out, const Buffer& norm_weight,
+                       const Buffer& w, const Buffer& w_scales, const Buffer& act, const Buffer& workspace,
+                       std::size_t m, std::size_t intermediate, std::size_t k, float eps) const {
+    product_i8(true, x, residual, residual_out, norm_weight, w, w_scales, act, workspace, m, intermediate, k, eps);
+}
+
 std::size_t Gpu::attention_tree_workspace(std::size_t rows, std::size_t qheads, std::size_t kvheads,
                                           std::size_t head_dim, std::size_t batch_size, std::size_t max_nodes,
                                           std::size_t max_context) const {

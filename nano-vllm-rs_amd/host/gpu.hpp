@@ -75,6 +75,11 @@ void require_head_layout(std::size_t qheads, std::size_t kvheads, std::size_t he
 std::vector<uint16_t> tile_gate_up_rows(const std::vector<uint16_t>& gate_up, std::size_t intermediate,
                                         std::size_t k);
 
+// The longest rows of products in 8-bit integers, and the bytes from one row of
+// k such integers to the next.
+constexpr std::size_t kI8MaxK = 131071;
+constexpr std::size_t i8_pitch(std::size_t k) { return (k + 15) / 16 * 16; }
+
 // Trees of drafted tokens have at most this many nodes.
 constexpr std::size_t kMaxTreeNodes = 64;
 // The attention masks of one tree's nodes: each node's own bit and its
@@ -256,6 +261,24 @@ public:
                   std::size_t rows, std::size_t kvheads, std::size_t head_dim, std::size_t block_size,
                   std::size_t num_blocks) const;
 
+    // ---- weights in 8-bit integers (no Rust caller in the reference) ----
+    // Rows of bf16 as 8-bit integers, i8_pitch(k) bytes a row, with an f32 scale
+    // a row: its largest magnitude over 127. Makes the weights of gemm_i8.
+    void quantize_rows(const Buffer& x, const Buffer& q, const Buffer& scales, std::size_t rows, std::size_t k) const;
+    std::size_t gemm_i8_workspace(std::size_t m, std::size_t n, std::size_t k) const;
+    // y = bf16(tokens W^T) with the tokens x, RMSNorm(x) (norm_weight not empty)
+    // or RMSNorm(x + residual) (neither empty; residual_out, when not empty,
+    // <- bf16(x + residual), another buffer) in 8-bit integers with a scale each.
+    void gemm_i8(const Buffer& x, const Buffer& residual, const Buffer& residual_out, const Buffer& norm_weight,
+                 const Buffer& w, const Buffer& w_scales, const Buffer& y, const Buffer& workspace, std::size_t m,
+                 std::size_t n, std::size_t k, float eps) const;
+    std::size_t gemm_i8_silu_workspace(std::size_t m, std::size_t intermediate, std::size_t k) const;
+    // gemm_i8 with the [2 * intermediate, k] gate_up weight (gate rows, then up
+    // rows): act [m, intermediate] = bf16(silu(gate) * up).
+    void gemm_i8_silu(const Buffer& x, const Buffer& residual, const Buffer& residual_out, const Buffer& norm_weight,
+                      const Buffer& w, const Buffer& w_scales, const Buffer& act, const Buffer& workspace,
+                      std::size_t m, std::size_t intermediate, std::size_t k, float eps) const;
+
     // ---- trees of drafted tokens (no Rust caller in the reference) ----
     // Bytes of workspace that attention_tree needs for these arguments (0: none).
     std::size_t attention_tree_workspace(std::size_t rows, std::size_t qheads, std::size_t kvheads,
@@ -294,6 +317,9 @@ public:
                         std::size_t head_dim, std::size_t block_size, std::size_t num_blocks) const;
 
 private:
+    void product_i8(bool gated, const Buffer& x, const Buffer& residual, const Buffer& residual_out,
+                    const Buffer& norm_weight, const Buffer& w, const Buffer& w_scales, const Buffer& y,
+                    const Buffer& workspace, std::size_t m, std::size_t n, std::size_t k, float eps) const;
     nv_context* context() const;
     std::shared_ptr<detail::Device> device_;
 };

@@ -87,6 +87,11 @@ SIGNATURES = {
     "nv_verify_tree": (_i, [_vp] * 13 + [_i] * 4),
     "nv_kv_compact": (_i, [_vp] * 7 + [_i] * 8),
     "nv_kv_copy_blocks": (_i, [_vp] * 6 + [_i] * 6),
+    "nv_quantize_rows": (_i, [_vp] * 4 + [_i, _i]),
+    "nv_gemm_i8_workspace": (_i, [_i] * 3 + [ctypes.POINTER(_sz)]),
+    "nv_gemm_i8": (_i, [_vp] * 9 + [_i] * 3 + [_f]),
+    "nv_gemm_i8_silu_workspace": (_i, [_i] * 3 + [ctypes.POINTER(_sz)]),
+    "nv_gemm_i8_silu": (_i, [_vp] * 9 + [_i] * 3 + [_f]),
     "nv_sampling_seed": (ctypes.c_uint64, [ctypes.c_uint64] * 3),
 }
 
@@ -149,6 +154,14 @@ def tile_gate_up_rows(gate_up: np.ndarray, intermediate: int) -> np.ndarray:
     rows 8t..8t+7."""
     w = np.asarray(gate_up).reshape(2, intermediate // 8, 8, -1)
     return np.ascontiguousarray(w.transpose(1, 0, 2, 3).reshape(2 * intermediate, -1))
+
+
+I8_MAX_K = 131071
+
+
+def i8_pitch(k: int) -> int:
+    """Bytes from a row of k 8-bit integers to the next."""
+    return -(-as_dim(k) // 16) * 16
 
 
 MAX_TREE_NODES = 64
@@ -497,6 +510,75 @@ class Gpu:
         ptr = lambda b: None if b is None else b.ptr  # noqa: E731
         self._call(self.lib.nv_rms_gemm_silu(self.handle, x.ptr, ptr(residual), ptr(residual_out), norm_weight.ptr,
                                              w_tiled.ptr, ptr(gate_up), act.ptr, ptr(normed), m, intermediate, k, eps))
+
+    @staticmethod
+    def _i8_limit(op: str, k: int) -> None:
+        if not 1 <= k <= I8_MAX_K:
+            raise ArgumentError("value", f"{op}: k {k} outside [1, {I8_MAX_K}]")
+
+    def quantize_rows(self, x: Buffer, q: Buffer, scales: Buffer, rows: int, k: int) -> None:
+        """Rows of bf16 as 8-bit integers, i8_pitch(k) bytes a row, with an f32 scale a row: its largest magnitude
+        over 127. Makes the weights of gemm_i8 and gemm_i8_silu."""
+        self._i8_limit("quantize_rows", k)
+        self._admit("quantize_rows", [_r("x", x, 2, rows, k), _w("q", q, 16, rows, i8_pitch(k) // 16),
+                                      _w("scales", scales, 4, rows)])
+        self._call(self.lib.nv_quantize_rows(self.handle, x.ptr, q.ptr, scales.ptr, rows, k))
+
+    def gemm_i8_workspace(self, m: int, n: int, k: int) -> int:
+        """Bytes of workspace that gemm_i8 needs for these arguments."""
+        return self._i8_workspace("gemm_i8_workspace", m, n, k)
+
+    def gemm_i8_silu_workspace(self, m: int, intermediate: int, k: int) -> int:
+        """Bytes of workspace that gemm_i8_silu needs for these arguments."""
+        return self._i8_workspace("gemm_i8_silu_workspace", m, intermediate, k)
+
+    def _i8_workspace(self, op: str, m: int, n: int, k: int) -> int:
+        self._i8_limit(op, k)
+        as_dim(m), as_dim(n)
+        need, lib = _sz(), self.lib or library()
+        check_status(getattr(lib, "nv_" + op)(m, n, k, ctypes.byref(need)), lib)
+        return need.value
+
+    def gemm_i8(self, x: Buffer, residual: Buffer | None, residual_out: Buffer | None, norm_weight: Buffer | None,
+                w: Buffer, w_scales: Buffer, y: Buffer, workspace: Buffer, m: int, n: int, k: int,
+                eps: float) -> None:
+        """y = bf16(tokens W^T), with the tokens x, RMSNorm(x) (a norm_weight) or RMSNorm(x + residual) (both;
+        residual_out <- bf16(x + residual), another buffer, when given) in 8-bit integers with a scale each, and w,
+        w_scales as quantize_rows makes them. workspace holds gemm_i8_workspace bytes; eps is read with a
+        norm_weight only."""
+        self._product_i8("gemm_i8", x, residual, residual_out, norm_weight, w, w_scales, y, workspace, m, n, n, k, eps)
+
+    def gemm_i8_silu(self, x: Buffer, residual: Buffer | None, residual_out: Buffer | None,
+                     norm_weight: Buffer | None, w: Buffer, w_scales: Buffer, act: Buffer, workspace: Buffer, m: int,
+                     intermediate: int, k: int, eps: float) -> None:
+        """gemm_i8 with the [2 * intermediate, k] gate_up weight (gate rows, then up rows):
+        act [m, intermediate] = bf16(silu(gate) * up) of the products before rounding."""
+        if intermediate > INT_MAX // 2:
+            raise ArgumentError("dimension", f"gemm_i8_silu: {intermediate} gates are more than 2^30")
+        self._product_i8("gemm_i8_silu", x, residual, residual_out, norm_weight, w, w_scales, act, workspace, m,
+                         intermediate, 2 * intermediate, k, eps)
+
+    def _product_i8(self, op, x, residual, residual_out, norm_weight, w, w_scales, y, workspace, m, n, channels, k,
+                    eps) -> None:
+        if norm_weight is not None:
+            require_positive(eps, f"{op} eps")
+        elif residual is not None:
+            raise ArgumentError("value", f"{op}: a residual needs a norm_weight")
+        if residual is None and residual_out is not None:
+            raise ArgumentError("value", f"{op}: residual_out needs a residual to add")
+        need = self._i8_workspace(op + "_workspace", m, n, k)
+        args = [_r("x", x, 2, m, k), _r("w", w, 16, channels, i8_pitch(k) // 16), _r("w_scales", w_scales, 4, channels),
+                _w("y", y, 2, m, n)]
+        if need:
+            args.append(self._workspace(op, workspace, need))
+        for name, buf, dims, writes in (("residual", residual, (m, k), False), ("residual_out", residual_out, (m, k), True),
+                                        ("norm_weight", norm_weight, (k,), False)):
+            if buf is not None:
+                args.append((_w if writes else _r)(name, buf, 2, *dims))
+        self._admit(op, args)
+        ptr = lambda b: None if b is None else b.ptr  # noqa: E731
+        self._call(getattr(self.lib, "nv_" + op)(self.handle, x.ptr, ptr(residual), ptr(residual_out), ptr(norm_weight),
+                                                 w.ptr, w_scales.ptr, y.ptr, ptr(workspace), m, n, k, eps))
 
     def add_rms_norm_gather(self, x: Buffer, residual: Buffer, weight: Buffer, indices: Buffer, out: Buffer,
                             rows: int, hidden: int, input_rows: int, eps: float) -> None:
