@@ -98,6 +98,10 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     nvr::launch_quantize(c, t, xq, xs, pitch);
     const nvr::ProductArgs p{xq, xs, static_cast<const uint8_t*>(w), static_cast<const float*>(w_scales),
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
+    if (m >= 64) {
+        nvr::launch_product_tiles(c, p, GATED);
+        return nvr::launch_status();
+    }
     const dim3 grid(unsigned((int64_t(n) + 127) / 128), unsigned(std::min<int64_t>((int64_t(m) + 31) / 32, 65535)));
     hipLaunchKernelGGL(gemm_direct<GATED>, grid, dim3(256), 0, c->stream, p);
     return nvr::launch_status();

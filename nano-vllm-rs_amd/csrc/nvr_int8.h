@@ -69,6 +69,9 @@ struct ProductArgs {
     int m, n, x_pitch, w_pitch;
 };
 
+// Products of whole tiles (gemm_int_tiles.hip).
+void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated);
+
 // Elements j .. j + 7 of a row, +0 from k on.
 template <bool VEC>
 __device__ __forceinline__ void load_chunk(const uint16_t* row, int j, int k, float* f) {
