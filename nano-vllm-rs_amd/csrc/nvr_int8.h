@@ -230,5 +230,8 @@ __device__ __forceinline__ Scale split_scale(float s) {
 __device__ __forceinline__ float scaled(int acc, Scale x, Scale w) {
     return __builtin_amdgcn_ldexpf(float(acc) * x.mantissa * w.mantissa, x.exponent + w.exponent);
 }
+// Whether float(acc) s t is the same bits as scaled's for all such scales s, t and any sum: nothing on the way overflows
+// or becomes subnormal, and powers of two change no rounding.
+__device__ __forceinline__ bool middling(float s) { return s == 0.0f || (s >= 0x1.0p-60f && s <= 0x1.0p40f); }
 
 }  // namespace nvr

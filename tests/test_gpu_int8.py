@@ -140,6 +140,15 @@ def test_products_of_long_rows(gpu, m, n, k, norm):
     call.check()
 
 
+@pytest.mark.parametrize("m,n,k,gated", [(4100, 4097, 40, False), (3900, 4344, 136, False), (4100, 2050, 72, True),
+                                         (4111, 2059, 160, True)])
+@pytest.mark.parametrize("norm", ["none", "add"])
+def test_products_of_many_tokens(gpu, m, n, k, gated, norm):
+    call = Call(gpu, m, n, k, norm, gated, seed=n)
+    call.run()
+    call.check()
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 def test_sums_of_the_longest_rows_stay_exact(gpu, m):
     """The largest sums that 32 bits hold: 131071 times 127 times -128."""
