@@ -19,42 +19,205 @@ namespace {
 
 using nvr::kWave;
 using nvr::Scale;
+using nvr::Tokens;
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
-// Any size: a wave forms 32 channels of 32 tokens, its operands read from memory in the matrix
-// instruction's layout (lane l: row l % 32, 16 bytes at 16 (l / 32) of each 32).
-template <bool GATED>
-__global__ __launch_bounds__(256) void gemm_direct(nvr::ProductArgs p) {
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int i = lane % 32, half = lane / 32;
-    const int n0 = (blockIdx.x * 4 + wave) * 32;
-    if (n0 >= p.n) return;
-    for (int64_t m0 = int64_t(blockIdx.y) * 32; m0 < p.m; m0 += int64_t(gridDim.y) * 32) {
-        const int64_t token = min(m0 + i, int64_t(p.m) - 1);
-        const int channel = min(n0 + i, p.n - 1);
-        const uint8_t* x = p.xq + token * p.x_pitch;
-        const uint8_t* w = p.wq + int64_t(channel) * p.w_pitch;
-        i32x16_t acc = {}, up = {};
-        for (int k = 0; k < p.x_pitch; k += 32) {
-            const int kx = k + 16 * half, kw = min(kx, p.w_pitch - 16);  // x is zero from w's pitch on
-            const i32x4_t b = *reinterpret_cast<const i32x4_t*>(x + kx);
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*reinterpret_cast<const i32x4_t*>(w + kw), b, acc, 0, 0, 0);
-            if constexpr (GATED)
-                up = __builtin_amdgcn_mfma_i32_32x32x32_i8(
-                    *reinterpret_cast<const i32x4_t*>(w + int64_t(p.n) * p.w_pitch + kw), b, up, 0, 0, 0);
-        }
-        if (m0 + i >= p.m) continue;
-        const Scale xs = nvr::split_scale(p.xs[token]);
+constexpr int kWaves = 8, kThreads = kWaves * kWave;
+constexpr int kUnit = 8;     // steps of 64 bytes of k whose weights are in flight together
+constexpr int kRowPad = 16;  // behind a token's row in LDS: 16 tokens' pieces of one column lie in different banks
+constexpr int kFewTokens = 32;
+constexpr int kKeptChunks = 8;       // a made token's row stays in registers: k <= 4096
+constexpr int kMadeTokens = 32768;   // values that each block makes
+constexpr int kMostLds = 160 * 1024;
+
+// Where the tokens' integers come from: made by each block (of x, the norm, or the norm of the sum), or by a launch of
+// quantize_rows, and then brought to LDS, or read where they are used.
+enum class Source { kPlain, kNorm, kAddNorm, kCopied, kMemory };
+
+struct RowsArgs {
+    nvr::ProductArgs p;
+    nvr::TokenArgs t;
+    int parts;  // waves that share the k of a tile: 1, 2, 4 or 8
+};
+
+// LDS of a block: partial sums (parts > 1), scales, tokens.
+template <int MT>
+constexpr int kSumBytes = 2 * kWaves * MT * kWave * 16;
+template <Source SRC, int MT>
+int64_t rows_lds(int m, int x_pitch) {
+    return kSumBytes<MT> + MT * 16 * 4 + (SRC == Source::kMemory ? 0 : int64_t(m) * (x_pitch + kRowPad));
+}
+
+// Few tokens: the weights stream through registers, once.
+template <Source SRC, int MT, bool GATED>
+__global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
+    constexpr bool kMade = SRC != Source::kCopied && SRC != Source::kMemory;
+    constexpr int kChannels = GATED ? 8 : 16;  // of a tile: 16 rows of the weight, or 8 of gate, then 8 of up
+    extern __shared__ __align__(16) unsigned char smem[];
+    const nvr::ProductArgs& p = a.p;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int i = lane % 16, g = lane / 16;
+    const int parts = a.parts, groups = kWaves / parts, group = wave / parts, part = wave % parts;
+    // A block's tiles lie side by side, so the pieces of y's rows fill lines in one XCD's L2.
+    const int tiles = (p.n + kChannels - 1) / kChannels;
+    const int first = int(int64_t(blockIdx.x) * tiles / gridDim.x);
+    const int mine = int(int64_t(blockIdx.x + 1) * tiles / gridDim.x) - first;  // >= 1
+    const int rounds = (mine + groups - 1) / groups;                            // the same in every wave
+    // A wave's steps of each of its tiles: whole lines of 128 bytes.
+    const int lines = p.x_pitch / 128, share = (lines + parts - 1) / parts;
+    const int s0 = min(part * share, lines) * 2, s1 = min((part + 1) * share, lines) * 2;
+    const int units = (share * 2 + kUnit - 1) / kUnit;
+
+    i32x4_t* red = reinterpret_cast<i32x4_t*>(smem);                   // [2][kWaves][MT][64]
+    float* xs = reinterpret_cast<float*>(smem + kSumBytes<MT>);        // [MT * 16]
+    unsigned char* xq = reinterpret_cast<unsigned char*>(xs + MT * 16);  // [m][pitch]
+    const int pitch = SRC == Source::kMemory ? p.x_pitch : p.x_pitch + kRowPad;
+
+    // The weights of a unit: lane l has row l % 16, 16 bytes at 16 (l / 16) of each step. Behind a row's end, where x is
+    // zero, and behind the wave's steps, which are not multiplied, any bytes of the row will do.
+    struct Unit {
+        uint4 w[kUnit];
+        float ws[4];  // of the lane's outputs; with a tile's first unit
+    };
+    Unit unit[2];
+    int ahead_round = 0, ahead = 0;  // the next unit to load
+    auto load = [&](Unit& u) {
+        const int tile = first + min(ahead_round * groups + group, mine - 1);
+        const int64_t row = GATED ? int64_t(i < 8 ? 0 : p.n) + min(tile * 8 + i % 8, p.n - 1) : min(tile * 16 + i, p.n - 1);
+        const uint8_t* w = p.wq + row * p.w_pitch;
+        const int s = s0 + ahead * kUnit;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int j = n0 + 8 * (r / 4) + 4 * half + r % 4;
-            if (j >= p.n) continue;
-            float y = nvr::scaled(acc[r], xs, nvr::split_scale(p.ws[j]));
-            if constexpr (GATED) y = nvr::silu_mul(y, nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + j])));
-            p.y[token * p.n + j] = nvr::f32_to_bf16(y);
+        for (int e = 0; e < kUnit; ++e) u.w[e] = nvr::load_stream(w + min((s + e) * 64 + 16 * g, p.w_pitch - 16));
+        if (ahead == 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                u.ws[r] = GATED ? p.ws[int64_t(g < 2 ? 0 : p.n) + min(tile * 8 + 4 * (g % 2) + r, p.n - 1)]
+                                : p.ws[min(tile * 16 + 4 * g + r, p.n - 1)];
         }
+        if (++ahead == units) {
+            ahead = 0;
+            ++ahead_round;
+        }
+    };
+    load(unit[0]);
+
+    if constexpr (kMade) {
+        constexpr Tokens T = SRC == Source::kPlain ? Tokens::kPlain : SRC == Source::kNorm ? Tokens::kNorm : Tokens::kAddNorm;
+        for (int row = wave; row < p.m; row += kWaves) {
+            const nvr::RowStep step = nvr::quantize_row<T, true, true, kKeptChunks, 1>(
+                a.t, row, p.x_pitch, blockIdx.x == 0 && a.t.residual_out != nullptr, lane, 0, nvr::NoJoin{},
+                [&](int j, uint2 eight) { *reinterpret_cast<uint2*>(xq + row * pitch + j) = eight; });
+            if (lane == 0) xs[row] = step.scale;
+        }
+    } else {
+        if constexpr (SRC == Source::kCopied) {
+            const int pieces = p.x_pitch / 16;
+            for (int at = threadIdx.x; at < p.m * pieces; at += kThreads)
+                *reinterpret_cast<uint4*>(xq + at / pieces * pitch + at % pieces * 16) =
+                    *reinterpret_cast<const uint4*>(p.xq + int64_t(at) * 16);
+        }
+        if (int(threadIdx.x) < p.m) xs[threadIdx.x] = p.xs[threadIdx.x];
     }
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // leaves the weights in flight
+
+    // Tokens behind the last repeat it and are not stored.
+    const unsigned char* xrow[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+        xrow[t] = (SRC == Source::kMemory ? p.xq : xq) + int64_t(min(t * 16 + i, p.m - 1)) * pitch + 16 * g;
+    i32x4_t acc[MT];
+    float ws[4];
+    int round = 0, at = 0;  // the unit to multiply
+    // Lane l has token l % 16 of 16, rows 4 (l / 16) .. + 3 of the tile.
+    auto finish = [&](int t, const i32x4_t& sum) {
+        const int token = t * 16 + i, tile = round * groups + group;
+        const Scale x = nvr::split_scale(xs[min(token, p.m - 1)]);
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            y[r] = nvr::scaled(sum[r], x, nvr::split_scale(ws[r]));
+            if constexpr (GATED) y[r] = nvr::silu_mul(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
+        }
+        if (tile >= mine || token >= p.m || (GATED && g >= 2)) return;
+        const int channel = (first + tile) * kChannels + 4 * (GATED ? g % 2 : g);
+        uint16_t* out = p.y + int64_t(token) * p.n + channel;
+        if (p.n % 4 == 0 && nvr::aligned(p.y, 8)) {
+            if (channel < p.n)
+                *reinterpret_cast<uint2*>(out) = make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (channel + r < p.n) out[r] = nvr::f32_to_bf16(y[r]);
+        }
+    };
+    auto multiply = [&](const Unit& u) {
+        if (at == 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int r = 0; r < 4; ++r) ws[r] = u.ws[r];
+        }
+        const int s = s0 + at * kUnit;
+#pragma unroll
+        for (int e = 0; e < kUnit; ++e) {
+            if (s + e >= s1) break;
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]),
+                                                               *reinterpret_cast<const i32x4_t*>(xrow[t] + (s + e) * 64),
+                                                               acc[t], 0, 0, 0);
+        }
+        if (++at < units) return;
+        if (parts == 1) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) finish(t, acc[t]);
+        } else {
+            i32x4_t* sums = red + (round & 1) * (kWaves * MT * kWave) + lane;
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sums[(wave * MT + t) * kWave] = acc[t];
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                if ((round * MT + t) % parts != part) continue;  // the waves take turns
+                i32x4_t sum = sums[(group * parts * MT + t) * kWave];
+                for (int q = 1; q < parts; ++q) sum += sums[((group * parts + q) * MT + t) * kWave];
+                finish(t, sum);
+            }
+        }
+        at = 0;
+        ++round;
+    };
+    const int total = rounds * units;
+    for (int u = 0; u < total; u += 2) {
+        if (u + 1 < total) load(unit[1]);
+        multiply(unit[0]);
+        if (u + 1 >= total) break;
+        if (u + 2 < total) load(unit[0]);
+        multiply(unit[1]);
+    }
+}
+
+template <Source SRC, int MT, bool GATED>
+void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
+    hipLaunchKernelGGL((gemm_rows_i8<SRC, MT, GATED>), dim3(unsigned(blocks)), dim3(kThreads),
+                       size_t(rows_lds<SRC, MT>(a.p.m, a.p.x_pitch)), c->stream, a);
+}
+
+template <Source SRC, bool GATED>
+void launch_rows(nv_context* c, RowsArgs a) {
+    const int tiles = (a.p.n + (GATED ? 8 : 16) - 1) / (GATED ? 8 : 16);
+    const int cus = c->cu_count > 0 ? c->cu_count : 256;
+    const int units = (a.p.x_pitch / 64 + kUnit - 1) / kUnit;
+    a.parts = 8;
+    while (a.parts > 1 && (units * 2 <= a.parts || int64_t(tiles) * a.parts > int64_t(cus) * kWaves * 4)) a.parts /= 2;
+    const int blocks = std::min(cus, (tiles * a.parts + kWaves - 1) / kWaves);
+    a.p.m <= 16 ? launch_rows_as<SRC, 1, GATED>(c, a, blocks) : launch_rows_as<SRC, 2, GATED>(c, a, blocks);
+}
+
+// Whether each block makes the tokens' integers by itself: they fit its LDS and registers, and are few enough.
+bool tokens_in_block(const nvr::TokenArgs& t) {
+    return t.k <= kKeptChunks * nvr::kWaveChunk && nvr::tokens_aligned(t) && int64_t(t.rows) * t.k <= kMadeTokens;
 }
 
 constexpr int kStepBytes = 128;  // tokens' rows in the workspace end in zeros at a multiple of this
@@ -95,15 +258,20 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     const int pitch = int(token_pitch(k));
     uint8_t* xq = static_cast<uint8_t*>(workspace);
     float* xs = reinterpret_cast<float*>(xq + int64_t(m) * pitch);
-    nvr::launch_quantize(c, t, xq, xs, pitch);
     const nvr::ProductArgs p{xq, xs, static_cast<const uint8_t*>(w), static_cast<const float*>(w_scales),
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
-    if (m >= 64) {
-        nvr::launch_product_tiles(c, p, GATED);
+    const RowsArgs few{p, t, 0};
+    if (m <= kFewTokens && tokens_in_block(t)) {
+        if (norm_weight == nullptr) launch_rows<Source::kPlain, GATED>(c, few);
+        else if (residual == nullptr) launch_rows<Source::kNorm, GATED>(c, few);
+        else launch_rows<Source::kAddNorm, GATED>(c, few);
         return nvr::launch_status();
     }
-    const dim3 grid(unsigned((int64_t(n) + 127) / 128), unsigned(std::min<int64_t>((int64_t(m) + 31) / 32, 65535)));
-    hipLaunchKernelGGL(gemm_direct<GATED>, grid, dim3(256), 0, c->stream, p);
+    nvr::launch_quantize(c, t, xq, xs, pitch);
+    if (m > kFewTokens) nvr::launch_product_tiles(c, p, GATED);
+    else if ((m <= 16 ? rows_lds<Source::kCopied, 1>(m, pitch) : rows_lds<Source::kCopied, 2>(m, pitch)) <= kMostLds)
+        launch_rows<Source::kCopied, GATED>(c, few);
+    else launch_rows<Source::kMemory, GATED>(c, few);
     return nvr::launch_status();
 }
 
