@@ -27,8 +27,6 @@ constexpr int kWaves = 8, kThreads = kWaves * kWave;
 constexpr int kUnit = 8;     // steps of 64 bytes of k whose weights are in flight together
 constexpr int kRowPad = 16;  // behind a token's row in LDS: 16 tokens' pieces of one column lie in different banks
 constexpr int kFewTokens = 32;
-constexpr int kKeptChunks = 8;       // a made token's row stays in registers: k <= 4096
-constexpr int kMadeTokens = 32768;   // values that each block makes
 constexpr int kMostLds = 160 * 1024;
 
 // Where the tokens' integers come from: made by each block (of x, the norm, or the norm of the sum), or by a launch of
@@ -38,7 +36,9 @@ enum class Source { kPlain, kNorm, kAddNorm, kCopied, kMemory };
 struct RowsArgs {
     nvr::ProductArgs p;
     nvr::TokenArgs t;
-    int parts;  // waves that share the k of a tile: 1, 2, 4 or 8
+    int log_parts;              // 2^log_parts waves share the k of a tile: 1, 2, 4 or 8
+    int tiles, per, more;       // a block has `per` tiles, the first `more` blocks one more
+    int share, units;           // lines of 128 bytes of k a wave has of a tile; loads of kUnit steps
 };
 
 // LDS of a block: partial sums (parts > 1), scales, tokens.
@@ -49,8 +49,8 @@ int64_t rows_lds(int m, int x_pitch) {
     return kSumBytes<MT> + MT * 16 * 4 + (SRC == Source::kMemory ? 0 : int64_t(m) * (x_pitch + kRowPad));
 }
 
-// Few tokens: the weights stream through registers, once.
-template <Source SRC, int MT, bool GATED>
+// Few tokens: the weights stream through registers, once. ONE: every wave has one unit at most in all.
+template <Source SRC, int CH, int MT, bool GATED, bool ONE>
 __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     constexpr bool kMade = SRC != Source::kCopied && SRC != Source::kMemory;
     constexpr int kChannels = GATED ? 8 : 16;  // of a tile: 16 rows of the weight, or 8 of gate, then 8 of up
@@ -58,16 +58,17 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     const nvr::ProductArgs& p = a.p;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int i = lane % 16, g = lane / 16;
-    const int parts = a.parts, groups = kWaves / parts, group = wave / parts, part = wave % parts;
-    // A block's tiles lie side by side, so the pieces of y's rows fill lines in one XCD's L2.
-    const int tiles = (p.n + kChannels - 1) / kChannels;
-    const int first = int(int64_t(blockIdx.x) * tiles / gridDim.x);
-    const int mine = int(int64_t(blockIdx.x + 1) * tiles / gridDim.x) - first;  // >= 1
-    const int rounds = (mine + groups - 1) / groups;                            // the same in every wave
-    // A wave's steps of each of its tiles: whole lines of 128 bytes.
-    const int lines = p.x_pitch / 128, share = (lines + parts - 1) / parts;
-    const int s0 = min(part * share, lines) * 2, s1 = min((part + 1) * share, lines) * 2;
-    const int units = (share * 2 + kUnit - 1) / kUnit;
+    const int parts = 1 << a.log_parts, groups = kWaves >> a.log_parts, group = wave >> a.log_parts, part = wave & (parts - 1);
+    const int first = int(blockIdx.x) * a.per + min(int(blockIdx.x), a.more);
+    // Of a block's tiles, and of a group's of waves.
+    const int mine = a.per + (int(blockIdx.x) < a.more ? 1 : 0);  // >= 1
+    const int rounds = (mine + groups - 1) >> (3 - a.log_parts);  // the same in every wave
+    static_assert(kWaves == 8, "rounds");
+    const int even = mine >> (3 - a.log_parts), odd = mine & (groups - 1);
+    const int tile0 = first + group * even + min(group, odd), tile_count = even + (group < odd ? 1 : 0);
+    // A wave's steps of each of its tiles.
+    const int lines = p.x_pitch / 128, units = a.units;
+    const int s0 = min(part * a.share, lines) * 2, s1 = min((part + 1) * a.share, lines) * 2;
 
     i32x4_t* red = reinterpret_cast<i32x4_t*>(smem);                   // [2][kWaves][MT][64]
     float* xs = reinterpret_cast<float*>(smem + kSumBytes<MT>);        // [MT * 16]
@@ -78,48 +79,52 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     // zero, and behind the wave's steps, which are not multiplied, any bytes of the row will do.
     struct Unit {
         uint4 w[kUnit];
-        float ws[4];  // of the lane's outputs; with a tile's first unit
+        float ws[4];  // of the lane's outputs
     };
     Unit unit[2];
     int ahead_round = 0, ahead = 0;  // the next unit to load
     auto load = [&](Unit& u) {
-        const int tile = first + min(ahead_round * groups + group, mine - 1);
+        const int tile = tile0 + max(min(ahead_round, tile_count - 1), 0);  // its own last one, if any, where it has no more
         const int64_t row = GATED ? int64_t(i < 8 ? 0 : p.n) + min(tile * 8 + i % 8, p.n - 1) : min(tile * 16 + i, p.n - 1);
         const uint8_t* w = p.wq + row * p.w_pitch;
         const int s = s0 + ahead * kUnit;
 #pragma unroll
         for (int e = 0; e < kUnit; ++e) u.w[e] = nvr::load_stream(w + min((s + e) * 64 + 16 * g, p.w_pitch - 16));
-        if (ahead == 0) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                u.ws[r] = GATED ? p.ws[int64_t(g < 2 ? 0 : p.n) + min(tile * 8 + 4 * (g % 2) + r, p.n - 1)]
-                                : p.ws[min(tile * 16 + 4 * g + r, p.n - 1)];
-        }
+        for (int r = 0; r < 4; ++r)
+            u.ws[r] = GATED ? p.ws[int64_t(g < 2 ? 0 : p.n) + min(tile * 8 + 4 * (g % 2) + r, p.n - 1)]
+                            : p.ws[min(tile * 16 + 4 * g + r, p.n - 1)];
         if (++ahead == units) {
             ahead = 0;
             ++ahead_round;
         }
     };
-    load(unit[0]);
-
     if constexpr (kMade) {
+        // A wave's loads return in order: its tokens' come before the weights'.
         constexpr Tokens T = SRC == Source::kPlain ? Tokens::kPlain : SRC == Source::kNorm ? Tokens::kNorm : Tokens::kAddNorm;
-        for (int row = wave; row < p.m; row += kWaves) {
-            const nvr::RowStep step = nvr::quantize_row<T, true, true, kKeptChunks, 1>(
-                a.t, row, p.x_pitch, blockIdx.x == 0 && a.t.residual_out != nullptr, lane, 0, nvr::NoJoin{},
+        const int row = min(wave, p.m - 1);
+        const nvr::NormChunks<CH> norm = nvr::load_norm<T, true, CH, 1>(a.t, lane, 0);
+        const nvr::RowChunks<T, CH> chunks = nvr::load_row<T, true, CH, 1>(a.t, row, lane, 0);
+        load(unit[0]);
+        if (wave < p.m) {
+            const nvr::RowStep step = nvr::quantize_row<T, true, CH, 1>(
+                a.t, row, chunks, norm, p.x_pitch, blockIdx.x == 0 && a.t.residual_out != nullptr, lane, 0, nvr::NoJoin{},
                 [&](int j, uint2 eight) { *reinterpret_cast<uint2*>(xq + row * pitch + j) = eight; });
             if (lane == 0) xs[row] = step.scale;
         }
     } else {
+        load(unit[0]);
         if constexpr (SRC == Source::kCopied) {
-            const int pieces = p.x_pitch / 16;
-            for (int at = threadIdx.x; at < p.m * pieces; at += kThreads)
-                *reinterpret_cast<uint4*>(xq + at / pieces * pitch + at % pieces * 16) =
-                    *reinterpret_cast<const uint4*>(p.xq + int64_t(at) * 16);
+            for (int row = wave; row < p.m; row += kWaves)
+#pragma unroll 4
+                for (int c = lane * 16; c < p.x_pitch; c += kWave * 16)
+                    *reinterpret_cast<uint4*>(xq + row * pitch + c) =
+                        *reinterpret_cast<const uint4*>(p.xq + int64_t(row) * p.x_pitch + c);
         }
         if (int(threadIdx.x) < p.m) xs[threadIdx.x] = p.xs[threadIdx.x];
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // leaves the weights in flight
+    if constexpr (!ONE) load(unit[1]);
 
     // Tokens behind the last repeat it and are not stored.
     const unsigned char* xrow[MT];
@@ -128,10 +133,14 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         xrow[t] = (SRC == Source::kMemory ? p.xq : xq) + int64_t(min(t * 16 + i, p.m - 1)) * pitch + 16 * g;
     i32x4_t acc[MT];
     float ws[4];
+    // A wave that has its tiles to itself, and several, keeps its outputs until they fill lines of 128 bytes.
+    const bool lines_kept = !ONE && parts == 1 && p.n % 8 == 0 && nvr::aligned(p.y, 16);
+    unsigned char* kept = smem + wave * (MT * 16 * 128);  // [MT * 16][128], where the sums would be
+    static_assert(kWaves * MT * 16 * 128 == kSumBytes<MT>, "its place");
     int round = 0, at = 0;  // the unit to multiply
     // Lane l has token l % 16 of 16, rows 4 (l / 16) .. + 3 of the tile.
     auto finish = [&](int t, const i32x4_t& sum) {
-        const int token = t * 16 + i, tile = round * groups + group;
+        const int token = t * 16 + i;
         const Scale x = nvr::split_scale(xs[min(token, p.m - 1)]);
         float y[4];
 #pragma unroll
@@ -139,39 +148,75 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
             y[r] = nvr::scaled(sum[r], x, nvr::split_scale(ws[r]));
             if constexpr (GATED) y[r] = nvr::silu_mul(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
         }
-        if (tile >= mine || token >= p.m || (GATED && g >= 2)) return;
-        const int channel = (first + tile) * kChannels + 4 * (GATED ? g % 2 : g);
+        if (round >= tile_count) return;
+        const int channel = (tile0 + round) * kChannels + 4 * (GATED ? g % 2 : g);
+        const bool stored = token < p.m && !(GATED && g >= 2);
+        if (lines_kept) {
+            if (stored)
+                *reinterpret_cast<uint2*>(kept + token * 128 + channel % 64 * 2) =
+                    make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+            return;
+        }
         uint16_t* out = p.y + int64_t(token) * p.n + channel;
         if (p.n % 4 == 0 && nvr::aligned(p.y, 8)) {
-            if (channel < p.n)
+            if (stored && channel < p.n)
                 *reinterpret_cast<uint2*>(out) = make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
-        } else {
+        } else if (stored) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (channel + r < p.n) out[r] = nvr::f32_to_bf16(y[r]);
         }
     };
+    // A wave's tiles that fill a line of 64 channels, or its last: 8 tokens' lines a store.
+    auto flush = [&] {
+        const int end = (tile0 + round + 1) * kChannels;
+        if (round >= tile_count || (end % 64 != 0 && round + 1 < tile_count)) return;
+        const int channel = (end - 1) / 64 * 64 + lane % 8 * 8;
+        if (channel < tile0 * kChannels || channel >= min(end, p.n)) return;
+#pragma unroll
+        for (int r = 0; r < MT * 16; r += 8)
+            if (r + lane / 8 < p.m)
+                *reinterpret_cast<uint4*>(p.y + int64_t(r + lane / 8) * p.n + channel) =
+                    *reinterpret_cast<const uint4*>(kept + (r + lane / 8) * 128 + lane % 8 * 16);
+    };
     auto multiply = [&](const Unit& u) {
         if (at == 0) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = i32x4_t{0, 0, 0, 0};
-#pragma unroll
-            for (int r = 0; r < 4; ++r) ws[r] = u.ws[r];
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ws[r] = u.ws[r];
         const int s = s0 + at * kUnit;
+        auto tokens = [&](int t, int e) { return *reinterpret_cast<const i32x4_t*>(xrow[t] + (s + e) * 64); };
+        if (s + kUnit <= s1) {
+            i32x4_t x[kUnit][MT];
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) {
-            if (s + e >= s1) break;
+            for (int e = 0; e < kUnit; ++e)
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
-                acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]),
-                                                               *reinterpret_cast<const i32x4_t*>(xrow[t] + (s + e) * 64),
-                                                               acc[t], 0, 0, 0);
+                for (int t = 0; t < MT; ++t) x[e][t] = tokens(t, e);
+#pragma unroll
+            for (int e = 0; e < kUnit; ++e)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]), x[e][t], acc[t], 0, 0, 0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kUnit; ++e) {
+                if (s + e >= s1) break;
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]), tokens(t, e), acc[t], 0, 0, 0);
+            }
         }
-        if (++at < units) return;
+        ++at;
+    };
+    // After the loads that follow: a wait for those of one unit then leaves the stores of the one before in flight.
+    auto settle = [&] {
+        if (at < units) return;
         if (parts == 1) {
 #pragma unroll
             for (int t = 0; t < MT; ++t) finish(t, acc[t]);
+            if (lines_kept) flush();
         } else {
             i32x4_t* sums = red + (round & 1) * (kWaves * MT * kWave) + lane;
 #pragma unroll
@@ -179,29 +224,63 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                if ((round * MT + t) % parts != part) continue;  // the waves take turns
-                i32x4_t sum = sums[(group * parts * MT + t) * kWave];
-                for (int q = 1; q < parts; ++q) sum += sums[((group * parts + q) * MT + t) * kWave];
-                finish(t, sum);
+                if (((round * MT + t) & (parts - 1)) != part) continue;  // the waves take turns
+                i32x4_t sum[kWaves];
+#pragma unroll
+                for (int q = 0; q < kWaves; ++q)
+                    if (q < parts) sum[q] = sums[(((wave & -parts) + q) * MT + t) * kWave];
+#pragma unroll
+                for (int q = 1; q < kWaves; ++q)
+                    if (q < parts) sum[0] += sum[q];
+                finish(t, sum[0]);
             }
         }
         at = 0;
         ++round;
     };
-    const int total = rounds * units;
-    for (int u = 0; u < total; u += 2) {
-        if (u + 1 < total) load(unit[1]);
+    if constexpr (ONE) {
         multiply(unit[0]);
-        if (u + 1 >= total) break;
-        if (u + 2 < total) load(unit[0]);
+        settle();
+        return;
+    }
+    for (int left = rounds * units;; left -= 2) {
+        multiply(unit[0]);
+        if (left <= 2) {
+            settle();
+            if (left == 2) {
+                multiply(unit[1]);
+                settle();
+            }
+            break;
+        }
+        load(unit[0]);
+        settle();
         multiply(unit[1]);
+        if (left == 3) {
+            settle();
+            multiply(unit[0]);
+            settle();
+            break;
+        }
+        load(unit[1]);
+        settle();
     }
 }
 
-template <Source SRC, int MT, bool GATED>
+template <Source SRC, int CH, int MT, bool GATED, bool ONE>
 void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
-    hipLaunchKernelGGL((gemm_rows_i8<SRC, MT, GATED>), dim3(unsigned(blocks)), dim3(kThreads),
+    hipLaunchKernelGGL((gemm_rows_i8<SRC, CH, MT, GATED, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
                        size_t(rows_lds<SRC, MT>(a.p.m, a.p.x_pitch)), c->stream, a);
+}
+
+void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
+    const int lines = a.p.x_pitch / 128;
+    a.log_parts = __builtin_ctz(unsigned(parts));
+    a.tiles = tiles;
+    a.per = tiles / blocks;
+    a.more = tiles % blocks;
+    a.share = (lines + parts - 1) / parts;
+    a.units = (a.share * 2 + kUnit - 1) / kUnit;
 }
 
 template <Source SRC, bool GATED>
@@ -209,15 +288,34 @@ void launch_rows(nv_context* c, RowsArgs a) {
     const int tiles = (a.p.n + (GATED ? 8 : 16) - 1) / (GATED ? 8 : 16);
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
     const int units = (a.p.x_pitch / 64 + kUnit - 1) / kUnit;
-    a.parts = 8;
-    while (a.parts > 1 && (units * 2 <= a.parts || int64_t(tiles) * a.parts > int64_t(cus) * kWaves * 4)) a.parts /= 2;
-    const int blocks = std::min(cus, (tiles * a.parts + kWaves - 1) / kWaves);
-    a.p.m <= 16 ? launch_rows_as<SRC, 1, GATED>(c, a, blocks) : launch_rows_as<SRC, 2, GATED>(c, a, blocks);
+    int parts = 8;
+    while (parts > 1 && (units * 2 <= parts || int64_t(tiles) * parts > int64_t(cus) * kWaves * 4)) parts /= 2;
+    const int blocks = std::min(cus, (tiles * parts + kWaves - 1) / kWaves);
+    plan_rows(a, tiles, parts, blocks);
+    const bool one = a.units == 1 && (a.per + (a.more != 0)) * parts <= kWaves;
+    auto run = [&](auto chunks, auto tiles16) {
+        constexpr int CH = decltype(chunks)::value, MT = decltype(tiles16)::value;
+        one ? launch_rows_as<SRC, CH, MT, GATED, true>(c, a, blocks) : launch_rows_as<SRC, CH, MT, GATED, false>(c, a, blocks);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one16;
+    if constexpr (SRC == Source::kCopied || SRC == Source::kMemory) {
+        if (a.p.m <= 16) run(integral_constant<int, 1>{}, one16);
+        else run(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+    } else {
+        if (a.p.x_pitch <= 2 * nvr::kWaveChunk) run(integral_constant<int, 2>{}, one16);
+        else if (a.p.x_pitch <= 4 * nvr::kWaveChunk) run(integral_constant<int, 4>{}, one16);
+        else if constexpr (SRC == Source::kPlain) run(integral_constant<int, 8>{}, one16);
+    }
 }
 
-// Whether each block makes the tokens' integers by itself: they fit its LDS and registers, and are few enough.
+// Whether each block makes the tokens' integers by itself, a row a wave: one launch less, for work that all blocks
+// repeat. On MI355X in a graph, n 4096, made and by a launch of their own, in us: 8 tokens at k 1024 5.7, 7.2 and with
+// sum and norm 6.3, 7.8; at k 2048 6.4, 7.6 and 7.8, 7.7 (4 tokens: 6.5, 7.4); at k 4096 9.1, 9.8 and 17.8, 12 (a row's
+// chunks, sums and norm weights no longer fit the registers beside the weights). 16 tokens, two rows a wave: at k 1024
+// 6.7, 7.5 and 8.0, 7.8; at k 2048 8.1, 8.1 and 10.9, 8.4.
 bool tokens_in_block(const nvr::TokenArgs& t) {
-    return t.k <= kKeptChunks * nvr::kWaveChunk && nvr::tokens_aligned(t) && int64_t(t.rows) * t.k <= kMadeTokens;
+    return t.rows <= kWaves && t.k % nvr::kChunk == 0 && t.k <= (t.norm_weight == nullptr ? 8 : 4) * nvr::kWaveChunk;
 }
 
 constexpr int kStepBytes = 128;  // tokens' rows in the workspace end in zeros at a multiple of this
@@ -260,7 +358,7 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     float* xs = reinterpret_cast<float*>(xq + int64_t(m) * pitch);
     const nvr::ProductArgs p{xq, xs, static_cast<const uint8_t*>(w), static_cast<const float*>(w_scales),
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
-    const RowsArgs few{p, t, 0};
+    const RowsArgs few{p, t, 0, 0, 0, 0, 0, 0};
     if (m <= kFewTokens && tokens_in_block(t)) {
         if (norm_weight == nullptr) launch_rows<Source::kPlain, GATED>(c, few);
         else if (residual == nullptr) launch_rows<Source::kNorm, GATED>(c, few);

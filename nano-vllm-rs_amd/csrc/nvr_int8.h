@@ -45,7 +45,7 @@ constexpr int kMostSummed = 131071;
 enum class Tokens { kPlain, kNorm, kAddNorm };
 
 // Tokens of a call: x, or RMSNorm(x) weight, or RMSNorm(x + residual) weight with
-// residual_out <- bf16(x + residual). VEC: k is a multiple of 8 and every pointer of 16 bytes.
+// residual_out <- bf16(x + residual).
 struct TokenArgs {
     const uint16_t* x;
     const uint16_t* residual;
@@ -56,7 +56,6 @@ struct TokenArgs {
 };
 
 // The tokens' integers (rows at `pitch` bytes, zeros behind k) and scales (quantize.hip).
-bool tokens_aligned(const TokenArgs& t);
 void launch_quantize(nv_context* c, const TokenArgs& t, uint8_t* q, float* scales, int pitch);
 
 // A product of m tokens and n channels (gated: n of gate, then n of up). Tokens' rows are zero from k to x_pitch.
@@ -72,22 +71,40 @@ struct ProductArgs {
 // Products of whole tiles (gemm_int_tiles.hip).
 void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated);
 
-// Elements j .. j + 7 of a row, +0 from k on.
-template <bool VEC>
-__device__ __forceinline__ void load_chunk(const uint16_t* row, int j, int k, float* f) {
-    if constexpr (VEC) {
-        unpack8(j < k ? *reinterpret_cast<const uint4*>(row + j) : make_uint4(0, 0, 0, 0), f);
-    } else {
+// Elements j .. j + 7 of a row (bf16 from any even address on), +0 from k on; nothing outside the row is read. WHOLE: k is
+// a multiple of 8.
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int j, int k) {
+    struct __attribute__((packed, aligned(2))) Eight { uint64_t lo, hi; };
+    if (!WHOLE && k < kChunk) {
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) f[i] = j + i < k ? bf16_to_f32(row[j + i]) : 0.0f;
+        for (int i = 0; i < 4; ++i)
+            w[i] = (j + 2 * i < k ? row[j + 2 * i] : 0) | (j + 2 * i + 1 < k ? uint32_t(row[j + 2 * i + 1]) << 16 : 0);
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    const int at = min(j, k - kChunk), past = min(j - at, kChunk);  // the row's last eight, of which `past` are before j
+    const Eight e = *reinterpret_cast<const Eight*>(row + at);
+    uint64_t lo = e.lo, hi = e.hi;
+    if constexpr (WHOLE) {
+        if (past != 0) lo = hi = 0;
+    } else {
+        if (past & 4) { lo = hi; hi = 0; }
+        const int bits = past & 3 ? 16 * (past & 3) : 0;
+        lo = lo >> bits | (bits ? hi << (64 - bits) : 0);
+        hi >>= bits;
+        if (past == kChunk) lo = hi = 0;
+    }
+    return make_uint4(uint32_t(lo), uint32_t(lo >> 32), uint32_t(hi), uint32_t(hi >> 32));
 }
 
-template <bool VEC>
+template <bool WHOLE>
 __device__ __forceinline__ void store_chunk(uint16_t* row, int j, int k, const float* f) {
-    if constexpr (VEC) {
-        if (j < k) *reinterpret_cast<uint4*>(row + j) = pack8_split(f);
-    } else {
+    struct __attribute__((packed, aligned(2))) Eight { uint32_t w[4]; };
+    if (j + kChunk <= k) {
+        const uint4 w = pack8_split(f);
+        *reinterpret_cast<Eight*>(row + j) = Eight{{w.x, w.y, w.z, w.w}};
+    } else if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
             if (j + i < k) row[j + i] = f32_to_bf16(f[i]);
@@ -139,84 +156,162 @@ __device__ __forceinline__ uint2 whole_numbers(const float* u, const RowStep& s)
     return make_uint2(four(b[0], b[1], b[2], b[3]), four(b[4], b[5], b[6], b[7]));
 }
 
-// A row of tokens by one wave: its step (in every lane), and put(j, eight numbers) for each chunk j < width that the lane
-// holds, from k on zeros. KEEP: the row stays in registers, CH chunks a lane (width <= CH * 512); else it is read again.
-// WAVES 1: this wave has the whole row. WAVES 4: four do, this one class `wave`, and join(sum or bits, ...) gathers.
-template <Tokens T, bool VEC, bool KEEP, int CH, int WAVES, class Join, class Put>
-__device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row, int width, bool keep_sum, int lane,
-                                                int wave, Join join, Put put) {
-    static_assert(WAVES == 1 || WAVES == kClasses, "a wave has all classes of a row, or one");
-    const uint16_t* x = t.x + row * t.k;
-    const uint16_t* res = T == Tokens::kAddNorm ? t.residual + row * t.k : nullptr;
-    const int stride = WAVES * kWaveChunk, first = wave * kWaveChunk + lane * kChunk;
-    const int chunks = (width + stride - 1) / stride;  // uniform in the block
-    float v[KEEP ? CH : 1][kChunk];
-    auto load = [&](int c, float* f) {
-        const int j = first + c * stride;
-        load_chunk<VEC>(x, j, t.k, f);
-        if constexpr (T == Tokens::kAddNorm) {
-            float r[kChunk];
-            load_chunk<VEC>(res, j, t.k, r);
+// A row of tokens by one wave (WAVES 1) or a class of it by each of four (WAVES 4), CH chunks a lane: what a lane loads
+// of it, always as many loads, so that later ones can stay in flight while the row is worked on.
+template <Tokens T, int CH>
+struct RowChunks {
+    uint4 x[CH], residual[T == Tokens::kAddNorm ? CH : 1];
+};
+template <int CH>
+struct NormChunks {
+    uint4 g[CH];
+};
+template <int WAVES>
+__device__ __forceinline__ int chunk_at(int c, int lane, int wave) {
+    return (c * WAVES + wave) * kWaveChunk + lane * kChunk;
+}
+template <Tokens T, bool WHOLE, int CH, int WAVES>
+__device__ __forceinline__ RowChunks<T, CH> load_row(const TokenArgs& t, int64_t row, int lane, int wave) {
+    RowChunks<T, CH> r;
 #pragma unroll
-            for (int i = 0; i < kChunk; ++i) f[i] = f[i] + r[i];
-        }
-    };
-    auto each = [&](auto&& f) {  // f(c, values as loaded)
-        if constexpr (KEEP) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-                if (c < chunks) f(c, v[c]);
-        } else {
-            for (int c = 0; c < chunks; ++c) {
-                load(c, v[0]);
-                f(c, v[0]);
-            }
-        }
-    };
-    if constexpr (KEEP) {
+    for (int c = 0; c < CH; ++c) r.x[c] = load_chunk<WHOLE>(t.x + row * t.k, chunk_at<WAVES>(c, lane, wave), t.k);
+    if constexpr (T == Tokens::kAddNorm) {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-            if (c < chunks) load(c, v[c]);
+            r.residual[c] = load_chunk<WHOLE>(t.residual + row * t.k, chunk_at<WAVES>(c, lane, wave), t.k);
     }
-    float inv = 1.0f;
+    return r;
+}
+template <Tokens T, bool WHOLE, int CH, int WAVES>
+__device__ __forceinline__ NormChunks<CH> load_norm(const TokenArgs& t, int lane, int wave) {
+    NormChunks<CH> n;
+    if constexpr (T != Tokens::kPlain) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) n.g[c] = load_chunk<WHOLE>(t.norm_weight, chunk_at<WAVES>(c, lane, wave), t.k);
+    }
+    return n;
+}
+
+template <Tokens T>
+__device__ __forceinline__ void row_values(const uint4& x, const uint4& residual, float* v) {
+    unpack8(x, v);
+    if constexpr (T == Tokens::kAddNorm) {
+        float r[kChunk];
+        unpack8(residual, r);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) v[i] = v[i] + r[i];
+    }
+}
+// A chunk's squares onto its class's sum.
+__device__ __forceinline__ float add_squares(float sum, const float* v) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) sum = __builtin_fmaf(v[i], v[i], sum);
+    return sum;
+}
+__device__ __forceinline__ float row_inverse(const float* s, const TokenArgs& t) {
+    return inv_sqrt_rn(((s[0] + s[1]) + (s[2] + s[3])) / float(t.k) + t.eps);
+}
+__device__ __forceinline__ void scale_norm(float* v, float inv, const uint4& weight) {
+    float g[kChunk];
+    unpack8(weight, g);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) v[i] = (v[i] * inv) * g[i];
+}
+__device__ __forceinline__ uint32_t most_of(uint32_t top, const float* v) {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) top = max(top, magnitude(v[i]));
+    return top;
+}
+
+struct NoJoin {
+    __device__ void sums(float*) const {}
+    __device__ void most(uint32_t&) const {}
+};
+
+// The row's step (in every lane), and put(j, eight numbers) for each chunk j < width that the lane holds: zeros from k on.
+// With WAVES 4, join brings the waves' sums and largest bits together.
+template <Tokens T, bool WHOLE, int CH, int WAVES, class Join, class Put>
+__device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row, const RowChunks<T, CH>& r,
+                                                const NormChunks<CH>& norm, int width, bool keep_sum, int lane,
+                                                int wave, Join join, Put put) {
+    static_assert(WAVES == 1 || WAVES == kClasses, "a wave has all classes of a row, or one");
+    float v[CH][kChunk];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) row_values<T>(r.x[c], r.residual[T == Tokens::kAddNorm ? c : 0], v[c]);
     if constexpr (T != Tokens::kPlain) {
         float s[kClasses] = {};
-        each([&](int c, const float* f) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
             float& sum = s[WAVES == 1 ? c % kClasses : 0];
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) sum = __builtin_fmaf(f[i], f[i], sum);
-        });
-#pragma unroll
-        for (int i = 0; i < (WAVES == 1 ? kClasses : 1); ++i) s[i] = wave_sum(s[i]);
-        if constexpr (WAVES != 1) join.sums(s);
-        inv = inv_sqrt_rn(((s[0] + s[1]) + (s[2] + s[3])) / float(t.k) + t.eps);
-    }
-    auto normed = [&](int c, float* f) {
-        if constexpr (T != Tokens::kPlain) {
-            float g[kChunk];
-            load_chunk<VEC>(t.norm_weight, first + c * stride, t.k, g);
-#pragma unroll
-            for (int i = 0; i < kChunk; ++i) f[i] = (f[i] * inv) * g[i];
+            sum = add_squares(sum, v[c]);
         }
-    };
-    uint32_t top = 0;
-    each([&](int c, float* f) {
-        if (T == Tokens::kAddNorm && keep_sum) store_chunk<VEC>(t.residual_out + row * t.k, first + c * stride, t.k, f);
-        normed(c, f);
 #pragma unroll
-        for (int i = 0; i < kChunk; ++i) top = max(top, magnitude(f[i]));
-    });
+        for (int i = 0; i < (WAVES == 1 ? (CH < kClasses ? CH : kClasses) : 1); ++i) s[i] = wave_sum(s[i]);
+        join.sums(s);
+        const float inv = row_inverse(s, t);
+        if (T == Tokens::kAddNorm && keep_sum) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                store_chunk<WHOLE>(t.residual_out + row * t.k, chunk_at<WAVES>(c, lane, wave), t.k, v[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) scale_norm(v[c], inv, norm.g[c]);
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) top = most_of(top, v[c]);
     top = wave_max(top);
-    if constexpr (WAVES != 1) join.most(top);
+    join.most(top);
     const RowStep step = row_step(top);
-    each([&](int c, float* f) {
-        if constexpr (!KEEP) normed(c, f);
-        if (first + c * stride < width) put(first + c * stride, whole_numbers(f, step));
-    });
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int j = chunk_at<WAVES>(c, lane, wave);
+        if (j < width) put(j, whole_numbers(v[c], step));
+    }
     return step;
 }
 
-struct NoJoin {};
+// The same for a row of any length by four waves, which read it anew for each of its three passes.
+template <Tokens T, bool WHOLE, class Join, class Put>
+__device__ __forceinline__ RowStep quantize_long_row(const TokenArgs& t, int64_t row, int width, bool keep_sum, int lane,
+                                                     int wave, Join join, Put put) {
+    const int chunks = (width + kClasses * kWaveChunk - 1) / (kClasses * kWaveChunk);
+    auto load = [&](int c, float* v) {
+        const int j = chunk_at<kClasses>(c, lane, wave);
+        const uint4 x = load_chunk<WHOLE>(t.x + row * t.k, j, t.k);
+        row_values<T>(x, T == Tokens::kAddNorm ? load_chunk<WHOLE>(t.residual + row * t.k, j, t.k) : x, v);
+        return j;
+    };
+    float inv = 1.0f, v[kChunk];
+    if constexpr (T != Tokens::kPlain) {
+        float s[kClasses] = {};
+        for (int c = 0; c < chunks; ++c) {
+            load(c, v);
+            s[0] = add_squares(s[0], v);
+        }
+        s[0] = wave_sum(s[0]);
+        join.sums(s);
+        inv = row_inverse(s, t);
+    }
+    uint32_t top = 0;
+    for (int c = 0; c < chunks; ++c) {
+        const int j = load(c, v);
+        if constexpr (T != Tokens::kPlain) {
+            if (T == Tokens::kAddNorm && keep_sum) store_chunk<WHOLE>(t.residual_out + row * t.k, j, t.k, v);
+            scale_norm(v, inv, load_chunk<WHOLE>(t.norm_weight, j, t.k));
+        }
+        top = most_of(top, v);
+    }
+    top = wave_max(top);
+    join.most(top);
+    const RowStep step = row_step(top);
+    for (int c = 0; c < chunks; ++c) {
+        const int j = load(c, v);
+        if constexpr (T != Tokens::kPlain) scale_norm(v, inv, load_chunk<WHOLE>(t.norm_weight, j, t.k));
+        if (j < width) put(j, whole_numbers(v, step));
+    }
+    return step;
+}
 
 // acc xs ws with both scales as mantissa and exponent: no product of two of the three leaves the range of fp32
 // where the result does not.

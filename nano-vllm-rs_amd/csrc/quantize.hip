@@ -17,7 +17,7 @@ namespace {
 using nvr::kWave;
 using nvr::Tokens;
 
-constexpr int kThreads = 256, kRowChunks = 8;
+constexpr int kThreads = 256;
 
 // The four waves of a row exchange through LDS.
 struct BlockJoin {
@@ -37,61 +37,73 @@ struct BlockJoin {
     }
 };
 
-template <Tokens T, bool VEC, bool KEEP, int WAVES>
+// CH chunks a lane of WAVES waves hold a row; 0: a row of any length, read anew for each pass.
+template <Tokens T, bool WHOLE, int CH, int WAVES>
 __global__ __launch_bounds__(kThreads) void quantize_rows(nvr::TokenArgs t, uint8_t* __restrict__ q,
                                                           float* __restrict__ scales, int pitch) {
     __shared__ float sum[nvr::kClasses];
     __shared__ uint32_t top[nvr::kClasses];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, of_row = WAVES == 1 ? 0 : wave;
     constexpr int kRows = kThreads / kWave / WAVES;  // rows of a block at a time
-    for (int64_t row = int64_t(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0); row < t.rows;
-         row += int64_t(gridDim.x) * kRows) {
+    const int64_t first = int64_t(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0), step = int64_t(gridDim.x) * kRows;
+    const bool keep_sum = t.residual_out != nullptr;
+    using Join = std::conditional_t<WAVES == 1, nvr::NoJoin, BlockJoin>;
+    Join join;
+    if constexpr (WAVES != 1) join = {sum, top, lane, wave};
+    nvr::NormChunks<CH == 0 ? 1 : CH> norm;
+    if constexpr (CH != 0) norm = nvr::load_norm<T, WHOLE, CH, WAVES>(t, lane, of_row);
+    for (int64_t row = first; row < t.rows; row += step) {
         uint8_t* out = q + row * pitch;
         auto put = [&](int j, uint2 eight) { *reinterpret_cast<uint2*>(out + j) = eight; };
-        const bool keep_sum = t.residual_out != nullptr;
-        nvr::RowStep step;
-        if constexpr (WAVES == 1) {
-            step = nvr::quantize_row<T, VEC, KEEP, kRowChunks, 1>(t, row, pitch, keep_sum, lane, 0, nvr::NoJoin{}, put);
-        } else {
-            step = nvr::quantize_row<T, VEC, KEEP, kRowChunks, WAVES>(t, row, pitch, keep_sum, lane, wave,
-                                                                     BlockJoin{sum, top, lane, wave}, put);
-        }
-        if (lane == 0 && (WAVES == 1 || wave == 0)) scales[row] = step.scale;
+        nvr::RowStep made;
+        if constexpr (CH != 0)
+            made = nvr::quantize_row<T, WHOLE, CH, WAVES>(t, row, nvr::load_row<T, WHOLE, CH, WAVES>(t, row, lane, of_row),
+                                                          norm, pitch, keep_sum, lane, of_row, join, put);
+        else
+            made = nvr::quantize_long_row<T, WHOLE>(t, row, pitch, keep_sum, lane, wave, join, put);
+        if (lane == 0 && of_row == 0) scales[row] = made.scale;
         if constexpr (WAVES != 1) __syncthreads();  // sum and top are read
     }
 }
 
-template <Tokens T, bool VEC>
+template <Tokens T, bool WHOLE>
 void launch(nv_context* c, const nvr::TokenArgs& t, uint8_t* q, float* scales, int pitch) {
-    constexpr int kWaveRow = kRowChunks * nvr::kWaveChunk, kBlockRow = 4 * kWaveRow;
-    constexpr int64_t kMostBlocks = 1 << 20;  // further rows are taken in turn
-    const int64_t quarter = (int64_t(t.rows) + 3) / 4;
-    const dim3 block(kThreads);
-    if (pitch <= kWaveRow && quarter >= c->cu_count)
-        hipLaunchKernelGGL((quantize_rows<T, VEC, true, 1>), dim3(unsigned(std::min(quarter, kMostBlocks))), block, 0,
-                           c->stream, t, q, scales, pitch);
-    else if (pitch <= kBlockRow)
-        hipLaunchKernelGGL((quantize_rows<T, VEC, true, 4>), dim3(unsigned(std::min<int64_t>(t.rows, kMostBlocks))), block,
-                           0, c->stream, t, q, scales, pitch);
-    else
-        hipLaunchKernelGGL((quantize_rows<T, VEC, false, 4>), dim3(unsigned(std::min<int64_t>(t.rows, kMostBlocks))), block,
-                           0, c->stream, t, q, scales, pitch);
+    const int cus = c->cu_count > 0 ? c->cu_count : 256;
+    const int64_t rows = t.rows;
+    auto run = [&](auto chunks, auto waves) {
+        constexpr int CH = decltype(chunks)::value, WAVES = decltype(waves)::value, kRows = kThreads / kWave / WAVES;
+        const int64_t blocks = std::min<int64_t>((rows + kRows - 1) / kRows, 1 << 20);  // further rows are taken in turn
+        hipLaunchKernelGGL((quantize_rows<T, WHOLE, CH, WAVES>), dim3(unsigned(blocks)), dim3(kThreads), 0, c->stream, t, q,
+                           scales, pitch);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 4> four;
+    const integral_constant<int, 0> any;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 8> eight;
+    if (rows >= 4 * cus && pitch <= 8 * nvr::kWaveChunk) {
+        if (pitch <= 2 * nvr::kWaveChunk) run(two, one);
+        else if (pitch <= 4 * nvr::kWaveChunk) run(four, one);
+        else run(eight, one);
+    } else {
+        const int chunk = 4 * nvr::kWaveChunk;
+        if (pitch <= chunk) run(one, four);
+        else if (pitch <= 2 * chunk) run(two, four);
+        else if (pitch <= 4 * chunk) run(four, four);
+        else if (pitch <= 8 * chunk) run(eight, four);
+        else run(any, four);
+    }
 }
 
 }  // namespace
 
 namespace nvr {
 
-bool tokens_aligned(const TokenArgs& t) {
-    return t.k % kChunk == 0 && aligned(t.x, 16) && aligned(t.residual, 16) && aligned(t.residual_out, 16) &&
-           aligned(t.norm_weight, 16);
-}
-
 void launch_quantize(nv_context* c, const TokenArgs& t, uint8_t* q, float* scales, int pitch) {
-    const bool vec = tokens_aligned(t);
     auto run = [&](auto tokens) {
         constexpr Tokens T = decltype(tokens)::value;
-        vec ? launch<T, true>(c, t, q, scales, pitch) : launch<T, false>(c, t, q, scales, pitch);
+        t.k % kChunk == 0 ? launch<T, true>(c, t, q, scales, pitch) : launch<T, false>(c, t, q, scales, pitch);
     };
     if (t.norm_weight == nullptr) run(std::integral_constant<Tokens, Tokens::kPlain>{});
     else if (t.residual == nullptr) run(std::integral_constant<Tokens, Tokens::kNorm>{});
