@@ -8,7 +8,6 @@ namespace {
 using nvr::kWave;
 using nvr::Scale;
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kXcds = 8;
 
@@ -18,27 +17,25 @@ template <int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
 struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
     static constexpr int WAVES = WM * WN, THREADS = WAVES * kWave;
-    static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 32, NI = TN / 32;  // a wave's products of 32 x 32
-    static constexpr int SUB = KB / 32;                                          // products' depths in a stage
+    static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;  // a wave's products of 16 x 16
+    static constexpr int SUB = KB / 64;                                          // products' depths of a stage
     static constexpr int PIECES = KB / 16, ROWS = kWave / PIECES;                // of a copy: pieces of a row, rows
     static constexpr int XR = BM / WAVES, WR = BN / WAVES;                       // rows that a wave copies
     static constexpr int COPIES = (XR + WR) / ROWS;                              // instructions of a wave a stage
     static constexpr int kStageBytes = (BM + BN) * KB;
-    static_assert(XR % ROWS == 0 && WR % ROWS == 0 && TM % 32 == 0 && TN % 32 == 0, "whole copies and products");
+    static_assert(XR % ROWS == 0 && WR % ROWS == 0 && TM % 16 == 0 && TN % 32 == 0, "whole copies and products");
     static_assert(STAGES * kStageBytes <= 160 * 1024 && (KB == 64 || KB == 128), "LDS");
 };
 
 // Waits until all but the last `late` stages' copies of this wave have landed.
 template <class S>
 __device__ __forceinline__ void wait_stages(int late) {
-    static_assert(S::STAGES <= 6 && (S::STAGES - 2) * S::COPIES < 64, "vmcnt");
-    switch (late) {
-        case 0: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
-        case 1: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(S::COPIES) : "memory"); break;
-        case 2: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * S::COPIES) : "memory"); break;
-        case 3: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * S::COPIES) : "memory"); break;
-        default: asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * S::COPIES) : "memory"); break;
-    }
+    constexpr int C = S::COPIES;
+    static_assert(S::STAGES <= 4 && (S::STAGES - 1) * C < 64, "vmcnt");
+    if (late == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else if (S::STAGES == 2 || late == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C) : "memory");
+    else if (S::STAGES == 3 || late == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(std::min(3 * C, 63)) : "memory");
 }
 
 // The tile of a block: neighbours in a group of 4 tiles of tokens share an XCD, so that the 32 blocks that run there
@@ -109,56 +106,68 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
         for (int u = 0; u < S::WR / S::ROWS; ++u) copy(wbase + step * S::KB, woff[u], dst + (S::BM + wave * S::WR + u * S::ROWS) * S::KB);
     };
 
-    // Operands: lane l has row l % 32, bytes 16 (l / 32) .. of each 32.
+    // Operands: lane l has row l % 16, bytes 16 (l / 16) .. of each 64.
     const int wm = wave % S::WM, wn = wave / S::WM;
-    const int read = lane % 32 * S::KB + place(lane % 32, lane / 32) * 16;
+    const int lane_at = lane % 16 * S::KB + place(lane % 16, lane / 16) * 16;
     auto operand = [&](const unsigned char* rows, int i, int ks) {
-        return *reinterpret_cast<const i32x4_t*>(rows + i * 32 * S::KB + (read ^ (ks << 5)));
+        return *reinterpret_cast<const i32x4_t*>(rows + i * 16 * S::KB + (lane_at ^ (ks << 6)));
     };
-    i32x16_t acc[S::NI][S::MI];
+    i32x4_t acc[S::NI][S::MI];
 #pragma unroll
     for (int i = 0; i < S::NI; ++i)
 #pragma unroll
-        for (int j = 0; j < S::MI; ++j) acc[i][j] = i32x16_t{};
+        for (int j = 0; j < S::MI; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+    // Operands of two depths: those of the next are read while the products of one are formed, a read before a product.
+    constexpr int READS = S::NI + S::MI, PRODUCTS = S::NI * S::MI;
     i32x4_t xf[2][S::MI], wf[2][S::NI];
-    auto fetch = [&](int slot, int buffer, int ks) {
-        const unsigned char* at = smem + buffer * S::kStageBytes;
-#pragma unroll
-        for (int i = 0; i < S::NI; ++i) wf[slot][i] = operand(at + (S::BM + wn * S::TN) * S::KB, i, ks);
-#pragma unroll
-        for (int j = 0; j < S::MI; ++j) xf[slot][j] = operand(at + wm * S::TM * S::KB, j, ks);
+    auto fetch = [&](int slot, const unsigned char* stage_at, int ks, int r) {  // the r-th operand
+        if (r == 0) wf[slot][0] = operand(stage_at + (S::BM + wn * S::TN) * S::KB, 0, ks);
+        else if (r <= S::MI) xf[slot][r - 1] = operand(stage_at + wm * S::TM * S::KB, r - 1, ks);
+        else wf[slot][r - S::MI] = operand(stage_at + (S::BM + wn * S::TN) * S::KB, r - S::MI, ks);
+    };
+    auto product = [&](int slot, int q) {
+        const int i = q / S::MI, j = q % S::MI;
+        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[slot][i], xf[slot][j], acc[i][j], 0, 0, 0);
     };
     for (int s = 0; s < S::STAGES && s < steps; ++s) stage(s, s);
     wait_stages<S>(min(steps, S::STAGES) - 1);
     asm volatile("s_barrier" ::: "memory");
-    fetch(0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < READS; ++r) fetch(0, smem, 0, r);
     int buffer = 0;
     for (int step = 0; step < steps; ++step) {
         const int next = buffer + 1 == S::STAGES ? 0 : buffer + 1;
 #pragma unroll
         for (int ks = 0; ks < S::SUB; ++ks) {
-            if (ks + 1 < S::SUB) {
-                fetch((ks + 1) & 1, buffer, ks + 1);
-            } else if (step + 1 < steps) {
-                // This stage is read and the next one here, in every wave: its place takes another.
-                wait_stages<S>(min(steps - 2 - step, S::STAGES - 2));
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (step + S::STAGES < steps) stage(step + S::STAGES, buffer);
-                fetch(0, next, 0);
+            const bool last = ks + 1 == S::SUB;
+            const int slot = ks & 1;
+            static_assert(S::SUB == 2, "slots");
+            const int first = last ? PRODUCTS / 2 : 0;
+            if (last) {
+#pragma unroll
+                for (int q = 0; q < first; ++q) product(slot, q);
+                __builtin_amdgcn_sched_barrier(0);
+                if (step + 1 < steps) {
+                    // This stage is read and the next one here, in every wave: its place takes another.
+                    wait_stages<S>(min(steps - 2 - step, S::STAGES - 2));
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (step + S::STAGES < steps) stage(step + S::STAGES, buffer);
+                }
             }
-            __builtin_amdgcn_sched_barrier(0);
+            // Behind the last stage: what lies in LDS is read and not used.
+            const unsigned char* at = smem + (last ? next : buffer) * S::kStageBytes;
 #pragma unroll
-            for (int i = 0; i < S::NI; ++i)
-#pragma unroll
-                for (int j = 0; j < S::MI; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[ks & 1][i], xf[ks & 1][j], acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < std::max(READS, PRODUCTS - first); ++q) {
+                if (q < READS) fetch(slot ^ 1, at, last ? 0 : ks + 1, q);
+                if (first + q < PRODUCTS) product(slot, first + q);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         buffer = next;
     }
 
-    // Lane l has token l % 32 of each 32, and channels 8 q + 4 (l / 32) + r, in its element 4 q + r. A wave brings its
-    // outputs through LDS, so that it stores rows of OUT channels.
+    // Lane l has token l % 16 of each 16, and channels 4 (l / 16) .. + 3 of each 16. A wave brings its outputs through LDS,
+    // so that it stores rows of OUT channels.
     constexpr int OUT = GATED ? S::TN / 2 : S::TN, UNITS = OUT / 8;
     static_assert(S::WAVES * S::TM * OUT * 2 <= S::STAGES * S::kStageBytes, "a wave's outputs");
     static_assert(UNITS == 4 || UNITS == 8, "banks");
@@ -171,42 +180,39 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     bool plain = true;
 #pragma unroll
     for (int j = 0; j < S::MI; ++j) {
-        xs[j] = p.xs[min(t0 + j * 32 + lane % 32, int64_t(p.m) - 1)];
+        xs[j] = p.xs[min(t0 + j * 16 + lane % 16, int64_t(p.m) - 1)];
         plain = plain && nvr::middling(xs[j]);
+    }
+    if (lane < OUT) {
+        plain = plain && nvr::middling(p.ws[min(c0 + lane, p.n - 1)]);
+        if constexpr (GATED) plain = plain && nvr::middling(p.ws[int64_t(p.n) + min(c0 + lane, p.n - 1)]);
     }
     auto outputs = [&](auto scale) {
 #pragma unroll
-        for (int i = 0; i < S::NI; i += GATED ? 2 : 1) {
+        for (int o = 0; o < OUT / 16; ++o) {
+            const int i = GATED ? o / 2 * 4 + o % 2 : o;  // gated: 32 rows of gate, 32 of up
+            const int at = o * 16 + 4 * (lane / 16);
+            float ws[4], us[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int at = (GATED ? i / 2 : i) * 32 + 8 * q + 4 * (lane / 32);
-                float ws[4], us[4];
+            for (int r = 0; r < 4; ++r) {
+                const int channel = min(c0 + at + r, p.n - 1);
+                ws[r] = p.ws[channel];
+                if constexpr (GATED) us[r] = p.ws[int64_t(p.n) + channel];
+            }
+#pragma unroll
+            for (int j = 0; j < S::MI; ++j) {
+                float y[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int channel = min(c0 + at + r, p.n - 1);
-                    ws[r] = p.ws[channel];
-                    if constexpr (GATED) us[r] = p.ws[int64_t(p.n) + channel];
+                    y[r] = scale(acc[i][j][r], xs[j], ws[r]);
+                    if constexpr (GATED) y[r] = nvr::silu_mul(y[r], scale(acc[i + 2][j][r], xs[j], us[r]));
                 }
-#pragma unroll
-                for (int j = 0; j < S::MI; ++j) {
-                    float y[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        y[r] = scale(acc[i][j][4 * q + r], xs[j], ws[r]);
-                        if constexpr (GATED) y[r] = nvr::silu_mul(y[r], scale(acc[i + 1][j][4 * q + r], xs[j], us[r]));
-                    }
-                    const int row = j * 32 + lane % 32;
-                    *reinterpret_cast<uint2*>(mine + row * (OUT * 2) + unit(row, at / 8) * 16 + lane / 32 * 8) =
-                        make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
-                }
+                const int row = j * 16 + lane % 16;
+                *reinterpret_cast<uint2*>(mine + row * (OUT * 2) + unit(row, at / 8) * 16 + at % 8 * 2) =
+                    make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
             }
         }
     };
-#pragma unroll 1
-    for (int c = lane; c < OUT; c += kWave) {
-        plain = plain && nvr::middling(p.ws[min(c0 + c, p.n - 1)]);
-        if constexpr (GATED) plain = plain && nvr::middling(p.ws[int64_t(p.n) + min(c0 + c, p.n - 1)]);
-    }
     if (__all(plain)) outputs([](int sum, float x, float w) { return float(sum) * x * w; });
     else outputs([](int sum, float x, float w) { return nvr::scaled(sum, nvr::split_scale(x), nvr::split_scale(w)); });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its own region only
@@ -227,6 +233,160 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     else store(uint16_t{});
 }
 
+// Fewer tokens: tiles of 64 tokens by 64 rows of the weight (gated: 32 of gate, 32 of up), a wave for every fourth unit of
+// 128 bytes of k. A wave copies and reads its units by itself, two in LDS, so the loop has no barrier; each byte of LDS is
+// read once, where four waves that share a tile's k would read it twice, and 16 products a read group cover its latency.
+constexpr int kSide = 64, kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
+constexpr int kSlotBytes = 2 * kSide * kUnitBytes, kSplitLds = kSplit * 2 * kSlotBytes;
+
+template <bool GATED>
+__global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, int mt, int nt) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int2 tile = tile_of(blockIdx.x, gridDim.x, mt, nt);
+    const int64_t m0 = int64_t(tile.x) * kSide;
+    const int n0 = tile.y * (GATED ? kSide / 2 : kSide);  // < n
+    const int units = (p.w_pitch + kUnitBytes - 1) / kUnitBytes;  // x holds zeros to the end of the last
+    const int mine = (units - wave + kSplit - 1) / kSplit;        // wave, wave + 4, ...
+
+    // A copy brings 8 rows of 128 bytes; the piece c of row r goes to place c ^ (r / 2 % 8), as in gemm_tiles.
+    auto place = [](int r, int c) { return c ^ (r / 2 % 8); };
+    constexpr int kCopies = kSide / 8;
+    uint32_t xoff[kCopies], woff[kCopies];
+#pragma unroll
+    for (int u = 0; u < kCopies; ++u) {
+        const int r = u * 8 + lane / 8, piece = place(r, lane % 8);
+        xoff[u] = uint32_t(min(m0 + r, int64_t(p.m) - 1) - m0) * uint32_t(p.x_pitch) + piece * 16;
+        woff[u] = uint32_t(min(n0 + (GATED ? r % 32 : r), p.n - 1) - n0) * uint32_t(p.w_pitch) + piece * 16;
+    }
+    const uint8_t* xbase = p.xq + m0 * p.x_pitch;
+    const uint8_t* wbase = p.wq + int64_t(n0) * p.w_pitch;
+    const uint8_t* ubase = GATED ? wbase + int64_t(p.n) * p.w_pitch : wbase;  // of the tile's upper 32 rows
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem)) + wave * (2 * kSlotBytes);
+    // Four copies to places of 1 KB side by side; inline asm for the reasons given in gemm_tiles.
+    auto copy4 = [&](const uint8_t* base, const uint32_t* off, uint32_t dst) {
+        uint32_t saved;
+        asm volatile(
+            "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\t"
+            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
+            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %1\n\t"
+            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\ts_mov_b32 m0, %0"
+            : "=&s"(saved)
+            : "s"(base), "s"(dst), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3])
+            : "memory", "scc");
+    };
+    auto copy = [&](int i) {  // this wave's i-th unit
+        const int k = (wave + i * kSplit) * kUnitBytes;
+        const uint32_t dst = lds + (i & 1) * kSlotBytes;
+        const int past = p.w_pitch - 16 - k;
+        if (past < kUnitBytes - 16) {  // past its row a weight's bytes meet zeros of x: any bytes of the row will do
+#pragma unroll
+            for (int u = 0; u < kCopies; ++u) woff[u] -= max(place(u * 8 + lane / 8, lane % 8) * 16 - past, 0);
+        }
+        copy4(xbase + k, xoff, dst);
+        copy4(xbase + k, xoff + 4, dst + 4096);
+        copy4(wbase + k, woff, dst + 8192);
+        copy4(ubase + k, woff + 4, dst + 12288);
+    };
+    const int lane_at = lane % 16 * kUnitBytes + place(lane % 16, lane / 16) * 16;
+    const unsigned char* ring = smem + wave * (2 * kSlotBytes);
+    struct Operands {
+        i32x4_t x[4], w[4];
+    };
+    auto fetch = [&](Operands& o, int i, int ks) {
+        const unsigned char* at = ring + (i & 1) * kSlotBytes + (lane_at ^ (ks << 6));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o.x[j] = *reinterpret_cast<const i32x4_t*>(at + j * 2048);
+            o.w[j] = *reinterpret_cast<const i32x4_t*>(at + 8192 + j * 2048);
+        }
+    };
+    i32x4_t acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+    auto products = [&](const Operands& o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[i], o.x[j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto landed = [&](bool another) {  // this wave's copies, but those of one unit behind them
+        if (another) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopies) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    };
+    Operands a, b;
+    if (mine > 0) {
+        copy(0);
+        if (mine > 1) copy(1);
+        landed(mine > 1);
+        fetch(a, 0, 0);
+        for (int i = 0; i < mine; ++i) {
+            fetch(b, i, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            products(a);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the unit is read
+            if (i + 2 < mine) copy(i + 2);
+            if (i + 1 < mine) {
+                landed(i + 2 < mine);
+                fetch(a, i + 1, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            products(b);
+        }
+    }
+    // The waves' sums: each wave takes 16 of the tokens.
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    i32x4_t* sums = reinterpret_cast<i32x4_t*>(smem) + lane;  // [wave][16 tokens][16 rows][64]
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[((wave * 4 + j) * 4 + i) * kWave] = acc[i][j];
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    i32x4_t sum[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum[i] = sums[(wave * 4 + i) * kWave];
+#pragma unroll
+        for (int v = 1; v < kSplit; ++v) sum[i] += sums[((v * 4 + wave) * 4 + i) * kWave];
+    }
+    const int64_t token = m0 + wave * 16 + lane % 16;
+    if (token >= p.m) return;
+    const Scale xs = nvr::split_scale(p.xs[token]);
+    const bool pieces = p.n % 4 == 0 && nvr::aligned(p.y, 8);
+#pragma unroll
+    for (int i = 0; i < (GATED ? 2 : 4); ++i) {
+        const int channel = n0 + i * 16 + 4 * (lane / 16);
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int c = min(channel + r, p.n - 1);
+            y[r] = nvr::scaled(sum[i][r], xs, nvr::split_scale(p.ws[c]));
+            if constexpr (GATED)
+                y[r] = nvr::silu_mul(y[r], nvr::scaled(sum[i + 2][r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+        }
+        uint16_t* out = p.y + token * p.n + channel;
+        if (pieces) {
+            if (channel < p.n)
+                *reinterpret_cast<uint2*>(out) = make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (channel + r < p.n) out[r] = nvr::f32_to_bf16(y[r]);
+        }
+    }
+}
+
+template <bool GATED>
+void launch_split(nv_context* c, const nvr::ProductArgs& p) {
+    constexpr int kChannels = GATED ? kSide / 2 : kSide;
+    const int mt = int((int64_t(p.m) + kSide - 1) / kSide), nt = (p.n + kChannels - 1) / kChannels;
+    hipLaunchKernelGGL((gemm_split<GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplitLds, c->stream, p,
+                       mt, nt);
+}
+
 template <class S, bool GATED>
 void launch(nv_context* c, const nvr::ProductArgs& p) {
     constexpr int kChannels = GATED ? S::BN / 2 : S::BN;
@@ -241,11 +401,12 @@ namespace nvr {
 
 void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
     using Large = Shape<256, 256, 2, 4, 128, 2>;
-    using Small = Shape<128, 128, 2, 2, 128, 2>;
+    using Medium = Shape<128, 256, 2, 4, 128, 2>;
     const int channels = gated ? 2 * p.n : p.n;
     const int64_t large = ((int64_t(p.m) + 255) / 256) * ((int64_t(channels) + 255) / 256);
     if (large >= c->cu_count) gated ? launch<Large, true>(c, p) : launch<Large, false>(c, p);
-    else gated ? launch<Small, true>(c, p) : launch<Small, false>(c, p);
+    else if (p.m > 1024) gated ? launch<Medium, true>(c, p) : launch<Medium, false>(c, p);
+    else gated ? launch_split<true>(c, p) : launch_split<false>(c, p);
 }
 
 }  // namespace nvr
