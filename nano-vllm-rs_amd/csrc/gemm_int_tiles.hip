@@ -233,88 +233,92 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     else store(uint16_t{});
 }
 
-// Fewer tokens: tiles of 64 tokens by 64 rows of the weight (gated: 32 of gate, 32 of up), a wave for every fourth unit of
-// 128 bytes of k. A wave copies and reads its units by itself, two in LDS, so the loop has no barrier; each byte of LDS is
-// read once, where four waves that share a tile's k would read it twice, and 16 products a read group cover its latency.
-constexpr int kSide = 64, kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
-constexpr int kSlotBytes = 2 * kSide * kUnitBytes, kSplitLds = kSplit * 2 * kSlotBytes;
+// Fewer tokens: tiles of 64 tokens by SIDE rows of the weight (gated: half of gate, half of up), a wave for every fourth
+// unit of 128 bytes of k. A wave copies and reads its units by itself, two in LDS, so the loop has no barrier; each byte of LDS is
+// read once, where four waves that share a tile's k would read it twice, and a group's products cover the next one's reads.
+constexpr int kTokens = 64, kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
+template <int SIDE>
+constexpr int kSlotBytes = (kTokens + SIDE) * kUnitBytes;
 
-template <bool GATED>
+template <int SIDE, bool GATED>
 __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, int mt, int nt) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int2 tile = tile_of(blockIdx.x, gridDim.x, mt, nt);
-    const int64_t m0 = int64_t(tile.x) * kSide;
-    const int n0 = tile.y * (GATED ? kSide / 2 : kSide);  // < n
+    const int64_t m0 = int64_t(tile.x) * kTokens;
+    const int n0 = tile.y * (GATED ? SIDE / 2 : SIDE);  // < n
+    constexpr int NI = SIDE / 16, SLOT = kSlotBytes<SIDE>;
     const int units = (p.w_pitch + kUnitBytes - 1) / kUnitBytes;  // x holds zeros to the end of the last
     const int mine = (units - wave + kSplit - 1) / kSplit;        // wave, wave + 4, ...
 
     // A copy brings 8 rows of 128 bytes; the piece c of row r goes to place c ^ (r / 2 % 8), as in gemm_tiles.
     auto place = [](int r, int c) { return c ^ (r / 2 % 8); };
-    constexpr int kCopies = kSide / 8;
-    uint32_t xoff[kCopies], woff[kCopies];
+    constexpr int XC = kTokens / 8, WC = SIDE / 8;
+    uint32_t xoff[XC], woff[WC];
 #pragma unroll
-    for (int u = 0; u < kCopies; ++u) {
-        const int r = u * 8 + lane / 8, piece = place(r, lane % 8);
-        xoff[u] = uint32_t(min(m0 + r, int64_t(p.m) - 1) - m0) * uint32_t(p.x_pitch) + piece * 16;
-        woff[u] = uint32_t(min(n0 + (GATED ? r % 32 : r), p.n - 1) - n0) * uint32_t(p.w_pitch) + piece * 16;
+    for (int u = 0; u < XC; ++u) {
+        const int r = u * 8 + lane / 8;
+        xoff[u] = uint32_t(min(m0 + r, int64_t(p.m) - 1) - m0) * uint32_t(p.x_pitch) + place(r, lane % 8) * 16;
+    }
+#pragma unroll
+    for (int u = 0; u < WC; ++u) {
+        const int r = u * 8 + lane / 8;
+        woff[u] = uint32_t(min(n0 + (GATED ? r % (SIDE / 2) : r), p.n - 1) - n0) * uint32_t(p.w_pitch) + place(r, lane % 8) * 16;
     }
     const uint8_t* xbase = p.xq + m0 * p.x_pitch;
     const uint8_t* wbase = p.wq + int64_t(n0) * p.w_pitch;
-    const uint8_t* ubase = GATED ? wbase + int64_t(p.n) * p.w_pitch : wbase;  // of the tile's upper 32 rows
-    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem)) + wave * (2 * kSlotBytes);
-    // Four copies to places of 1 KB side by side; inline asm for the reasons given in gemm_tiles.
-    auto copy4 = [&](const uint8_t* base, const uint32_t* off, uint32_t dst) {
+    const uint8_t* ubase = GATED ? wbase + int64_t(p.n) * p.w_pitch : wbase;  // of the tile's upper half
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem)) + wave * (2 * SLOT);
+    // Two copies to places of 1 KB side by side; inline asm for the reasons given in gemm_tiles.
+    auto copy2 = [&](const uint8_t* base, uint32_t off0, uint32_t off1, uint32_t dst) {
         uint32_t saved;
         asm volatile(
             "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\t"
-            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %1\n\t"
-            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %1\n\t"
-            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %1\n\ts_mov_b32 m0, %0"
+            "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %1\n\ts_mov_b32 m0, %0"
             : "=&s"(saved)
-            : "s"(base), "s"(dst), "v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3])
+            : "s"(base), "s"(dst), "v"(off0), "v"(off1)
             : "memory", "scc");
     };
     auto copy = [&](int i) {  // this wave's i-th unit
         const int k = (wave + i * kSplit) * kUnitBytes;
-        const uint32_t dst = lds + (i & 1) * kSlotBytes;
+        const uint32_t dst = lds + (i & 1) * SLOT;
         const int past = p.w_pitch - 16 - k;
         if (past < kUnitBytes - 16) {  // past its row a weight's bytes meet zeros of x: any bytes of the row will do
 #pragma unroll
-            for (int u = 0; u < kCopies; ++u) woff[u] -= max(place(u * 8 + lane / 8, lane % 8) * 16 - past, 0);
+            for (int u = 0; u < WC; ++u) woff[u] -= max(place(u * 8 + lane / 8, lane % 8) * 16 - past, 0);
         }
-        copy4(xbase + k, xoff, dst);
-        copy4(xbase + k, xoff + 4, dst + 4096);
-        copy4(wbase + k, woff, dst + 8192);
-        copy4(ubase + k, woff + 4, dst + 12288);
+#pragma unroll
+        for (int u = 0; u < XC; u += 2) copy2(xbase + k, xoff[u], xoff[u + 1], dst + u * 1024);
+#pragma unroll
+        for (int u = 0; u < WC; u += 2)
+            copy2((u < WC / 2 ? wbase : ubase) + k, woff[u], woff[u + 1], dst + (XC + u) * 1024);
     };
     const int lane_at = lane % 16 * kUnitBytes + place(lane % 16, lane / 16) * 16;
-    const unsigned char* ring = smem + wave * (2 * kSlotBytes);
+    const unsigned char* ring = smem + wave * (2 * SLOT);
     struct Operands {
-        i32x4_t x[4], w[4];
+        i32x4_t x[4], w[NI];
     };
     auto fetch = [&](Operands& o, int i, int ks) {
-        const unsigned char* at = ring + (i & 1) * kSlotBytes + (lane_at ^ (ks << 6));
+        const unsigned char* at = ring + (i & 1) * SLOT + (lane_at ^ (ks << 6));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o.x[j] = *reinterpret_cast<const i32x4_t*>(at + j * 2048);
-            o.w[j] = *reinterpret_cast<const i32x4_t*>(at + 8192 + j * 2048);
-        }
+        for (int j = 0; j < 4; ++j) o.x[j] = *reinterpret_cast<const i32x4_t*>(at + j * 2048);
+#pragma unroll
+        for (int i16 = 0; i16 < NI; ++i16) o.w[i16] = *reinterpret_cast<const i32x4_t*>(at + (4 + i16) * 2048);
     };
-    i32x4_t acc[4][4];
+    i32x4_t acc[NI][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
     auto products = [&](const Operands& o) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NI; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[i], o.x[j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
     auto landed = [&](bool another) {  // this wave's copies, but those of one unit behind them
-        if (another) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopies) : "memory");
+        if (another) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XC + WC) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
     Operands a, b;
@@ -343,21 +347,21 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[((wave * 4 + j) * 4 + i) * kWave] = acc[i][j];
+        for (int i = 0; i < NI; ++i) sums[((wave * 4 + j) * NI + i) * kWave] = acc[i][j];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    i32x4_t sum[4];
+    i32x4_t sum[NI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        sum[i] = sums[(wave * 4 + i) * kWave];
+    for (int i = 0; i < NI; ++i) {
+        sum[i] = sums[(wave * NI + i) * kWave];
 #pragma unroll
-        for (int v = 1; v < kSplit; ++v) sum[i] += sums[((v * 4 + wave) * 4 + i) * kWave];
+        for (int v = 1; v < kSplit; ++v) sum[i] += sums[((v * 4 + wave) * NI + i) * kWave];
     }
     const int64_t token = m0 + wave * 16 + lane % 16;
     if (token >= p.m) return;
     const Scale xs = nvr::split_scale(p.xs[token]);
     const bool pieces = p.n % 4 == 0 && nvr::aligned(p.y, 8);
 #pragma unroll
-    for (int i = 0; i < (GATED ? 2 : 4); ++i) {
+    for (int i = 0; i < (GATED ? NI / 2 : NI); ++i) {
         const int channel = n0 + i * 16 + 4 * (lane / 16);
         float y[4];
 #pragma unroll
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
             const int c = min(channel + r, p.n - 1);
             y[r] = nvr::scaled(sum[i][r], xs, nvr::split_scale(p.ws[c]));
             if constexpr (GATED)
-                y[r] = nvr::silu_mul(y[r], nvr::scaled(sum[i + 2][r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+                y[r] = nvr::silu_mul(y[r], nvr::scaled(sum[i + NI / 2][r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
         }
         uint16_t* out = p.y + token * p.n + channel;
         if (pieces) {
@@ -379,11 +383,11 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     }
 }
 
-template <bool GATED>
+template <int SIDE, bool GATED>
 void launch_split(nv_context* c, const nvr::ProductArgs& p) {
-    constexpr int kChannels = GATED ? kSide / 2 : kSide;
-    const int mt = int((int64_t(p.m) + kSide - 1) / kSide), nt = (p.n + kChannels - 1) / kChannels;
-    hipLaunchKernelGGL((gemm_split<GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplitLds, c->stream, p,
+    constexpr int kChannels = GATED ? SIDE / 2 : SIDE;
+    const int mt = int((int64_t(p.m) + kTokens - 1) / kTokens), nt = (p.n + kChannels - 1) / kChannels;
+    hipLaunchKernelGGL((gemm_split<SIDE, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplit * 2 * kSlotBytes<SIDE>, c->stream, p,
                        mt, nt);
 }
 
@@ -401,12 +405,14 @@ namespace nvr {
 
 void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
     using Large = Shape<256, 256, 2, 4, 128, 2>;
-    using Medium = Shape<128, 256, 2, 4, 128, 2>;
-    const int channels = gated ? 2 * p.n : p.n;
-    const int64_t large = ((int64_t(p.m) + 255) / 256) * ((int64_t(channels) + 255) / 256);
-    if (large >= c->cu_count) gated ? launch<Large, true>(c, p) : launch<Large, false>(c, p);
-    else if (p.m > 1024) gated ? launch<Medium, true>(c, p) : launch<Medium, false>(c, p);
-    else gated ? launch_split<true>(c, p) : launch_split<false>(c, p);
+    using Medium = Shape<128, 128, 4, 2, 128, 2>;
+    const int64_t cus = c->cu_count > 0 ? c->cu_count : 256, rows = gated ? 2 * int64_t(p.n) : p.n;
+    auto tiles = [&](int tokens, int side) { return (int64_t(p.m) + tokens - 1) / tokens * ((rows + side - 1) / side); };
+    auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
+    if (tiles(kTokens, 32) <= cus) gated ? launch_split<32, true>(c, p) : launch_split<32, false>(c, p);
+    else if (tiles(kTokens, 64) <= cus) gated ? launch_split<64, true>(c, p) : launch_split<64, false>(c, p);
+    else if (3 * turns(tiles(256, 256)) > turns(tiles(128, 128))) gated ? launch<Medium, true>(c, p) : launch<Medium, false>(c, p);
+    else gated ? launch<Large, true>(c, p) : launch<Large, false>(c, p);
 }
 
 }  // namespace nvr
