@@ -30,8 +30,8 @@ constexpr int kFewTokens = 32;
 constexpr int kMostLds = 160 * 1024;
 
 // Where the tokens' integers come from: made by each block (of x, the norm, or the norm of the sum), or by a launch of
-// quantize_rows, and then brought to LDS, or read where they are used.
-enum class Source { kPlain, kNorm, kAddNorm, kCopied, kMemory };
+// quantize_rows and brought to LDS.
+enum class Source { kPlain, kNorm, kAddNorm, kCopied };
 
 struct RowsArgs {
     nvr::ProductArgs p;
@@ -44,15 +44,15 @@ struct RowsArgs {
 // LDS of a block: partial sums (parts > 1), scales, tokens.
 template <int MT>
 constexpr int kSumBytes = 2 * kWaves * MT * kWave * 16;
-template <Source SRC, int MT>
+template <int MT>
 int64_t rows_lds(int m, int x_pitch) {
-    return kSumBytes<MT> + MT * 16 * 4 + (SRC == Source::kMemory ? 0 : int64_t(m) * (x_pitch + kRowPad));
+    return kSumBytes<MT> + MT * 16 * 4 + int64_t(m) * (x_pitch + kRowPad);
 }
 
 // Few tokens: the weights stream through registers, once. ONE: every wave has one unit at most in all.
 template <Source SRC, int CH, int MT, bool GATED, bool ONE>
 __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
-    constexpr bool kMade = SRC != Source::kCopied && SRC != Source::kMemory;
+    constexpr bool kMade = SRC != Source::kCopied;
     constexpr int kChannels = GATED ? 8 : 16;  // of a tile: 16 rows of the weight, or 8 of gate, then 8 of up
     extern __shared__ __align__(16) unsigned char smem[];
     const nvr::ProductArgs& p = a.p;
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     i32x4_t* red = reinterpret_cast<i32x4_t*>(smem);                   // [2][kWaves][MT][64]
     float* xs = reinterpret_cast<float*>(smem + kSumBytes<MT>);        // [MT * 16]
     unsigned char* xq = reinterpret_cast<unsigned char*>(xs + MT * 16);  // [m][pitch]
-    const int pitch = SRC == Source::kMemory ? p.x_pitch : p.x_pitch + kRowPad;
+    const int pitch = p.x_pitch + kRowPad;
 
     // The weights of a unit: lane l has row l % 16, 16 bytes at 16 (l / 16) of each step. Behind a row's end, where x is
     // zero, and behind the wave's steps, which are not multiplied, any bytes of the row will do.
@@ -114,13 +114,11 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         }
     } else {
         load(unit[0]);
-        if constexpr (SRC == Source::kCopied) {
-            for (int row = wave; row < p.m; row += kWaves)
+        for (int row = wave; row < p.m; row += kWaves)
 #pragma unroll 4
-                for (int c = lane * 16; c < p.x_pitch; c += kWave * 16)
-                    *reinterpret_cast<uint4*>(xq + row * pitch + c) =
-                        *reinterpret_cast<const uint4*>(p.xq + int64_t(row) * p.x_pitch + c);
-        }
+            for (int c = lane * 16; c < p.x_pitch; c += kWave * 16)
+                *reinterpret_cast<uint4*>(xq + row * pitch + c) =
+                    *reinterpret_cast<const uint4*>(p.xq + int64_t(row) * p.x_pitch + c);
         if (int(threadIdx.x) < p.m) xs[threadIdx.x] = p.xs[threadIdx.x];
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // leaves the weights in flight
@@ -130,7 +128,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     const unsigned char* xrow[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-        xrow[t] = (SRC == Source::kMemory ? p.xq : xq) + int64_t(min(t * 16 + i, p.m - 1)) * pitch + 16 * g;
+        xrow[t] = xq + min(t * 16 + i, p.m - 1) * pitch + 16 * g;
     i32x4_t acc[MT];
     float ws[4];
     // A wave that has its tiles to itself, and several, keeps its outputs until they fill lines of 128 bytes.
@@ -270,7 +268,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
 template <Source SRC, int CH, int MT, bool GATED, bool ONE>
 void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
     hipLaunchKernelGGL((gemm_rows_i8<SRC, CH, MT, GATED, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
-                       size_t(rows_lds<SRC, MT>(a.p.m, a.p.x_pitch)), c->stream, a);
+                       size_t(rows_lds<MT>(a.p.m, a.p.x_pitch)), c->stream, a);
 }
 
 void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
@@ -299,7 +297,7 @@ void launch_rows(nv_context* c, RowsArgs a) {
     };
     using std::integral_constant;
     const integral_constant<int, 1> one16;
-    if constexpr (SRC == Source::kCopied || SRC == Source::kMemory) {
+    if constexpr (SRC == Source::kCopied) {
         if (a.p.m <= 16) run(integral_constant<int, 1>{}, one16);
         else run(integral_constant<int, 1>{}, integral_constant<int, 2>{});
     } else {
@@ -316,6 +314,16 @@ void launch_rows(nv_context* c, RowsArgs a) {
 // 6.7, 7.5 and 8.0, 7.8; at k 2048 8.1, 8.1 and 10.9, 8.4.
 bool tokens_in_block(const nvr::TokenArgs& t) {
     return t.rows <= kWaves && t.k % nvr::kChunk == 0 && t.k <= (t.norm_weight == nullptr ? 8 : 4) * nvr::kWaveChunk;
+}
+
+// Whether few tokens, made by a launch of their own, take gemm_rows_i8: where a CU would have more than two of
+// gemm_split's tiles in turn and the tokens fit LDS. On MI355X, this and that in us: 16 tokens at k 1024 over n 8192 5.6,
+// 3.9; 16384 6.0, 5.1; 32768 9.6, 10.2; at k 4096 over 8192 11.2, 9.4; 16384 16.7, 19.2; 32768 26.7, 33.1; 32 tokens over
+// 151936 x 1024 37.8, 41.8.
+bool weight_streams(const nv_context* c, const nvr::ProductArgs& p, bool gated) {
+    const int64_t rows = gated ? 2 * int64_t(p.n) : p.n, cus = c->cu_count > 0 ? c->cu_count : 256;
+    return p.m <= kFewTokens && (rows + 31) / 32 > 2 * cus &&
+           (p.m <= 16 ? rows_lds<1>(p.m, p.x_pitch) : rows_lds<2>(p.m, p.x_pitch)) <= kMostLds;
 }
 
 constexpr int kStepBytes = 128;  // tokens' rows in the workspace end in zeros at a multiple of this
@@ -359,17 +367,15 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     const nvr::ProductArgs p{xq, xs, static_cast<const uint8_t*>(w), static_cast<const float*>(w_scales),
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
     const RowsArgs few{p, t, 0, 0, 0, 0, 0, 0};
-    if (m <= kFewTokens && tokens_in_block(t)) {
+    if (tokens_in_block(t)) {
         if (norm_weight == nullptr) launch_rows<Source::kPlain, GATED>(c, few);
         else if (residual == nullptr) launch_rows<Source::kNorm, GATED>(c, few);
         else launch_rows<Source::kAddNorm, GATED>(c, few);
         return nvr::launch_status();
     }
     nvr::launch_quantize(c, t, xq, xs, pitch);
-    if (m > kFewTokens) nvr::launch_product_tiles(c, p, GATED);
-    else if ((m <= 16 ? rows_lds<Source::kCopied, 1>(m, pitch) : rows_lds<Source::kCopied, 2>(m, pitch)) <= kMostLds)
-        launch_rows<Source::kCopied, GATED>(c, few);
-    else launch_rows<Source::kMemory, GATED>(c, few);
+    if (weight_streams(c, p, GATED)) launch_rows<Source::kCopied, GATED>(c, few);
+    else nvr::launch_product_tiles(c, p, GATED);
     return nvr::launch_status();
 }
 

@@ -233,27 +233,25 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     else store(uint16_t{});
 }
 
-// Fewer tokens: tiles of 64 tokens by SIDE rows of the weight (gated: half of gate, half of up), a wave for every fourth
+// Fewer tokens: tiles of TOK tokens by SIDE rows of the weight (gated: half of gate, half of up), a wave for every fourth
 // unit of 128 bytes of k. A wave copies and reads its units by itself, two in LDS, so the loop has no barrier; each byte of LDS is
 // read once, where four waves that share a tile's k would read it twice, and a group's products cover the next one's reads.
-constexpr int kTokens = 64, kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
-template <int SIDE>
-constexpr int kSlotBytes = (kTokens + SIDE) * kUnitBytes;
+constexpr int kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
 
-template <int SIDE, bool GATED>
+template <int TOK, int SIDE, int SLOTS, bool GATED>
 __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, int mt, int nt) {
     extern __shared__ __align__(16) unsigned char smem[];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int2 tile = tile_of(blockIdx.x, gridDim.x, mt, nt);
-    const int64_t m0 = int64_t(tile.x) * kTokens;
+    const int64_t m0 = int64_t(tile.x) * TOK;
     const int n0 = tile.y * (GATED ? SIDE / 2 : SIDE);  // < n
-    constexpr int NI = SIDE / 16, SLOT = kSlotBytes<SIDE>;
+    constexpr int NI = SIDE / 16, MJ = TOK / 16, SLOT = (TOK + SIDE) * kUnitBytes;
     const int units = (p.w_pitch + kUnitBytes - 1) / kUnitBytes;  // x holds zeros to the end of the last
     const int mine = (units - wave + kSplit - 1) / kSplit;        // wave, wave + 4, ...
 
     // A copy brings 8 rows of 128 bytes; the piece c of row r goes to place c ^ (r / 2 % 8), as in gemm_tiles.
     auto place = [](int r, int c) { return c ^ (r / 2 % 8); };
-    constexpr int XC = kTokens / 8, WC = SIDE / 8;
+    constexpr int XC = TOK / 8, WC = SIDE / 8;
     uint32_t xoff[XC], woff[WC];
 #pragma unroll
     for (int u = 0; u < XC; ++u) {
@@ -268,7 +266,7 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     const uint8_t* xbase = p.xq + m0 * p.x_pitch;
     const uint8_t* wbase = p.wq + int64_t(n0) * p.w_pitch;
     const uint8_t* ubase = GATED ? wbase + int64_t(p.n) * p.w_pitch : wbase;  // of the tile's upper half
-    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem)) + wave * (2 * SLOT);
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(nvr::lds_address(smem)) + wave * (SLOTS * SLOT);
     // Two copies to places of 1 KB side by side; inline asm for the reasons given in gemm_tiles.
     auto copy2 = [&](const uint8_t* base, uint32_t off0, uint32_t off1, uint32_t dst) {
         uint32_t saved;
@@ -281,7 +279,7 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     };
     auto copy = [&](int i) {  // this wave's i-th unit
         const int k = (wave + i * kSplit) * kUnitBytes;
-        const uint32_t dst = lds + (i & 1) * SLOT;
+        const uint32_t dst = lds + i % SLOTS * SLOT;
         const int past = p.w_pitch - 16 - k;
         if (past < kUnitBytes - 16) {  // past its row a weight's bytes meet zeros of x: any bytes of the row will do
 #pragma unroll
@@ -294,83 +292,90 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
             copy2((u < WC / 2 ? wbase : ubase) + k, woff[u], woff[u + 1], dst + (XC + u) * 1024);
     };
     const int lane_at = lane % 16 * kUnitBytes + place(lane % 16, lane / 16) * 16;
-    const unsigned char* ring = smem + wave * (2 * SLOT);
+    const unsigned char* ring = smem + wave * (SLOTS * SLOT);
     struct Operands {
-        i32x4_t x[4], w[NI];
+        i32x4_t x[MJ], w[NI];
     };
     auto fetch = [&](Operands& o, int i, int ks) {
-        const unsigned char* at = ring + (i & 1) * SLOT + (lane_at ^ (ks << 6));
+        const unsigned char* at = ring + i % SLOTS * SLOT + (lane_at ^ (ks << 6));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o.x[j] = *reinterpret_cast<const i32x4_t*>(at + j * 2048);
+        for (int j = 0; j < MJ; ++j) o.x[j] = *reinterpret_cast<const i32x4_t*>(at + j * 2048);
 #pragma unroll
-        for (int i16 = 0; i16 < NI; ++i16) o.w[i16] = *reinterpret_cast<const i32x4_t*>(at + (4 + i16) * 2048);
+        for (int i16 = 0; i16 < NI; ++i16) o.w[i16] = *reinterpret_cast<const i32x4_t*>(at + (MJ + i16) * 2048);
     };
-    i32x4_t acc[NI][4];
+    i32x4_t acc[NI][MJ];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
+        for (int j = 0; j < MJ; ++j) acc[i][j] = i32x4_t{0, 0, 0, 0};
     auto products = [&](const Operands& o) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[i], o.x[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < MJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.w[i], o.x[j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto landed = [&](bool another) {  // this wave's copies, but those of one unit behind them
-        if (another) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(XC + WC) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto landed = [&](int late) {  // this wave's copies, but those of the last `late` units
+        constexpr int C = XC + WC;
+        static_assert(SLOTS <= 4 && 3 * C < 64, "vmcnt");
+        if (late == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        else if (SLOTS == 2 || late == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C) : "memory");
+        else if (SLOTS == 3 || late == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * C) : "memory");
     };
     Operands a, b;
     if (mine > 0) {
-        copy(0);
-        if (mine > 1) copy(1);
-        landed(mine > 1);
+        for (int i = 0; i < SLOTS && i < mine; ++i) copy(i);
+        landed(min(mine, SLOTS) - 1);
         fetch(a, 0, 0);
         for (int i = 0; i < mine; ++i) {
             fetch(b, i, 1);
             __builtin_amdgcn_sched_barrier(0);
             products(a);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the unit is read
-            if (i + 2 < mine) copy(i + 2);
+            if (i + SLOTS < mine) copy(i + SLOTS);
             if (i + 1 < mine) {
-                landed(i + 2 < mine);
+                landed(min(mine - i - 2, SLOTS - 1));
                 fetch(a, i + 1, 0);
             }
             __builtin_amdgcn_sched_barrier(0);
             products(b);
         }
     }
-    // The waves' sums: each wave takes 16 of the tokens.
+    // The waves' sums, of 16 tokens by 16 rows (gated: and the 16 of up), each in one wave.
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     i32x4_t* sums = reinterpret_cast<i32x4_t*>(smem) + lane;  // [wave][16 tokens][16 rows][64]
+    static_assert(MJ * NI * kWave * 16 <= SLOTS * SLOT, "its place");
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < MJ; ++j)
 #pragma unroll
-        for (int i = 0; i < NI; ++i) sums[((wave * 4 + j) * NI + i) * kWave] = acc[i][j];
+        for (int i = 0; i < NI; ++i) sums[((wave * MJ + j) * NI + i) * kWave] = acc[i][j];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    i32x4_t sum[NI];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        sum[i] = sums[(wave * NI + i) * kWave];
-#pragma unroll
-        for (int v = 1; v < kSplit; ++v) sum[i] += sums[((v * 4 + wave) * NI + i) * kWave];
-    }
-    const int64_t token = m0 + wave * 16 + lane % 16;
-    if (token >= p.m) return;
-    const Scale xs = nvr::split_scale(p.xs[token]);
     const bool pieces = p.n % 4 == 0 && nvr::aligned(p.y, 8);
+    constexpr int OI = GATED ? NI / 2 : NI;  // a token's 16 channels
 #pragma unroll
-    for (int i = 0; i < (GATED ? NI / 2 : NI); ++i) {
+    for (int at = 0; at < MJ * OI; at += kSplit) {
+        const int q = at + wave, j = q / OI, i = q % OI;
+        if (q >= MJ * OI) break;
+        auto whole = [&](int row16) {
+            i32x4_t part[kSplit];
+#pragma unroll
+            for (int v = 0; v < kSplit; ++v) part[v] = sums[((v * MJ + j) * NI + row16) * kWave];
+            return part[0] + part[1] + (part[2] + part[3]);
+        };
+        static_assert(kSplit == 4, "whole");
+        const i32x4_t sum = whole(i), up = GATED ? whole(i + NI / 2) : sum;
+        const int64_t token = m0 + j * 16 + lane % 16;
         const int channel = n0 + i * 16 + 4 * (lane / 16);
+        const Scale xs = nvr::split_scale(p.xs[min(token, int64_t(p.m) - 1)]);
         float y[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int c = min(channel + r, p.n - 1);
-            y[r] = nvr::scaled(sum[i][r], xs, nvr::split_scale(p.ws[c]));
-            if constexpr (GATED)
-                y[r] = nvr::silu_mul(y[r], nvr::scaled(sum[i + NI / 2][r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+            y[r] = nvr::scaled(sum[r], xs, nvr::split_scale(p.ws[c]));
+            if constexpr (GATED) y[r] = nvr::silu_mul(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
         }
+        if (token >= p.m) continue;
         uint16_t* out = p.y + token * p.n + channel;
         if (pieces) {
             if (channel < p.n)
@@ -383,11 +388,11 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     }
 }
 
-template <int SIDE, bool GATED>
+template <int TOK, int SIDE, int SLOTS, bool GATED>
 void launch_split(nv_context* c, const nvr::ProductArgs& p) {
     constexpr int kChannels = GATED ? SIDE / 2 : SIDE;
-    const int mt = int((int64_t(p.m) + kTokens - 1) / kTokens), nt = (p.n + kChannels - 1) / kChannels;
-    hipLaunchKernelGGL((gemm_split<SIDE, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplit * 2 * kSlotBytes<SIDE>, c->stream, p,
+    const int mt = int((int64_t(p.m) + TOK - 1) / TOK), nt = (p.n + kChannels - 1) / kChannels;
+    hipLaunchKernelGGL((gemm_split<TOK, SIDE, SLOTS, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplit * SLOTS * (TOK + SIDE) * kUnitBytes, c->stream, p,
                        mt, nt);
 }
 
@@ -406,13 +411,21 @@ namespace nvr {
 void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
     using Large = Shape<256, 256, 2, 4, 128, 2>;
     using Medium = Shape<128, 128, 4, 2, 128, 2>;
+    using Wide = Shape<64, 128, 4, 2, 128, 3>;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256, rows = gated ? 2 * int64_t(p.n) : p.n;
     auto tiles = [&](int tokens, int side) { return (int64_t(p.m) + tokens - 1) / tokens * ((rows + side - 1) / side); };
     auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
-    if (tiles(kTokens, 32) <= cus) gated ? launch_split<32, true>(c, p) : launch_split<32, false>(c, p);
-    else if (tiles(kTokens, 64) <= cus) gated ? launch_split<64, true>(c, p) : launch_split<64, false>(c, p);
-    else if (3 * turns(tiles(256, 256)) > turns(tiles(128, 128))) gated ? launch<Medium, true>(c, p) : launch<Medium, false>(c, p);
-    else gated ? launch<Large, true>(c, p) : launch<Large, false>(c, p);
+    auto run = [&](auto g) {
+        constexpr bool G = decltype(g)::value;
+        if (p.m <= 16) launch_split<16, 32, 2, G>(c, p);
+        else if (p.m <= 32) launch_split<32, 32, 2, G>(c, p);
+        else if (tiles(64, 32) <= cus) launch_split<64, 32, 2, G>(c, p);
+        else if (tiles(64, 64) <= cus) launch_split<64, 64, 2, G>(c, p);
+        else if (p.m <= 64) launch<Wide, G>(c, p);
+        else if (3 * turns(tiles(256, 256)) > turns(tiles(128, 128))) launch<Medium, G>(c, p);
+        else launch<Large, G>(c, p);
+    };
+    gated ? run(std::true_type{}) : run(std::false_type{});
 }
 
 }  // namespace nvr

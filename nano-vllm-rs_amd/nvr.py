@@ -28,6 +28,7 @@ from __future__ import annotations
 
 import atexit
 import ctypes
+import functools
 import math
 import os
 import sys
@@ -162,6 +163,14 @@ I8_MAX_K = 131071
 def i8_pitch(k: int) -> int:
     """Bytes from a row of k 8-bit integers to the next."""
     return -(-as_dim(k) // 16) * 16
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(lib: ctypes.CDLL, name: str, *sizes: int) -> int:
+    """What the library's function `name` says of these sizes; it depends on nothing else."""
+    need = _sz()
+    check_status(getattr(lib, name)(*sizes, ctypes.byref(need)), lib)
+    return need.value
 
 
 MAX_TREE_NODES = 64
@@ -535,9 +544,7 @@ class Gpu:
     def _i8_workspace(self, op: str, m: int, n: int, k: int) -> int:
         self._i8_limit(op, k)
         as_dim(m), as_dim(n)
-        need, lib = _sz(), self.lib or library()
-        check_status(getattr(lib, "nv_" + op)(m, n, k, ctypes.byref(need)), lib)
-        return need.value
+        return _workspace_bytes(self.lib or library(), "nv_" + op, m, n, k)
 
     def gemm_i8(self, x: Buffer, residual: Buffer | None, residual_out: Buffer | None, norm_weight: Buffer | None,
                 w: Buffer, w_scales: Buffer, y: Buffer, workspace: Buffer, m: int, n: int, k: int,
@@ -561,24 +568,30 @@ class Gpu:
     def _product_i8(self, op, x, residual, residual_out, norm_weight, w, w_scales, y, workspace, m, n, channels, k,
                     eps) -> None:
         if norm_weight is not None:
-            require_positive(eps, f"{op} eps")
+            require_positive(eps, op)
         elif residual is not None:
             raise ArgumentError("value", f"{op}: a residual needs a norm_weight")
-        if residual is None and residual_out is not None:
-            raise ArgumentError("value", f"{op}: residual_out needs a residual to add")
         need = self._i8_workspace(op + "_workspace", m, n, k)
-        args = [_r("x", x, 2, m, k), _r("w", w, 16, channels, i8_pitch(k) // 16), _r("w_scales", w_scales, 4, channels),
-                _w("y", y, 2, m, n)]
+        args = [("x", x, 2, (m, k), False), ("w", w, 16, (channels, (k + 15) // 16), False),
+                ("w_scales", w_scales, 4, (channels,), False), ("y", y, 2, (m, n), True)]
         if need:
             args.append(self._workspace(op, workspace, need))
-        for name, buf, dims, writes in (("residual", residual, (m, k), False), ("residual_out", residual_out, (m, k), True),
-                                        ("norm_weight", norm_weight, (k,), False)):
-            if buf is not None:
-                args.append((_w if writes else _r)(name, buf, 2, *dims))
+        if norm_weight is not None:
+            args.append(("norm_weight", norm_weight, 2, (k,), False))
+        if residual is not None:
+            args.append(("residual", residual, 2, (m, k), False))
+        if residual_out is not None:
+            if residual is None:
+                raise ArgumentError("value", f"{op}: residual_out needs a residual to add")
+            args.append(("residual_out", residual_out, 2, (m, k), True))
         self._admit(op, args)
-        ptr = lambda b: None if b is None else b.ptr  # noqa: E731
-        self._call(getattr(self.lib, "nv_" + op)(self.handle, x.ptr, ptr(residual), ptr(residual_out), ptr(norm_weight),
-                                                 w.ptr, w_scales.ptr, y.ptr, ptr(workspace), m, n, k, eps))
+        call = self.lib.nv_gemm_i8 if channels == n else self.lib.nv_gemm_i8_silu
+        status = call(self._device.ctx, x.ptr, None if residual is None else residual.ptr,
+                      None if residual_out is None else residual_out.ptr,
+                      None if norm_weight is None else norm_weight.ptr, w.ptr, w_scales.ptr, y.ptr,
+                      None if workspace is None else workspace.ptr, m, n, k, eps)
+        if status:
+            check_status(status, self.lib)
 
     def add_rms_norm_gather(self, x: Buffer, residual: Buffer, weight: Buffer, indices: Buffer, out: Buffer,
                             rows: int, hidden: int, input_rows: int, eps: float) -> None:
