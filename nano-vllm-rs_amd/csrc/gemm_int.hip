@@ -24,7 +24,6 @@ typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 8, kThreads = kWaves * kWave;
-constexpr int kUnit = 8;     // steps of 64 bytes of k whose weights are in flight together
 constexpr int kRowPad = 16;  // behind a token's row in LDS: 16 tokens' pieces of one column lie in different banks
 constexpr int kFewTokens = 32;
 constexpr int kMostLds = 160 * 1024;
@@ -38,7 +37,7 @@ struct RowsArgs {
     nvr::TokenArgs t;
     int log_parts;              // 2^log_parts waves share the k of a tile: 1, 2, 4 or 8
     int tiles, per, more;       // a block has `per` tiles, the first `more` blocks one more
-    int share, units;           // lines of 128 bytes of k a wave has of a tile; loads of kUnit steps
+    int share, units;           // lines of 128 bytes of k a wave has of a tile; loads of STEPS steps
 };
 
 // LDS of a block: partial sums (parts > 1), scales, tokens.
@@ -49,8 +48,9 @@ int64_t rows_lds(int m, int x_pitch) {
     return kSumBytes<MT> + MT * 16 * 4 + int64_t(m) * (x_pitch + kRowPad);
 }
 
-// Few tokens: the weights stream through registers, once. ONE: every wave has one unit at most in all.
-template <Source SRC, int CH, int MT, bool GATED, bool ONE>
+// Few tokens: the weights stream through registers, once, STEPS pieces of 64 bytes of k in flight together as a unit, and
+// two units. ONE: every wave has one unit at most in all.
+template <Source SRC, int CH, int MT, bool GATED, int STEPS, bool ONE>
 __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     constexpr bool kMade = SRC != Source::kCopied;
     constexpr int kChannels = GATED ? 8 : 16;  // of a tile: 16 rows of the weight, or 8 of gate, then 8 of up
@@ -75,10 +75,12 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     unsigned char* xq = reinterpret_cast<unsigned char*>(xs + MT * 16);  // [m][pitch]
     const int pitch = p.x_pitch + kRowPad;
 
-    // The weights of a unit: lane l has row l % 16, 16 bytes at 16 (l / 16) of each step. Behind a row's end, where x is
-    // zero, and behind the wave's steps, which are not multiplied, any bytes of the row will do.
+    // The weights of a unit: lane l has row l % 16, 16 bytes at 16 (l / 16) of each step. Behind the wave's steps, which are
+    // not multiplied, its last one again (lines of another wave's would cost: 4 tokens over 4096 x 1024 6.0 us for 4.3), and
+    // behind a row's end, where x is zero, any bytes of the row.
+    const int last_step = max(s1, 1) - 1;
     struct Unit {
-        uint4 w[kUnit];
+        uint4 w[STEPS];
         float ws[4];  // of the lane's outputs
     };
     Unit unit[2];
@@ -87,9 +89,9 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         const int tile = tile0 + max(min(ahead_round, tile_count - 1), 0);  // its own last one, if any, where it has no more
         const int64_t row = GATED ? int64_t(i < 8 ? 0 : p.n) + min(tile * 8 + i % 8, p.n - 1) : min(tile * 16 + i, p.n - 1);
         const uint8_t* w = p.wq + row * p.w_pitch;
-        const int s = s0 + ahead * kUnit;
+        const int s = s0 + ahead * STEPS;
 #pragma unroll
-        for (int e = 0; e < kUnit; ++e) u.w[e] = nvr::load_stream(w + min((s + e) * 64 + 16 * g, p.w_pitch - 16));
+        for (int e = 0; e < STEPS; ++e) u.w[e] = *reinterpret_cast<const uint4*>(w + min(min(s + e, last_step) * 64 + 16 * g, p.w_pitch - 16));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             u.ws[r] = GATED ? p.ws[int64_t(g < 2 ? 0 : p.n) + min(tile * 8 + 4 * (g % 2) + r, p.n - 1)]
@@ -184,22 +186,22 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) ws[r] = u.ws[r];
-        const int s = s0 + at * kUnit;
+        const int s = s0 + at * STEPS;
         auto tokens = [&](int t, int e) { return *reinterpret_cast<const i32x4_t*>(xrow[t] + (s + e) * 64); };
-        if (s + kUnit <= s1) {
-            i32x4_t x[kUnit][MT];
+        if (s + STEPS <= s1) {
+            i32x4_t x[STEPS][MT];
 #pragma unroll
-            for (int e = 0; e < kUnit; ++e)
+            for (int e = 0; e < STEPS; ++e)
 #pragma unroll
                 for (int t = 0; t < MT; ++t) x[e][t] = tokens(t, e);
 #pragma unroll
-            for (int e = 0; e < kUnit; ++e)
+            for (int e = 0; e < STEPS; ++e)
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
                     acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]), x[e][t], acc[t], 0, 0, 0);
         } else {
 #pragma unroll
-            for (int e = 0; e < kUnit; ++e) {
+            for (int e = 0; e < STEPS; ++e) {
                 if (s + e >= s1) break;
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
@@ -265,9 +267,9 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     }
 }
 
-template <Source SRC, int CH, int MT, bool GATED, bool ONE>
+template <Source SRC, int CH, int MT, bool GATED, int STEPS, bool ONE>
 void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
-    hipLaunchKernelGGL((gemm_rows_i8<SRC, CH, MT, GATED, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
+    hipLaunchKernelGGL((gemm_rows_i8<SRC, CH, MT, GATED, STEPS, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
                        size_t(rows_lds<MT>(a.p.m, a.p.x_pitch)), c->stream, a);
 }
 
@@ -278,22 +280,33 @@ void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
     a.per = tiles / blocks;
     a.more = tiles % blocks;
     a.share = (lines + parts - 1) / parts;
-    a.units = (a.share * 2 + kUnit - 1) / kUnit;
 }
 
 template <Source SRC, bool GATED>
 void launch_rows(nv_context* c, RowsArgs a) {
     const int tiles = (a.p.n + (GATED ? 8 : 16) - 1) / (GATED ? 8 : 16);
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
-    const int units = (a.p.x_pitch / 64 + kUnit - 1) / kUnit;
-    int parts = 8;
-    while (parts > 1 && (units * 2 <= parts || int64_t(tiles) * parts > int64_t(cus) * kWaves * 4)) parts /= 2;
+    const int lines = a.p.x_pitch / 128;
+    // As many waves for a tile as leave each one tile, if its share of k is then one unit; else up to four turns of them.
+    auto fits = [&](int parts) { return int64_t(tiles) * parts <= int64_t(cus) * kWaves && (lines + parts - 1) / parts <= 4; };
+    int parts = fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : fits(1) ? 1 : 8;
+    if (!fits(parts))
+        while (parts > 1 && (parts > lines || int64_t(tiles) * parts > int64_t(cus) * kWaves * 4)) parts /= 2;
     const int blocks = std::min(cus, (tiles * parts + kWaves - 1) / kWaves);
     plan_rows(a, tiles, parts, blocks);
-    const bool one = a.units == 1 && (a.per + (a.more != 0)) * parts <= kWaves;
+    const bool alone = (a.per + (a.more != 0)) * parts <= kWaves;  // a wave has one tile at most
     auto run = [&](auto chunks, auto tiles16) {
         constexpr int CH = decltype(chunks)::value, MT = decltype(tiles16)::value;
-        one ? launch_rows_as<SRC, CH, MT, GATED, true>(c, a, blocks) : launch_rows_as<SRC, CH, MT, GATED, false>(c, a, blocks);
+        auto with = [&](auto steps, auto one) {
+            constexpr int STEPS = decltype(steps)::value;
+            a.units = (a.share * 2 + STEPS - 1) / STEPS;
+            launch_rows_as<SRC, CH, MT, GATED, STEPS, decltype(one)::value>(c, a, blocks);
+        };
+        if (alone && a.share == 1) with(std::integral_constant<int, 2>{}, std::true_type{});
+        else if (alone && a.share == 2) with(std::integral_constant<int, 4>{}, std::true_type{});
+        else if (alone && a.share <= 4) with(std::integral_constant<int, 8>{}, std::true_type{});
+        else if (a.share <= 2) with(std::integral_constant<int, 4>{}, std::false_type{});
+        else with(std::integral_constant<int, 8>{}, std::false_type{});
     };
     using std::integral_constant;
     const integral_constant<int, 1> one16;

@@ -14,13 +14,13 @@
 // lies within 2^-17 of such a point, and fp32 is within 2^-18 of it below 128: the
 // row's numbers are those of exact arithmetic.
 //
-// A norm's values are those of fp32, not rounded to bf16 in between: the norm's
-// output feeds one product only, and 8 bits of a step keep more of them.
-// Its sum of squares has one order, whoever computes it: element j belongs to
-// lane (j / 8) % 64 and class (j / 512) % 4; a lane sums each class in order of
-// j, the 64 lanes by a butterfly, the classes as (0 + 1) + (2 + 3). A wave that
-// holds all of a row and four waves that hold a class each give the same bits, so
-// a token's outputs do not depend on the call's other tokens.
+// Of a norm, u_j = v_j g_j / rms(v), the whole numbers need the products v_j g_j alone: their common factor leaves 127 u_j /
+// a as it is, and goes into the scale. So a row's sum of squares and its largest product are found in one pass, and the
+// norm's values are never rounded, to bf16 or otherwise: they feed one product only, and 8 bits of a step keep more.
+// The sum of squares has one order, whoever computes it: element j belongs to lane (j / 8) % 64 and class (j / 512) % 4; a
+// lane sums each class in order of j, then come the 64 lanes, in wave_sum's order, and the classes as (0 + 1) + (2 + 3). A
+// wave that holds all of a row and four waves that hold a class each give the same bits, so a token's outputs do not depend
+// on the call's other tokens.
 #pragma once
 
 #include <algorithm>
@@ -111,17 +111,32 @@ __device__ __forceinline__ void store_chunk(uint16_t* row, int j, int k, const f
     }
 }
 
+// Sums over a wave by shifts inside each row of 16 lanes, then of rows' last lanes into the rows behind them: no LDS
+// crossbar. Every lane gets lane 63's value.
+constexpr int kDppRowShr = 0x110, kDppRowBcast15 = 0x142, kDppRowBcast31 = 0x143;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t v) {
+    return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, ROWS, 0xF, false));
+}
+template <class Op>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, Op op) {
+    v = op(v, dpp_or_zero<kDppRowShr + 1, 0xF>(v));
+    v = op(v, dpp_or_zero<kDppRowShr + 2, 0xF>(v));
+    v = op(v, dpp_or_zero<kDppRowShr + 4, 0xF>(v));
+    v = op(v, dpp_or_zero<kDppRowShr + 8, 0xF>(v));
+    v = op(v, dpp_or_zero<kDppRowBcast15, 0xA>(v));
+    v = op(v, dpp_or_zero<kDppRowBcast31, 0xC>(v));
+    return uint32_t(__builtin_amdgcn_readlane(int(v), 63));
+}
 __device__ __forceinline__ float wave_sum(float s) {
-#pragma unroll
-    for (int w = 1; w < kWave; w <<= 1) s = s + xor_lane(s, w);
-    return s;
+    return __uint_as_float(wave_fold(__float_as_uint(s), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
 }
 // The largest |u| of values as bits: a NaN's are above those of infinity, which are above all others.
 __device__ __forceinline__ uint32_t magnitude(float u) { return __float_as_uint(u) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t wave_max(uint32_t a) {
-#pragma unroll
-    for (int w = 1; w < kWave; w <<= 1) a = max(a, xor_lane_bits(a, w));
-    return a;
+    return wave_fold(a, [](uint32_t x, uint32_t y) { return max(x, y); });
 }
 
 // The step of a row whose largest magnitude has the bits `top`.
@@ -211,11 +226,11 @@ __device__ __forceinline__ float add_squares(float sum, const float* v) {
 __device__ __forceinline__ float row_inverse(const float* s, const TokenArgs& t) {
     return inv_sqrt_rn(((s[0] + s[1]) + (s[2] + s[3])) / float(t.k) + t.eps);
 }
-__device__ __forceinline__ void scale_norm(float* v, float inv, const uint4& weight) {
+__device__ __forceinline__ void times(float* v, const uint4& weight) {
     float g[kChunk];
     unpack8(weight, g);
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) v[i] = (v[i] * inv) * g[i];
+    for (int i = 0; i < kChunk; ++i) v[i] = v[i] * g[i];
 }
 __device__ __forceinline__ uint32_t most_of(uint32_t top, const float* v) {
 #pragma unroll
@@ -224,8 +239,7 @@ __device__ __forceinline__ uint32_t most_of(uint32_t top, const float* v) {
 }
 
 struct NoJoin {
-    __device__ void sums(float*) const {}
-    __device__ void most(uint32_t&) const {}
+    __device__ void operator()(float*, uint32_t&) const {}
 };
 
 // The row's step (in every lane), and put(j, eight numbers) for each chunk j < width that the lane holds: zeros from k on.
@@ -238,31 +252,32 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     float v[CH][kChunk];
 #pragma unroll
     for (int c = 0; c < CH; ++c) row_values<T>(r.x[c], r.residual[T == Tokens::kAddNorm ? c : 0], v[c]);
+    float s[kClasses] = {};
     if constexpr (T != Tokens::kPlain) {
-        float s[kClasses] = {};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             float& sum = s[WAVES == 1 ? c % kClasses : 0];
             sum = add_squares(sum, v[c]);
         }
-#pragma unroll
-        for (int i = 0; i < (WAVES == 1 ? (CH < kClasses ? CH : kClasses) : 1); ++i) s[i] = wave_sum(s[i]);
-        join.sums(s);
-        const float inv = row_inverse(s, t);
         if (T == Tokens::kAddNorm && keep_sum) {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
                 store_chunk<WHOLE>(t.residual_out + row * t.k, chunk_at<WAVES>(c, lane, wave), t.k, v[c]);
         }
 #pragma unroll
-        for (int c = 0; c < CH; ++c) scale_norm(v[c], inv, norm.g[c]);
+        for (int c = 0; c < CH; ++c) times(v[c], norm.g[c]);
     }
     uint32_t top = 0;
 #pragma unroll
     for (int c = 0; c < CH; ++c) top = most_of(top, v[c]);
     top = wave_max(top);
-    join.most(top);
-    const RowStep step = row_step(top);
+    if constexpr (T != Tokens::kPlain) {
+#pragma unroll
+        for (int i = 0; i < (WAVES == 1 ? (CH < kClasses ? CH : kClasses) : 1); ++i) s[i] = wave_sum(s[i]);
+    }
+    join(s, top);
+    RowStep step = row_step(top);
+    if constexpr (T != Tokens::kPlain) step.scale = step.scale * row_inverse(s, t);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int j = chunk_at<WAVES>(c, lane, wave);
@@ -271,7 +286,7 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     return step;
 }
 
-// The same for a row of any length by four waves, which read it anew for each of its three passes.
+// The same for a row of any length by four waves, which read it twice.
 template <Tokens T, bool WHOLE, class Join, class Put>
 __device__ __forceinline__ RowStep quantize_long_row(const TokenArgs& t, int64_t row, int width, bool keep_sum, int lane,
                                                      int wave, Join join, Put put) {
@@ -282,32 +297,25 @@ __device__ __forceinline__ RowStep quantize_long_row(const TokenArgs& t, int64_t
         row_values<T>(x, T == Tokens::kAddNorm ? load_chunk<WHOLE>(t.residual + row * t.k, j, t.k) : x, v);
         return j;
     };
-    float inv = 1.0f, v[kChunk];
-    if constexpr (T != Tokens::kPlain) {
-        float s[kClasses] = {};
-        for (int c = 0; c < chunks; ++c) {
-            load(c, v);
-            s[0] = add_squares(s[0], v);
-        }
-        s[0] = wave_sum(s[0]);
-        join.sums(s);
-        inv = row_inverse(s, t);
-    }
+    float v[kChunk], s[kClasses] = {};
     uint32_t top = 0;
     for (int c = 0; c < chunks; ++c) {
         const int j = load(c, v);
         if constexpr (T != Tokens::kPlain) {
+            s[0] = add_squares(s[0], v);
             if (T == Tokens::kAddNorm && keep_sum) store_chunk<WHOLE>(t.residual_out + row * t.k, j, t.k, v);
-            scale_norm(v, inv, load_chunk<WHOLE>(t.norm_weight, j, t.k));
+            times(v, load_chunk<WHOLE>(t.norm_weight, j, t.k));
         }
         top = most_of(top, v);
     }
     top = wave_max(top);
-    join.most(top);
-    const RowStep step = row_step(top);
+    if constexpr (T != Tokens::kPlain) s[0] = wave_sum(s[0]);
+    join(s, top);
+    RowStep step = row_step(top);
+    if constexpr (T != Tokens::kPlain) step.scale = step.scale * row_inverse(s, t);
     for (int c = 0; c < chunks; ++c) {
         const int j = load(c, v);
-        if constexpr (T != Tokens::kPlain) scale_norm(v, inv, load_chunk<WHOLE>(t.norm_weight, j, t.k));
+        if constexpr (T != Tokens::kPlain) times(v, load_chunk<WHOLE>(t.norm_weight, j, t.k));
         if (j < width) put(j, whole_numbers(v, step));
     }
     return step;

@@ -5,8 +5,7 @@
 //
 // Bound by memory: 3 bytes an element move (7 with a residual). A row is read
 // once and stays in registers: up to 4096 values by one wave, so no barrier is
-// waited for, up to 16384 by the four waves of a block; longer rows are read again
-// for each step. With few rows four waves a row are taken below 4096 too, for
+// waited for, up to 16384 by the four waves of a block; longer rows are read twice. With few rows four waves a row are taken below 4096 too, for
 // more loads in flight.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
@@ -24,20 +23,19 @@ struct BlockJoin {
     float* sum;
     uint32_t* top;
     int lane, wave;
-    __device__ void sums(float* s) const {
-        if (lane == 0) sum[wave] = s[0];
+    __device__ void operator()(float* s, uint32_t& t) const {
+        if (lane == 0) {
+            sum[wave] = s[0];
+            top[wave] = t;
+        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < nvr::kClasses; ++i) s[i] = sum[i];
-    }
-    __device__ void most(uint32_t& t) const {
-        if (lane == 0) top[wave] = t;
-        __syncthreads();
         t = max(max(top[0], top[1]), max(top[2], top[3]));
     }
 };
 
-// CH chunks a lane of WAVES waves hold a row; 0: a row of any length, read anew for each pass.
+// CH chunks a lane of WAVES waves hold a row; 0: a row of any length, read twice.
 template <Tokens T, bool WHOLE, int CH, int WAVES>
 __global__ __launch_bounds__(kThreads) void quantize_rows(nvr::TokenArgs t, uint8_t* __restrict__ q,
                                                           float* __restrict__ scales, int pitch) {
