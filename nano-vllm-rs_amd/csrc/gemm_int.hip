@@ -50,7 +50,7 @@ int64_t rows_lds(int m, int x_pitch) {
 
 // Few tokens: the weights stream through registers, once, STEPS pieces of 64 bytes of k in flight together as a unit, and
 // two units. ONE: every wave has one unit at most in all.
-template <Source SRC, int CH, int MT, bool GATED, int STEPS, bool ONE>
+template <Source SRC, bool WHOLE, int CH, int RW, int MT, bool GATED, int STEPS, bool ONE>
 __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     constexpr bool kMade = SRC != Source::kCopied;
     constexpr int kChannels = GATED ? 8 : 16;  // of a tile: 16 rows of the weight, or 8 of gate, then 8 of up
@@ -104,24 +104,32 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     if constexpr (kMade) {
         // A wave's loads return in order: its tokens' come before the weights'.
         constexpr Tokens T = SRC == Source::kPlain ? Tokens::kPlain : SRC == Source::kNorm ? Tokens::kNorm : Tokens::kAddNorm;
-        const int row = min(wave, p.m - 1);
-        const nvr::NormChunks<CH> norm = nvr::load_norm<T, true, CH, 1>(a.t, lane, 0);
-        const nvr::RowChunks<T, CH> chunks = nvr::load_row<T, true, CH, 1>(a.t, row, lane, 0);
+        const nvr::NormChunks<CH> norm = nvr::load_norm<T, WHOLE, CH, 1>(a.t, lane, 0);
+        nvr::RowChunks<T, CH> chunks[RW];
+#pragma unroll
+        for (int i = 0; i < RW; ++i)
+            chunks[i] = nvr::load_row<T, WHOLE, CH, 1>(a.t, min(wave + i * kWaves, p.m - 1), lane, 0);
+        // The compiler would mix them otherwise (1 token over 1024 x 2048 4.5 us for 3.4).
+        __builtin_amdgcn_sched_barrier(0);
         load(unit[0]);
-        if (wave < p.m) {
-            const nvr::RowStep step = nvr::quantize_row<T, true, CH, 1>(
-                a.t, row, chunks, norm, p.x_pitch, blockIdx.x == 0 && a.t.residual_out != nullptr, lane, 0, nvr::NoJoin{},
-                [&](int j, uint2 eight) { *reinterpret_cast<uint2*>(xq + row * pitch + j) = eight; });
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < RW; ++i) {
+            const int row = wave + i * kWaves;
+            if (row >= p.m) break;
+            const nvr::RowStep step = nvr::quantize_row<T, WHOLE, CH, 1>(
+                a.t, row, chunks[i], norm, p.x_pitch, blockIdx.x == 0 && a.t.residual_out != nullptr, lane, 0,
+                nvr::NoJoin{}, [&](int j, uint2 eight) { *reinterpret_cast<uint2*>(xq + row * pitch + j) = eight; });
             if (lane == 0) xs[row] = step.scale;
         }
     } else {
-        load(unit[0]);
         for (int row = wave; row < p.m; row += kWaves)
 #pragma unroll 4
             for (int c = lane * 16; c < p.x_pitch; c += kWave * 16)
                 *reinterpret_cast<uint4*>(xq + row * pitch + c) =
                     *reinterpret_cast<const uint4*>(p.xq + int64_t(row) * p.x_pitch + c);
         if (int(threadIdx.x) < p.m) xs[threadIdx.x] = p.xs[threadIdx.x];
+        load(unit[0]);  // behind the tokens, for the same reason (16 tokens over 16384 x 4096 18.8 us for 16.2)
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // leaves the weights in flight
     if constexpr (!ONE) load(unit[1]);
@@ -267,9 +275,9 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     }
 }
 
-template <Source SRC, int CH, int MT, bool GATED, int STEPS, bool ONE>
+template <Source SRC, bool WHOLE, int CH, int RW, int MT, bool GATED, int STEPS, bool ONE>
 void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
-    hipLaunchKernelGGL((gemm_rows_i8<SRC, CH, MT, GATED, STEPS, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
+    hipLaunchKernelGGL((gemm_rows_i8<SRC, WHOLE, CH, RW, MT, GATED, STEPS, ONE>), dim3(unsigned(blocks)), dim3(kThreads),
                        size_t(rows_lds<MT>(a.p.m, a.p.x_pitch)), c->stream, a);
 }
 
@@ -282,7 +290,7 @@ void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
     a.share = (lines + parts - 1) / parts;
 }
 
-template <Source SRC, bool GATED>
+template <Source SRC, bool WHOLE, bool GATED>
 void launch_rows(nv_context* c, RowsArgs a) {
     const int tiles = (a.p.n + (GATED ? 8 : 16) - 1) / (GATED ? 8 : 16);
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
@@ -295,28 +303,32 @@ void launch_rows(nv_context* c, RowsArgs a) {
     const int blocks = std::min(cus, (tiles * parts + kWaves - 1) / kWaves);
     plan_rows(a, tiles, parts, blocks);
     const bool alone = (a.per + (a.more != 0)) * parts <= kWaves;  // a wave has one tile at most
-    auto run = [&](auto chunks, auto tiles16) {
-        constexpr int CH = decltype(chunks)::value, MT = decltype(tiles16)::value;
+    auto run = [&](auto chunks, auto rows, auto tiles16) {
+        constexpr int CH = decltype(chunks)::value, RW = decltype(rows)::value, MT = decltype(tiles16)::value;
         auto with = [&](auto steps, auto one) {
             constexpr int STEPS = decltype(steps)::value;
             a.units = (a.share * 2 + STEPS - 1) / STEPS;
-            launch_rows_as<SRC, CH, MT, GATED, STEPS, decltype(one)::value>(c, a, blocks);
+            launch_rows_as<SRC, WHOLE, CH, RW, MT, GATED, STEPS, decltype(one)::value>(c, a, blocks);
         };
-        if (alone && a.share == 1) with(std::integral_constant<int, 2>{}, std::true_type{});
-        else if (alone && a.share == 2) with(std::integral_constant<int, 4>{}, std::true_type{});
-        else if (alone && a.share <= 4) with(std::integral_constant<int, 8>{}, std::true_type{});
-        else if (a.share <= 2) with(std::integral_constant<int, 4>{}, std::false_type{});
+        const auto one = std::true_type{};
+        if constexpr (WHOLE) {
+            if (alone && a.share == 1) return with(std::integral_constant<int, 2>{}, one);
+            if (!alone && a.share <= 2) return with(std::integral_constant<int, 4>{}, std::false_type{});
+        }
+        if (alone && a.share <= 2) with(std::integral_constant<int, 4>{}, one);
+        else if (alone && a.share <= 4) with(std::integral_constant<int, 8>{}, one);
         else with(std::integral_constant<int, 8>{}, std::false_type{});
     };
     using std::integral_constant;
-    const integral_constant<int, 1> one16;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
     if constexpr (SRC == Source::kCopied) {
-        if (a.p.m <= 16) run(integral_constant<int, 1>{}, one16);
-        else run(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+        a.p.m <= 16 ? run(one, one, one) : run(one, one, two);
     } else {
-        if (a.p.x_pitch <= 2 * nvr::kWaveChunk) run(integral_constant<int, 2>{}, one16);
-        else if (a.p.x_pitch <= 4 * nvr::kWaveChunk) run(integral_constant<int, 4>{}, one16);
-        else if constexpr (SRC == Source::kPlain) run(integral_constant<int, 8>{}, one16);
+        if (a.p.m > kWaves) run(two, two, one);
+        else if (a.p.x_pitch <= 2 * nvr::kWaveChunk) run(two, one, one);
+        else if (a.p.x_pitch <= 4 * nvr::kWaveChunk) run(integral_constant<int, 4>{}, one, one);
+        else if constexpr (SRC == Source::kPlain) run(integral_constant<int, 8>{}, one, one);
     }
 }
 
@@ -326,7 +338,8 @@ void launch_rows(nv_context* c, RowsArgs a) {
 // chunks, sums and norm weights no longer fit the registers beside the weights). 16 tokens, two rows a wave: at k 1024
 // 6.7, 7.5 and 8.0, 7.8; at k 2048 8.1, 8.1 and 10.9, 8.4.
 bool tokens_in_block(const nvr::TokenArgs& t) {
-    return t.rows <= kWaves && t.k % nvr::kChunk == 0 && t.k <= (t.norm_weight == nullptr ? 8 : 4) * nvr::kWaveChunk;
+    const int chunks = t.rows > kWaves ? 2 : t.norm_weight == nullptr ? 8 : 4;
+    return t.rows <= 2 * kWaves && t.k <= chunks * nvr::kWaveChunk;
 }
 
 // Whether few tokens, made by a launch of their own, take gemm_rows_i8: where a CU would have more than two of
@@ -381,13 +394,17 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
     const RowsArgs few{p, t, 0, 0, 0, 0, 0, 0};
     if (tokens_in_block(t)) {
-        if (norm_weight == nullptr) launch_rows<Source::kPlain, GATED>(c, few);
-        else if (residual == nullptr) launch_rows<Source::kNorm, GATED>(c, few);
-        else launch_rows<Source::kAddNorm, GATED>(c, few);
+        auto run = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
+            if (norm_weight == nullptr) launch_rows<Source::kPlain, WHOLE, GATED>(c, few);
+            else if (residual == nullptr) launch_rows<Source::kNorm, WHOLE, GATED>(c, few);
+            else launch_rows<Source::kAddNorm, WHOLE, GATED>(c, few);
+        };
+        k % nvr::kChunk == 0 ? run(std::true_type{}) : run(std::false_type{});
         return nvr::launch_status();
     }
     nvr::launch_quantize(c, t, xq, xs, pitch);
-    if (weight_streams(c, p, GATED)) launch_rows<Source::kCopied, GATED>(c, few);
+    if (weight_streams(c, p, GATED)) launch_rows<Source::kCopied, true, GATED>(c, few);
     else nvr::launch_product_tiles(c, p, GATED);
     return nvr::launch_status();
 }
