@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     i32x4_t acc[MT];
     float ws[4];
     // A wave that has its tiles to itself, and several, keeps its outputs until they fill lines of 128 bytes.
-    const bool lines_kept = !ONE && parts == 1 && p.n % 8 == 0 && nvr::aligned(p.y, 16);
+    const bool lines_kept = !ONE && parts == 1 && p.n % 8 == 0;
     unsigned char* kept = smem + wave * (MT * 16 * 128);  // [MT * 16][128], where the sums would be
     static_assert(kWaves * MT * 16 * 128 == kSumBytes<MT>, "its place");
     int round = 0, at = 0;  // the unit to multiply
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             y[r] = nvr::scaled(sum[r], x, nvr::split_scale(ws[r]));
-            if constexpr (GATED) y[r] = nvr::silu_mul(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
+            if constexpr (GATED) y[r] = nvr::gated(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
         }
         if (round >= tile_count) return;
         const int channel = (tile0 + round) * kChannels + 4 * (GATED ? g % 2 : g);
@@ -165,15 +165,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
                     make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
             return;
         }
-        uint16_t* out = p.y + int64_t(token) * p.n + channel;
-        if (p.n % 4 == 0 && nvr::aligned(p.y, 8)) {
-            if (stored && channel < p.n)
-                *reinterpret_cast<uint2*>(out) = make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
-        } else if (stored) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (channel + r < p.n) out[r] = nvr::f32_to_bf16(y[r]);
-        }
+        if (stored) nvr::store_outputs(p.y + int64_t(token) * p.n + channel, y, channel, p.n);
     };
     // A wave's tiles that fill a line of 64 channels, or its last: 8 tokens' lines a store.
     auto flush = [&] {
@@ -184,8 +176,8 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
 #pragma unroll
         for (int r = 0; r < MT * 16; r += 8)
             if (r + lane / 8 < p.m)
-                *reinterpret_cast<uint4*>(p.y + int64_t(r + lane / 8) * p.n + channel) =
-                    *reinterpret_cast<const uint4*>(kept + (r + lane / 8) * 128 + lane % 8 * 16);
+                nvr::store8(p.y + int64_t(r + lane / 8) * p.n + channel,
+                            *reinterpret_cast<const uint4*>(kept + (r + lane / 8) * 128 + lane % 8 * 16));
     };
     auto multiply = [&](const Unit& u) {
         if (at == 0) {

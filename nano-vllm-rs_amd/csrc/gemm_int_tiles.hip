@@ -205,7 +205,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     y[r] = scale(acc[i][j][r], xs[j], ws[r]);
-                    if constexpr (GATED) y[r] = nvr::silu_mul(y[r], scale(acc[i + 2][j][r], xs[j], us[r]));
+                    if constexpr (GATED) y[r] = nvr::gated(y[r], scale(acc[i + 2][j][r], xs[j], us[r]));
                 }
                 const int row = j * 16 + lane % 16;
                 *reinterpret_cast<uint2*>(mine + row * (OUT * 2) + unit(row, at / 8) * 16 + at % 8 * 2) =
@@ -216,21 +216,19 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     if (__all(plain)) outputs([](int sum, float x, float w) { return float(sum) * x * w; });
     else outputs([](int sum, float x, float w) { return nvr::scaled(sum, nvr::split_scale(x), nvr::split_scale(w)); });
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its own region only
-    auto store = [&](auto kind) {
-        using T = decltype(kind);
-        constexpr int PER = sizeof(T) / 2, LANES = OUT / PER, ROWS = kWave / LANES;
-        const int c = lane % LANES * PER;
-        if (c0 + c >= p.n) return;  // a T lies inside n or outside
+    constexpr int ROWS = kWave / UNITS;
+    const int c = lane % UNITS * 8;
 #pragma unroll 4
-        for (int r = lane / LANES; r < S::TM; r += ROWS) {
-            if (t0 + r >= p.m) break;
-            const T v = *reinterpret_cast<const T*>(mine + r * (OUT * 2) + unit(r, c / 8) * 16 + c % 8 * 2);
-            *reinterpret_cast<T*>(p.y + (t0 + r) * p.n + c0 + c) = v;
+    for (int r = lane / UNITS; r < S::TM; r += ROWS) {
+        if (t0 + r >= p.m) break;
+        const unsigned char* at = mine + r * (OUT * 2) + unit(r, c / 8) * 16;
+        uint16_t* out = p.y + (t0 + r) * p.n + c0 + c;
+        if (c0 + c + 8 <= p.n) {
+            nvr::store8(out, *reinterpret_cast<const uint4*>(at));
+        } else {
+            for (int e = 0; e < 8 && c0 + c + e < p.n; ++e) out[e] = *reinterpret_cast<const uint16_t*>(at + 2 * e);
         }
-    };
-    if (p.n % 8 == 0 && nvr::aligned(p.y, 16)) store(uint4{});
-    else if (p.n % 2 == 0 && nvr::aligned(p.y, 4)) store(uint32_t{});
-    else store(uint16_t{});
+    }
 }
 
 // Fewer tokens: tiles of TOK tokens by SIDE rows of the weight (gated: half of gate, half of up), a wave for every fourth
@@ -351,7 +349,6 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
 #pragma unroll
         for (int i = 0; i < NI; ++i) sums[((wave * MJ + j) * NI + i) * kWave] = acc[i][j];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool pieces = p.n % 4 == 0 && nvr::aligned(p.y, 8);
     constexpr int OI = GATED ? NI / 2 : NI;  // a token's 16 channels
 #pragma unroll
     for (int at = 0; at < MJ * OI; at += kSplit) {
@@ -373,18 +370,10 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
         for (int r = 0; r < 4; ++r) {
             const int c = min(channel + r, p.n - 1);
             y[r] = nvr::scaled(sum[r], xs, nvr::split_scale(p.ws[c]));
-            if constexpr (GATED) y[r] = nvr::silu_mul(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+            if constexpr (GATED) y[r] = nvr::gated(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
         }
         if (token >= p.m) continue;
-        uint16_t* out = p.y + token * p.n + channel;
-        if (pieces) {
-            if (channel < p.n)
-                *reinterpret_cast<uint2*>(out) = make_uint2(nvr::pack_bf16x2(y[0], y[1]), nvr::pack_bf16x2(y[2], y[3]));
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (channel + r < p.n) out[r] = nvr::f32_to_bf16(y[r]);
-        }
+        nvr::store_outputs(p.y + token * p.n + channel, y, channel, p.n);
     }
 }
 

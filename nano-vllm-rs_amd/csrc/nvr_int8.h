@@ -17,10 +17,10 @@
 // Of a norm, u_j = v_j g_j / rms(v), the whole numbers need the products v_j g_j alone: their common factor leaves 127 u_j /
 // a as it is, and goes into the scale. So a row's sum of squares and its largest product are found in one pass, and the
 // norm's values are never rounded, to bf16 or otherwise: they feed one product only, and 8 bits of a step keep more.
-// The sum of squares has one order, whoever computes it: element j belongs to lane (j / 8) % 64 and class (j / 512) % 4; a
-// lane sums each class in order of j, then come the 64 lanes, in wave_sum's order, and the classes as (0 + 1) + (2 + 3). A
-// wave that holds all of a row and four waves that hold a class each give the same bits, so a token's outputs do not depend
-// on the call's other tokens.
+// The sum of squares has one order, whoever computes it: element j belongs to lane (j / 8) % 64 and class (j / 512) % 16; a
+// lane sums each class in order of j, then come the 64 lanes, in wave_sum's order, and the classes in pairs. A wave that
+// holds all of a row, 4 that hold 4 classes each and 16 that hold one give the same bits, so a token's outputs do not
+// depend on the call's other tokens.
 #pragma once
 
 #include <algorithm>
@@ -34,7 +34,7 @@ namespace nvr {
 
 constexpr int kChunk = 8;                      // elements of a lane's load (16 bytes of bf16)
 constexpr int kWaveChunk = kChunk * kWave;     // elements a wave covers with one load a lane
-constexpr int kClasses = 4;
+constexpr int kClasses = 16;
 
 // Rows of 8-bit integers start at multiples of 16 bytes.
 __host__ __device__ constexpr int64_t i8_pitch(int64_t k) { return (k + 15) / 16 * 16; }
@@ -71,6 +71,8 @@ struct ProductArgs {
 // Products of whole tiles (gemm_int_tiles.hip).
 void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated);
 
+__device__ __forceinline__ void store8(uint16_t* to, uint4 v);
+
 // Elements j .. j + 7 of a row (bf16 from any even address on), +0 from k on; nothing outside the row is read. WHOLE: k is
 // a multiple of 8.
 template <bool WHOLE>
@@ -100,10 +102,8 @@ __device__ __forceinline__ uint4 load_chunk(const uint16_t* row, int j, int k) {
 
 template <bool WHOLE>
 __device__ __forceinline__ void store_chunk(uint16_t* row, int j, int k, const float* f) {
-    struct __attribute__((packed, aligned(2))) Eight { uint32_t w[4]; };
     if (j + kChunk <= k) {
-        const uint4 w = pack8_split(f);
-        *reinterpret_cast<Eight*>(row + j) = Eight{{w.x, w.y, w.z, w.w}};
+        store8(row + j, pack8_split(f));
     } else if constexpr (!WHOLE) {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
@@ -171,8 +171,8 @@ __device__ __forceinline__ uint2 whole_numbers(const float* u, const RowStep& s)
     return make_uint2(four(b[0], b[1], b[2], b[3]), four(b[4], b[5], b[6], b[7]));
 }
 
-// A row of tokens by one wave (WAVES 1) or a class of it by each of four (WAVES 4), CH chunks a lane: what a lane loads
-// of it, always as many loads, so that later ones can stay in flight while the row is worked on.
+// A row of tokens by WAVES waves (1, 4 or 16), CH chunks a lane: what a lane loads of it, always as many loads, so that
+// later ones can stay in flight while the row is worked on.
 template <Tokens T, int CH>
 struct RowChunks {
     uint4 x[CH], residual[T == Tokens::kAddNorm ? CH : 1];
@@ -224,7 +224,14 @@ __device__ __forceinline__ float add_squares(float sum, const float* v) {
     return sum;
 }
 __device__ __forceinline__ float row_inverse(const float* s, const TokenArgs& t) {
-    return inv_sqrt_rn(((s[0] + s[1]) + (s[2] + s[3])) / float(t.k) + t.eps);
+    float total[kClasses];
+#pragma unroll
+    for (int i = 0; i < kClasses; ++i) total[i] = s[i];
+#pragma unroll
+    for (int w = 1; w < kClasses; w *= 2)
+#pragma unroll
+        for (int i = 0; i < kClasses; i += 2 * w) total[i] = total[i] + total[i + w];
+    return inv_sqrt_rn(total[0] / float(t.k) + t.eps);
 }
 __device__ __forceinline__ void times(float* v, const uint4& weight) {
     float g[kChunk];
@@ -243,12 +250,13 @@ struct NoJoin {
 };
 
 // The row's step (in every lane), and put(j, eight numbers) for each chunk j < width that the lane holds: zeros from k on.
-// With WAVES 4, join brings the waves' sums and largest bits together.
+// With more than one wave, join brings their sums and largest bits together.
 template <Tokens T, bool WHOLE, int CH, int WAVES, class Join, class Put>
 __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row, const RowChunks<T, CH>& r,
                                                 const NormChunks<CH>& norm, int width, bool keep_sum, int lane,
                                                 int wave, Join join, Put put) {
-    static_assert(WAVES == 1 || WAVES == kClasses, "a wave has all classes of a row, or one");
+    constexpr int MINE = kClasses / WAVES, SUMS = CH < MINE ? CH : MINE;  // a wave's classes, and those that it has chunks of
+    static_assert(WAVES * MINE == kClasses, "whole classes");
     float v[CH][kChunk];
 #pragma unroll
     for (int c = 0; c < CH; ++c) row_values<T>(r.x[c], r.residual[T == Tokens::kAddNorm ? c : 0], v[c]);
@@ -256,7 +264,7 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     if constexpr (T != Tokens::kPlain) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            float& sum = s[WAVES == 1 ? c % kClasses : 0];
+            float& sum = s[c % MINE];
             sum = add_squares(sum, v[c]);
         }
         if (T == Tokens::kAddNorm && keep_sum) {
@@ -273,7 +281,7 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     top = wave_max(top);
     if constexpr (T != Tokens::kPlain) {
 #pragma unroll
-        for (int i = 0; i < (WAVES == 1 ? (CH < kClasses ? CH : kClasses) : 1); ++i) s[i] = wave_sum(s[i]);
+        for (int i = 0; i < SUMS; ++i) s[i] = wave_sum(s[i]);
     }
     join(s, top);
     RowStep step = row_step(top);
@@ -286,7 +294,7 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     return step;
 }
 
-// The same for a row of any length by four waves, which read it twice.
+// The same for a row of any length by 16 waves, which read it twice.
 template <Tokens T, bool WHOLE, class Join, class Put>
 __device__ __forceinline__ RowStep quantize_long_row(const TokenArgs& t, int64_t row, int width, bool keep_sum, int lane,
                                                      int wave, Join join, Put put) {
@@ -333,6 +341,37 @@ __device__ __forceinline__ Scale split_scale(float s) {
 __device__ __forceinline__ float scaled(int acc, Scale x, Scale w) {
     return __builtin_amdgcn_ldexpf(float(acc) * x.mantissa * w.mantissa, x.exponent + w.exponent);
 }
+// silu(g) u, with g / (1 + e^-g) at 2^-64 of both sides where e^-g is large: neither the exponential overflows nor the
+// reciprocal is flushed while the result is one of fp32. Hardware exponential and reciprocal, each within a step; without
+// the division that nv_silu takes there, whose instructions every lane would run.
+__device__ __forceinline__ float gated(float g, float u) {
+    const float t = g * -1.44269504088896340736f;
+    const bool large = t > 64.0f;
+    const float a = large ? 0x1.0p-64f : 1.0f;
+    const float d = a + __builtin_amdgcn_exp2f(large ? t - 64.0f : t);
+    return (g * a) * __builtin_amdgcn_rcpf(d) * u;
+}
+
+// Stores of four and eight bf16 to any even address.
+__device__ __forceinline__ void store4(uint16_t* to, uint2 v) {
+    struct __attribute__((packed, aligned(2))) Four { uint32_t w[2]; };
+    *reinterpret_cast<Four*>(to) = Four{{v.x, v.y}};
+}
+__device__ __forceinline__ void store8(uint16_t* to, uint4 v) {
+    struct __attribute__((packed, aligned(2))) Eight { uint32_t w[4]; };
+    *reinterpret_cast<Eight*>(to) = Eight{{v.x, v.y, v.z, v.w}};
+}
+// Four outputs of a row from `channel` on, those below n.
+__device__ __forceinline__ void store_outputs(uint16_t* to, const float* y, int channel, int n) {
+    if (channel + 4 <= n) {
+        store4(to, make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])));
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (channel + r < n) to[r] = f32_to_bf16(y[r]);
+    }
+}
+
 // Whether float(acc) s t is the same bits as scaled's for all such scales s, t and any sum: nothing on the way overflows
 // or becomes subnormal, and powers of two change no rounding.
 __device__ __forceinline__ bool middling(float s) { return s == 0.0f || (s >= 0x1.0p-60f && s <= 0x1.0p40f); }

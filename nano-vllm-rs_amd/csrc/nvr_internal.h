@@ -54,7 +54,7 @@ bool gemm_rows_fits(const nv_context* c, const void* x, const void* w, int m, in
 // Status of the most recent launch on this thread.
 inline int launch_status() { return hip_status(hipGetLastError(), "HIP kernel launch"); }
 
-__host__ __device__ inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 }  // namespace nvr
 

@@ -3,10 +3,6 @@
 // No counterpart in the reference, whose weights and products are bf16
 // (kernels/kernels.cu:98-106). The arithmetic is in nvr_int8.h.
 //
-// Bound by memory: 3 bytes an element move (7 with a residual). A row is read
-// once and stays in registers: up to 4096 values by one wave, so no barrier is
-// waited for, up to 16384 by the four waves of a block; longer rows are read twice. With few rows four waves a row are taken below 4096 too, for
-// more loads in flight.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
@@ -16,36 +12,40 @@ namespace {
 using nvr::kWave;
 using nvr::Tokens;
 
-constexpr int kThreads = 256;
-
-// The four waves of a row exchange through LDS.
+// The waves of a row exchange through LDS.
+template <int WAVES>
 struct BlockJoin {
     float* sum;
     uint32_t* top;
     int lane, wave;
     __device__ void operator()(float* s, uint32_t& t) const {
+        constexpr int MINE = nvr::kClasses / WAVES;
         if (lane == 0) {
-            sum[wave] = s[0];
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) sum[i * WAVES + wave] = s[i];
             top[wave] = t;
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < nvr::kClasses; ++i) s[i] = sum[i];
-        t = max(max(top[0], top[1]), max(top[2], top[3]));
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) t = max(t, top[i]);
     }
 };
 
 // CH chunks a lane of WAVES waves hold a row; 0: a row of any length, read twice.
+template <int WAVES>
+constexpr int kThreads = WAVES == 16 ? 1024 : 256;
 template <Tokens T, bool WHOLE, int CH, int WAVES>
-__global__ __launch_bounds__(kThreads) void quantize_rows(nvr::TokenArgs t, uint8_t* __restrict__ q,
-                                                          float* __restrict__ scales, int pitch) {
+__global__ __launch_bounds__(kThreads<WAVES>) void quantize_rows(nvr::TokenArgs t, uint8_t* __restrict__ q,
+                                                                 float* __restrict__ scales, int pitch) {
     __shared__ float sum[nvr::kClasses];
-    __shared__ uint32_t top[nvr::kClasses];
+    __shared__ uint32_t top[WAVES];
+    constexpr int kRows = kThreads<WAVES> / kWave / WAVES;  // rows of a block at a time
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, of_row = WAVES == 1 ? 0 : wave;
-    constexpr int kRows = kThreads / kWave / WAVES;  // rows of a block at a time
     const int64_t first = int64_t(blockIdx.x) * kRows + (WAVES == 1 ? wave : 0), step = int64_t(gridDim.x) * kRows;
     const bool keep_sum = t.residual_out != nullptr;
-    using Join = std::conditional_t<WAVES == 1, nvr::NoJoin, BlockJoin>;
+    using Join = std::conditional_t<WAVES == 1, nvr::NoJoin, BlockJoin<WAVES>>;
     Join join;
     if constexpr (WAVES != 1) join = {sum, top, lane, wave};
     nvr::NormChunks<CH == 0 ? 1 : CH> norm;
@@ -64,33 +64,41 @@ __global__ __launch_bounds__(kThreads) void quantize_rows(nvr::TokenArgs t, uint
     }
 }
 
+// Bound by memory: 3 bytes an element move (7 with a residual): 8192 rows of 4096 in 25 us, 4.0 TB/s, with sum and norm
+// 4096 rows in 28 us, 4.2 TB/s. A row is read once and stays in registers. With many rows one wave takes up to 4096
+// values, so that it waits for no barrier, four up to 16384. With few, latency counts: 4 waves take up to 2048, 16 up to
+// 16384, in as little code as that gives (it is read anew by each launch: 3 odd rows of 8989 by 4 waves of 8 chunks 10 us).
+// Longer rows are read twice.
 template <Tokens T, bool WHOLE>
 void launch(nv_context* c, const nvr::TokenArgs& t, uint8_t* q, float* scales, int pitch) {
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
     const int64_t rows = t.rows;
     auto run = [&](auto chunks, auto waves) {
-        constexpr int CH = decltype(chunks)::value, WAVES = decltype(waves)::value, kRows = kThreads / kWave / WAVES;
+        constexpr int CH = decltype(chunks)::value, WAVES = decltype(waves)::value;
+        constexpr int kRows = kThreads<WAVES> / kWave / WAVES;
         const int64_t blocks = std::min<int64_t>((rows + kRows - 1) / kRows, 1 << 20);  // further rows are taken in turn
-        hipLaunchKernelGGL((quantize_rows<T, WHOLE, CH, WAVES>), dim3(unsigned(blocks)), dim3(kThreads), 0, c->stream, t, q,
-                           scales, pitch);
+        hipLaunchKernelGGL((quantize_rows<T, WHOLE, CH, WAVES>), dim3(unsigned(blocks)), dim3(kThreads<WAVES>), 0, c->stream,
+                           t, q, scales, pitch);
     };
     using std::integral_constant;
-    const integral_constant<int, 1> one;
-    const integral_constant<int, 4> four;
     const integral_constant<int, 0> any;
+    const integral_constant<int, 1> one;
     const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
     const integral_constant<int, 8> eight;
-    if (rows >= 4 * cus && pitch <= 8 * nvr::kWaveChunk) {
-        if (pitch <= 2 * nvr::kWaveChunk) run(two, one);
-        else if (pitch <= 4 * nvr::kWaveChunk) run(four, one);
-        else run(eight, one);
+    const integral_constant<int, 16> sixteen;
+    const int chunks = (pitch + nvr::kWaveChunk - 1) / nvr::kWaveChunk;
+    if (rows >= 4 * cus && chunks <= 32) {
+        if (chunks <= 2) run(two, one);
+        else if (chunks <= 4) run(four, one);
+        else if (chunks <= 8) run(eight, one);
+        else if (chunks <= 16) run(four, four);
+        else run(eight, four);
     } else {
-        const int chunk = 4 * nvr::kWaveChunk;
-        if (pitch <= chunk) run(one, four);
-        else if (pitch <= 2 * chunk) run(two, four);
-        else if (pitch <= 4 * chunk) run(four, four);
-        else if (pitch <= 8 * chunk) run(eight, four);
-        else run(any, four);
+        if (chunks <= 4) run(one, four);
+        else if (chunks <= 16) run(one, sixteen);
+        else if (chunks <= 32) run(two, sixteen);
+        else run(any, sixteen);
     }
 }
 
