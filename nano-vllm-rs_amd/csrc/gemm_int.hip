@@ -396,8 +396,8 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
         return nvr::launch_status();
     }
     nvr::launch_quantize(c, t, xq, xs, pitch);
-    if (weight_streams(c, p, GATED)) launch_rows<Source::kCopied, true, GATED>(c, few);
-    else nvr::launch_product_tiles(c, p, GATED);
+    if (!weight_streams(c, p, GATED)) return nvr::launch_product_tiles(c, p, GATED);
+    launch_rows<Source::kCopied, true, GATED>(c, few);
     return nvr::launch_status();
 }
 

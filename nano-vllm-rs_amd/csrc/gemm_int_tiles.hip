@@ -23,8 +23,9 @@ struct Shape {
     static constexpr int XR = BM / WAVES, WR = BN / WAVES;                       // rows that a wave copies
     static constexpr int COPIES = (XR + WR) / ROWS;                              // instructions of a wave a stage
     static constexpr int kStageBytes = (BM + BN) * KB;
+    static constexpr int kLds = STAGES * kStageBytes + (BM + BN) * 4;            // and the scales
     static_assert(XR % ROWS == 0 && WR % ROWS == 0 && TM % 16 == 0 && TN % 32 == 0, "whole copies and products");
-    static_assert(STAGES * kStageBytes <= 160 * 1024 && (KB == 64 || KB == 128), "LDS");
+    static_assert(kLds <= 160 * 1024 && (KB == 64 || KB == 128), "LDS");
 };
 
 // Waits until all but the last `late` stages' copies of this wave have landed.
@@ -129,9 +130,17 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
         const int i = q / S::MI, j = q % S::MI;
         acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[slot][i], xf[slot][j], acc[i][j], 0, 0, 0);
     };
+    // The scales come first, so that no epilogue waits for them: [BM] of tokens, [BN] of channels (gated: half of gate, half
+    // of up).
+    float* scales = reinterpret_cast<float*>(smem + S::STAGES * S::kStageBytes);
+    for (int i = threadIdx.x; i < S::BM + S::BN; i += S::THREADS) {
+        const int c = i - S::BM, half = GATED ? S::BN / 2 : S::BN;
+        scales[i] = c < 0 ? p.xs[min(m0 + i, int64_t(p.m) - 1)]
+                          : p.ws[(c < half ? 0 : int64_t(p.n)) + min(n0 + (c < half ? c : c - half), p.n - 1)];
+    }
     for (int s = 0; s < S::STAGES && s < steps; ++s) stage(s, s);
     wait_stages<S>(min(steps, S::STAGES) - 1);
-    asm volatile("s_barrier" ::: "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
     for (int r = 0; r < READS; ++r) fetch(0, smem, 0, r);
     int buffer = 0;
@@ -180,12 +189,13 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     bool plain = true;
 #pragma unroll
     for (int j = 0; j < S::MI; ++j) {
-        xs[j] = p.xs[min(t0 + j * 16 + lane % 16, int64_t(p.m) - 1)];
+        xs[j] = scales[wm * S::TM + j * 16 + lane % 16];
         plain = plain && nvr::middling(xs[j]);
     }
+    const float* wscales = scales + S::BM + wn * OUT;
     if (lane < OUT) {
-        plain = plain && nvr::middling(p.ws[min(c0 + lane, p.n - 1)]);
-        if constexpr (GATED) plain = plain && nvr::middling(p.ws[int64_t(p.n) + min(c0 + lane, p.n - 1)]);
+        plain = plain && nvr::middling(wscales[lane]);
+        if constexpr (GATED) plain = plain && nvr::middling(wscales[S::BN / 2 + lane]);
     }
     auto outputs = [&](auto scale) {
 #pragma unroll
@@ -195,9 +205,8 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
             float ws[4], us[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int channel = min(c0 + at + r, p.n - 1);
-                ws[r] = p.ws[channel];
-                if constexpr (GATED) us[r] = p.ws[int64_t(p.n) + channel];
+                ws[r] = wscales[at + r];
+                us[r] = GATED ? wscales[S::BN / 2 + at + r] : 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < S::MI; ++j) {
@@ -377,44 +386,67 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     }
 }
 
-template <int TOK, int SIDE, int SLOTS, bool GATED>
-void launch_split(nv_context* c, const nvr::ProductArgs& p) {
-    constexpr int kChannels = GATED ? SIDE / 2 : SIDE;
-    const int mt = int((int64_t(p.m) + TOK - 1) / TOK), nt = (p.n + kChannels - 1) / kChannels;
-    hipLaunchKernelGGL((gemm_split<TOK, SIDE, SLOTS, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads), kSplit * SLOTS * (TOK + SIDE) * kUnitBytes, c->stream, p,
-                       mt, nt);
+// A grid dimension holds fewer than 2^32 work-items.
+int refuse_grid(int64_t mt, int64_t nt, int threads) {
+    if (mt * nt < (int64_t(1) << 32) / threads) return 0;
+    return nvr::fail(-2, "gemm_i8: %lld tiles of tokens by %lld of channels are more than one launch", (long long)mt,
+                     (long long)nt);
 }
 
 template <class S, bool GATED>
-void launch(nv_context* c, const nvr::ProductArgs& p) {
+int launch(nv_context* c, const nvr::ProductArgs& p) {
     constexpr int kChannels = GATED ? S::BN / 2 : S::BN;
     const int mt = int((int64_t(p.m) + S::BM - 1) / S::BM), nt = (p.n + kChannels - 1) / kChannels;
-    hipLaunchKernelGGL((gemm_tiles<S, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(S::THREADS), S::STAGES * S::kStageBytes,
-                       c->stream, p, mt, nt);
+    if (int error = refuse_grid(mt, nt, S::THREADS)) return error;
+    hipLaunchKernelGGL((gemm_tiles<S, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(S::THREADS), S::kLds, c->stream, p, mt,
+                       nt);
+    return nvr::launch_status();
+}
+
+template <int TOK, int SIDE, int SLOTS, bool GATED>
+int launch_split(nv_context* c, const nvr::ProductArgs& p) {
+    constexpr int kChannels = GATED ? SIDE / 2 : SIDE;
+    const int mt = int((int64_t(p.m) + TOK - 1) / TOK), nt = (p.n + kChannels - 1) / kChannels;
+    if (int error = refuse_grid(mt, nt, kSplitThreads)) return error;
+    hipLaunchKernelGGL((gemm_split<TOK, SIDE, SLOTS, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads),
+                       kSplit * SLOTS * (TOK + SIDE) * kUnitBytes, c->stream, p, mt, nt);
+    return nvr::launch_status();
 }
 
 }  // namespace
 
 namespace nvr {
 
-void launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
+// The tile by tokens and by turns: how often the CUs are filled. On MI355X, weights cold, in us of the product alone:
+//   a tile's k over four waves while there is a tile a CU: 256 tokens over 1024 x 2048 by tiles of 64 x 32, 64 x 64 and
+//   128 x 128 5.2, 7.3, 11.2; 100 over 6144 x 4096 13.1 (in two turns), 10.9, 15.2; 512 over 4096 x 1024 (two turns of 64 x
+//   64) -, 10.7, 7.9;
+//   up to 64 tokens over wide weights, 64 x 128 and 128 x 128: 64 over 151936 x 1024 41.2, 46.1; over 32768 x 4096 38.8,
+//   44.8 (and 64 x 64 40.6);
+//   256 x 256 against 128 x 128, two of which share a CU: 8192 over 12288 x 4096 (6 turns, 24) 356, 422; 4096 over 4096 x
+//   1024 (1, 4) 23.2, 24.6; 768 over 12288 x 4096 (1, 3) 48.9, 52.1; 1500 over 4096 x 12288 (1, 2) 125, 85; 2048 over 4096 x
+//   1024 (1, 2) 20.8, 14.2. Where k is short, a tile is mostly its outputs, which two blocks overlap: 5327 over 18704 x 176
+//   (7, 25) 77.6, 67.6; 8192 over 8192 x 512 (4, 16) 59.9, 65.8; gated 2244 over 8001 x 1024 (3, 9) 63.2, 57.0.
+int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
     using Large = Shape<256, 256, 2, 4, 128, 2>;
     using Medium = Shape<128, 128, 4, 2, 128, 2>;
     using Wide = Shape<64, 128, 4, 2, 128, 3>;
+    constexpr int kShort = 384;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256, rows = gated ? 2 * int64_t(p.n) : p.n;
     auto tiles = [&](int tokens, int side) { return (int64_t(p.m) + tokens - 1) / tokens * ((rows + side - 1) / side); };
     auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
     auto run = [&](auto g) {
         constexpr bool G = decltype(g)::value;
-        if (p.m <= 16) launch_split<16, 32, 2, G>(c, p);
-        else if (p.m <= 32) launch_split<32, 32, 2, G>(c, p);
-        else if (tiles(64, 32) <= cus) launch_split<64, 32, 2, G>(c, p);
-        else if (tiles(64, 64) <= cus) launch_split<64, 64, 2, G>(c, p);
-        else if (p.m <= 64) launch<Wide, G>(c, p);
-        else if (3 * turns(tiles(256, 256)) > turns(tiles(128, 128))) launch<Medium, G>(c, p);
-        else launch<Large, G>(c, p);
+        if (p.m <= 16) return launch_split<16, 32, 2, G>(c, p);
+        if (p.m <= 32) return launch_split<32, 32, 2, G>(c, p);
+        if (tiles(64, 32) <= cus) return launch_split<64, 32, 2, G>(c, p);
+        if (tiles(64, 64) <= cus) return launch_split<64, 64, 2, G>(c, p);
+        if (p.m <= 64) return launch<Wide, G>(c, p);
+        const int64_t large = 3 * turns(tiles(256, 256)) + (p.w_pitch <= 1024 ? 1 : 0);
+        if (p.w_pitch <= kShort || large > turns(tiles(128, 128))) return launch<Medium, G>(c, p);
+        return launch<Large, G>(c, p);
     };
-    gated ? run(std::true_type{}) : run(std::false_type{});
+    return gated ? run(std::true_type{}) : run(std::false_type{});
 }
 
 }  // namespace nvr
