@@ -395,8 +395,11 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
         k % nvr::kChunk == 0 ? run(std::true_type{}) : run(std::false_type{});
         return nvr::launch_status();
     }
+    const bool streams = weight_streams(c, p, GATED);
+    if (!streams)
+        if (int error = nvr::launch_product_tiles(c, p, GATED, true)) return error;
     nvr::launch_quantize(c, t, xq, xs, pitch);
-    if (!weight_streams(c, p, GATED)) return nvr::launch_product_tiles(c, p, GATED);
+    if (!streams) return nvr::launch_product_tiles(c, p, GATED, false);
     launch_rows<Source::kCopied, true, GATED>(c, few);
     return nvr::launch_status();
 }

@@ -65,12 +65,12 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     // different ones of the 64 banks.
     auto place = [](int r, int c) { return S::PIECES == 8 ? c ^ (r / 2 % 8) : c ^ (r / 4 % 4); };
     const int at = lane / S::PIECES;  // a copy's row of this lane
-    auto piece = [&](int u) { return place(u * S::ROWS + at, lane % S::PIECES); };
+    auto piece = [&](int rows, int u) { return place(wave * rows + u * S::ROWS + at, lane % S::PIECES); };
     uint32_t xoff[S::XR / S::ROWS], woff[S::WR / S::ROWS];
 #pragma unroll
     for (int u = 0; u < S::XR / S::ROWS; ++u) {
         const int64_t row = min(m0 + wave * S::XR + u * S::ROWS + at, int64_t(p.m) - 1);
-        xoff[u] = uint32_t(row - m0) * uint32_t(p.x_pitch) + piece(u) * 16;
+        xoff[u] = uint32_t(row - m0) * uint32_t(p.x_pitch) + piece(S::XR, u) * 16;
     }
     // Gated, every 32 rows of gate are followed by the 32 of up for the same channels.
     const bool up = GATED && (wave * S::WR / 32) % 2 != 0;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     for (int u = 0; u < S::WR / S::ROWS; ++u) {
         const int r = wave * S::WR + u * S::ROWS + at;
         const int row = min(n0 + (GATED ? r / 64 * 32 + r % 32 : r), p.n - 1);
-        woff[u] = uint32_t(row - n0) * uint32_t(p.w_pitch) + piece(u) * 16;
+        woff[u] = uint32_t(row - n0) * uint32_t(p.w_pitch) + piece(S::WR, u) * 16;
     }
     const uint8_t* xbase = p.xq + m0 * p.x_pitch;
     const uint8_t* wbase = p.wq + (int64_t(n0) + (up ? int64_t(p.n) : 0)) * p.w_pitch;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
         const int past = p.w_pitch - 16 - step * S::KB;
         if (past < S::KB - 16) {  // the last: past its row a weight's bytes meet zeros of x, any bytes of the row will do
 #pragma unroll
-            for (int u = 0; u < S::WR / S::ROWS; ++u) woff[u] -= max(piece(u) * 16 - past, 0);
+            for (int u = 0; u < S::WR / S::ROWS; ++u) woff[u] -= max(piece(S::WR, u) * 16 - past, 0);
         }
 #pragma unroll
         for (int u = 0; u < S::XR / S::ROWS; ++u)
@@ -394,20 +394,20 @@ int refuse_grid(int64_t mt, int64_t nt, int threads) {
 }
 
 template <class S, bool GATED>
-int launch(nv_context* c, const nvr::ProductArgs& p) {
+int launch(nv_context* c, const nvr::ProductArgs& p, bool check) {
     constexpr int kChannels = GATED ? S::BN / 2 : S::BN;
     const int mt = int((int64_t(p.m) + S::BM - 1) / S::BM), nt = (p.n + kChannels - 1) / kChannels;
-    if (int error = refuse_grid(mt, nt, S::THREADS)) return error;
+    if (check) return refuse_grid(mt, nt, S::THREADS);
     hipLaunchKernelGGL((gemm_tiles<S, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(S::THREADS), S::kLds, c->stream, p, mt,
                        nt);
     return nvr::launch_status();
 }
 
 template <int TOK, int SIDE, int SLOTS, bool GATED>
-int launch_split(nv_context* c, const nvr::ProductArgs& p) {
+int launch_split(nv_context* c, const nvr::ProductArgs& p, bool check) {
     constexpr int kChannels = GATED ? SIDE / 2 : SIDE;
     const int mt = int((int64_t(p.m) + TOK - 1) / TOK), nt = (p.n + kChannels - 1) / kChannels;
-    if (int error = refuse_grid(mt, nt, kSplitThreads)) return error;
+    if (check) return refuse_grid(mt, nt, kSplitThreads);
     hipLaunchKernelGGL((gemm_split<TOK, SIDE, SLOTS, GATED>), dim3(unsigned(mt) * unsigned(nt)), dim3(kSplitThreads),
                        kSplit * SLOTS * (TOK + SIDE) * kUnitBytes, c->stream, p, mt, nt);
     return nvr::launch_status();
@@ -427,7 +427,7 @@ namespace nvr {
 //   1024 (1, 4) 23.2, 24.6; 768 over 12288 x 4096 (1, 3) 48.9, 52.1; 1500 over 4096 x 12288 (1, 2) 125, 85; 2048 over 4096 x
 //   1024 (1, 2) 20.8, 14.2. Where k is short, a tile is mostly its outputs, which two blocks overlap: 5327 over 18704 x 176
 //   (7, 25) 77.6, 67.6; 8192 over 8192 x 512 (4, 16) 59.9, 65.8; gated 2244 over 8001 x 1024 (3, 9) 63.2, 57.0.
-int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
+int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated, bool check) {
     using Large = Shape<256, 256, 2, 4, 128, 2>;
     using Medium = Shape<128, 128, 4, 2, 128, 2>;
     using Wide = Shape<64, 128, 4, 2, 128, 3>;
@@ -437,14 +437,14 @@ int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated) {
     auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
     auto run = [&](auto g) {
         constexpr bool G = decltype(g)::value;
-        if (p.m <= 16) return launch_split<16, 32, 2, G>(c, p);
-        if (p.m <= 32) return launch_split<32, 32, 2, G>(c, p);
-        if (tiles(64, 32) <= cus) return launch_split<64, 32, 2, G>(c, p);
-        if (tiles(64, 64) <= cus) return launch_split<64, 64, 2, G>(c, p);
-        if (p.m <= 64) return launch<Wide, G>(c, p);
+        if (p.m <= 16) return launch_split<16, 32, 2, G>(c, p, check);
+        if (p.m <= 32) return launch_split<32, 32, 2, G>(c, p, check);
+        if (tiles(64, 32) <= cus) return launch_split<64, 32, 2, G>(c, p, check);
+        if (tiles(64, 64) <= cus) return launch_split<64, 64, 2, G>(c, p, check);
+        if (p.m <= 64) return launch<Wide, G>(c, p, check);
         const int64_t large = 3 * turns(tiles(256, 256)) + (p.w_pitch <= 1024 ? 1 : 0);
-        if (p.w_pitch <= kShort || large > turns(tiles(128, 128))) return launch<Medium, G>(c, p);
-        return launch<Large, G>(c, p);
+        if (p.w_pitch <= kShort || large > turns(tiles(128, 128))) return launch<Medium, G>(c, p, check);
+        return launch<Large, G>(c, p, check);
     };
     return gated ? run(std::true_type{}) : run(std::false_type{});
 }

@@ -68,8 +68,8 @@ struct ProductArgs {
     int m, n, x_pitch, w_pitch;
 };
 
-// Products of whole tiles (gemm_int_tiles.hip); the launch's status.
-int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated);
+// Products of whole tiles (gemm_int_tiles.hip): the launch's status; with `check`, whether one launch holds them.
+int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated, bool check);
 
 __device__ __forceinline__ void store8(uint16_t* to, uint4 v);
 

@@ -140,10 +140,19 @@ def test_products_of_long_rows(gpu, m, n, k, norm):
     call.check()
 
 
-@pytest.mark.parametrize("m,n,k,gated", [(4100, 4097, 40, False), (3900, 4344, 136, False), (4100, 2050, 72, True),
-                                         (4111, 2059, 160, True)])
+@pytest.mark.parametrize("m,n,k,gated", [
+    # few tokens over wide weights: made in the block, several tiles a wave, lines of outputs kept and not
+    (1, 40000, 136, False), (3, 20001, 264, False), (8, 70000, 72, False), (8, 12001, 520, True), (5, 9000, 2048, False),
+    (2, 12000, 4096, False), (16, 33000, 1000, False), (13, 9001, 64, True), (1, 12345, 1111, False), (7, 20008, 333, True),
+    # made by a launch of their own, then brought to LDS
+    (9, 20000, 1032, False), (16, 18001, 2056, False), (24, 17000, 264, False), (32, 40008, 144, False), (29, 9001, 1030, True),
+    (32, 8400, 2048, True),
+    # tiles of 64 tokens by 128 rows of the weight, of 128 by 128 where k is short, and of 256 by 256
+    (40, 17001, 72, False), (64, 16700, 400, False), (63, 8300, 264, True), (300, 4001, 500, False), (4100, 4097, 40, False),
+    (260, 4200, 1030, True), (3900, 4344, 136, False), (4111, 2059, 160, True), (4090, 4089, 1050, False),
+    (4090, 2043, 1040, True)])
 @pytest.mark.parametrize("norm", ["none", "add"])
-def test_products_of_many_tokens(gpu, m, n, k, gated, norm):
+def test_products_in_every_form(gpu, m, n, k, gated, norm):
     call = Call(gpu, m, n, k, norm, gated, seed=n)
     call.run()
     call.check()
@@ -163,7 +172,7 @@ def test_sums_of_the_longest_rows_stay_exact(gpu, m):
 
 @pytest.mark.parametrize("m,batches", [(300, (1, 5, 16, 17, 32, 33, 64, 130))])
 @pytest.mark.parametrize("norm", ["none", "add"])
-@pytest.mark.parametrize("n,k", [(300, 1024), (128, 4096), (72, 1111), (4500, 512)])
+@pytest.mark.parametrize("n,k", [(300, 1024), (128, 4096), (72, 1111), (4500, 512), (17000, 264), (2100, 10000)])
 def test_a_token_has_the_same_bits_in_any_batch(gpu, m, batches, n, k, norm):
     whole = Call(gpu, m, n, k, norm, seed=9)
     whole.run()
@@ -334,6 +343,8 @@ def test_the_library_refuses(gpu):
                    dict(w_scales=None), dict(y=None), dict(w=p + 8), dict(x=p + 1), dict(y=far + 1), dict(w_scales=p + 2),
                    dict(residual=p), dict(residual_out=p), dict(norm_weight=p, residual_out=p), dict(workspace=p + 4104)):
         assert product(**change) == (-2, -2), change
+    # More tiles than one launch holds: nothing is read or written.
+    assert lib.nv_gemm_i8(h, p, None, None, None, p, p, far, p + 4096, 40, 2 ** 31 - 1000, 16, 1e-6) == -2
     for args in ((None, p, p, 1, 16), (p, None, p, 1, 16), (p, p, None, 1, 16), (p, far, p, 0, 16), (p, far, p, 1, 0),
                  (p, far, p, 1, 131072), (p + 1, far, p, 1, 16), (p, far + 8, p, 1, 16), (p, far, p + 2, 1, 16)):
         assert lib.nv_quantize_rows(h, *args) == -2, args
