@@ -171,6 +171,9 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     auto flush = [&] {
         const int end = (tile0 + round + 1) * kChannels;
         if (round >= tile_count || (end % 64 != 0 && round + 1 < tile_count)) return;
+        // finish wrote values of another type, which the compiler may take to be elsewhere; the wave's LDS accesses themselves
+        // are in order, and so are the next lines' writes behind these reads.
+        asm volatile("" ::: "memory");
         const int channel = (end - 1) / 64 * 64 + lane % 8 * 8;
         if (channel < tile0 * kChannels || channel >= min(end, p.n)) return;
 #pragma unroll
@@ -178,6 +181,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
             if (r + lane / 8 < p.m)
                 nvr::store8(p.y + int64_t(r + lane / 8) * p.n + channel,
                             *reinterpret_cast<const uint4*>(kept + (r + lane / 8) * 128 + lane % 8 * 16));
+        asm volatile("" ::: "memory");
     };
     auto multiply = [&](const Unit& u) {
         if (at == 0) {

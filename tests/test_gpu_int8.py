@@ -246,6 +246,43 @@ def test_a_captured_product_follows_its_inputs(gpu, m, gated):
         c.check()
 
 
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_two_graphs_share_a_workspace(gpu, m):
+    """Captured products that use one workspace in turn on one stream, each replayed several times in changing order."""
+    calls = [Call(gpu, m, 264, 2056, "add", False, seed=1), Call(gpu, m, 136, 1000, "rms", True, seed=2)]
+    shared = gpu.upload_array(np.full(max(c.need for c in calls) + GUARD, 0x5A, np.uint8))
+    for c in calls:
+        c.work = shared
+    graphs = [gpu.capture(c.run) for c in calls]
+    for order in ((0, 1), (1, 0), (1, 1, 0), (0, 0, 1)):
+        for i in order:
+            calls[i].by.upload(np.full(calls[i].by.bytes, 0xA5, np.uint8))
+            graphs[i].replay()
+        for c in calls:
+            c.check()
+
+
+@pytest.mark.parametrize("m", [2, 14, 60, 300])
+def test_x_and_the_residual_may_be_one_buffer(gpu, m):
+    c = Call(gpu, m, 72, 520, "add", seed=5)
+    c.residual, c.bres = c.x, c.bx
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("rows,k", [(3, 700), (1200, 512)])
+def test_a_captured_quantize_rows_follows_its_rows(gpu, rows, k):
+    bx, q, s = gpu.alloc(rows * k * 2), gpu.alloc(rows * ref.pitch(k)), gpu.alloc(rows * 4)
+    bx.upload(ora.normal_bf16((rows, k), 1))
+    graph = gpu.capture(lambda: gpu.quantize_rows(bx, q, s, rows, k))
+    for replay in range(3):
+        x = ora.normal_bf16((rows, k), 60 + replay)
+        bx.upload(x)
+        graph.replay()
+        want, _ = ref.whole_numbers(f64(x))
+        assert_bits_equal(q.download(np.int8, rows * ref.pitch(k)).reshape(rows, -1)[:, :k], want)
+
+
 def test_two_programs_at_once(gpu):
     """Calls of two contexts, each with a workspace of its own, in turns without waiting."""
     other = nvr.Gpu(0)
