@@ -330,8 +330,9 @@ int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
  *   x                            norm_weight NULL (residual and residual_out too),
  *   RMSNorm(x)                   residual NULL (residual_out too),
  *   RMSNorm(x + residual)        with residual_out <- bf16(x + residual), unless NULL;
- * the norm in fp32 (as nv_rms but for roundings, its values not rounded to bf16). x, residual, residual_out: [m, k] bf16, residual_out another buffer than
- * the others; norm_weight: [k] bf16; w, w_scales as nv_quantize_rows' q and scales
+ * the norm in fp32 (as nv_rms but for roundings, its values not rounded to bf16).
+ * x, residual, residual_out: [m, k] bf16, residual_out another buffer than the
+ * others; norm_weight: [k] bf16; w, w_scales as nv_quantize_rows' q and scales
  * (integers of any source; -128 too); y: [m, n] bf16. Sums of products are exact,
  * so a token's outputs are the same bits in any batch. A token with a NaN or an
  * infinity (or whose product with the norm's weight leaves fp32) has NaN in its row

@@ -11,6 +11,14 @@
 // those fp32 values of channels j and inter + j: bf16(g / (1 + e^-g) * u).
 // Integer sums have no order, so every form gives the same bits for a token,
 // whatever the batch.
+//
+// Three forms. Up to 16 tokens over short rows are made into integers by every
+// block, and up to 32 over wide weights are brought to LDS; gemm_rows_i8 then
+// streams the weights through registers, each byte once, bound by HBM and, in the
+// smallest calls, by one chain: tokens, their largest value, products, outputs. All
+// others go by tiles (gemm_int_tiles.hip). On MI355X: 1 token over 1024 x 2048 3.4
+// us, 8 with sum and norm over 4096 x 1024 4.2 us; 32 over 151936 x 1024 38.7 us with
+// the tokens' launch, 4.3 TB/s.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
@@ -21,7 +29,6 @@ using nvr::kWave;
 using nvr::Scale;
 using nvr::Tokens;
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
-typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int kWaves = 8, kThreads = kWaves * kWave;
 constexpr int kRowPad = 16;  // behind a token's row in LDS: 16 tokens' pieces of one column lie in different banks
@@ -36,7 +43,7 @@ struct RowsArgs {
     nvr::ProductArgs p;
     nvr::TokenArgs t;
     int log_parts;              // 2^log_parts waves share the k of a tile: 1, 2, 4 or 8
-    int tiles, per, more;       // a block has `per` tiles, the first `more` blocks one more
+    int per, more;              // a block has `per` tiles, the first `more` blocks one more
     int share, units;           // lines of 128 bytes of k a wave has of a tile; loads of STEPS steps
 };
 
@@ -49,7 +56,8 @@ int64_t rows_lds(int m, int x_pitch) {
 }
 
 // Few tokens: the weights stream through registers, once, STEPS pieces of 64 bytes of k in flight together as a unit, and
-// two units. ONE: every wave has one unit at most in all.
+// two units; 16 rows of the weight are a product's first operand, so that nothing of it passes LDS. ONE: every wave has one
+// unit at most in all.
 template <Source SRC, bool WHOLE, int CH, int RW, int MT, bool GATED, int STEPS, bool ONE>
 __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
     constexpr bool kMade = SRC != Source::kCopied;
@@ -91,7 +99,8 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         const uint8_t* w = p.wq + row * p.w_pitch;
         const int s = s0 + ahead * STEPS;
 #pragma unroll
-        for (int e = 0; e < STEPS; ++e) u.w[e] = *reinterpret_cast<const uint4*>(w + min(min(s + e, last_step) * 64 + 16 * g, p.w_pitch - 16));
+        for (int e = 0; e < STEPS; ++e)
+            u.w[e] = *reinterpret_cast<const uint4*>(w + min(min(s + e, last_step) * 64 + 16 * g, p.w_pitch - 16));
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             u.ws[r] = GATED ? p.ws[int64_t(g < 2 ? 0 : p.n) + min(tile * 8 + 4 * (g % 2) + r, p.n - 1)]
@@ -192,6 +201,9 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
         for (int r = 0; r < 4; ++r) ws[r] = u.ws[r];
         const int s = s0 + at * STEPS;
         auto tokens = [&](int t, int e) { return *reinterpret_cast<const i32x4_t*>(xrow[t] + (s + e) * 64); };
+        auto product = [](i32x4_t& sum, const uint4& w, i32x4_t x) {
+            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, w), x, sum, 0, 0, 0);
+        };
         if (s + STEPS <= s1) {
             i32x4_t x[STEPS][MT];
 #pragma unroll
@@ -202,14 +214,14 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
             for (int e = 0; e < STEPS; ++e)
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]), x[e][t], acc[t], 0, 0, 0);
+                    product(acc[t], u.w[e], x[e][t]);
         } else {
 #pragma unroll
             for (int e = 0; e < STEPS; ++e) {
                 if (s + e >= s1) break;
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
-                    acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, u.w[e]), tokens(t, e), acc[t], 0, 0, 0);
+                    product(acc[t], u.w[e], tokens(t, e));
             }
         }
         ++at;
@@ -280,7 +292,6 @@ void launch_rows_as(nv_context* c, const RowsArgs& a, int blocks) {
 void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
     const int lines = a.p.x_pitch / 128;
     a.log_parts = __builtin_ctz(unsigned(parts));
-    a.tiles = tiles;
     a.per = tiles / blocks;
     a.more = tiles % blocks;
     a.share = (lines + parts - 1) / parts;
@@ -321,27 +332,39 @@ void launch_rows(nv_context* c, RowsArgs a) {
     if constexpr (SRC == Source::kCopied) {
         a.p.m <= 16 ? run(one, one, one) : run(one, one, two);
     } else {
-        if (a.p.m > kWaves) run(two, two, one);
-        else if (a.p.x_pitch <= 2 * nvr::kWaveChunk) run(two, one, one);
-        else if (a.p.x_pitch <= 4 * nvr::kWaveChunk) run(integral_constant<int, 4>{}, one, one);
-        else if constexpr (SRC == Source::kPlain) run(integral_constant<int, 8>{}, one, one);
+        const integral_constant<int, 4> four;
+        const int chunks = (a.p.x_pitch + nvr::kWaveChunk - 1) / nvr::kWaveChunk;
+        if (a.p.m > kWaves) {
+            if constexpr (SRC == Source::kPlain)
+                if (chunks > 2) return run(four, two, one);
+            run(two, two, one);
+        } else if (chunks <= 2) {
+            run(two, one, one);
+        } else if (chunks <= 4) {
+            run(four, one, one);
+        } else {
+            run(integral_constant<int, 8>{}, one, one);
+        }
     }
 }
 
-// Whether each block makes the tokens' integers by itself, a row a wave: one launch less, for work that all blocks
-// repeat. On MI355X in a graph, n 4096, made and by a launch of their own, in us: 8 tokens at k 1024 5.7, 7.2 and with
-// sum and norm 6.3, 7.8; at k 2048 6.4, 7.6 and 7.8, 7.7 (4 tokens: 6.5, 7.4); at k 4096 9.1, 9.8 and 17.8, 12 (a row's
-// chunks, sums and norm weights no longer fit the registers beside the weights). 16 tokens, two rows a wave: at k 1024
-// 6.7, 7.5 and 8.0, 7.8; at k 2048 8.1, 8.1 and 10.9, 8.4.
+// Whether each block makes the tokens' integers by itself, a row or two a wave: one launch less, for work that all blocks
+// repeat. On MI355X in a graph, weights cold, n 4096, made and by a launch of their own, in us:
+//   k 1024: 1 token 3.1, 5.8; 8 with sum and norm 4.2, 6.2; 16 4.3, 5.9, with sum and norm 5.4, 6.4;
+//   k 2048: 8 5.0, 7.3, with sum and norm 6.3, 7.7; 9 to 16 5.1 to 6.1, 7.3 (n 16384 10.9 to 12.3, 11.3); 16 with sum and
+//   norm 8.8, 7.8;
+//   k 4096: 8 8.2, 9.5; with sum and norm 4 8.1, 9.8, but 6 10.5, 9.5: two waves of a SIMD then have a row each, and a row's
+//   chunks, sums and norm weights fill the registers beside the weights.
 bool tokens_in_block(const nvr::TokenArgs& t) {
-    const int chunks = t.rows > kWaves ? 2 : t.norm_weight == nullptr ? 8 : 4;
+    const int most = t.rows <= 4 ? 8 : t.rows <= kWaves ? 4 : 2;  // chunks of a row with a norm
+    const int chunks = t.norm_weight != nullptr ? most : t.rows <= kWaves ? 8 : 4;
     return t.rows <= 2 * kWaves && t.k <= chunks * nvr::kWaveChunk;
 }
 
 // Whether few tokens, made by a launch of their own, take gemm_rows_i8: where a CU would have more than two of
-// gemm_split's tiles in turn and the tokens fit LDS. On MI355X, this and that in us: 16 tokens at k 1024 over n 8192 5.6,
-// 3.9; 16384 6.0, 5.1; 32768 9.6, 10.2; at k 4096 over 8192 11.2, 9.4; 16384 16.7, 19.2; 32768 26.7, 33.1; 32 tokens over
-// 151936 x 1024 37.8, 41.8.
+// gemm_split's tiles of 32 rows in turn and the tokens fit LDS. On MI355X, weights cold, this and that in us: 16 tokens at k
+// 4096 over n 8192 13.4, 12.3; 16384 20.2, 22.4 (at k 3000 17.3, 15.5, at k 5120 27.3, 21.8); 20480 23.6, 23.8; 32768 32.9,
+// 36.7; 32 tokens over 151936 x 1024 42.0, 47.7; gated 24 over 11008 x 4096 26.2, 26.8.
 bool weight_streams(const nv_context* c, const nvr::ProductArgs& p, bool gated) {
     const int64_t rows = gated ? 2 * int64_t(p.n) : p.n, cus = c->cu_count > 0 ? c->cu_count : 256;
     return p.m <= kFewTokens && (rows + 31) / 32 > 2 * cus &&
@@ -388,7 +411,7 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     float* xs = reinterpret_cast<float*>(xq + int64_t(m) * pitch);
     const nvr::ProductArgs p{xq, xs, static_cast<const uint8_t*>(w), static_cast<const float*>(w_scales),
                              static_cast<uint16_t*>(y), m, n, pitch, int(nvr::i8_pitch(k))};
-    const RowsArgs few{p, t, 0, 0, 0, 0, 0, 0};
+    const RowsArgs few{p, t, 0, 0, 0, 0, 0};
     if (tokens_in_block(t)) {
         auto run = [&](auto whole) {
             constexpr bool WHOLE = decltype(whole)::value;

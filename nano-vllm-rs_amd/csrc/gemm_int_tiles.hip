@@ -1,4 +1,16 @@
-// Tiles of nv_gemm_i8 and nv_gemm_i8_silu (gemm_int.hip has the semantics).
+// Tiles of nv_gemm_i8 and nv_gemm_i8_silu (gemm_int.hip has the semantics). No counterpart in the reference
+// (kernels/kernels.cu:98-106 calls a library's bf16 product).
+//
+// gemm_tiles is bound by the matrix units' power: products of random integers alone, from registers, run at 4.0 POPS in
+// 16 x 16 x 64 and 3.35 in 32 x 32 x 32 (the same work a cycle, more energy), with their operands' LDS reads at 3.4 and 3.0,
+// at clocks near 1.8 GHz; of constant data at 4.9. Therefore 16 x 16 x 64 (8192 tokens over 12288 x 4096 349 us for 380), and
+// tiles of 256 x 256, whose operands are read from LDS 64 rows for 128, the largest that registers hold beside two depths of
+// operands. 8192 over 12288 x 4096 takes 350 us, 2.36 POPS; the library's product without scales, in raw 32-bit integers,
+// 389 us, and at 8192 x 8192 x 8192 2.07 POPS.
+//   The two stages of 128 bytes of k take 128 KB of LDS. Three or four stages of 64 bytes, whose barriers come twice as often,
+//   380 us for 349. A depth's operands are read one depth ahead, a read between two products, so that the units never wait.
+//   Outputs go through LDS, so that a store writes whole rows of 128 bytes: 8 bytes a lane into 16 rows at once 631 us for
+//   393. What is left over the products, about 15%, is the first stage's way to LDS and the outputs, in each of 6 turns.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
@@ -13,9 +25,9 @@ constexpr int kXcds = 8;
 
 // A block's tile of BM tokens and BN channels (gated: BN / 2 of gate and of up), by WM x WN waves; STAGES stages in LDS of
 // KB bytes of k of each row.
-template <int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_>
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = 128, STAGES = STAGES_;
     static constexpr int WAVES = WM * WN, THREADS = WAVES * kWave;
     static constexpr int TM = BM / WM, TN = BN / WN, MI = TM / 16, NI = TN / 16;  // a wave's products of 16 x 16
     static constexpr int SUB = KB / 64;                                          // products' depths of a stage
@@ -25,18 +37,17 @@ struct Shape {
     static constexpr int kStageBytes = (BM + BN) * KB;
     static constexpr int kLds = STAGES * kStageBytes + (BM + BN) * 4;            // and the scales
     static_assert(XR % ROWS == 0 && WR % ROWS == 0 && TM % 16 == 0 && TN % 32 == 0, "whole copies and products");
-    static_assert(kLds <= 160 * 1024 && (KB == 64 || KB == 128), "LDS");
+    static_assert(kLds <= 160 * 1024, "LDS");
 };
 
 // Waits until all but the last `late` stages' copies of this wave have landed.
 template <class S>
 __device__ __forceinline__ void wait_stages(int late) {
     constexpr int C = S::COPIES;
-    static_assert(S::STAGES <= 4 && (S::STAGES - 1) * C < 64, "vmcnt");
+    static_assert(S::STAGES <= 3 && (S::STAGES - 1) * C < 64, "vmcnt");
     if (late == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     else if (S::STAGES == 2 || late == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C) : "memory");
-    else if (S::STAGES == 3 || late == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
-    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(std::min(3 * C, 63)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
 }
 
 // The tile of a block: neighbours in a group of 4 tiles of tokens share an XCD, so that the 32 blocks that run there
@@ -61,9 +72,9 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
     const int steps = (p.w_pitch + S::KB - 1) / S::KB;  // x holds zeros to the end of the last
 
     // Copies: a wave's instruction brings ROWS rows of KB bytes, 16 a lane, to LDS in order of lanes. The 16-byte piece c
-    // of row r goes to place c ^ (r / 2 % 8) (of 4 places: c ^ (r / 4 % 4)), so that 16 rows' pieces of one column lie in
-    // different ones of the 64 banks.
-    auto place = [](int r, int c) { return S::PIECES == 8 ? c ^ (r / 2 % 8) : c ^ (r / 4 % 4); };
+    // of row r goes to place c ^ (r / 2 % 8), so that 16 rows' pieces of one column lie in different ones of the 64 banks.
+    static_assert(S::PIECES == 8, "place");
+    auto place = [](int r, int c) { return c ^ (r / 2 % 8); };
     const int at = lane / S::PIECES;  // a copy's row of this lane
     auto piece = [&](int rows, int u) { return place(wave * rows + u * S::ROWS + at, lane % S::PIECES); };
     uint32_t xoff[S::XR / S::ROWS], woff[S::WR / S::ROWS];
@@ -104,7 +115,8 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
         for (int u = 0; u < S::XR / S::ROWS; ++u)
             copy(xbase + step * S::KB, xoff[u], dst + (wave * S::XR + u * S::ROWS) * S::KB);
 #pragma unroll
-        for (int u = 0; u < S::WR / S::ROWS; ++u) copy(wbase + step * S::KB, woff[u], dst + (S::BM + wave * S::WR + u * S::ROWS) * S::KB);
+        for (int u = 0; u < S::WR / S::ROWS; ++u)
+            copy(wbase + step * S::KB, woff[u], dst + (S::BM + wave * S::WR + u * S::ROWS) * S::KB);
     };
 
     // Operands: lane l has row l % 16, bytes 16 (l / 16) .. of each 64.
@@ -241,8 +253,11 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
 }
 
 // Fewer tokens: tiles of TOK tokens by SIDE rows of the weight (gated: half of gate, half of up), a wave for every fourth
-// unit of 128 bytes of k. A wave copies and reads its units by itself, two in LDS, so the loop has no barrier; each byte of LDS is
-// read once, where four waves that share a tile's k would read it twice, and a group's products cover the next one's reads.
+// unit of 128 bytes of k. A wave copies and reads its units by itself, SLOTS of them in LDS, so the loop has no barrier; each
+// byte of LDS is read once, where four waves side by side would read it twice, and one group's products cover the next one's
+// reads. Bound by the copies: what a CU brings to LDS from L2 (110 to 130 bytes a ns; 27 from beyond), or by their
+// latency: 16 tokens over 4096 x 12288, 50 MB of cold weights, 17.0 us with the tokens' launch, 3.0 TB/s; 100 over 6144 x 4096
+// 10.9 us without it, 460 TOPS.
 constexpr int kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
 
 template <int TOK, int SIDE, int SLOTS, bool GATED>
@@ -324,11 +339,11 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     };
     auto landed = [&](int late) {  // this wave's copies, but those of the last `late` units
         constexpr int C = XC + WC;
-        static_assert(SLOTS <= 4 && 3 * C < 64, "vmcnt");
+        static_assert((SLOTS == 2 || SLOTS == 4) && (SLOTS - 1) * C < 64, "vmcnt");
         if (late == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         else if (SLOTS == 2 || late == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(C) : "memory");
-        else if (SLOTS == 3 || late == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(3 * C) : "memory");
+        else if (late == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * C) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(SLOTS == 2 ? 0 : 3 * C) : "memory");
     };
     Operands a, b;
     if (mine > 0) {
@@ -417,7 +432,14 @@ int launch_split(nv_context* c, const nvr::ProductArgs& p, bool check) {
 
 namespace nvr {
 
-// The tile by tokens and by turns: how often the CUs are filled. On MI355X, weights cold, in us of the product alone:
+// The tile by tokens and by turns: how often the CUs are filled. On MI355X, weights cold, in us, first of whole calls:
+//   tiles of 16 rows of the weight while there is at most one a CU, against 32 rows, which leave half of the CUs without:
+//   16 tokens over 4096 at k 2056, 4104, 12288 7.6, 9.6, 17.0 and 8.4, 11.2, 20.7; over 6144 (more than one) 9.0, 12.7, 25.4
+//   and 8.8, 12.0, 23.6; 32 tokens over 4096 at k 4104 11.1, 12.5; 64 12.8, 14.9; 256 over 1000 at k 1030 6.7, 7.7. Few
+//   such tokens are latency: four units of k in LDS instead of two, 16 over 1024 at k 12288 13.3, 14.7; 64 tokens
+//   by two over 1024 at k 4104 10.4, by three 10.7. Eight waves for a tile's k: 32 over 4096 at k 8192 14.8,
+//   four 14.7; over 200 9.9, 10.6. Gated tiles have 16 rows of gate and of up at least.
+// Of the product alone:
 //   a tile's k over four waves while there is a tile a CU: 256 tokens over 1024 x 2048 by tiles of 64 x 32, 64 x 64 and
 //   128 x 128 5.2, 7.3, 11.2; 100 over 6144 x 4096 13.1 (in two turns), 10.9, 15.2; 512 over 4096 x 1024 (two turns of 64 x
 //   64) -, 10.7, 7.9;
@@ -428,15 +450,20 @@ namespace nvr {
 //   1024 (1, 2) 20.8, 14.2. Where k is short, a tile is mostly its outputs, which two blocks overlap: 5327 over 18704 x 176
 //   (7, 25) 77.6, 67.6; 8192 over 8192 x 512 (4, 16) 59.9, 65.8; gated 2244 over 8001 x 1024 (3, 9) 63.2, 57.0.
 int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated, bool check) {
-    using Large = Shape<256, 256, 2, 4, 128, 2>;
-    using Medium = Shape<128, 128, 4, 2, 128, 2>;
-    using Wide = Shape<64, 128, 4, 2, 128, 3>;
+    using Large = Shape<256, 256, 2, 4, 2>;
+    using Medium = Shape<128, 128, 4, 2, 2>;
+    using Wide = Shape<64, 128, 4, 2, 3>;
     constexpr int kShort = 384;
     const int64_t cus = c->cu_count > 0 ? c->cu_count : 256, rows = gated ? 2 * int64_t(p.n) : p.n;
     auto tiles = [&](int tokens, int side) { return (int64_t(p.m) + tokens - 1) / tokens * ((rows + side - 1) / side); };
     auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
     auto run = [&](auto g) {
         constexpr bool G = decltype(g)::value;
+        if constexpr (!G) {
+            if (p.m <= 16 && tiles(16, 16) <= cus) return launch_split<16, 16, 4, false>(c, p, check);
+            if (p.m <= 32 && tiles(32, 16) <= cus) return launch_split<32, 16, 4, false>(c, p, check);
+            if (tiles(64, 16) <= cus) return launch_split<64, 16, 2, false>(c, p, check);
+        }
         if (p.m <= 16) return launch_split<16, 32, 2, G>(c, p, check);
         if (p.m <= 32) return launch_split<32, 32, 2, G>(c, p, check);
         if (tiles(64, 32) <= cus) return launch_split<64, 32, 2, G>(c, p, check);

@@ -2,7 +2,6 @@
 // tokens of nv_gemm_i8 and nv_gemm_i8_silu where a launch of its own makes them.
 // No counterpart in the reference, whose weights and products are bf16
 // (kernels/kernels.cu:98-106). The arithmetic is in nvr_int8.h.
-//
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
