@@ -17,8 +17,8 @@
 // streams the weights through registers, each byte once, bound by HBM and, in the
 // smallest calls, by one chain: tokens, their largest value, products, outputs. All
 // others go by tiles (gemm_int_tiles.hip). On MI355X: 1 token over 1024 x 2048 3.4
-// us, 8 with sum and norm over 4096 x 1024 4.2 us; 32 over 151936 x 1024 38.7 us with
-// the tokens' launch, 4.3 TB/s.
+// us, 8 with sum and norm over 4096 x 1024 4.2 us; 32 over 151936 x 1024 39.6 us with
+// the tokens' launch, 4.2 TB/s.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
