@@ -158,6 +158,20 @@ def test_products_in_every_form(gpu, m, n, k, gated, norm):
     call.check()
 
 
+# The longest rows that each block makes by itself, and the ones behind them; tiles of 16 rows up to one a CU, and one more.
+@pytest.mark.parametrize("m,n,k,norm", [
+    (4, 50, 4096, "add"), (4, 50, 4095, "rms"), (5, 50, 4096, "add"), (3, 50, 4097, "add"), (1, 9, 2049, "rms"), (5, 50, 2048, "rms"),
+    (8, 50, 2041, "add"), (6, 50, 2049, "add"), (8, 50, 4096, "none"), (7, 50, 4090, "none"), (8, 50, 4104, "none"),
+    (9, 50, 2048, "none"), (16, 50, 2047, "none"), (16, 5000, 1500, "none"), (10, 50, 2049, "none"), (16, 50, 1024, "rms"),
+    (11, 50, 1025, "add"), (16, 4096, 2056, "none"), (16, 4097, 2056, "none"), (32, 4090, 136, "add"), (32, 4100, 136, "add"),
+    (64, 4081, 72, "none"), (64, 4112, 72, "none"), (129, 1360, 200, "none"), (1025, 200, 96, "add"), (1025, 241, 96, "add")])
+@pytest.mark.parametrize("gated", [False, True])
+def test_products_on_both_sides_of_each_rule(gpu, m, n, k, norm, gated):
+    call = Call(gpu, m, n, k, norm, gated, seed=k + m)
+    call.run()
+    call.check()
+
+
 @pytest.mark.parametrize("m", [1, 20, 150])
 def test_sums_of_the_longest_rows_stay_exact(gpu, m):
     """The largest sums that 32 bits hold: 131071 times 127 times -128."""
