@@ -335,14 +335,14 @@ void launch_rows(nv_context* c, RowsArgs a) {
         const integral_constant<int, 4> four;
         const int chunks = (a.p.x_pitch + nvr::kWaveChunk - 1) / nvr::kWaveChunk;
         if (a.p.m > kWaves) {
-            if constexpr (SRC == Source::kPlain)
+            if constexpr (SRC == Source::kPlain && WHOLE)
                 if (chunks > 2) return run(four, two, one);
             run(two, two, one);
         } else if (chunks <= 2) {
             run(two, one, one);
-        } else if (chunks <= 4) {
+        } else if (!WHOLE || chunks <= 4) {
             run(four, one, one);
-        } else {
+        } else if constexpr (WHOLE) {
             run(integral_constant<int, 8>{}, one, one);
         }
     }
@@ -350,15 +350,17 @@ void launch_rows(nv_context* c, RowsArgs a) {
 
 // Whether each block makes the tokens' integers by itself, a row or two a wave: one launch less, for work that all blocks
 // repeat. On MI355X in a graph, weights cold, n 4096, made and by a launch of their own, in us:
-//   k 1024: 1 token 3.1, 5.8; 8 with sum and norm 4.2, 6.2; 16 4.3, 5.9, with sum and norm 5.4, 6.4;
-//   k 2048: 8 5.0, 7.3, with sum and norm 6.3, 7.7; 9 to 16 5.1 to 6.1, 7.3 (n 16384 10.9 to 12.3, 11.3); 16 with sum and
-//   norm 8.8, 7.8;
-//   k 4096: 8 8.2, 9.5; with sum and norm 4 8.1, 9.8, but 6 10.5, 9.5: two waves of a SIMD then have a row each, and a row's
+//   k 1024: 1 token 3.1, 5.6; 8 with sum and norm 4.2, 6.2; 16 4.3, 5.7, with sum and norm 5.4, 6.2;
+//   k 2048: 8 5.0, 6.7, with sum and norm 6.3, 7.5; 9 to 16 5.0 to 6.1, 6.7 (over n 16384 10.9 to 12.4, 11.3); 16 with sum
+//   and norm 8.8, 7.8;
+//   k 4096: 8 8.2, 8.6; with sum and norm 4 8.1, 9.0, but 6 10.5, 9.1: two waves of a SIMD then have a row each, and a row's
 //   chunks, sums and norm weights fill the registers beside the weights.
+// Chunks of a k that is no multiple of 8 take shifts, so half as many: 8 at k 2041 5.2, 6.8, at 4090 9.7, 8.8; 1 with sum and
+// norm at 2041 6.8, 7.6, at 4090 15.0, 9.6; 8 at 1001 5.2, 6.7, at 1111 7.5, 7.0; 16 at 1001 5.0, 5.9, at 1111 7.1, 6.4.
 bool tokens_in_block(const nvr::TokenArgs& t) {
     const int most = t.rows <= 4 ? 8 : t.rows <= kWaves ? 4 : 2;  // chunks of a row with a norm
     const int chunks = t.norm_weight != nullptr ? most : t.rows <= kWaves ? 8 : 4;
-    return t.rows <= 2 * kWaves && t.k <= chunks * nvr::kWaveChunk;
+    return t.rows <= 2 * kWaves && t.k <= (t.k % nvr::kChunk == 0 ? chunks : chunks / 2) * nvr::kWaveChunk;
 }
 
 // Whether few tokens, made by a launch of their own, take gemm_rows_i8: where a CU would have more than two of

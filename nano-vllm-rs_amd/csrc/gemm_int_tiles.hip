@@ -267,6 +267,7 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
     const int2 tile = tile_of(blockIdx.x, gridDim.x, mt, nt);
     const int64_t m0 = int64_t(tile.x) * TOK;
     const int n0 = tile.y * (GATED ? SIDE / 2 : SIDE);  // < n
+    constexpr bool kHalves = GATED && SIDE == 16;  // a product's 16 rows are 8 of gate, then 8 of up
     constexpr int NI = SIDE / 16, MJ = TOK / 16, SLOT = (TOK + SIDE) * kUnitBytes;
     const int units = (p.w_pitch + kUnitBytes - 1) / kUnitBytes;  // x holds zeros to the end of the last
     const int mine = (units - wave + kSplit - 1) / kSplit;        // wave, wave + 4, ...
@@ -283,7 +284,8 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
 #pragma unroll
     for (int u = 0; u < WC; ++u) {
         const int r = u * 8 + lane / 8;
-        woff[u] = uint32_t(min(n0 + (GATED ? r % (SIDE / 2) : r), p.n - 1) - n0) * uint32_t(p.w_pitch) + place(r, lane % 8) * 16;
+        const int row = min(n0 + (GATED ? r % (SIDE / 2) : r), p.n - 1);
+        woff[u] = uint32_t(row - n0) * uint32_t(p.w_pitch) + place(r, lane % 8) * 16;
     }
     const uint8_t* xbase = p.xq + m0 * p.x_pitch;
     const uint8_t* wbase = p.wq + int64_t(n0) * p.w_pitch;
@@ -299,6 +301,13 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
             : "s"(base), "s"(dst), "v"(off0), "v"(off1)
             : "memory", "scc");
     };
+    auto copy1 = [&](const uint8_t* base, uint32_t off, uint32_t dst) {
+        uint32_t saved;
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %1\n\ts_mov_b32 m0, %0"
+                     : "=&s"(saved)
+                     : "s"(base), "s"(dst), "v"(off)
+                     : "memory");
+    };
     auto copy = [&](int i) {  // this wave's i-th unit
         const int k = (wave + i * kSplit) * kUnitBytes;
         const uint32_t dst = lds + i % SLOTS * SLOT;
@@ -309,9 +318,14 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
         }
 #pragma unroll
         for (int u = 0; u < XC; u += 2) copy2(xbase + k, xoff[u], xoff[u + 1], dst + u * 1024);
+        if constexpr (kHalves) {
+            copy1(wbase + k, woff[0], dst + XC * 1024);
+            copy1(ubase + k, woff[1], dst + (XC + 1) * 1024);
+        } else {
 #pragma unroll
-        for (int u = 0; u < WC; u += 2)
-            copy2((u < WC / 2 ? wbase : ubase) + k, woff[u], woff[u + 1], dst + (XC + u) * 1024);
+            for (int u = 0; u < WC; u += 2)
+                copy2((u < WC / 2 ? wbase : ubase) + k, woff[u], woff[u + 1], dst + (XC + u) * 1024);
+        }
     };
     const int lane_at = lane % 16 * kUnitBytes + place(lane % 16, lane / 16) * 16;
     const unsigned char* ring = smem + wave * (SLOTS * SLOT);
@@ -373,7 +387,7 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
 #pragma unroll
         for (int i = 0; i < NI; ++i) sums[((wave * MJ + j) * NI + i) * kWave] = acc[i][j];
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    constexpr int OI = GATED ? NI / 2 : NI;  // a token's 16 channels
+    constexpr int OI = GATED && !kHalves ? NI / 2 : NI;  // a token's 16 channels (8)
 #pragma unroll
     for (int at = 0; at < MJ * OI; at += kSplit) {
         const int q = at + wave, j = q / OI, i = q % OI;
@@ -385,18 +399,20 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
             return part[0] + part[1] + (part[2] + part[3]);
         };
         static_assert(kSplit == 4, "whole");
-        const i32x4_t sum = whole(i), up = GATED ? whole(i + NI / 2) : sum;
+        const i32x4_t sum = whole(i), up = GATED && !kHalves ? whole(i + NI / 2) : sum;
         const int64_t token = m0 + j * 16 + lane % 16;
-        const int channel = n0 + i * 16 + 4 * (lane / 16);
+        const int channel = n0 + i * 16 + 4 * (kHalves ? lane / 16 % 2 : lane / 16);
+        const float* ws = p.ws + (kHalves && lane >= 32 ? int64_t(p.n) : 0);
         const Scale xs = nvr::split_scale(p.xs[min(token, int64_t(p.m) - 1)]);
         float y[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int c = min(channel + r, p.n - 1);
-            y[r] = nvr::scaled(sum[r], xs, nvr::split_scale(p.ws[c]));
-            if constexpr (GATED) y[r] = nvr::gated(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+            y[r] = nvr::scaled(sum[r], xs, nvr::split_scale(ws[c]));
+            if constexpr (kHalves) y[r] = nvr::gated(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
+            else if constexpr (GATED) y[r] = nvr::gated(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
         }
-        if (token >= p.m) continue;
+        if (token >= p.m || (kHalves && lane >= 32)) continue;
         nvr::store_outputs(p.y + token * p.n + channel, y, channel, p.n);
     }
 }
@@ -438,7 +454,8 @@ namespace nvr {
 //   and 8.8, 12.0, 23.6; 32 tokens over 4096 at k 4104 11.1, 12.5; 64 12.8, 14.9; 256 over 1000 at k 1030 6.7, 7.7. Few
 //   such tokens are latency: four units of k in LDS instead of two, 16 over 1024 at k 12288 13.3, 14.7; 64 tokens
 //   by two over 1024 at k 4104 10.4, by three 10.7. Eight waves for a tile's k: 32 over 4096 at k 8192 14.8,
-//   four 14.7; over 200 9.9, 10.6. Gated tiles have 16 rows of gate and of up at least.
+//   four 14.7; over 200 9.9, 10.6. Gated, 8 rows of gate and of up against 16: 32 over 1376 at k 4104 10.5, 12.1; over 2048 at
+//   k 1111 7.0, 7.3.
 // Of the product alone:
 //   a tile's k over four waves while there is a tile a CU: 256 tokens over 1024 x 2048 by tiles of 64 x 32, 64 x 64 and
 //   128 x 128 5.2, 7.3, 11.2; 100 over 6144 x 4096 13.1 (in two turns), 10.9, 15.2; 512 over 4096 x 1024 (two turns of 64 x
@@ -459,11 +476,9 @@ int launch_product_tiles(nv_context* c, const ProductArgs& p, bool gated, bool c
     auto turns = [&](int64_t t) { return (t + cus - 1) / cus; };
     auto run = [&](auto g) {
         constexpr bool G = decltype(g)::value;
-        if constexpr (!G) {
-            if (p.m <= 16 && tiles(16, 16) <= cus) return launch_split<16, 16, 4, false>(c, p, check);
-            if (p.m <= 32 && tiles(32, 16) <= cus) return launch_split<32, 16, 4, false>(c, p, check);
-            if (tiles(64, 16) <= cus) return launch_split<64, 16, 2, false>(c, p, check);
-        }
+        if (p.m <= 16 && tiles(16, 16) <= cus) return launch_split<16, 16, 4, G>(c, p, check);
+        if (p.m <= 32 && tiles(32, 16) <= cus) return launch_split<32, 16, 4, G>(c, p, check);
+        if (tiles(64, 16) <= cus) return launch_split<64, 16, 2, G>(c, p, check);
         if (p.m <= 16) return launch_split<16, 32, 2, G>(c, p, check);
         if (p.m <= 32) return launch_split<32, 32, 2, G>(c, p, check);
         if (tiles(64, 32) <= cus) return launch_split<64, 32, 2, G>(c, p, check);
