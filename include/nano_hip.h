@@ -331,14 +331,14 @@ int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
  *   RMSNorm(x)                   residual NULL (residual_out too),
  *   RMSNorm(x + residual)        with residual_out <- bf16(x + residual), unless NULL;
  * the norm in fp32 (as nv_rms but for roundings, its values not rounded to bf16).
- * x, residual, residual_out: [m, k] bf16, residual_out another buffer than the
- * others; norm_weight: [k] bf16; w, w_scales as nv_quantize_rows' q and scales
- * (integers of any source; -128 too); y: [m, n] bf16. Sums of products are exact,
- * so a token's outputs are the same bits in any batch. A token with a NaN or an
- * infinity (or whose product with the norm's weight leaves fp32) has NaN in its row
- * of y, and no other has. eps is read with a norm_weight only. Any m and n that one
- * launch holds (2^32 threads; else -2) and any k; tensors of bf16 start at any even
- * address, scales at multiples of 4 bytes. */
+ * x, residual, residual_out: [m, k] bf16; residual_out and y overlap neither x nor
+ * residual nor each other (else -2), nor any other argument; norm_weight: [k] bf16;
+ * w, w_scales as nv_quantize_rows' q and scales (integers of any source; -128 too);
+ * y: [m, n] bf16. Sums of products are exact, so a token's outputs are the same bits
+ * in any batch. A token with a NaN or an infinity (or whose product with the norm's
+ * weight leaves fp32) has NaN in its row of y, and no other has. eps is read with a
+ * norm_weight only. Any m and n that one launch holds (2^32 threads; else -2) and any
+ * k; tensors of bf16 start at any even address, scales at multiples of 4 bytes. */
 int nv_gemm_i8(nv_context* c, const void* x, const void* residual, void* residual_out, const void* norm_weight,
                const void* w, const void* w_scales, void* y, void* workspace, int m, int n, int k, float eps);
 

@@ -394,6 +394,13 @@ def test_the_library_refuses(gpu):
                    dict(w_scales=None), dict(y=None), dict(w=p + 8), dict(x=p + 1), dict(y=far + 1), dict(w_scales=p + 2),
                    dict(residual=p), dict(residual_out=p), dict(norm_weight=p, residual_out=p), dict(workspace=p + 4104)):
         assert product(**change) == (-2, -2), change
+    # An output over the tokens or the other output: blocks read while others write.
+    apart = dict(residual=p + 8192, residual_out=p + 12288, norm_weight=p)
+    assert product(**apart) == (0, 0)
+    for change in (dict(residual_out=p + 8192), dict(residual_out=p + 8192 + 62), dict(residual_out=p), dict(y=p + 62), dict(y=p),
+                   dict(y=p + 8192), dict(y=p + 12288 - 2), dict(y=p + 12288 + 62)):
+        assert product(**{**apart, **change}) == (-2, -2), change
+    assert product(**{**apart, "y": p + 12288 + 64}) == (0, 0)  # right behind it
     # More tiles than one launch holds: nothing is read or written.
     assert lib.nv_gemm_i8(h, p, None, None, None, p, p, far, p + 4096, 40, 2 ** 31 - 1000, 16, 1e-6) == -2
     for args in ((None, p, p, 1, 16), (p, None, p, 1, 16), (p, p, None, 1, 16), (p, far, p, 0, 16), (p, far, p, 1, 0),
