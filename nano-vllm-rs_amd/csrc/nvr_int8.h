@@ -341,15 +341,17 @@ __device__ __forceinline__ Scale split_scale(float s) {
 __device__ __forceinline__ float scaled(int acc, Scale x, Scale w) {
     return __builtin_amdgcn_ldexpf(float(acc) * x.mantissa * w.mantissa, x.exponent + w.exponent);
 }
-// silu(g) u, with g / (1 + e^-g) at 2^-64 of both sides where e^-g is large: neither the exponential overflows nor the
-// reciprocal is flushed while the result is one of fp32. Hardware exponential and reciprocal, each within a step; without
-// the division that nv_silu takes there, whose instructions every lane would run.
+// silu(g) u = g u / (1 + e^-g). Far below zero, where the 1 no longer counts, it is g e^g u with e^g in three equal factors
+// and u between them: nothing on the way is flushed or overflows while the result is one of fp32, though e^g alone may be far
+// below. At -512 that is 0 for any u, and so it is for all gates below, -inf among them. Hardware exponential and reciprocal,
+// each within a step; without the division that nv_silu takes there, whose instructions every lane would run.
 __device__ __forceinline__ float gated(float g, float u) {
-    const float t = g * -1.44269504088896340736f;
-    const bool large = t > 64.0f;
-    const float a = large ? 0x1.0p-64f : 1.0f;
-    const float d = a + __builtin_amdgcn_exp2f(large ? t - 64.0f : t);
-    return (g * a) * __builtin_amdgcn_rcpf(d) * u;
+    const float at = g < -512.0f ? -512.0f : g;  // a NaN stays
+    const float t = at * -1.44269504088896340736f;
+    const bool far = t > 64.0f;
+    const float e = __builtin_amdgcn_exp2f(far ? t * -0x1.555556p-2f : t);
+    const float rest = far ? e : 1.0f;
+    return at * (far ? e : __builtin_amdgcn_rcpf(1.0f + e)) * u * rest * rest;
 }
 
 // Stores of four and eight bf16 to any even address.
