@@ -1,7 +1,9 @@
-"""Values at the ends of the range in nv_gemm_i8 and nv_gemm_i8_silu, against 64 bits: gates far below zero."""
+"""Values at the ends of the range in nv_gemm_i8 and nv_gemm_i8_silu, against 64 bits: gates far below zero,
+rows with a norm whose squares leave fp32, NaN and infinities in them."""
 import numpy as np
 import pytest
 
+import int8_reference as ref
 from helpers import bf16_of, f32_of
 from int8_reference import HALF16, HALF32, TINY
 from test_gpu_int8 import Call, f64
@@ -75,3 +77,65 @@ def test_a_gate_of_minus_infinity_is_closed(gpu, m, n, k):
     assert far.size
     closed = f64(call.outputs())[sign > 0][:, far]
     assert closed.size and (closed == 0).all()
+
+
+# ------------------------------------------------------------- rows with a norm --
+KINDS = ("normal", "zeros", "nan", "infinite", "large", "largest", "one large", "product past fp32")
+
+
+def norm_rows(m, k, shift, residual):
+    """Row i is of kind (i + shift): x, the residual (or None), and the norm's weight, whose first value is 4."""
+    rng = np.random.default_rng(100 * m + k + shift)
+    v, r = rng.standard_normal((m, k)), rng.standard_normal((m, k))
+    kinds = [KINDS[(i + shift) % len(KINDS)] for i in range(m)]
+    for i, kind in enumerate(kinds):
+        at = int(rng.integers(k))
+        if kind == "zeros":
+            v[i] = -f32_of(bf16_of(r[i].astype(np.float32))) if residual else 0
+        elif kind == "nan":
+            v[i, at] = np.nan
+        elif kind == "infinite":
+            v[i, at] = -np.inf
+        elif kind == "large":
+            v[i], r[i] = v[i] * 2.0 ** 70, r[i] * 2.0 ** 69
+        elif kind == "largest":
+            v[i], r[i] = rng.uniform(-1, 1, k) * 2.0 ** 124, rng.uniform(-1, 1, k) * 2.0 ** 120
+        elif kind == "one large":
+            v[i, at], r[i, at] = 2.0 ** 100, 0
+        elif kind == "product past fp32":
+            v[i, 0], r[i, 0] = 3e38, 0
+    weight = bf16_of((1.0 + 0.2 * rng.standard_normal(k)).astype(np.float32))
+    weight[0] = bf16_of(np.float32(4.0))
+    up = lambda a: bf16_of(a.astype(np.float32))  # noqa: E731
+    return kinds, up(v), up(r) if residual else None, weight
+
+
+# One wave a row in the block; a launch of its own with 4 waves, 16, 16 of two chunks, 16 that read a row twice; many rows by
+# one wave of 2, 4 and 8 chunks, by 4 of 4 and of 8.
+NORM_FORMS = [(1, 40), (4, 1000), (4, 1111), (4, 4096), (8, 1111), (8, 2048), (16, 505), (16, 1024),
+              (20, 200), (20, 2041), (40, 2500), (17, 5000), (40, 9000), (17, 16000), (40, 17000), (3, 20001),
+              (1030, 200), (1030, 2000), (1030, 2041), (1030, 4000), (1030, 8000), (1030, 16001)]
+
+
+@pytest.mark.parametrize("norm", ["rms", "add"])
+@pytest.mark.parametrize("m,k", NORM_FORMS)
+def test_rows_of_every_kind_with_a_norm(gpu, m, k, norm):
+    """Rows whose sum of squares leaves fp32 have the values of any others; a NaN or an infinity, and a product with the norm's
+    weight past fp32, make their row NaN and no other."""
+    for shift in range(len(KINDS) if m < len(KINDS) else 1):
+        kinds, x, residual, weight = norm_rows(m, k, shift, norm == "add")
+        call = Call(gpu, m, 33, k, norm, seed=k, x=x, residual=residual)
+        call.weight = weight
+        call.bnw.upload(weight)
+        call.run()
+        with np.errstate(invalid="ignore", over="ignore"):
+            want, bound = ref.product(f64(x), None if residual is None else f64(residual), f64(weight), 1e-6, call.wq,
+                                      call.ws.astype(np.float64))
+        got = f64(call.outputs())
+        for i, kind in enumerate(kinds):
+            if kind in ("nan", "infinite", "product past fp32"):
+                assert np.isnan(got[i]).all(), (shift, i, kind)
+            else:
+                assert not np.isnan(got[i]).any(), (shift, i, kind)
+                assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (shift, i, kind, got[i][:4], want[i][:4])
+            assert kind != "zeros" or not got[i].any()
