@@ -13,6 +13,10 @@
 // numbers is one of fp32 and comes out as it is. No other quotient of such t and a
 // lies within 2^-17 of such a point, and fp32 is within 2^-18 of it below 128: the
 // row's numbers are those of exact arithmetic.
+// So are RMSNorm(x)'s, of products of two bf16 (16 bits; t 23): a quotient that is
+// not half way is further from such a point than half a step of fp32, which rounds
+// none to it. A sum of two bf16 times a weight has more bits and is rounded to fp32
+// first, so a quotient within 2^-16 of such a point may take either number.
 //
 // Of a norm, u_j = v_j g_j / rms(v), the whole numbers need the products v_j g_j alone: their common factor leaves 127 u_j /
 // a as it is, and goes into the scale. So a row's sum of squares and its largest product are found in one pass, and the

@@ -1,10 +1,11 @@
 """Values at the ends of the range in nv_gemm_i8 and nv_gemm_i8_silu, against 64 bits: gates far below zero,
-rows with a norm whose squares leave fp32, NaN and infinities in them."""
+rows with a norm whose squares leave fp32, NaN and infinities in them; a norm's whole numbers; the same bits again and in any
+batch."""
 import numpy as np
 import pytest
 
 import int8_reference as ref
-from helpers import bf16_of, f32_of
+from helpers import assert_bits_equal, bf16_of, f32_of
 from int8_reference import HALF16, HALF32, TINY
 from test_gpu_int8 import Call, f64
 
@@ -139,3 +140,82 @@ def test_rows_of_every_kind_with_a_norm(gpu, m, k, norm):
                 assert not np.isnan(got[i]).any(), (shift, i, kind)
                 assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (shift, i, kind, got[i][:4], want[i][:4])
             assert kind != "zeros" or not got[i].any()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_a_channel_with_a_nan_is_nan_for_every_token(gpu, m, gated):
+    """quantize_rows gives such a channel a scale of NaN; no other channel has one."""
+    n, k = 40, 200
+    w = np.random.default_rng(m).standard_normal(((2 if gated else 1) * n, k)).astype(np.float32)
+    w[7, 3], w[-1, k - 1] = np.nan, np.inf  # gated: channel 7 of the gate, the last of up
+    q, s = gpu.alloc(w.shape[0] * ref.pitch(k)), gpu.alloc(w.shape[0] * 4)
+    gpu.quantize_rows(gpu.upload_array(bf16_of(w)), q, s, *w.shape)
+    call = Call(gpu, m, n, k, "rms", gated)
+    call.bw, call.bs = q, s
+    call.run()
+    assert np.array_equal(np.isnan(f64(call.outputs())), np.isin(np.arange(n), (7, n - 1))[None].repeat(m, 0))
+
+
+# ------------------------------------------------------- whole numbers of a norm --
+@pytest.mark.parametrize("m,k", [(1, 40), (4, 1000), (4, 4096), (8, 2041), (16, 1024), (20, 200), (20, 2041), (40, 2500),
+                                 (17, 5000), (17, 16000), (18, 17000), (1030, 1024), (1030, 2041), (1030, 4000), (1030, 5000)])
+def test_whole_numbers_of_a_norm_are_exact(gpu, m, k):
+    """Of RMSNorm(x) they are those of exact arithmetic: x_j g_j has 16 bits, 127 times that 23, so no step of fp32 rounds
+    before the quotient, and none that is not half way between two numbers can round to such a point. Channels of one 1 give
+    one number times the token's scale, which bf16 tells apart: 127 / (1 + 2^8) < 1/2."""
+    rng = np.random.default_rng(m + k)
+    x, weight = bf16_of(rng.standard_normal((m, k)).astype(np.float32)), bf16_of((1 + 0.2 * rng.standard_normal(k)).astype(np.float32))
+    x[:, 0], weight[0] = bf16_of(np.float32(4.0)), bf16_of(np.float32(2.0))  # a power of two at the top: quotients end in a half
+    places = np.unique(np.r_[np.arange(min(k, 300)), k - 1, rng.integers(0, k, 200)])
+    wq = np.zeros((places.size, k), np.int8)
+    wq[np.arange(places.size), places] = 1
+    call = Call(gpu, m, places.size, k, "rms", x=x, wq=wq, ws=np.ones(places.size, np.float32))
+    call.weight = weight
+    call.bnw.upload(weight)
+    call.run()
+    products = f64(x) * f64(weight)
+    want, top = ref.whole_numbers(products)
+    scale = top / np.sqrt((f64(x) ** 2).mean(-1) + 1e-6) / 127
+    assert_bits_equal(np.rint(f64(call.outputs()) / scale[:, None]).astype(np.int8), want[:, places])
+
+
+@pytest.mark.parametrize("norm", ["rms", "add"])
+@pytest.mark.parametrize("m,n,k,gated", [(8, 4096, 1024, False), (32, 20000, 1024, False), (100, 6144, 1030, False),
+                                         (520, 2000, 1030, True), (2048, 4096, 512, False), (1200, 4096, 1050, True)])
+def test_a_call_repeats_itself(gpu, m, n, k, gated, norm):
+    call = Call(gpu, m, n, k, norm, gated)
+    call.run()
+    first, summed = call.outputs(), None if call.bout is None else call.bout.download(np.uint16, m * k)
+    for _ in range(5):
+        call.by.upload(np.full(call.by.bytes, 0xA5, np.uint8))
+        call.run()
+        assert_bits_equal(call.outputs(), first)
+        assert summed is None or (call.bout.download(np.uint16, m * k) == summed).all()
+
+
+# Every form, on both sides of the rules by tokens: made in the block, streamed, split tiles of each size, whole tiles.
+@pytest.mark.parametrize("norm", ["none", "rms", "add"])
+@pytest.mark.parametrize("n,k", [(150, 1024), (64, 4104), (72, 1111), (2250, 512), (9001, 264), (1100, 3000), (6000, 1050)])
+def test_a_gated_token_has_the_same_bits_in_any_batch(gpu, n, k, norm):
+    m = 600
+    whole = Call(gpu, m, n, k, norm, True, seed=9)
+    whole.run()
+    want = whole.outputs()
+    for rows in (1, 5, 16, 17, 32, 33, 64, 130, 300):
+        part = Call(gpu, rows, n, k, norm, True, x=whole.x[m - rows:].copy(), wq=whole.wq, ws=whole.ws, seed=9,
+                    residual=None if whole.residual is None else whole.residual[m - rows:].copy())
+        part.run()
+        assert_bits_equal(part.outputs(), want[m - rows:], f"{rows} tokens")
+
+
+@pytest.mark.parametrize("n,k", [(300, 1024), (128, 4096), (72, 1111), (17000, 264), (2100, 10000)])
+def test_a_token_behind_a_norm_has_the_same_bits_in_any_batch(gpu, n, k):
+    m = 300
+    whole = Call(gpu, m, n, k, "rms", seed=9)
+    whole.run()
+    want = whole.outputs()
+    for rows in (1, 5, 16, 17, 32, 33, 64, 130):
+        part = Call(gpu, rows, n, k, "rms", x=whole.x[m - rows:].copy(), wq=whole.wq, ws=whole.ws, seed=9)
+        part.run()
+        assert_bits_equal(part.outputs(), want[m - rows:], f"{rows} tokens")
