@@ -16,7 +16,7 @@
 // So are RMSNorm(x)'s, of products of two bf16 (16 bits; t 23): a quotient that is
 // not half way is further from such a point than half a step of fp32, which rounds
 // none to it. A sum of two bf16 times a weight has more bits and is rounded to fp32
-// first, so a quotient within 2^-16 of such a point may take either number.
+// first, so a quotient within 2^-15 of such a point may take either number.
 //
 // Of a norm, u_j = v_j g_j / rms(v), the whole numbers need the products v_j g_j alone: their common factor leaves 127 u_j /
 // a as it is, and goes into the scale. So a row's sum of squares and its largest product are found in one pass, and the

@@ -640,8 +640,8 @@ void Gpu::product_i8(bool gated, const Buffer& x, const Buffer& residual, const 
     const std::size_t need = gated ? gemm_i8_silu_workspace(m, n, k) : gemm_i8_workspace(m, n, k);
     const std::size_t channels = gated ? 2 * n : n;
     std::vector<TensorArg> args = {read_arg("x", x, 2, {m, k}), read_arg("w", w, 16, {channels, i8_pitch(k) / 16}),
-                                   read_arg("w_scales", w_scales, 4, {channels}), write_arg("y", y, 2, {m, n})};
-    if (need != 0) args.push_back(workspace_arg(workspace, need));
+                                   read_arg("w_scales", w_scales, 4, {channels}), write_arg("y", y, 2, {m, n}),
+                                   workspace_arg(workspace, need)};
     if (!residual.empty()) args.push_back(read_arg("residual", residual, 2, {m, k}));
     if (!residual_out.empty()) args.push_back(write_arg("residual_out", residual_out, 2, {m, k}));
     if (!norm_weight.empty()) args.push_back(read_arg("norm_weight", norm_weight, 2, {k}));
@@ -649,7 +649,7 @@ void Gpu::product_i8(bool gated, const Buffer& x, const Buffer& residual, const 
     auto ptr = [](const Buffer& b) { return b.empty() ? nullptr : b.address(); };
     const auto call = gated ? nv_gemm_i8_silu : nv_gemm_i8;
     require_status(call(context(), x.address(), ptr(residual), ptr(residual_out), ptr(norm_weight), w.address(),
-                        w_scales.address(), y.address(), ptr(workspace), as_dim(m), as_dim(n), as_dim(k), eps));
+                        w_scales.address(), y.address(), workspace.address(), as_dim(m), as_dim(n), as_dim(k), eps));
 }
 
 void Gpu::gemm_i8(const Buffer& x, const Buffer& residual, const Buffer& residual_out, const Buffer& norm_weight,

@@ -573,9 +573,8 @@ class Gpu:
             raise ArgumentError("value", f"{op}: a residual needs a norm_weight")
         need = self._i8_workspace(op + "_workspace", m, n, k)
         args = [("x", x, 2, (m, k), False), ("w", w, 16, (channels, (k + 15) // 16), False),
-                ("w_scales", w_scales, 4, (channels,), False), ("y", y, 2, (m, n), True)]
-        if need:
-            args.append(self._workspace(op, workspace, need))
+                ("w_scales", w_scales, 4, (channels,), False), ("y", y, 2, (m, n), True),
+                self._workspace(op, workspace, need)]
         if norm_weight is not None:
             args.append(("norm_weight", norm_weight, 2, (k,), False))
         if residual is not None:
@@ -588,8 +587,8 @@ class Gpu:
         call = self.lib.nv_gemm_i8 if channels == n else self.lib.nv_gemm_i8_silu
         status = call(self._device.ctx, x.ptr, None if residual is None else residual.ptr,
                       None if residual_out is None else residual_out.ptr,
-                      None if norm_weight is None else norm_weight.ptr, w.ptr, w_scales.ptr, y.ptr,
-                      None if workspace is None else workspace.ptr, m, n, k, eps)
+                      None if norm_weight is None else norm_weight.ptr, w.ptr, w_scales.ptr, y.ptr, workspace.ptr,
+                      m, n, k, eps)
         if status:
             check_status(status, self.lib)
 
