@@ -317,12 +317,14 @@ int nv_kv_copy_blocks(nv_context* c, void* kc, void* vc, const void* src, const 
  * Rows of bf16 as 8-bit integers: x [rows, k] bf16; q [rows, pitch] i8, zeros
  * behind k; scales [rows] f32. With a = max |x_j| of a row, its scale is a / 127 and
  * q_j = 127 x_j / a to the nearest whole number, half to even; 0 where a is 0. A
- * row that holds a NaN or an infinity has a scale of NaN and integers 0. */
+ * row that holds a NaN or an infinity has a scale of NaN and integers 0. Neither q nor
+ * scales overlaps another argument (else -2). */
 int nv_quantize_rows(nv_context* c, const void* x, void* q, void* scales, int rows, int k);
 
 /* Bytes of workspace that nv_gemm_i8 needs; a host function, no device work. A
  * workspace starts at a multiple of 16 bytes (else -2), its contents do not matter
- * before a call and are unspecified after; calls that may overlap need one each. */
+ * before a call and are unspecified after; calls that may overlap need one each.
+ * Every call takes one, a small one too that makes its tokens without it. */
 int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
 
 /* y[m, n] = bf16(sum_l xq[i, l] w[j, l] * xs[i] * w_scales[j]), where xq and xs are
@@ -331,8 +333,8 @@ int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
  *   RMSNorm(x)                   residual NULL (residual_out too),
  *   RMSNorm(x + residual)        with residual_out <- bf16(x + residual), unless NULL;
  * the norm in fp32 (as nv_rms but for roundings, its values not rounded to bf16).
- * x, residual, residual_out: [m, k] bf16; residual_out and y overlap neither x nor
- * residual nor each other (else -2), nor any other argument; norm_weight: [k] bf16;
+ * x, residual, residual_out: [m, k] bf16; residual_out, y and the workspace overlap
+ * neither each other nor any other argument (else -2); norm_weight: [k] bf16;
  * w, w_scales as nv_quantize_rows' q and scales (integers of any source; -128 too);
  * y: [m, n] bf16. Sums of products are exact, so a token's outputs are the same bits
  * in any batch. A token with a NaN or an infinity (or whose product with the norm's

@@ -386,12 +386,6 @@ int check_sizes(const char* op, int m, int n, int k, bool gated) {
     return 0;
 }
 
-// Whether two tensors have a byte in common; one that is absent has none.
-bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const auto at = reinterpret_cast<uintptr_t>(a), bt = reinterpret_cast<uintptr_t>(b);
-    return a != nullptr && b != nullptr && at < bt + uint64_t(b_bytes) && bt < at + uint64_t(a_bytes);
-}
-
 template <bool GATED>
 int product(nv_context* c, const char* op, const void* x, const void* residual, void* residual_out,
             const void* norm_weight, const void* w, const void* w_scales, void* y, void* workspace, int m, int n, int k,
@@ -407,12 +401,12 @@ int product(nv_context* c, const char* op, const void* x, const void* residual, 
     if (!nvr::aligned(w, 16) || !nvr::aligned(workspace, 16) || !nvr::aligned(w_scales, 4) || !nvr::aligned(x, 2) ||
         !nvr::aligned(residual, 2) || !nvr::aligned(residual_out, 2) || !nvr::aligned(norm_weight, 2) || !nvr::aligned(y, 2))
         return nvr::fail(-2, "%s: w and the workspace start at multiples of 16 bytes, scales of 4, others of 2", op);
-    // Blocks read the tokens while others write.
-    const int64_t in_bytes = int64_t(m) * k * 2, out_bytes = int64_t(m) * n * 2;
-    if (overlap(residual_out, in_bytes, x, in_bytes) || overlap(residual_out, in_bytes, residual, in_bytes) ||
-        overlap(y, out_bytes, x, in_bytes) || overlap(y, out_bytes, residual, in_bytes) ||
-        overlap(y, out_bytes, residual_out, in_bytes))
-        return nvr::fail(-2, "%s: an output overlaps the tokens or the other output", op);
+    // Blocks read while others write.
+    const int64_t in_bytes = int64_t(m) * k * 2, channels = GATED ? 2 * int64_t(n) : n;
+    if (nvr::overlap({{residual_out, in_bytes}, {y, int64_t(m) * n * 2}, {workspace, int64_t(workspace_bytes(m, k))}},
+                     {{x, in_bytes}, {residual, in_bytes}, {norm_weight, int64_t(k) * 2}, {w, channels * nvr::i8_pitch(k)},
+                      {w_scales, channels * 4}}))
+        return nvr::fail(-2, "%s: an output or the workspace overlaps another argument", op);
     const nvr::TokenArgs t{static_cast<const uint16_t*>(x),
                            static_cast<const uint16_t*>(residual),
                            static_cast<uint16_t*>(residual_out),

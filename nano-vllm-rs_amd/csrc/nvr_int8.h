@@ -28,6 +28,7 @@
 #pragma once
 
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 #include "nvr_device.h"
@@ -58,6 +59,26 @@ struct TokenArgs {
     int rows, k;
     float eps;
 };
+
+// A tensor's bytes; one that is absent has none.
+struct Span {
+    const void* at;
+    int64_t bytes;
+};
+// Whether one of the tensors that a call writes has a byte in common with another of them, or with one that it reads.
+inline bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    auto common = [](const Span& a, const Span& b) {
+        const auto at = reinterpret_cast<uintptr_t>(a.at), bt = reinterpret_cast<uintptr_t>(b.at);
+        return a.at != nullptr && b.at != nullptr && at < bt + uint64_t(b.bytes) && bt < at + uint64_t(a.bytes);
+    };
+    for (const Span* w = written.begin(); w != written.end(); ++w) {
+        for (const Span& r : read)
+            if (common(*w, r)) return true;
+        for (const Span* other = written.begin(); other != w; ++other)
+            if (common(*w, *other)) return true;
+    }
+    return false;
+}
 
 // The tokens' integers (rows at `pitch` bytes, zeros behind k) and scales (quantize.hip).
 void launch_quantize(nv_context* c, const TokenArgs& t, uint8_t* q, float* scales, int pitch);

@@ -125,6 +125,8 @@ extern "C" int nv_quantize_rows(nv_context* c, const void* x, void* q, void* sca
         return nvr::fail(-2, "quantize_rows: x, q and scales are required");
     if (!nvr::aligned(x, 2) || !nvr::aligned(q, 16) || !nvr::aligned(scales, 4))
         return nvr::fail(-2, "quantize_rows: q starts at a multiple of 16 bytes, x of 2, scales of 4");
+    if (nvr::overlap({{q, rows * nvr::i8_pitch(k)}, {scales, int64_t(rows) * 4}}, {{x, int64_t(rows) * k * 2}}))
+        return nvr::fail(-2, "quantize_rows: q or scales overlap another argument");
     const nvr::TokenArgs t{static_cast<const uint16_t*>(x), nullptr, nullptr, nullptr, rows, k, 0.0f};
     nvr::launch_quantize(c, t, static_cast<uint8_t*>(q), static_cast<float*>(scales), int(nvr::i8_pitch(k)));
     return nvr::launch_status();

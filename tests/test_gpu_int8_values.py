@@ -219,3 +219,31 @@ def test_a_token_behind_a_norm_has_the_same_bits_in_any_batch(gpu, n, k):
         part = Call(gpu, rows, n, k, "rms", x=whole.x[m - rows:].copy(), wq=whole.wq, ws=whole.ws, seed=9)
         part.run()
         assert_bits_equal(part.outputs(), want[m - rows:], f"{rows} tokens")
+
+
+# ---------------------------------------------------------------------- refusals --
+def test_the_library_refuses_what_overlaps(gpu):
+    """At the C entries: an output or the workspace over any other argument, the other outputs too."""
+    lib, h, m, n, k = gpu.lib, gpu.handle, 3, 40, 100
+    names = ("x", "residual", "residual_out", "norm_weight", "w", "w_scales", "y", "workspace")
+    for call, channels, need in ((lib.nv_gemm_i8, n, gpu.gemm_i8_workspace(m, n, k)),
+                                 (lib.nv_gemm_i8_silu, 2 * n, gpu.gemm_i8_silu_workspace(m, n, k))):
+        sizes = dict(zip(names, (m * k * 2, m * k * 2, m * k * 2, k * 2, channels * 112, channels * 4, m * n * 2, need)))
+        room = gpu.alloc(len(names) << 15)
+        at = {name: room.ptr + (i << 15) + (1 << 14) for i, name in enumerate(names)}
+        run = lambda **change: call(h, *{**at, **change}.values(), m, n, k, 1e-6)  # noqa: E731
+        assert run() == 0 and run(x=at["residual"]) == 0
+        for written in ("residual_out", "y", "workspace"):
+            for other in names:
+                if other == written:
+                    continue
+                for place in (at[other], at[other] + (sizes[other] - 1) // 16 * 16, at[other] - (sizes[written] - 1) // 16 * 16):
+                    assert run(**{written: place}) == -2, (written, other, place - at[other])
+                assert run(**{written: at[other] + (sizes[other] + 15) // 16 * 16}) == 0, (written, other)  # behind it
+    rows = 5
+    x, q, s = (room.ptr + (i << 15) for i in range(3))
+    assert lib.nv_quantize_rows(h, x, q, s, rows, k) == 0
+    for args in ((x, x, s), (x, x + 992, s), (x, q, x + 996), (x, q, q), (x, q, q + rows * 112 - 4)):
+        assert lib.nv_quantize_rows(h, *args, rows, k) == -2, args
+    assert lib.nv_quantize_rows(h, x, x + 1008, q, rows, k) == 0 and lib.nv_quantize_rows(h, x, q, q + rows * 112, rows, k) == 0
+    gpu.sync()
