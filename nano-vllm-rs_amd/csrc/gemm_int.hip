@@ -13,7 +13,7 @@
 // whatever the batch.
 //
 // Three forms. Up to 16 tokens over short rows are made into integers by every
-// block, and up to 32 over wide weights are brought to LDS; gemm_rows_i8 then
+// block, and up to 32 over some wide weights are brought to LDS; gemm_rows_i8 then
 // streams the weights through registers, each byte once, bound by HBM and, in the
 // smallest calls, by one chain: tokens, their largest value, products, outputs. All
 // others go by tiles (gemm_int_tiles.hip). On MI355X: 1 token over 1024 x 2048 3.4
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(kThreads) void gemm_rows_i8(RowsArgs a) {
                 *reinterpret_cast<uint4*>(xq + row * pitch + c) =
                     *reinterpret_cast<const uint4*>(p.xq + int64_t(row) * p.x_pitch + c);
         if (int(threadIdx.x) < p.m) xs[threadIdx.x] = p.xs[threadIdx.x];
-        load(unit[0]);  // behind the tokens, for the same reason (16 tokens over 16384 x 4096 18.8 us for 16.2)
+        load(unit[0]);  // behind the tokens, for the same reason
     }
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // leaves the weights in flight
     if constexpr (!ONE) load(unit[1]);
@@ -363,13 +363,26 @@ bool tokens_in_block(const nvr::TokenArgs& t) {
     return t.rows <= 2 * kWaves && t.k <= (t.k % nvr::kChunk == 0 ? chunks : chunks / 2) * nvr::kWaveChunk;
 }
 
-// Whether few tokens, made by a launch of their own, take gemm_rows_i8: where a CU would have more than two of
-// gemm_split's tiles of 32 rows in turn and the tokens fit LDS. On MI355X, weights cold, this and that in us: 16 tokens at k
-// 4096 over n 8192 13.4, 12.3; 16384 20.2, 22.4 (at k 3000 17.3, 15.5, at k 5120 27.3, 21.8); 20480 23.6, 23.8; 32768 32.9,
-// 36.7; 32 tokens over 151936 x 1024 42.0, 47.7; gated 24 over 11008 x 4096 26.2, 26.8.
+// Whether few tokens, made by a launch of their own, take gemm_rows_i8 rather than gemm_split's tiles of 32 rows of the weight.
+// On MI355X, weights cold, tokens' launch included, this and that in us:
+//   more than 16 tokens over a wide weight of short rows, of which a tile is mostly its start and its end: 32 over 151936 at
+//   k 520, 1024, 1030 27.2, 39.1, 43.2 and 32.7, 43.6, 48.5; over 65536 15.9, 21.7, 26.2 and 17.9, 23.8, 25.2; over 40000
+//   (five turns of the CUs) 12.8, 16.3, 20.1 and 13.0, 16.4, 18.5. Of longer rows the tiles are mostly the faster ones: at k
+//   2048 over 40000, 100000, 151936 25.9, 52.0, 70.6 and 23.4, 49.1, 70.6; 24 over 100000 x 4096 97, 84, but 32 over 151936 x
+//   3000 98, 106. 16 tokens: over 40000 x 1024 14.7, 13.6, over 151936 at k 1024, 4096 36.2, 132 and 36.2, 112;
+//   where the runs of tiles that the XCDs take lie a power of two apart, 8 MB or more, so that all eight read the same memory
+//   channels in step, and there is more than a tile a CU: 16 tokens over 16384 at k 4096, 8192 19.2, 30.8 and 21.5, 36.8; over
+//   32768 29.8, 52.4 and 33.6, 72.3; over 65536 56.3, 106 and 58.3, 133; gated over 16384 x 4096 31.0, 35.5; at 16384 x 16384
+//   53.4, 53.4. Beside them: 16384 at k 3000, 4104, 6144 17.6, 23.2, 27.5 and 15.3, 19.5, 22.8; 20480 at k 4096, 8192 22.2,
+//   39.9 and 22.1, 36.7; 8192 x 8192 (a tile a CU) 20.2, 17.9; 12288 x 8192 25.0, 25.5. Gated 24 over 11008 x 4096 24.7, 25.2.
+// Up to 8 tokens over one to two turns of long rows would gain: 8 over 11008, 12288, 13824 at k 12288 31.5, 32.7, 40.0 and
+// 37.0, 36.4, 38.5.
 bool weight_streams(const nv_context* c, const nvr::ProductArgs& p, bool gated) {
-    const int64_t rows = gated ? 2 * int64_t(p.n) : p.n, cus = c->cu_count > 0 ? c->cu_count : 256;
-    return p.m <= kFewTokens && (rows + 31) / 32 > 2 * cus &&
+    const int64_t rows = gated ? 2 * int64_t(p.n) : p.n, cus = c->cu_count > 0 ? c->cu_count : 256, tiles = (rows + 31) / 32;
+    const int64_t run = tiles / nvr::kXcds * (gated ? 16 : 32) * p.w_pitch;  // bytes from an XCD's tiles to the next one's
+    const bool in_step = tiles > cus && run >= 8 << 20 && (run & (run - 1)) == 0;
+    const bool wide = p.m > 16 && tiles >= 8 * cus && p.x_pitch <= 1152;
+    return p.m <= kFewTokens && (in_step || wide) &&
            (p.m <= 16 ? rows_lds<1>(p.m, p.x_pitch) : rows_lds<2>(p.m, p.x_pitch)) <= kMostLds;
 }
 

@@ -21,8 +21,6 @@ using nvr::kWave;
 using nvr::Scale;
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kXcds = 8;
-
 // A block's tile of BM tokens and BN channels (gated: BN / 2 of gate and of up), by WM x WN waves; STAGES stages in LDS of
 // KB bytes of k of each row.
 template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
@@ -54,7 +52,7 @@ __device__ __forceinline__ void wait_stages(int late) {
 // read few rows of either operand.
 __device__ __forceinline__ int2 tile_of(unsigned block, unsigned blocks, int mt, int nt) {
     // Blocks go to XCDs in turn; each XCD takes a run of tiles.
-    const unsigned xcd = block % kXcds, at = block / kXcds, whole = blocks / kXcds, more = blocks % kXcds;
+    const unsigned xcd = block % nvr::kXcds, at = block / nvr::kXcds, whole = blocks / nvr::kXcds, more = blocks % nvr::kXcds;
     const unsigned tile = xcd * whole + min(xcd, more) + at;
     constexpr unsigned kGroup = 4;
     const unsigned per = kGroup * unsigned(nt), group = tile / per, in = tile % per;

@@ -41,6 +41,8 @@ constexpr int kChunk = 8;                      // elements of a lane's load (16 
 constexpr int kWaveChunk = kChunk * kWave;     // elements a wave covers with one load a lane
 constexpr int kClasses = 16;
 
+constexpr int kXcds = 8;
+
 // Rows of 8-bit integers start at multiples of 16 bytes.
 __host__ __device__ constexpr int64_t i8_pitch(int64_t k) { return (k + 15) / 16 * 16; }
 

@@ -247,3 +247,33 @@ def test_the_library_refuses_what_overlaps(gpu):
         assert lib.nv_quantize_rows(h, *args, rows, k) == -2, args
     assert lib.nv_quantize_rows(h, x, x + 1008, q, rows, k) == 0 and lib.nv_quantize_rows(h, x, q, q + rows * 112, rows, k) == 0
     gpu.sync()
+
+
+# ------------------------------------------------------------- tokens brought to LDS --
+# Made by a launch of their own, for weights that stream: more than 16 tokens over wide weights of short rows, and weights whose
+# parts lie a power of two apart; and the shapes beside them, which go by tiles.
+@pytest.mark.parametrize("m,n,k,gated", [
+    (17, 65540, 72, False), (24, 65600, 400, False), (32, 70001, 1030, False), (29, 33000, 264, True), (32, 33001, 1000, True),
+    (31, 66000, 1152, False), (20, 66008, 130, False), (24, 65504, 72, False), (24, 65500, 264, False), (18, 66000, 1160, False),
+    (12, 16384, 4096, False), (16, 16390, 4090, False), (3, 16384, 8190, False), (20, 32768, 2048, False), (12, 16384, 4104, False),
+    (10, 16384, 4096, True), (9, 32760, 2040, True), (17, 8192, 8192, False)])
+@pytest.mark.parametrize("norm", ["none", "add"])
+def test_products_over_wide_weights(gpu, m, n, k, gated, norm):
+    call = Call(gpu, m, n, k, norm, gated, seed=n + k)
+    call.run()
+    got = f64(call.outputs())
+    # The first and the last channels, and those of places in between.
+    some = np.unique(np.r_[np.arange(100), np.arange(n - 100, n), np.random.default_rng(n).integers(0, n, 300)])
+    rows = np.r_[some, n + some] if gated else some
+    want, bound = ref.product(f64(call.x), None if call.residual is None else f64(call.residual),
+                              None if call.weight is None else f64(call.weight), 1e-6, call.wq[rows],
+                              call.ws[rows].astype(np.float64), gated)
+    assert (np.abs(got[:, some] - want) <= bound).all()
+    assert not np.isnan(got).any() and np.abs(got).max() < 1e6  # the others: no byte of 0xA5 is left
+    assert (got == f64(np.uint16(0xA5A5))).mean() < 1e-3
+    assert (call.by.download(np.uint8, call.by.bytes)[-256:] == 0xA5).all()
+    # A token by itself has the same bits: other forms made it.
+    one = Call(gpu, 1, n, k, norm, gated, x=call.x[-1:].copy(), wq=call.wq, ws=call.ws, seed=n + k,
+               residual=None if call.residual is None else call.residual[-1:].copy())
+    one.run()
+    assert_bits_equal(one.outputs()[0], call.outputs()[-1])
