@@ -299,10 +299,16 @@ void plan_rows(RowsArgs& a, int tiles, int parts, int blocks) {
 
 template <Source SRC, bool WHOLE, bool GATED>
 void launch_rows(nv_context* c, RowsArgs a) {
+    constexpr bool kMade = SRC != Source::kCopied;
     const int tiles = (a.p.n + (GATED ? 8 : 16) - 1) / (GATED ? 8 : 16);
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
     const int lines = a.p.x_pitch / 128;
-    // As many waves for a tile as leave each one tile, if its share of k is then one unit; else up to four turns of them.
+    // As many waves for a tile as leave each one tile, if its share of k is then one unit; else up to four turns of them. On
+    // MI355X, weights cold, in us by 1, 2, 4 and 8 waves a tile: 1 token over 4096 x 1024 6.1, 4.4, 3.5, 3.1; over 16384 x 1024
+    // 6.7, 5.6, 6.2, 7.7; 16 over 4096 x 1024 7.2, 4.9, 4.6, 4.4; gated 1 over 4096 x 1024 6.9, 5.3, 4.6, 5.8, over 11008 x 4096
+    // 21.8, 24.3, 19.5, 21.8; 4 with sum and norm over 8192 x 4096 21.3, 14.3, 11.4, 11.7, over 65536 x 4096 57.1, 50.6, 49.6,
+    // 51.3; 8 with norm over 151936 x 1024 32.6, 33.1, 34.4, 48.8. Takes more waves than are best for 1 over 65536 at k 256, 1024
+    // (2, where 1 and 2 are 5.8, 14.9 and 7.9, 16.0) and 16384 x 4096 (8: 19.6, 14.2, 14.6, 16.2).
     auto fits = [&](int parts) { return int64_t(tiles) * parts <= int64_t(cus) * kWaves && (lines + parts - 1) / parts <= 4; };
     int parts = fits(8) ? 8 : fits(4) ? 4 : fits(2) ? 2 : fits(1) ? 1 : 8;
     if (!fits(parts))
@@ -317,14 +323,22 @@ void launch_rows(nv_context* c, RowsArgs a) {
             a.units = (a.share * 2 + STEPS - 1) / STEPS;
             launch_rows_as<SRC, WHOLE, CH, RW, MT, GATED, STEPS, decltype(one)::value>(c, a, blocks);
         };
+        // The fewest loads that hold a wave's share: each is made, also behind it. On MI355X, in us, as here, by the next larger
+        // unit, and by two of 8 steps in turn: 1 token over 4096 at k 1024 (2 steps) 3.1, 3.3, 5.6, with sum and norm 3.5, 3.8,
+        // 5.9; at k 2048 (4) 4.2, 5.2, 6.4; at k 4096 (8) 6.1, -, 7.9. Of several tiles in turn, over 65536 at k 128, 256 (4)
+        // 5.0, 7.9, by 8 6.4, 11.2. Tokens brought to LDS meet wide weights: several tiles a wave, without one unit's forms.
         const auto one = std::true_type{};
-        if constexpr (WHOLE) {
+        if constexpr (WHOLE && kMade) {
             if (alone && a.share == 1) return with(std::integral_constant<int, 2>{}, one);
+        }
+        if constexpr (WHOLE) {
             if (!alone && a.share <= 2) return with(std::integral_constant<int, 4>{}, std::false_type{});
         }
-        if (alone && a.share <= 2) with(std::integral_constant<int, 4>{}, one);
-        else if (alone && a.share <= 4) with(std::integral_constant<int, 8>{}, one);
-        else with(std::integral_constant<int, 8>{}, std::false_type{});
+        if constexpr (kMade) {
+            if (alone && a.share <= 2) return with(std::integral_constant<int, 4>{}, one);
+            if (alone && a.share <= 4) return with(std::integral_constant<int, 8>{}, one);
+        }
+        with(std::integral_constant<int, 8>{}, std::false_type{});
     };
     using std::integral_constant;
     const integral_constant<int, 1> one;
@@ -350,11 +364,13 @@ void launch_rows(nv_context* c, RowsArgs a) {
 
 // Whether each block makes the tokens' integers by itself, a row or two a wave: one launch less, for work that all blocks
 // repeat. On MI355X in a graph, weights cold, n 4096, made and by a launch of their own, in us:
-//   k 1024: 1 token 3.1, 5.6; 8 with sum and norm 4.2, 6.2; 16 4.3, 5.7, with sum and norm 5.4, 6.2;
-//   k 2048: 8 5.0, 6.7, with sum and norm 6.3, 7.5; 9 to 16 5.0 to 6.1, 6.7 (over n 16384 10.9 to 12.4, 11.3); 16 with sum
-//   and norm 8.8, 7.8;
+//   k 1024: 1 token 3.1, 5.6; 8 with sum and norm 4.2, 6.2; 16 4.4, 5.7, with sum and norm 5.6, 6.1;
+//   k 2048: 8 5.0, 6.7, with sum and norm 6.3, 7.3; 9 and 16 5.1, 6.2 and 6.8, 7.0; 16 with sum and norm 8.8, 7.8;
 //   k 4096: 8 8.2, 8.6; with sum and norm 4 8.1, 9.0, but 6 10.5, 9.1: two waves of a SIMD then have a row each, and a row's
 //   chunks, sums and norm weights fill the registers beside the weights.
+// What every block repeats does not grow with n, and neither does what it saves. 16 at k 2048 over n 1024, 8192, 16384, 32768,
+// 65536: 5.4, 7.7, 11.8, 17.5, 28.4 and 6.0, 8.0, 11.2, 19.0, 30.8; 16 with sum and norm at k 1024 5.3, 6.2, 7.9, 12.0, 17.7 and
+// 5.9, 7.3, 8.6, 13.2, 19.9; 8 at k 4096 5.9, 12.2, 17.4, 28.2, 51.3 and 7.3, 12.0, 18.8, 29.2, 53.1.
 // Chunks of a k that is no multiple of 8 take shifts, so half as many: 8 at k 2041 5.2, 6.8, at 4090 9.7, 8.8; 1 with sum and
 // norm at 2041 6.8, 7.6, at 4090 15.0, 9.6; 8 at 1001 5.2, 6.7, at 1111 7.5, 7.0; 16 at 1001 5.0, 5.9, at 1111 7.1, 6.4.
 bool tokens_in_block(const nvr::TokenArgs& t) {

@@ -458,8 +458,10 @@ namespace nvr {
 //   a tile's k over four waves while there is a tile a CU: 256 tokens over 1024 x 2048 by tiles of 64 x 32, 64 x 64 and
 //   128 x 128 5.2, 7.3, 11.2; 100 over 6144 x 4096 13.1 (in two turns), 10.9, 15.2; 512 over 4096 x 1024 (two turns of 64 x
 //   64) -, 10.7, 7.9;
-//   up to 64 tokens over wide weights, 64 x 128 and 128 x 128: 64 over 151936 x 1024 41.2, 46.1; over 32768 x 4096 38.8,
-//   44.8 (and 64 x 64 40.6);
+//   up to 64 tokens past a tile of 64 x 64 a CU, by 64 x 128 (just past it 129 blocks), 64 x 64 in two turns and 128 x 128,
+//   whole calls: 64 over 16640 x 1024 11.3, 15.9, 13.8, at k 4096 27.2, 33.3, 36.3; over 22016 x 4096 29.2, 35.1, 38.2; 33 over
+//   16640 x 4096 25.2, 30.1, 35.9; over 32768 x 4096 36.8, 37.7, 41.9; 64 over 40000 x 4096 48.3, 50.6, 47.5; over 65536 x 4096
+//   65.9, 75.9, 71.0; gated 64 over 11008 x 4096 28.6, 35.0, 38.4; the product of 64 over 151936 x 1024 41.2, -, 46.1;
 //   256 x 256 against 128 x 128, two of which share a CU: 8192 over 12288 x 4096 (6 turns, 24) 356, 422; 4096 over 4096 x
 //   1024 (1, 4) 23.2, 24.6; 768 over 12288 x 4096 (1, 3) 48.9, 52.1; 1500 over 4096 x 12288 (1, 2) 125, 85; 2048 over 4096 x
 //   1024 (1, 2) 20.8, 14.2. Where k is short, a tile is mostly its outputs, which two blocks overlap: 5327 over 18704 x 176
