@@ -251,8 +251,9 @@ __device__ __forceinline__ float add_squares(float sum, const float* v) {
     return sum;
 }
 // A row's scale with 1 / rms in it, s its classes' sums. Where the squares leave fp32 the row is read once more, by each of
-// its waves, with the values at 2^-80, eps at 2^-160: their mean square is 2^111 at least, so what is lost below does not count.
-template <Tokens T, bool WHOLE>
+// its waves, and summed in 64 bits, in little code, which every launch has to fetch; 1 / rms is then formed at 2^80 and eps
+// put in at 2^-160 (it does not count beside a mean square of 2^111 and more unless it is as large).
+template <Tokens T>
 __device__ __forceinline__ float normed_scale(float scale, const float* s, const TokenArgs& t, int64_t row, int lane) {
     float total[kClasses];
 #pragma unroll
@@ -262,19 +263,14 @@ __device__ __forceinline__ float normed_scale(float scale, const float* s, const
 #pragma unroll
         for (int i = 0; i < kClasses; i += 2 * w) total[i] = total[i] + total[i + w];
     if (__builtin_expect(total[0] != __builtin_inff(), 1)) return scale * inv_sqrt_rn(total[0] / float(t.k) + t.eps);
-    float sums[kChunk] = {};
+    double squares = 0.0;
 #pragma unroll 1
-    for (int j = lane * kChunk; j < t.k; j += kWaveChunk) {
-        const uint4 x = load_chunk<WHOLE>(t.x + row * t.k, j, t.k);
-        float v[kChunk];
-        row_values<T>(x, T == Tokens::kAddNorm ? load_chunk<WHOLE>(t.residual + row * t.k, j, t.k) : x, v);
-#pragma unroll
-        for (int i = 0; i < kChunk; ++i) {
-            const float small = __builtin_amdgcn_ldexpf(v[i], -80);
-            sums[i] = __builtin_fmaf(small, small, sums[i]);
-        }
+    for (int j = lane; j < t.k; j += kWave) {
+        float v = bf16_to_f32(t.x[row * t.k + j]);
+        if constexpr (T == Tokens::kAddNorm) v = v + bf16_to_f32(t.residual[row * t.k + j]);
+        squares = __builtin_fma(double(v), double(v), squares);
     }
-    const float sum = wave_sum(((sums[0] + sums[1]) + (sums[2] + sums[3])) + ((sums[4] + sums[5]) + (sums[6] + sums[7])));
+    const float sum = wave_sum(float(squares * 0x1.0p-160));
     const float inverse = inv_sqrt_rn(sum / float(t.k) + __builtin_amdgcn_ldexpf(t.eps, -160));
     return __builtin_amdgcn_ldexpf(scale, -40) * __builtin_amdgcn_ldexpf(inverse, -40);
 }
@@ -330,7 +326,7 @@ __device__ __forceinline__ RowStep quantize_row(const TokenArgs& t, int64_t row,
     }
     join(s, top);
     RowStep step = row_step(top);
-    if constexpr (T != Tokens::kPlain) step.scale = normed_scale<T, WHOLE>(step.scale, s, t, row, lane);
+    if constexpr (T != Tokens::kPlain) step.scale = normed_scale<T>(step.scale, s, t, row, lane);
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         const int j = chunk_at<WAVES>(c, lane, wave);
@@ -365,7 +361,7 @@ __device__ __forceinline__ RowStep quantize_long_row(const TokenArgs& t, int64_t
     if constexpr (T != Tokens::kPlain) s[0] = wave_sum(s[0]);
     join(s, top);
     RowStep step = row_step(top);
-    if constexpr (T != Tokens::kPlain) step.scale = normed_scale<T, WHOLE>(step.scale, s, t, row, lane);
+    if constexpr (T != Tokens::kPlain) step.scale = normed_scale<T>(step.scale, s, t, row, lane);
     for (int c = 0; c < chunks; ++c) {
         const int j = load(c, v);
         if constexpr (T != Tokens::kPlain) times(v, load_chunk<WHOLE>(t.norm_weight, j, t.k));
