@@ -402,13 +402,17 @@ __global__ __launch_bounds__(kSplitThreads) void gemm_split(nvr::ProductArgs p, 
         const int channel = n0 + i * 16 + 4 * (kHalves ? lane / 16 % 2 : lane / 16);
         const float* ws = p.ws + (kHalves && lane >= 32 ? int64_t(p.n) : 0);
         const Scale xs = nvr::split_scale(p.xs[min(token, int64_t(p.m) - 1)]);
-        float y[4];
+        float y[4], u[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < 4; ++r) {  // all scales are asked for before the first gate's branch
             const int c = min(channel + r, p.n - 1);
             y[r] = nvr::scaled(sum[r], xs, nvr::split_scale(ws[c]));
-            if constexpr (kHalves) y[r] = nvr::gated(y[r], nvr::xor_lane(y[r], 32));  // the other half has the up rows
-            else if constexpr (GATED) y[r] = nvr::gated(y[r], nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c])));
+            if constexpr (kHalves) u[r] = nvr::xor_lane(y[r], 32);  // the other half has the up rows
+            else if constexpr (GATED) u[r] = nvr::scaled(up[r], xs, nvr::split_scale(p.ws[int64_t(p.n) + c]));
+        }
+        if constexpr (GATED) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = nvr::gated(y[r], u[r]);
         }
         if (token >= p.m || (kHalves && lane >= 32)) continue;
         nvr::store_outputs(p.y + token * p.n + channel, y, channel, p.n);
