@@ -352,7 +352,7 @@ int nv_gemm_i8_silu_workspace(int m, int intermediate, int k, size_t* bytes);
  * (as a bf16 gate_up weight has them), and act[m, intermediate] =
  * bf16(g / (1 + e^-g) * u) with g and u the products of nv_gemm_i8 before its
  * rounding, in fp32: one past its range is an infinity, and a gate of -inf gives 0
- * for any finite u. Everything else as nv_gemm_i8. */
+ * for any finite u (an infinity times 0 is NaN). Everything else as nv_gemm_i8. */
 int nv_gemm_i8_silu(nv_context* c, const void* x, const void* residual, void* residual_out, const void* norm_weight,
                     const void* w, const void* w_scales, void* act, void* workspace, int m, int intermediate, int k,
                     float eps);

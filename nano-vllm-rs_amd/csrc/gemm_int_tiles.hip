@@ -10,7 +10,9 @@
 //   The two stages of 128 bytes of k take 128 KB of LDS. Three or four stages of 64 bytes, whose barriers come twice as often,
 //   380 us for 349. A depth's operands are read one depth ahead, a read between two products, so that the units never wait.
 //   Outputs go through LDS, so that a store writes whole rows of 128 bytes: 8 bytes a lane into 16 rows at once 631 us for
-//   393. What is left over the products, about 15%, is the first stage's way to LDS and the outputs, in each of 6 turns.
+//   393. Products with their operands' reads alone would take 241 us. Of the 108 over them 53 do not grow with k (k 2048,
+//   4096, 8192 199, 349, 635 us): the first stage's way to LDS and the outputs, in each of 6 turns. The others, in the loop,
+//   are its barriers, copies and waits, not told apart.
 #include "../../include/nano_hip.h"
 #include "nvr_int8.h"
 #include "nvr_internal.h"
@@ -254,8 +256,9 @@ __global__ __launch_bounds__(S::THREADS) void gemm_tiles(nvr::ProductArgs p, int
 // unit of 128 bytes of k. A wave copies and reads its units by itself, SLOTS of them in LDS, so the loop has no barrier; each
 // byte of LDS is read once, where four waves side by side would read it twice, and one group's products cover the next one's
 // reads. Bound by the copies: what a CU brings to LDS from L2 (110 to 130 bytes a ns; 27 from beyond), or by their
-// latency: 16 tokens over 4096 x 12288, 50 MB of cold weights, 17.0 us with the tokens' launch, 3.0 TB/s; 100 over 6144 x 4096
-// 10.9 us without it, 460 TOPS.
+// latency: 16 tokens over 4096 x 12288, 50 MB of cold weights, 16.6 us with the tokens' launch, 3.0 TB/s. 100 over 6144 x 4096
+// 11.4 us without it, 5.1 of them at any k (the launch, first copies, the waves' sums, outputs); the others are 84 bytes a ns
+// a CU, with cold weights 61.
 constexpr int kUnitBytes = 128, kSplit = 4, kSplitThreads = kSplit * kWave;
 
 template <int TOK, int SIDE, int SLOTS, bool GATED>

@@ -277,3 +277,15 @@ def test_products_over_wide_weights(gpu, m, n, k, gated, norm):
                residual=None if call.residual is None else call.residual[-1:].copy())
     one.run()
     assert_bits_equal(one.outputs()[0], call.outputs()[-1])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 1024), (8, 1111), (20, 200), (40, 2500), (17, 9000), (3, 20001), (1030, 2000), (1030, 5000)])
+def test_the_sum_may_stay_inside(gpu, m, k, gated):
+    """A residual without residual_out: the same outputs."""
+    call = Call(gpu, m, 70, k, "add", gated)
+    call.run()
+    want, call.bout = call.outputs(), None
+    call.by.upload(np.full(call.by.bytes, 0xA5, np.uint8))
+    call.run()
+    assert_bits_equal(call.outputs(), want)
