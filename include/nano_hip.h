@@ -340,8 +340,9 @@ int nv_gemm_i8_workspace(int m, int n, int k, size_t* bytes);
  * in any batch. A token with a NaN or an infinity (or whose product with the norm's
  * weight leaves fp32) has NaN in its row of y, and no other has where the scales are
  * finite: a channel of scale NaN, as nv_quantize_rows makes it of a row with a NaN,
- * is NaN for every token. eps is read with a norm_weight only. Any m and n that one launch holds (2^32 threads; else -2) and any
- * k; tensors of bf16 start at any even address, scales at multiples of 4 bytes. */
+ * is NaN for every token. eps is read with a norm_weight only. Any m and n that one
+ * launch holds (2^32 threads; else -2) and any k; tensors of bf16 start at any even
+ * address, scales at multiples of 4 bytes. */
 int nv_gemm_i8(nv_context* c, const void* x, const void* residual, void* residual_out, const void* norm_weight,
                const void* w, const void* w_scales, void* y, void* workspace, int m, int n, int k, float eps);
 

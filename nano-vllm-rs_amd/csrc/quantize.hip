@@ -63,15 +63,15 @@ __global__ __launch_bounds__(kThreads<WAVES>) void quantize_rows(nvr::TokenArgs 
     }
 }
 
-// Bound by memory: 3 bytes an element move (7 with a residual): 8192 rows of 4096 in 25 us, 4.0 TB/s, with sum and norm
-// 4096 rows in 28 us, 4.2 TB/s. A row is read once and stays in registers. With many rows one wave takes up to 4096
-// values, so that it waits for no barrier, four up to 16384. With few, latency counts: 4 waves take up to 2048, 16 up to
-// 16384, in as little code as that gives (it is read anew by each launch: 3 odd rows of 8989 by 4 waves of 8 chunks 10 us).
-// Longer rows are read twice. Inputs cold, in us, as for few rows and as for many, 256, 1024, 2048, 8192 rows: k 1024 2.3, 3.1,
-// 3.7, 9.6 and 2.1, 2.8, 3.4, 6.5; k 2048 2.7, 3.6, 4.6, 11.7 and 3.5, 3.8, 5.2, 11.0; k 4096 3.0, 5.9, 10.3, 30.9 and 3.3, 4.7,
-// 6.8, 17.7; k 4090 3.2, 6.3, 11.2, 33.8 and 4.9, 6.6, 8.7, 20.7; k 16384 4.6, 11.2, 18.4, 71.1 and 4.8, 10.8, 17.3, 72.8. With
-// sum and norm and a product of 16 channels behind it, 1024 and 8192 rows: k 1024 7.4, 19.2 and 6.8, 15.7; k 4096 15.0, 53.4 and
-// 14.0, 45.8; but k 1111 8.3, 22.9 and 9.9, 27.3, k 8192 21.4, 103 and 22.0, 107.
+// Bound by memory: 3 bytes an element move (7 with a residual): 8192 rows of 4096 in 17.7 us of a graph, inputs cold, 5.7
+// TB/s, with sum and norm 4096 rows in 28 us, 4.2 TB/s. A row is read once and stays in registers. With many rows one wave
+// takes up to 4096 values, so that it waits for no barrier, four up to 16384. With few, latency counts: 4 waves take up to
+// 2048, 16 up to 16384, in as little code as that gives (it is read anew by each launch: 3 odd rows of 8989 by 4 waves of 8
+// chunks 10 us). Longer rows are read twice. Inputs cold, in us, as for few rows and as for many, 256, 1024, 2048, 8192
+// rows: k 1024 2.3, 3.1, 3.7, 9.6 and 2.1, 2.8, 3.4, 6.5; k 2048 2.7, 3.6, 4.6, 11.7 and 3.5, 3.8, 5.2, 11.0; k 4096 3.0,
+// 5.9, 10.3, 30.9 and 3.3, 4.7, 6.8, 17.7; k 4090 3.2, 6.3, 11.2, 33.8 and 4.9, 6.6, 8.7, 20.7; k 16384 4.6, 11.2, 18.4,
+// 71.1 and 4.8, 10.8, 17.3, 72.8. With sum and norm and a product of 16 channels behind it, 1024 and 8192 rows: k 1024 7.4,
+// 19.2 and 6.8, 15.7; k 4096 15.0, 53.4 and 14.0, 45.8; but k 1111 8.3, 22.9 and 9.9, 27.3, k 8192 21.4, 103 and 22.0, 107.
 template <Tokens T, bool WHOLE>
 void launch(nv_context* c, const nvr::TokenArgs& t, uint8_t* q, float* scales, int pitch) {
     const int cus = c->cu_count > 0 ? c->cu_count : 256;
